@@ -30,6 +30,7 @@ __all__ = [
     "LIB_PATH", "DyninferError", "QWeight", "Context", "library", "candidates", "registry_select",
     "registry_require", "precision_check", "supports", "ENC_Q4_0", "ENC_Q4_1", "ENC_Q8_0", "ENC_Q6_K", "ENC_Q4_K", "ENC_Q5_K", "ENC_IQ4_XS", "ENC_MLX_U4",
     "DTYPE_F32", "DTYPE_F16", "DTYPE_BF16", "block_geometry", "weight_bytes", "prefill_workspace_bytes",
+    "KV_Q8", "KV_Q4", "KVCache", "KVBatch", "Rope", "ROPE_INTERLEAVED", "ROPE_HALF", "ROPE_SCALINGS",
     "ERR_INVALID_ARGUMENT",
     "ERR_UNSUPPORTED", "ERR_HIP", "ERR_DEVICE", "ERR_BUFFER_TOO_SMALL",
 ]
@@ -41,6 +42,10 @@ ENC_Q4_0, ENC_Q4_1, ENC_Q8_0, ENC_Q6_K, ENC_MLX_U4 = 2, 3, 8, 14, 0x1004
 # GGML's block_q4_K / block_q5_K / block_iq4_xs: schema-only types in the reference (gguf_block.rs:183-316)
 ENC_Q4_K, ENC_Q5_K, ENC_IQ4_XS = 12, 13, 23
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+KV_Q8, KV_Q4 = 1, 2  # DYNINFER_KV_*
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ROPE_LAYOUTS = {"interleaved": ROPE_INTERLEAVED, "half": ROPE_HALF}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "yarn": 2, "bands": 3}
 NOALLOC_SCRATCH_BYTES = 32 << 20  # DYNINFER_MI355X_NOALLOC_SCRATCH_BYTES
 ENCODING_IDS = {ENC_Q4_0: "gguf.q4_0", ENC_Q4_1: "gguf.q4_1", ENC_Q8_0: "gguf.q8_0", ENC_Q6_K: "gguf.q6_k",
                 ENC_Q4_K: "gguf.q4_k", ENC_Q5_K: "gguf.q5_k", ENC_IQ4_XS: "gguf.iq4_xs", ENC_MLX_U4: "mlx.affine.u4"}
@@ -60,6 +65,10 @@ EXPORTED_SYMBOLS = (
     "dyninfer_mi355x_safetensors_tensor_count", "dyninfer_mi355x_safetensors_metadata_json",
     "dyninfer_mi355x_safetensors_tensor", "dyninfer_mi355x_safetensors_find", "dyninfer_mi355x_safetensors_upload",
     "dyninfer_mi355x_safetensors_mlx_qweight", "dyninfer_mi355x_prefill_workspace_bytes",
+    "dyninfer_mi355x_rope_table", "dyninfer_mi355x_rope", "dyninfer_mi355x_kv_cache_bytes", "dyninfer_mi355x_kv_append",
+    "dyninfer_mi355x_kv_read", "dyninfer_mi355x_kv_commit", "dyninfer_mi355x_tree_attention",
+    "dyninfer_mi355x_tree_attention_workspace_bytes", "dyninfer_mi355x_draft_verify",
+    "dyninfer_mi355x_draft_verify_workspace_bytes",
 )
 
 
@@ -82,6 +91,14 @@ class _QWeightC(ctypes.Structure):
 
 
 _pack_qweight = struct.Struct("@2I5Q2I3Q").pack  # _QWeightC's layout
+
+# the descriptors of the calls around attention, as the bytes of their C structs
+_pack_kvcache = struct.Struct("@6I5Q").pack
+_pack_kvbatch = struct.Struct("@3Q4IQ").pack
+_pack_rows = struct.Struct("@Q2I2q").pack
+_pack_rope = struct.Struct("@2Q4I").pack
+_pack_rope_params = struct.Struct("@2I8d").pack
+_pack_verify = struct.Struct("@2Q2I2q6Qq4I3Q").pack
 
 _lib: Optional[ctypes.CDLL] = None
 
@@ -143,6 +160,16 @@ def library() -> ctypes.CDLL:
         "dyninfer_mi355x_safetensors_find": (I, [P, ctypes.c_char_p, ctypes.POINTER(_StTensorC)]),
         "dyninfer_mi355x_safetensors_upload": (I, [P, ctypes.c_char_p, P, ctypes.c_uint64, P]),
         "dyninfer_mi355x_safetensors_mlx_qweight": (I, [P, ctypes.c_char_p, P, P, P, W]),
+        "dyninfer_mi355x_rope_table": (I, [P, P, U32, P, P]),
+        "dyninfer_mi355x_rope": (I, [P, P, P, U32, U32, P, P]),
+        "dyninfer_mi355x_kv_cache_bytes": (I, [P, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)]),
+        "dyninfer_mi355x_kv_append": (I, [P, P, P, P, P, P, P, P, P]),
+        "dyninfer_mi355x_kv_read": (I, [P, P, P, P, P, P]),
+        "dyninfer_mi355x_kv_commit": (I, [P, P, P, P, U32, P, P]),
+        "dyninfer_mi355x_tree_attention": (I, [P, P, P, P, P, U32, ctypes.c_float, P, P, P, ctypes.c_uint64, P]),
+        "dyninfer_mi355x_tree_attention_workspace_bytes": (I, [P, P, U32, U32, ctypes.POINTER(ctypes.c_uint64)]),
+        "dyninfer_mi355x_draft_verify": (I, [P, P, P, ctypes.c_uint64, P]),
+        "dyninfer_mi355x_draft_verify_workspace_bytes": (I, [U32, U32, U32, U32, ctypes.POINTER(ctypes.c_uint64)]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -289,6 +316,118 @@ def _workspace_bytes(packed: bytes, count: int, rows: int, x_dtype: int, y_dtype
     return n.value
 
 
+def _bad(message: str):
+    raise DyninferError(ERR_INVALID_ARGUMENT, message)
+
+
+def _table(t, dtype: str, shape, what: str) -> int:
+    """Address of a contiguous device tensor of that type and shape (None: any length)."""
+    if t is None:
+        _bad(f"{what} is missing")
+    if not t.is_cuda or str(t.dtype) != dtype or not t.is_contiguous() or t.dim() != len(shape) \
+            or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        want = ", ".join("n" if n is None else str(n) for n in shape)
+        _bad(f"{what} must be a contiguous device tensor [{want}] of {dtype[6:]}")
+    return t.data_ptr()
+
+
+def _rows(t, tokens: int, dim: int, what: str) -> bytes:
+    """The C descriptor of a device tensor [tokens, heads, dim] whose last axis is contiguous."""
+    if not t.is_cuda or t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != dim or t.stride(2) != 1:
+        _bad(f"{what} must be a device tensor [{tokens}, heads, {dim}] whose last axis is contiguous")
+    return _pack_rows(t.data_ptr(), _dtype_code(t), t.shape[1], t.stride(0), t.stride(1))
+
+
+@dataclass
+class KVCache:
+    """A paged key/value cache (dyninfer_kvcache_t): uint8 device tensors ``k`` and ``v`` in the
+    layout the C header states.  ``KVCache.empty`` allocates them through torch."""
+    k: object
+    v: object
+    pages: int
+    kv_heads: int
+    head_dim: int
+    page_size: int = 64
+    k_encoding: int = KV_Q8
+    v_encoding: int = KV_Q8
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, k_encoding: int = KV_Q8,
+              v_encoding: int = KV_Q8, device="cuda") -> "KVCache":
+        import torch
+        kb, vb = cls.bytes(pages, kv_heads, head_dim, page_size, k_encoding, v_encoding)
+        new = lambda n: torch.empty(n, dtype=torch.uint8, device=device)
+        return cls(new(kb), new(vb), pages, kv_heads, head_dim, page_size, k_encoding, v_encoding)
+
+    @staticmethod
+    def bytes(pages: int, kv_heads: int, head_dim: int, page_size: int = 64, k_encoding: int = KV_Q8,
+              v_encoding: int = KV_Q8):
+        """Bytes of the two buffers (dyninfer_mi355x_kv_cache_bytes)."""
+        kb, vb = ctypes.c_uint64(0), ctypes.c_uint64(0)
+        try:
+            packed = _pack_kvcache(k_encoding, v_encoding, kv_heads, head_dim, page_size, 0, pages, 0, 0, 0, 0)
+        except struct.error as e:
+            _bad(f"cache: {e}")
+        _check(library().dyninfer_mi355x_kv_cache_bytes(packed, ctypes.byref(kb), ctypes.byref(vb)))
+        return kb.value, vb.value
+
+    def pack(self) -> bytes:
+        """The C struct's bytes."""
+        for t in (self.k, self.v):
+            if not t.is_cuda or not t.is_contiguous():
+                _bad("cache buffers must be contiguous device tensors")
+        try:
+            return _pack_kvcache(self.k_encoding, self.v_encoding, self.kv_heads, self.head_dim, self.page_size, 0,
+                                 self.pages, self.k.data_ptr(), self.v.data_ptr(), self.k.numel() * self.k.element_size(),
+                                 self.v.numel() * self.v.element_size())
+        except struct.error as e:
+            _bad(f"cache: {e}")
+
+
+@dataclass
+class KVBatch:
+    """The sequences of a call (dyninfer_kvbatch_t): row starts[b] + i of the call's tensors is the
+    token at position lengths[b] + i of sequence b.  ``page_table`` [sequences, table_pages],
+    ``lengths`` [sequences] and ``starts`` [sequences + 1] are int32 device tensors; ``tokens``
+    the rows of the call's tensors, ``max_new`` the most rows of a sequence, ``max_length`` the
+    largest length with its rows."""
+    page_table: object
+    lengths: object
+    starts: object
+    tokens: int
+    max_new: int
+    max_length: int
+
+    def pack(self) -> bytes:
+        """The C struct's bytes."""
+        n = self.lengths.shape[0] if self.lengths.dim() == 1 else -1
+        try:
+            return _pack_kvbatch(_table(self.page_table, "torch.int32", (n, None), "page_table"),
+                                 _table(self.lengths, "torch.int32", (n,), "lengths"),
+                                 _table(self.starts, "torch.int32", (n + 1,), "starts"), n, self.page_table.shape[1],
+                                 self.tokens, self.max_new, self.max_length)
+        except struct.error as e:
+            _bad(f"batch: {e}")
+
+
+@dataclass
+class Rope:
+    """Rotary positions of a call (dyninfer_rope_t): ``table`` [positions, rot_dim / 2, 2] from
+    ``Context.rope_table``, ``positions`` int32 [tokens], ``layout`` "interleaved" or "half"."""
+    table: object
+    positions: object
+    rot_dim: int
+    layout: str = "half"
+
+    def pack(self, tokens: int) -> bytes:
+        """The C struct's bytes."""
+        if self.layout not in ROPE_LAYOUTS:
+            _bad(f"rope layout must be one of {sorted(ROPE_LAYOUTS)}")
+        return _pack_rope(_table(self.table, "torch.float32", (None, self.rot_dim // 2, 2), "rope table"),
+                          _table(self.positions, "torch.int32", (tokens,), "positions"), self.table.shape[0], self.rot_dim,
+                          ROPE_LAYOUTS[self.layout], 0)
+
+
 class Context:
     """An open library context on one gfx950 device (dyninfer_mi355x_open/close)."""
 
@@ -398,6 +537,155 @@ class Context:
         _check(self._lib.packed_embedding(self._h, w.pack(), ids.data_ptr() if n else None, n,
                                          out.data_ptr() if n else None, self._stream(stream)))
         return out
+
+    # ---- around attention: rotary positions, the quantized cache, attention over it, verification
+    @staticmethod
+    def _new(shape, dtype, device, stream):
+        """A tensor that belongs to the stream the call's work runs on."""
+        import torch
+        if stream is None:
+            return torch.empty(shape, dtype=dtype, device=device)
+        st = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream), device=device)
+        with torch.cuda.stream(st):
+            return torch.empty(shape, dtype=dtype, device=device)
+
+    def _work(self, need: int, workspace, device, stream):
+        """(pointer, bytes, keep-alive) of a call's workspace: the caller's, or a new one."""
+        if not need:
+            return None, 0, None
+        if workspace is None:
+            import torch
+            workspace = self._new((need,), torch.uint8, device, stream)
+        return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+
+    def rope_table(self, positions: int, rot_dim: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                   original_length: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                   attn_factor: float = 0.0, low_turns: float = 1.0, high_turns: float = 4.0, out=None, stream=None):
+        """Cosines and sines [positions, rot_dim / 2, 2] in f32 (dyninfer_mi355x_rope_table);
+        ``scaling``: "none", "linear", "yarn" or "bands"."""
+        import torch
+        if scaling not in ROPE_SCALINGS:
+            _bad(f"rope scaling must be one of {sorted(ROPE_SCALINGS)}")
+        if out is None:
+            out = self._new((positions, rot_dim // 2, 2), torch.float32, torch.device("cuda", self.device), stream)
+        p = _pack_rope_params(rot_dim, ROPE_SCALINGS[scaling], theta, factor, original_length, beta_fast, beta_slow,
+                              attn_factor, low_turns, high_turns)
+        ptr = _table(out, "torch.float32", (positions, rot_dim // 2, 2), "out")
+        _check(self._lib.dyninfer_mi355x_rope_table(self._h, p, positions, ptr, self._stream(stream)))
+        return out
+
+    def rope(self, x, rope: Rope, out=None, stream=None):
+        """x [tokens, heads, head_dim] with its first rot_dim dims rotated (dyninfer_mi355x_rope);
+        ``out`` may be x."""
+        if out is None:
+            out = self._new(x.shape, x.dtype, x.device, stream)
+        n, _, dim = x.shape if x.dim() == 3 else (0, 0, 0)
+        _check(self._lib.dyninfer_mi355x_rope(self._h, _rows(x, n, dim, "x"), _rows(out, n, dim, "out"), n, dim,
+                                              rope.pack(n), self._stream(stream)))
+        return out
+
+    def kv_append(self, cache: KVCache, batch: KVBatch, k, v, rope: Optional[Rope] = None, q=None, q_out=None,
+                  stream=None):
+        """Quantizes the rows k, v [tokens, kv_heads, head_dim] into the cache, k rotated first if
+        ``rope`` is given; then q [tokens, heads, head_dim] is rotated by the same launch and
+        returned (dyninfer_mi355x_kv_append)."""
+        n, dim = batch.tokens, cache.head_dim
+        if q is not None and q_out is None:
+            q_out = self._new(q.shape, q.dtype, q.device, stream)
+        _check(self._lib.dyninfer_mi355x_kv_append(
+            self._h, cache.pack(), batch.pack(), _rows(k, n, dim, "k"), _rows(v, n, dim, "v"),
+            None if rope is None else rope.pack(n), None if q is None else _rows(q, n, dim, "q"),
+            None if q_out is None else _rows(q_out, n, dim, "q_out"), self._stream(stream)))
+        return q_out
+
+    def kv_read(self, cache: KVCache, batch: KVBatch, dtype=None, k_out=None, v_out=None, stream=None):
+        """The batch's rows of the cache, (k, v) [tokens, kv_heads, head_dim] in ``dtype`` (f32 unless
+        given) or into k_out / v_out (dyninfer_mi355x_kv_read)."""
+        import torch
+        n, dim = batch.tokens, cache.head_dim
+        if k_out is None and v_out is None:
+            k_out, v_out = (self._new((n, cache.kv_heads, dim), dtype or torch.float32, cache.k.device, stream)
+                            for _ in range(2))
+        _check(self._lib.dyninfer_mi355x_kv_read(
+            self._h, cache.pack(), batch.pack(), None if k_out is None else _rows(k_out, n, dim, "k_out"),
+            None if v_out is None else _rows(v_out, n, dim, "v_out"), self._stream(stream)))
+        return k_out, v_out
+
+    def kv_commit(self, cache: KVCache, batch: KVBatch, path, counts, stream=None) -> None:
+        """Moves the rows of an accepted path (int32 [sequences, width], ``counts`` [sequences], as
+        draft_verify returns them) to the front of each sequence's rows (dyninfer_mi355x_kv_commit)."""
+        packed = batch.pack()
+        n = batch.lengths.shape[0]
+        _check(self._lib.dyninfer_mi355x_kv_commit(
+            self._h, cache.pack(), packed, _table(path, "torch.int32", (n, None), "path"), path.shape[1],
+            _table(counts, "torch.int32", (n,), "counts"), self._stream(stream)))
+
+    def tree_attention(self, cache: KVCache, batch: KVBatch, q, mask=None, scale: Optional[float] = None, out=None,
+                       lse=None, stream=None, workspace=None):
+        """Attention of q [tokens, heads, head_dim] over the cache, the batch's own rows included
+        (dyninfer_mi355x_tree_attention).  ``mask``: int64 [tokens, words], bit j of a row set where it
+        sees its sequence's row j; None: a chain.  ``scale``: head_dim ** -0.5 unless given.  ``lse``:
+        f32 [tokens, heads] to write the log-sum-exp to."""
+        n, dim = batch.tokens, cache.head_dim
+        if out is None:
+            out = self._new(q.shape, q.dtype, q.device, stream)
+        qr, cb, bb = _rows(q, n, dim, "q"), cache.pack(), batch.pack()
+        mp = None if mask is None else _table(mask, "torch.int64", (n, None), "mask")
+        if mask is not None and 64 * mask.shape[1] < batch.max_new:
+            _bad("mask has fewer bits than max_new")
+        lp = None if lse is None else _table(lse, "torch.float32", (n, q.shape[1]), "lse")
+        need = ctypes.c_uint64(0)
+        if workspace is None:
+            _check(self._lib.dyninfer_mi355x_tree_attention_workspace_bytes(cb, bb, q.shape[1], _dtype_code(q),
+                                                                            ctypes.byref(need)))
+            wp, wn, _keep = self._work(need.value, None, q.device, stream)
+        else:
+            wp, wn = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        _check(self._lib.dyninfer_mi355x_tree_attention(
+            self._h, cb, bb, qr, mp, 0 if mask is None else mask.shape[1], dim ** -0.5 if scale is None else scale,
+            _rows(out, n, dim, "out"), lp, wp, wn, self._stream(stream)))
+        return out
+
+    def tree_attention_workspace_bytes(self, cache: KVCache, batch: KVBatch, q_heads: int, dtype: int = DTYPE_F32) -> int:
+        """Device workspace bytes of a tree_attention call (dyninfer_mi355x_tree_attention_workspace_bytes)."""
+        need = ctypes.c_uint64(0)
+        _check(self._lib.dyninfer_mi355x_tree_attention_workspace_bytes(cache.pack(), batch.pack(), q_heads, dtype,
+                                                                        ctypes.byref(need)))
+        return need.value
+
+    def draft_verify(self, logits, draft_tokens, parents, starts, max_new: int, *, uniform, noise, draft_probs=None,
+                     temperature=None, stream=None, workspace=None):
+        """Checks drafted trees against the target's logits [tokens, vocab]
+        (dyninfer_mi355x_draft_verify): (path int32 [sequences, max_new], counts int32 [sequences],
+        next_token int64 [sequences]).  ``parents`` int32 [tokens] or None for chains; ``uniform`` f32
+        [tokens], ``noise`` f32 [sequences, vocab] exponentially distributed, ``temperature`` f32
+        [sequences] (0: greedy), ``draft_probs`` [tokens, vocab] or None."""
+        import torch
+        if not logits.is_cuda or logits.dim() != 2 or logits.stride(1) != 1:
+            _bad("logits must be a device tensor [tokens, vocab] whose last axis is contiguous")
+        n, vocab = logits.shape
+        seqs = starts.shape[0] - 1 if starts.dim() == 1 else -1
+        if draft_probs is not None and (not draft_probs.is_cuda or draft_probs.shape != logits.shape or draft_probs.stride(1) != 1):
+            _bad("draft_probs must be a device tensor of the logits' shape whose last axis is contiguous")
+        if not noise.is_cuda or noise.dtype != torch.float32 or noise.shape != (seqs, vocab) or noise.stride(1) != 1:
+            _bad("noise must be a device tensor [sequences, vocab] of float32 whose last axis is contiguous")
+        sp = _table(starts, "torch.int32", (None,), "starts")
+        tp = None if temperature is None else _table(temperature, "torch.float32", (seqs,), "temperature")
+        pp = None if parents is None else _table(parents, "torch.int32", (n,), "parents")
+        path = self._new((seqs, max_new), torch.int32, logits.device, stream)
+        counts = self._new((seqs,), torch.int32, logits.device, stream)
+        token = self._new((seqs,), torch.int64, logits.device, stream)
+        need = ctypes.c_uint64(0)
+        _check(self._lib.dyninfer_mi355x_draft_verify_workspace_bytes(seqs, n, vocab, max_new, ctypes.byref(need)))
+        wp, wn, _keep = self._work(need.value, workspace, logits.device, stream)
+        args = _pack_verify(
+            logits.data_ptr(), 0 if draft_probs is None else draft_probs.data_ptr(), _dtype_code(logits),
+            0 if draft_probs is None else _dtype_code(draft_probs), logits.stride(0),
+            0 if draft_probs is None else draft_probs.stride(0), _table(draft_tokens, "torch.int64", (n,), "draft_tokens"),
+            pp or 0, sp, tp or 0, _table(uniform, "torch.float32", (n,), "uniform"), noise.data_ptr(), noise.stride(0),
+            vocab, seqs, n, max_new, path.data_ptr(), counts.data_ptr(), token.data_ptr())
+        _check(self._lib.dyninfer_mi355x_draft_verify(self._h, args, wp, wn, self._stream(stream)))
+        return path, counts, token
 
 
 def candidates() -> list:

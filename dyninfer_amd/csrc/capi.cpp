@@ -20,6 +20,7 @@
 #include <string>
 #include <vector>
 
+#include "capi_common.hpp"
 #include "gguf.hpp"
 #include "safetensors.hpp"
 #include "kernels.hpp"
@@ -32,43 +33,14 @@
 constexpr size_t kScratchBytes = DYNINFER_MI355X_NOALLOC_SCRATCH_BYTES;
 static __device__ __align__(256) uint8_t scratch[kScratchBytes];
 
-// A context: the device it was opened on and that device's copy of `scratch`.
-// Immutable after dyninfer_mi355x_open, so calls from any number of threads
-// share it without locks; each call's temporary lives in the caller's
-// workspace (or, for the no-allocation entry point, in `scratch`).
-struct dyninfer_mi355x_ctx {
-    int device;
-    uint8_t* scratch;
-};
+using dmx::aligned;
+using dmx::check_ctx;
+using dmx::DeviceGuard;
+using dmx::fail;
+using dmx::g_last_error;
+using dmx::hip_fail;
 
 namespace {
-
-thread_local std::string g_last_error;
-
-int fail(int code, const std::string& msg) {
-    g_last_error = msg;
-    return code;
-}
-
-int hip_fail(hipError_t e, const char* what) {
-    return fail(DYNINFER_MI355X_ERR_HIP, std::string(what) + ": " + hipGetErrorName(e) + ": " + hipGetErrorString(e));
-}
-
-bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
-
-// Makes ctx->device current for the duration of a call, restoring the caller's.
-struct DeviceGuard {
-    int prev = -1;
-    hipError_t err = hipSuccess;
-    explicit DeviceGuard(int dev) {
-        err = hipGetDevice(&prev);
-        if (err == hipSuccess && prev != dev) err = hipSetDevice(dev);
-    }
-    ~DeviceGuard() {
-        int cur = -1;
-        if (prev >= 0 && hipGetDevice(&cur) == hipSuccess && cur != prev) (void)hipSetDevice(prev);
-    }
-};
 
 uint32_t block_weights(uint32_t enc) {
     switch (enc) {
@@ -187,11 +159,6 @@ int check_io(uint32_t x_dtype, uint32_t y_dtype, uint32_t rows) {
         return fail(DYNINFER_MI355X_ERR_UNSUPPORTED, "activations must be f32 or bf16");
     if (y_dtype != DYNINFER_DTYPE_F32 && y_dtype != DYNINFER_DTYPE_BF16)
         return fail(DYNINFER_MI355X_ERR_UNSUPPORTED, "outputs must be f32 or bf16");
-    return 0;
-}
-
-int check_ctx(dyninfer_mi355x_ctx_t* ctx) {
-    if (!ctx) return fail(DYNINFER_MI355X_ERR_INVALID_ARGUMENT, "context is NULL");
     return 0;
 }
 

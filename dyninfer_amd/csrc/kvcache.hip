@@ -1,0 +1,541 @@
+// Rotary positions and the quantized paged cache: writing, reading back, and
+// keeping an accepted path.  All are bound by memory (large calls) or by the
+// latency of one launch (small ones); the arithmetic is small beside either.
+//
+// Rows: a lane holds 8 consecutive dims of one head (16 bytes of bf16), a head
+// takes D / 8 lanes of one wave (rounded up to a power of two), so a block of
+// 32 dims is 4 lanes and its extremes take two shuffles, and the dims of a
+// rotary pair are in the lane itself (interleaved) or one more load away.
+//
+// Results are bit-identical to the plain sequence of f32 operations: products,
+// sums and quotients are rounded one by one (no contraction), the division by
+// a scale is the correctly rounded one.
+#include "kvcache.hpp"
+
+#include <type_traits>
+
+#pragma clang fp contract(off)
+
+namespace dmx {
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Lanes that hold one head of D dims.
+template <int D>
+constexpr int kLanes = D <= 64 ? 8 : D <= 128 ? 16 : 32;
+
+__device__ __forceinline__ float load1(const KvRows& r, int64_t at) {
+    return r.bf16 ? bf16_bits_to_f32(gptr<uint16_t>(r.p)[at]) : gptr<float>(r.p)[at];
+}
+
+// Eight elements from element offset `at` (of a row of 16-byte boundaries if r.vec).
+__device__ __forceinline__ void load8(const KvRows& r, int64_t at, float (&x)[8]) {
+    if (r.vec && r.bf16) {
+        const u32x4 w = *gptr<u32x4>(static_cast<const uint16_t*>(r.p) + at);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[2 * i] = bf16_bits_to_f32(w[i] & 0xFFFFu);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    } else if (r.vec) {
+        const f32x4 a = *gptr<f32x4>(static_cast<const float*>(r.p) + at);
+        const f32x4 b = *gptr<f32x4>(static_cast<const float*>(r.p) + at + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = a[i], x[4 + i] = b[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = load1(r, at + i);
+    }
+}
+
+__device__ __forceinline__ void store8(const KvRows& r, int64_t at, const float (&x)[8]) {
+    if (r.bf16) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = f32x2_to_bf16x2_bits(x[2 * i], x[2 * i + 1]);
+        uint16_t* p = static_cast<uint16_t*>(r.p) + at;
+        if (r.vec) {
+            *gptr_mut<u32x4>(p) = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) gptr_mut<uint16_t>(p)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        }
+    } else {
+        float* p = static_cast<float*>(r.p) + at;
+        if (r.vec) {
+            *gptr_mut<f32x4>(p) = f32x4{x[0], x[1], x[2], x[3]};
+            *gptr_mut<f32x4>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) gptr_mut<float>(p)[i] = x[i];
+        }
+    }
+}
+
+// x: dims d0..d0+7 of the row at element offset `row`; rotated in place.  The
+// wide forms need the pairs of the eight dims to be eight dims or eight pairs
+// of floats in a row: rot / 2 (half) a multiple of 8, rot (interleaved) too.
+__device__ __forceinline__ void rotate8(const KvRows& r, int64_t row, uint32_t token, uint32_t d0, const RopeView& rp,
+                                        float (&x)[8]) {
+    if (d0 >= rp.rot) return;
+    const uint32_t h = rp.rot / 2;
+    const int32_t pos = gptr<int32_t>(rp.positions)[token];
+    if (pos < 0 || (uint32_t)pos >= rp.table_positions) {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (d0 + i < rp.rot) x[i] = __builtin_nanf("");
+        return;
+    }
+    const float* t = rp.table + (size_t)pos * rp.rot;
+    if (rp.half && h % 8 == 0) {
+        const bool first = d0 < h;
+        float y[8];
+        load8(r, row + (first ? d0 + h : d0 - h), y);
+        const f32x4* cs = reinterpret_cast<const f32x4*>(t + 2 * (first ? d0 : d0 - h));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const f32x4 w = *gptr<f32x4>(cs + i);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int e = 2 * i + j;
+                const float c = w[2 * j], s = w[2 * j + 1];
+                // first half: a c - b s with b the partner; second: a s + b c with a the partner
+                x[e] = first ? x[e] * c - y[e] * s : y[e] * s + x[e] * c;
+            }
+        }
+    } else if (!rp.half && rp.rot % 8 == 0) {
+        const f32x4* cs = reinterpret_cast<const f32x4*>(t + d0);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const f32x4 w = *gptr<f32x4>(cs + i);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int e = 4 * i + 2 * j;
+                const float a = x[e], b = x[e + 1], c = w[2 * j], s = w[2 * j + 1];
+                x[e] = a * c - b * s;
+                x[e + 1] = a * s + b * c;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t d = d0 + i;
+            if (d >= rp.rot) continue;
+            const uint32_t f = rp.half ? (d < h ? d : d - h) : d / 2;
+            const bool first = rp.half ? d < h : d % 2 == 0;
+            const float y = load1(r, row + (rp.half ? (first ? d + h : d - h) : (d ^ 1u)));
+            const float c = gptr<float>(t)[2 * f], s = gptr<float>(t)[2 * f + 1], a = load1(r, row + d);
+            x[i] = first ? a * c - y * s : y * s + a * c;
+        }
+    }
+}
+
+// One head of one token: loads, rotates, stores.  In place is safe: a head's
+// lanes are one wave's, which has loaded all of it before its first store.
+template <int D>
+__device__ __forceinline__ void rope_row(const KvRows& x, const KvRows& y, uint32_t token, uint32_t head, uint32_t lane,
+                                         const RopeView& rp) {
+    const uint32_t d0 = 8 * lane;
+    const int64_t row = (int64_t)token * x.ts + (int64_t)head * x.hs;
+    float v[8];
+    if (d0 < D) {
+        load8(x, row + d0, v);
+        rotate8(x, row, token, d0, rp, v);
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (d0 < D) store8(y, (int64_t)token * y.ts + (int64_t)head * y.hs + d0, v);
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void rope_kernel(KvRows x, KvRows y, uint32_t tokens, uint32_t heads, RopeView rp) {
+    constexpr uint32_t L = kLanes<D>;
+    const uint64_t i = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (i >= (uint64_t)tokens * heads) return;
+    rope_row<D>(x, y, (uint32_t)(i / heads), (uint32_t)(i % heads), threadIdx.x % L, rp);
+}
+
+// Largest value of the N lanes around this one (N a power of two, aligned).
+template <int N>
+__device__ __forceinline__ float lanes_max(float x) {
+#pragma unroll
+    for (int m = 1; m < N; m *= 2) x = fmaxf(x, __shfl_xor(x, m));
+    return x;
+}
+
+// A block's scale and this lane's eight codes of it.  N lanes hold the block;
+// a lane without dims passes zeros.
+template <int BITS, int N>
+__device__ __forceinline__ uint16_t quantize(const float (&x)[8], int32_t (&c)[8]) {
+    float top = 0.0f, low = 0.0f;
+    uint32_t big = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        top = fmaxf(top, x[i]);
+        low = fmaxf(low, -x[i]);
+        big = max(big, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    }
+    top = lanes_max<N>(top);
+    low = lanes_max<N>(low);
+#pragma unroll
+    for (int m = 1; m < N; m *= 2) big = max(big, (uint32_t)__shfl_xor((int)big, m));
+    if (big >= 0x7F800000u) {  // an infinity or a NaN: the block reads back as NaN
+#pragma unroll
+        for (int i = 0; i < 8; i++) c[i] = 0;
+        return 0x7FC0u;
+    }
+    const float d = BITS == 8 ? fmaxf(top, low) / 127.0f : (top > low ? top : -low) / -8.0f;
+    const uint16_t bits = f32_to_bf16_bits(d);
+    const float s = bf16_bits_to_f32(bits);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        // the rounded scale may be a little small: the largest code is clamped
+        const float q = s == 0.0f ? 0.0f : rintf(x[i] / s);
+        c[i] = (int32_t)fminf(fmaxf(q, BITS == 8 ? -127.0f : -8.0f), BITS == 8 ? 127.0f : 7.0f);
+    }
+    return bits;
+}
+
+// Place of block b, part t of a K row, in codes.
+template <int D>
+__device__ __forceinline__ uint32_t k_place(uint32_t b, uint32_t t) {
+    return (b / 2) * 64 + ((b | 1u) * 32 < D ? t * 16 + (b & 1) * 8 : t * 8);
+}
+
+// Grid: `kv_blocks` workgroups for the keys, one per (sequence, chunk of 16
+// positions, head), as many for the values, then the queries' rows.  A chunk is
+// one workgroup's alone, so values of 4 bits, two tokens to a byte, are merged
+// without atomics.
+template <int D, int KB, int VB>
+__global__ __launch_bounds__(256) void append_kernel(KvView kv, KvBatch b, KvRows k, KvRows v, RopeView rp, KvRows q,
+                                                     KvRows q_out, uint32_t q_heads, uint32_t chunks,
+                                                     uint32_t kv_blocks) {
+    constexpr uint32_t L = kLanes<D>, ROWS = 256 / L;
+    const uint32_t lane = threadIdx.x % L, slot = threadIdx.x / L;
+    uint32_t blk = blockIdx.x;
+    if (blk >= 2 * kv_blocks) {
+        const uint64_t i = (uint64_t)(blk - 2 * kv_blocks) * ROWS + slot;
+        if (i < (uint64_t)b.tokens * q_heads)
+            rope_row<D>(q, q_out, (uint32_t)(i / q_heads), (uint32_t)(i % q_heads), lane, rp);
+        return;
+    }
+    const bool keys = blk < kv_blocks;
+    if (!keys) blk -= kv_blocks;
+    const uint32_t head = blk % kv.heads, rest = blk / kv.heads;
+    const uint32_t seq = rest / chunks;
+    const SeqRange r = seq_range(b, seq);
+    const uint32_t c = r.len / 16 + rest % chunks;
+    const uint64_t pos0 = 16ull * c;
+    if (r.n == 0 || pos0 >= (uint64_t)r.len + r.n) return;
+    const int64_t page = chunk_page(kv, b, seq, c);
+    if (page < 0) return;
+    const uint64_t s0 = chunk_slot(kv, page, head, c);
+    // the chunk's tokens lo..hi-1 are new; token t is row row0 + (pos0 + t - len)
+    const uint32_t lo = r.len > pos0 ? (uint32_t)(r.len - pos0) : 0u;
+    const uint32_t hi = (uint32_t)min((uint64_t)16, (uint64_t)r.len + r.n - pos0);
+    const uint32_t d0 = 8 * lane;
+    if (keys) {
+        for (uint32_t t = slot; t < 16; t += ROWS) {
+            if (t < lo || t >= hi) continue;  // whole rows leave together: the shuffles stay within a row
+            const uint32_t token = r.row0 + (uint32_t)(pos0 + t - r.len);
+            const int64_t row = (int64_t)token * k.ts + (int64_t)head * k.hs;
+            float x[8] = {};
+            if (d0 < D) {
+                load8(k, row + d0, x);
+                if (rp.table) rotate8(k, row, token, d0, rp, x);
+            }
+            int32_t code[8];
+            const uint16_t sc = quantize<KB, 4>(x, code);
+            if (d0 >= D) continue;
+            const uint32_t blk32 = lane / 4, part = lane % 4, at = k_place<D>(blk32, part);
+            if constexpr (KB == 8) {
+                u32x2 w = {0, 0};
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[i / 4] |= (uint32_t)(code[i] + 128) << (8 * (i % 4));
+                *gptr_mut<u32x2>(kv.k + (s0 + t) * D + at) = w;
+            } else {
+                uint32_t w = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) w |= (uint32_t)(code[i] + 8) << (8 * (i % 4) + 4 * (i / 4));
+                *gptr_mut<uint32_t>(kv.k + (s0 + t) * (D / 2) + at / 2) = w;
+            }
+            if (part == 0) gptr_mut<uint16_t>(kv.k + kv.k_scales)[(s0 + t) * (D / 32) + blk32] = sc;
+        }
+        return;
+    }
+    __shared__ uint8_t sm[D * 16];  // [dim][token]
+    for (uint32_t t = slot; t < 16; t += ROWS) {
+        if (t < lo || t >= hi) continue;
+        const uint32_t token = r.row0 + (uint32_t)(pos0 + t - r.len);
+        float x[8] = {};
+        if (d0 < D) load8(v, (int64_t)token * v.ts + (int64_t)head * v.hs + d0, x);
+        int32_t code[8];
+        const uint16_t sc = quantize<VB, (int)L>(x, code);
+        if (d0 < D) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) sm[(d0 + i) * 16 + t] = (uint8_t)code[i];
+        }
+        if (lane == 0) gptr_mut<uint16_t>(kv.v + kv.v_scales)[s0 + t] = sc;
+    }
+    __syncthreads();
+    const uint32_t dim = threadIdx.x;
+    if (dim >= D) return;
+    const u32x4 w = *reinterpret_cast<const u32x4*>(sm + dim * 16);
+    if constexpr (VB == 8) {
+        uint8_t* dst = kv.v + s0 * D + dim * 16;
+        if (lo == 0 && hi == 16) {
+            *gptr_mut<u32x4>(dst) = w;
+        } else {
+#pragma unroll
+            for (uint32_t t = 0; t < 16; t++)
+                if (t >= lo && t < hi) gptr_mut<uint8_t>(dst)[t] = (uint8_t)(w[t / 4] >> (8 * (t % 4)));
+        }
+    } else {
+        // dword j: tokens 8j..8j+3 in the low nibbles, 8j+4..8j+7 in the high ones
+        u32x2 x;
+#pragma unroll
+        for (int j = 0; j < 2; j++) x[j] = (w[2 * j] & 0x0F0F0F0Fu) | ((w[2 * j + 1] & 0x0F0F0F0Fu) << 4);
+        uint8_t* dst = kv.v + s0 * (D / 2) + dim * 8;
+        if (lo != 0 || hi != 16) {
+            const u32x2 old = *gptr<u32x2>(dst);
+            u32x2 m = {0, 0};
+#pragma unroll
+            for (uint32_t t = 0; t < 16; t++)
+                if (t >= lo && t < hi) m[t / 8] |= 15u << (8 * (t % 4) + 4 * (t % 8 / 4));
+            x = (x & m) | (old & ~m);
+        }
+        *gptr_mut<u32x2>(dst) = x;
+    }
+}
+
+// One workgroup per (sequence, chunk of 16 positions, head), keys then values.
+template <int D, int KB, int VB>
+__global__ __launch_bounds__(256) void read_kernel(KvView kv, KvBatch b, KvRows k, KvRows v, uint32_t chunks,
+                                                   uint32_t kv_blocks) {
+    constexpr uint32_t L = kLanes<D>, ROWS = 256 / L;
+    const uint32_t lane = threadIdx.x % L, slot = threadIdx.x / L;
+    uint32_t blk = blockIdx.x;
+    const bool keys = k.p != nullptr && blk < kv_blocks;
+    if (k.p != nullptr && !keys) blk -= kv_blocks;
+    const uint32_t head = blk % kv.heads, rest = blk / kv.heads;
+    const uint32_t seq = rest / chunks;
+    const SeqRange r = seq_range(b, seq);
+    const uint32_t c = r.len / 16 + rest % chunks;
+    const uint64_t pos0 = 16ull * c;
+    if (r.n == 0 || pos0 >= (uint64_t)r.len + r.n) return;
+    const int64_t page = chunk_page(kv, b, seq, c);
+    const uint64_t s0 = page < 0 ? 0 : chunk_slot(kv, page, head, c);
+    const uint32_t lo = r.len > pos0 ? (uint32_t)(r.len - pos0) : 0u;
+    const uint32_t hi = (uint32_t)min((uint64_t)16, (uint64_t)r.len + r.n - pos0);
+    const uint32_t d0 = 8 * lane;
+    __shared__ uint8_t sm[D * 16];  // [dim][token]
+    if (!keys && page >= 0) {
+        const uint32_t dim = threadIdx.x;
+        if (dim < D) {
+            u32x4 w;
+            if constexpr (VB == 8) {
+                w = *gptr<u32x4>(kv.v + s0 * D + dim * 16);
+            } else {
+                const u32x2 x = *gptr<u32x2>(kv.v + s0 * (D / 2) + dim * 8);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {  // nibble n (signed) as a byte: (n ^ 8) - 8, bytewise
+                    const uint32_t a = x[j] & 0x0F0F0F0Fu, h = (x[j] >> 4) & 0x0F0F0F0Fu;
+                    w[2 * j] = a | ((a & 0x08080808u) * 30u);  // bit 3 set: bits 4..7 too
+                    w[2 * j + 1] = h | ((h & 0x08080808u) * 30u);
+                }
+            }
+            *reinterpret_cast<u32x4*>(sm + dim * 16) = w;
+        }
+        __syncthreads();
+    }
+    for (uint32_t t = slot; t < 16; t += ROWS) {
+        if (t < lo || t >= hi || d0 >= D) continue;
+        const uint32_t token = r.row0 + (uint32_t)(pos0 + t - r.len);
+        float x[8], s = __builtin_nanf("");
+        int32_t code[8] = {};
+        if (page >= 0 && keys) {
+            const uint32_t at = k_place<D>(lane / 4, lane % 4);
+            s = bf16_bits_to_f32(gptr<uint16_t>(kv.k + kv.k_scales)[(s0 + t) * (D / 32) + lane / 4]);
+            if constexpr (KB == 8) {
+                const u32x2 w = *gptr<u32x2>(kv.k + (s0 + t) * D + at);
+#pragma unroll
+                for (int i = 0; i < 8; i++) code[i] = (int32_t)((w[i / 4] >> (8 * (i % 4))) & 255u) - 128;
+            } else {
+                const uint32_t w = *gptr<uint32_t>(kv.k + (s0 + t) * (D / 2) + at / 2);
+#pragma unroll
+                for (int i = 0; i < 8; i++) code[i] = (int32_t)((w >> (8 * (i % 4) + 4 * (i / 4))) & 15u) - 8;
+            }
+        } else if (page >= 0) {
+            s = bf16_bits_to_f32(gptr<uint16_t>(kv.v + kv.v_scales)[s0 + t]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) code[i] = (int8_t)sm[(d0 + i) * 16 + t];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (float)code[i] * s;
+        const KvRows& o = keys ? k : v;
+        store8(o, (int64_t)token * o.ts + (int64_t)head * o.hs + d0, x);
+    }
+}
+
+// One workgroup per (sequence, head, keys or values).  A thread owns the same
+// bytes of every row (a dword of a key, a dim of a value), so its moves are in
+// order by themselves: a row's source lies at or after every row written so far.
+template <int D, int KB, int VB>
+__global__ __launch_bounds__(256) void commit_kernel(KvView kv, KvBatch b, const int32_t* path, uint32_t path_stride,
+                                                     const int32_t* counts) {
+    const uint32_t head = blockIdx.x % kv.heads, seq = blockIdx.x / kv.heads % b.seqs;
+    const bool keys = blockIdx.x < kv.heads * b.seqs;
+    const SeqRange r = seq_range(b, seq);
+    const int32_t cn = counts[seq];
+    const uint32_t n = cn < 0 ? 0u : min((uint32_t)cn, min(r.n, path_stride));
+    const uint32_t i = threadIdx.x;
+    for (uint32_t j = 0; j < n; j++) {
+        const int32_t from = path[(size_t)seq * path_stride + j];
+        if (from <= (int32_t)j || (uint32_t)from >= r.n) continue;
+        const uint64_t ps = (uint64_t)r.len + (uint32_t)from, pd = (uint64_t)r.len + j;
+        const uint32_t cs = (uint32_t)(ps / 16), cd = (uint32_t)(pd / 16);
+        const int64_t gs = chunk_page(kv, b, seq, cs), gd = chunk_page(kv, b, seq, cd);
+        if (gs < 0 || gd < 0) continue;
+        const uint64_t ss = chunk_slot(kv, gs, head, cs), sd = chunk_slot(kv, gd, head, cd);
+        const uint32_t ts = ps % 16, td = pd % 16;
+        if (keys) {
+            constexpr uint32_t RB = D * KB / 8, NS = D / 32;
+            if (i < RB / 4)
+                *gptr_mut<uint32_t>(kv.k + (sd + td) * RB + 4 * i) = *gptr<uint32_t>(kv.k + (ss + ts) * RB + 4 * i);
+            else if (i >= 128 && i < 128 + NS) {
+                uint16_t* sc = reinterpret_cast<uint16_t*>(kv.k + kv.k_scales);
+                gptr_mut<uint16_t>(sc)[(sd + td) * NS + i - 128] = gptr<uint16_t>(sc)[(ss + ts) * NS + i - 128];
+            }
+        } else {
+            if (i < D) {
+                if constexpr (VB == 8) {
+                    gptr_mut<uint8_t>(kv.v)[sd * D + i * 16 + td] = gptr<uint8_t>(kv.v)[ss * D + i * 16 + ts];
+                } else {
+                    const uint32_t from_b = gptr<uint8_t>(kv.v)[ss * (D / 2) + i * 8 + ts / 8 * 4 + ts % 4];
+                    const uint64_t at = sd * (D / 2) + i * 8 + td / 8 * 4 + td % 4;
+                    const uint32_t sh = td % 8 / 4 * 4, nib = (from_b >> (ts % 8 / 4 * 4)) & 15u;
+                    const uint32_t old = gptr<uint8_t>(kv.v)[at];
+                    gptr_mut<uint8_t>(kv.v)[at] = (uint8_t)((old & ~(15u << sh)) | (nib << sh));
+                }
+            }
+            if (i == 0) {
+                uint16_t* sc = reinterpret_cast<uint16_t*>(kv.v + kv.v_scales);
+                gptr_mut<uint16_t>(sc)[sd + td] = gptr<uint16_t>(sc)[ss + ts];
+            }
+        }
+    }
+}
+
+// Angles in 64 bits: the frequency of a pair, times the position, and one
+// rounding of the cosine and sine.
+__global__ __launch_bounds__(256) void rope_table_kernel(uint32_t rot, uint32_t scaling, double theta, double factor,
+                                                         double original, double lo, double hi, double attn,
+                                                         uint32_t positions, float* out) {
+    const uint32_t h = rot / 2;
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (uint64_t)positions * h) return;
+    const uint32_t f = (uint32_t)(i % h);
+    double w = pow(theta, -2.0 * f / rot);
+    if (scaling == 1) {
+        w /= factor;
+    } else if (scaling == 2) {  // lo, hi: the pairs between which the scaling sets in
+        const double ramp = fmin(fmax((f - lo) / fmax(hi - lo, 0.001), 0.0), 1.0);
+        w = w / factor * ramp + w * (1.0 - ramp);
+    } else if (scaling == 3) {  // lo, hi: turns over the original length
+        const double turns = original * w / 6.283185307179586476925;
+        const double s = fmin(fmax((turns - lo) / (hi - lo), 0.0), 1.0);
+        w = (1.0 - s) * w / factor + s * w;
+    }
+    const double a = w * (double)(i / h);
+    out[2 * i] = (float)(cos(a) * attn);
+    out[2 * i + 1] = (float)(sin(a) * attn);
+}
+
+uint32_t chunk_bound(uint32_t max_new) { return max_new ? (max_new + 14u) / 16u + 1u : 0u; }
+
+template <class F>
+hipError_t by_dim(uint32_t dim, F f) {
+    switch (dim) {
+    case 64: return f(std::integral_constant<int, 64>());
+    case 96: return f(std::integral_constant<int, 96>());
+    case 128: return f(std::integral_constant<int, 128>());
+    case 256: return f(std::integral_constant<int, 256>());
+    }
+    return hipErrorInvalidValue;
+}
+
+template <class F>
+hipError_t by_cache(const KvView& kv, F f) {
+    return by_dim(kv.dim, [&](auto d) {
+        using A = std::integral_constant<int, 8>;
+        using B = std::integral_constant<int, 4>;
+        if (kv.k_bits == 8) return kv.v_bits == 8 ? f(d, A(), A()) : f(d, A(), B());
+        return kv.v_bits == 8 ? f(d, B(), A()) : f(d, B(), B());
+    });
+}
+
+}  // namespace
+
+hipError_t rope_table_launch(uint32_t rot, uint32_t scaling, double theta, double factor, double original, double lo,
+                             double hi, double attn, uint32_t positions, float* out, hipStream_t st) {
+    const uint64_t n = (uint64_t)positions * (rot / 2);
+    if (n == 0) return hipSuccess;
+    rope_table_kernel<<<(uint32_t)((n + 255) / 256), 256, 0, st>>>(rot, scaling, theta, factor, original, lo, hi, attn,
+                                                                   positions, out);
+    return hipGetLastError();
+}
+
+hipError_t rope_launch(const KvRows& x, const KvRows& y, uint32_t tokens, uint32_t heads, uint32_t dim,
+                       const RopeView& rope, hipStream_t st) {
+    if (tokens == 0) return hipSuccess;
+    return by_dim(dim, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        constexpr uint64_t rows = 256 / kLanes<D>;
+        rope_kernel<D><<<(uint32_t)(((uint64_t)tokens * heads + rows - 1) / rows), 256, 0, st>>>(x, y, tokens, heads, rope);
+        return hipGetLastError();
+    });
+}
+
+hipError_t kv_append_launch(const KvView& kv, const KvBatch& b, const KvRows& k, const KvRows& v, const RopeView& rope,
+                            const KvRows& q, const KvRows& q_out, uint32_t q_heads, hipStream_t st) {
+    return by_cache(kv, [&](auto d, auto kb, auto vb) {
+        constexpr int D = decltype(d)::value;
+        constexpr uint64_t rows = 256 / kLanes<D>;
+        const uint32_t chunks = chunk_bound(b.max_new);
+        const uint32_t kv_blocks = b.seqs * chunks * kv.heads;
+        const uint64_t grid = 2ull * kv_blocks + ((uint64_t)b.tokens * q_heads + rows - 1) / rows;
+        if (grid == 0) return hipSuccess;
+        append_kernel<D, decltype(kb)::value, decltype(vb)::value>
+            <<<(uint32_t)grid, 256, 0, st>>>(kv, b, k, v, rope, q, q_out, q_heads, chunks, kv_blocks);
+        return hipGetLastError();
+    });
+}
+
+hipError_t kv_read_launch(const KvView& kv, const KvBatch& b, const KvRows& k, const KvRows& v, hipStream_t st) {
+    return by_cache(kv, [&](auto d, auto kb, auto vb) {
+        constexpr int D = decltype(d)::value;
+        const uint32_t chunks = chunk_bound(b.max_new);
+        const uint32_t kv_blocks = b.seqs * chunks * kv.heads;
+        const uint32_t grid = kv_blocks * ((k.p != nullptr) + (v.p != nullptr));
+        if (grid == 0) return hipSuccess;
+        read_kernel<D, decltype(kb)::value, decltype(vb)::value><<<grid, 256, 0, st>>>(kv, b, k, v, chunks, kv_blocks);
+        return hipGetLastError();
+    });
+}
+
+hipError_t kv_commit_launch(const KvView& kv, const KvBatch& b, const int32_t* path, uint32_t path_stride,
+                            const int32_t* counts, hipStream_t st) {
+    return by_cache(kv, [&](auto d, auto kb, auto vb) {
+        constexpr int D = decltype(d)::value;
+        const uint32_t grid = 2 * b.seqs * kv.heads;
+        if (grid == 0) return hipSuccess;
+        commit_kernel<D, decltype(kb)::value, decltype(vb)::value>
+            <<<grid, 256, 0, st>>>(kv, b, path, path_stride, counts);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace dmx

@@ -252,6 +252,223 @@ int dyninfer_mi355x_embedding(dyninfer_mi355x_ctx_t* ctx, const dyninfer_qweight
                               const int64_t* ids, uint32_t n_ids, float* out, void* stream);
 
 /*
+ * ---- Speculative decoding on a quantized cache ----
+ *
+ * The calls between a step's qkv projection and its output projection, and after its
+ * lm_head, when drafted tokens are checked several at a time: rotary positions, a paged
+ * key/value cache quantized as it is written, attention of the drafted tokens over it,
+ * verification of the drafts, and removal of the rejected rows.  No counterpart in the
+ * reference.  A prompt is the same with one long chain of tokens, plain decoding with one
+ * token a sequence.
+ *
+ * Common rules: activations are f32 or bf16; sums, statistics and products are f32; all
+ * device tables (page tables, lengths, starts, positions, paths) are read on the device by
+ * kernels that check them: an entry out of its range never makes a kernel read or write
+ * outside the buffers described (what it does instead is said at each call).
+ */
+
+/* Codes of a cache's keys or values. */
+enum {
+    DYNINFER_KV_Q8 = 1, /* 8-bit codes -127..127, scale bf16(max|x| / 127) */
+    DYNINFER_KV_Q4 = 2  /* 4-bit codes -8..7, scale bf16(e / -8), e the value of largest magnitude
+                           (the negative one of two equal magnitudes) */
+};
+
+/*
+ * A paged key/value cache.  Pages hold page_size tokens (a power of two, 16..4096) of all
+ * kv_heads heads of head_dim (64, 96, 128 or 256) values.  A key has a scale for each block
+ * of 32 dims (rotated keys have a few strong channels, which then cost only their own block
+ * resolution); a value has one scale for the token's whole head.
+ * A code is rint(x / scale) clamped to its range, and stands for code * scale; scale 0 gives
+ * codes 0.  A block that holds an infinity or a NaN gets scale NaN and codes 0 (it reads back
+ * as NaN whole).
+ * k buffer: codes [pages][kv_heads][page_size][head_dim], then bf16 scales
+ *   [pages][kv_heads][page_size][head_dim / 32].  Within a row the blocks lie in pairs
+ *   (2p, 2p+1), a pair as [4 parts][block of the pair][8 dims], a last odd block as
+ *   [4 parts][8 dims]; part t of a block holds its dims 8t..8t+7.  Q8: byte = code + 128.
+ *   Q4: eight consecutive codes of this order in four bytes, byte t = (code t + 8) |
+ *   (code t+4 + 8) << 4.
+ * v buffer: codes [pages][kv_heads][page_size / 16][head_dim][16 tokens], then bf16 scales
+ *   [pages][kv_heads][page_size].  Q8: signed bytes.  Q4: eight tokens in four bytes, byte t =
+ *   (code t & 15) | (code t+4 & 15) << 4.
+ * Both orders are those in which the attention's matrix instructions take their operands, so
+ * that a lane's codes are one wide load and no value crosses lanes.  Buffers are 256-byte
+ * aligned; k_bytes and v_bytes must equal dyninfer_mi355x_kv_cache_bytes.  They need no
+ * initial contents.
+ */
+typedef struct dyninfer_kvcache {
+    uint32_t k_encoding, v_encoding;
+    uint32_t kv_heads, head_dim;
+    uint32_t page_size, reserved;
+    uint64_t pages;
+    void* k;
+    void* v;
+    uint64_t k_bytes, v_bytes;
+} dyninfer_kvcache_t;
+
+/*
+ * The sequences of a call.  Rows of the call's tensors are tokens packed sequence after
+ * sequence: row starts[b] + i is the token at position lengths[b] + i of sequence b, for
+ * i < starts[b+1] - starts[b].  Position p of sequence b lies in page
+ * page_table[b * table_pages + p / page_size].  All three are device int32, 4-byte aligned.
+ * max_new: the most rows of any sequence (rows past it are left out); max_length: the largest
+ * lengths[b] + rows of it, which only shapes the launches (any length is handled).
+ * A position beyond the page table, or on a page id outside [0, pages), is absent: writes to it
+ * are dropped, reads give NaN, attention does not see it.  A negative length counts as 0.
+ */
+typedef struct dyninfer_kvbatch {
+    const int32_t* page_table; /* [sequences, table_pages] */
+    const int32_t* lengths;    /* [sequences] */
+    const int32_t* starts;     /* [sequences + 1] */
+    uint32_t sequences, table_pages;
+    uint32_t tokens; /* rows of the call's tensors */
+    uint32_t max_new;
+    uint64_t max_length;
+} dyninfer_kvbatch_t;
+
+/* A tensor [tokens, heads, head_dim] whose last axis is contiguous; strides in elements. */
+typedef struct dyninfer_rows {
+    void* data;
+    uint32_t dtype, heads;
+    int64_t token_stride, head_stride;
+} dyninfer_rows_t;
+
+/* How the frequencies theta^(-2i / rot_dim) are scaled for contexts beyond the trained length. */
+enum {
+    DYNINFER_ROPE_PLAIN = 0,
+    DYNINFER_ROPE_LINEAR = 1, /* all divided by factor */
+    DYNINFER_ROPE_YARN = 2,   /* divided by factor below beta_slow turns over original_length, kept above beta_fast,
+                                 blended linearly between; cosine and sine times attn_factor
+                                 (0: 0.1 ln(factor) + 1) */
+    DYNINFER_ROPE_BANDS = 3   /* divided by factor below low_turns turns over original_length, kept above high_turns,
+                                 blended in the number of turns between */
+};
+typedef struct dyninfer_rope_params {
+    uint32_t rot_dim, scaling;
+    double theta, factor, original_length;
+    double beta_fast, beta_slow, attn_factor; /* YARN */
+    double low_turns, high_turns;             /* BANDS */
+} dyninfer_rope_params_t;
+
+/* Writes the table [positions, rot_dim / 2, 2] of cosines and sines (f32, rounded once from
+ * 64 bits; device, 16-byte aligned): at a million positions an angle computed in f32 would be
+ * off by several hundredths.  A program writes it once and keeps it. */
+int dyninfer_mi355x_rope_table(dyninfer_mi355x_ctx_t* ctx, const dyninfer_rope_params_t* params, uint32_t positions,
+                               float* table, void* stream);
+
+/* Pairs of the rotated dims: (2i, 2i+1), or (i, i + rot_dim / 2). */
+enum { DYNINFER_ROPE_INTERLEAVED = 0, DYNINFER_ROPE_HALF = 1 };
+typedef struct dyninfer_rope {
+    const float* table;       /* [table_positions, rot_dim / 2, 2], 16-byte aligned */
+    const int32_t* positions; /* [tokens], device: a drafted tree's siblings share one */
+    uint32_t table_positions;
+    uint32_t rot_dim; /* even, 2..head_dim: the dims from it on are left as they are */
+    uint32_t layout, reserved;
+} dyninfer_rope_t;
+
+/*
+ * y = x with its first rot_dim dims rotated: (a, b) -> (a c - b s, a s + b c), products and sums
+ * rounded to f32 one by one, y rounded once to its type (that of x).  y may be x itself (same
+ * pointer and strides) but must not overlap it otherwise.  A position outside the table gives
+ * NaN in the rotated dims.  head_dim 64, 96, 128 or 256.
+ */
+int dyninfer_mi355x_rope(dyninfer_mi355x_ctx_t* ctx, const dyninfer_rows_t* x, const dyninfer_rows_t* y,
+                         uint32_t tokens, uint32_t head_dim, const dyninfer_rope_t* rope, void* stream);
+
+/* Bytes of a cache's k and v buffers (from its encodings, heads, head_dim, page_size and pages). */
+int dyninfer_mi355x_kv_cache_bytes(const dyninfer_kvcache_t* cache, uint64_t* k_bytes, uint64_t* v_bytes);
+
+/*
+ * Quantizes the rows of k and v [tokens, kv_heads, head_dim] into the cache, one launch.  With
+ * rope given, keys are rotated first (in f32, quantized from there), and q, if given too, is
+ * rotated into q_out as dyninfer_mi355x_rope does; q without rope is refused.  k and v share a
+ * dtype.  Two calls that run at the same time must not write tokens of the same 16 (positions
+ * 16n..16n+15) of a sequence.
+ */
+int dyninfer_mi355x_kv_append(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache_t* cache,
+                              const dyninfer_kvbatch_t* batch, const dyninfer_rows_t* k, const dyninfer_rows_t* v,
+                              const dyninfer_rope_t* rope, const dyninfer_rows_t* q, const dyninfer_rows_t* q_out,
+                              void* stream);
+
+/* Reads the batch's rows back: k and v [tokens, kv_heads, head_dim], f32 (code * scale, exact) or
+ * bf16 (rounded once).  Either may be NULL. */
+int dyninfer_mi355x_kv_read(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache_t* cache,
+                            const dyninfer_kvbatch_t* batch, const dyninfer_rows_t* k, const dyninfer_rows_t* v,
+                            void* stream);
+
+/*
+ * Keeps an accepted path of each sequence's rows: for j < counts[b], the codes and scales at
+ * position lengths[b] + path[b * path_stride + j] move to lengths[b] + j, unchanged.  A path
+ * ascends (path[j] >= j); an entry that does not (or lies outside the sequence's rows) is left
+ * out.  path and counts as dyninfer_mi355x_draft_verify writes them (device int32).
+ */
+int dyninfer_mi355x_kv_commit(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache_t* cache,
+                              const dyninfer_kvbatch_t* batch, const int32_t* path, uint32_t path_stride,
+                              const int32_t* counts, void* stream);
+
+/*
+ * out[r, h] = sum_p softmax_p(scale * q[r, h] . k[p, h / group]) v[p, h / group] over the positions
+ * p of row r's sequence that it sees: every committed one (p < lengths[b]), and of the batch's own
+ * rows (already in the cache: dyninfer_mi355x_kv_append) row j iff bit j % 64 of word
+ * mask[r * mask_words + j / 64] is set.  mask NULL: row i sees rows j <= i (a chain: plain
+ * decoding, or a prompt).  mask_words >= ceil(max_new / 64).  A row that sees nothing gives 0 and
+ * lse -inf.  q and out share a dtype (f32 or bf16); group = heads / kv_heads, any whole number.
+ * lse: f32 [tokens, heads], the natural logarithm of the sum of exponentials, or NULL.
+ * What is masked has no influence, whatever it holds (NaN scales included).
+ * Rounding: scores as from exact products with f32 sums (f32 queries: to 22 bits of a row's
+ * largest); a probability times its value's scale is rounded to 16 bits of mantissa (f32: 24).
+ * workspace: device memory of dyninfer_mi355x_tree_attention_workspace_bytes, 256-byte aligned
+ * (NULL when that is 0), under the rules of dyninfer_mi355x_qlinear's.
+ */
+int dyninfer_mi355x_tree_attention(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache_t* cache,
+                                   const dyninfer_kvbatch_t* batch, const dyninfer_rows_t* q, const int64_t* mask,
+                                   uint32_t mask_words, float scale, const dyninfer_rows_t* out, float* lse,
+                                   void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Host-only; reads the cache's shape and the batch's numbers, no device memory. */
+int dyninfer_mi355x_tree_attention_workspace_bytes(const dyninfer_kvcache_t* cache, const dyninfer_kvbatch_t* batch,
+                                                   uint32_t q_heads, uint32_t dtype, uint64_t* out_bytes);
+
+/*
+ * Checks drafted tokens against the target model's logits.  Rows as in dyninfer_kvbatch_t: rows
+ * starts[b].. are the nodes of sequence b's tree, node 0 its root (the last token known), every
+ * other node a drafted token with a parent of smaller index.  Of the current node (first the
+ * root) with target distribution p = softmax(logits / temperature), the children are tried in
+ * order: with R = p at first, child c is accepted if uniform[c] * q(token c) < R(token c), and
+ * becomes the current node; otherwise R = max(R - q, 0) divided by its sum, and the next child's
+ * turn comes.  q is row (current node) of draft_probs, the distribution its children were drawn
+ * from; without draft_probs q is 1 at the child's token and 0 elsewhere.  If such a sum is 0, R = p
+ * and no more children of this node are tried.  Where none is accepted the next token is the
+ * argmax of R / noise (noise exponentially distributed: a draw from R).  Either way the tokens are
+ * distributed as the target model's own.  temperature[b] <= 0: p is 1 at the largest logit, and
+ * uniform and noise play no part.  Ties go to the lowest token.
+ * A NaN logit counts as -inf, +inf as the largest f32; a row of -inf only accepts nothing and gives token -1,
+ * as does R / noise without a positive value.  A token outside the vocabulary is never accepted.
+ */
+typedef struct dyninfer_verify {
+    const void* logits;       /* [tokens, vocab], f32 or bf16, rows logits_stride elements apart */
+    const void* draft_probs;  /* [tokens, vocab], f32 or bf16, rows probs_stride apart; or NULL */
+    uint32_t logits_dtype, probs_dtype;
+    int64_t logits_stride, probs_stride;
+    const int64_t* draft_tokens; /* [tokens] (a root's is not read) */
+    const int32_t* parents;      /* [tokens], index in the sequence (a root's is not read); NULL: chains */
+    const int32_t* starts;       /* [sequences + 1] */
+    const float* temperature;    /* [sequences]; NULL: all 1 */
+    const float* uniform;        /* [tokens], in [0, 1) (a root's is not read) */
+    const float* noise;          /* [sequences, vocab], > 0, rows noise_stride apart */
+    int64_t noise_stride;
+    uint32_t vocab, sequences, tokens, max_new;
+    int32_t* path;       /* out [sequences, max_new]: the accepted nodes, 0 first, then -1 */
+    int32_t* counts;     /* out [sequences]: how many (0 for a sequence without rows) */
+    int64_t* next_token; /* out [sequences] */
+} dyninfer_verify_t;
+
+int dyninfer_mi355x_draft_verify(dyninfer_mi355x_ctx_t* ctx, const dyninfer_verify_t* args, void* workspace,
+                                 uint64_t workspace_bytes, void* stream);
+int dyninfer_mi355x_draft_verify_workspace_bytes(uint32_t sequences, uint32_t tokens, uint32_t vocab, uint32_t max_new,
+                                                 uint64_t* out_bytes);
+
+/*
  * GGUF container index: the exact byte range of every tensor of a GGUF file, so a
  * weight reaches the device as a plain copy of its on-disk bytes (no repack).
  * Restates the reference's indexer (crates/dyninfer-checkpoint-gguf/src/container.rs:179-340:
