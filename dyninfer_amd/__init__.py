@@ -320,22 +320,36 @@ def _bad(message: str):
     raise DyninferError(ERR_INVALID_ARGUMENT, message)
 
 
-def _table(t, dtype: str, shape, what: str) -> int:
-    """Address of a contiguous device tensor of that type and shape (None: any length)."""
+def _table(t, code: int, shape, what: str) -> int:
+    """Address of a contiguous device tensor of that type (a code of _table_code) and shape (None:
+    any length)."""
     if t is None:
         _bad(f"{what} is missing")
-    if not t.is_cuda or str(t.dtype) != dtype or not t.is_contiguous() or t.dim() != len(shape) \
-            or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+    s = t.shape
+    if not t.is_cuda or _table_code(t.dtype) != code or not t.is_contiguous() or len(s) != len(shape) \
+            or any([n is not None and n != m for n, m in zip(shape, s)]):
         want = ", ".join("n" if n is None else str(n) for n in shape)
-        _bad(f"{what} must be a contiguous device tensor [{want}] of {dtype[6:]}")
+        _bad(f"{what} must be a contiguous device tensor [{want}] of {('f32', 'int32', 'int64')[code]}")
     return t.data_ptr()
+
+
+_T_F32, _T_I32, _T_I64 = 0, 1, 2
+_TABLE_CODES: dict = {}
+
+
+def _table_code(dtype) -> int:
+    if not _TABLE_CODES:
+        import torch
+        _TABLE_CODES.update({torch.float32: _T_F32, torch.int32: _T_I32, torch.int64: _T_I64})
+    return _TABLE_CODES.get(dtype, -1)
 
 
 def _rows(t, tokens: int, dim: int, what: str) -> bytes:
     """The C descriptor of a device tensor [tokens, heads, dim] whose last axis is contiguous."""
-    if not t.is_cuda or t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != dim or t.stride(2) != 1:
+    s, st = t.shape, t.stride()
+    if not t.is_cuda or len(s) != 3 or s[0] != tokens or s[2] != dim or st[2] != 1:
         _bad(f"{what} must be a device tensor [{tokens}, heads, {dim}] whose last axis is contiguous")
-    return _pack_rows(t.data_ptr(), _dtype_code(t), t.shape[1], t.stride(0), t.stride(1))
+    return _pack_rows(t.data_ptr(), _dtype_code(t), s[1], st[0], st[1])
 
 
 @dataclass
@@ -402,9 +416,9 @@ class KVBatch:
         """The C struct's bytes."""
         n = self.lengths.shape[0] if self.lengths.dim() == 1 else -1
         try:
-            return _pack_kvbatch(_table(self.page_table, "torch.int32", (n, None), "page_table"),
-                                 _table(self.lengths, "torch.int32", (n,), "lengths"),
-                                 _table(self.starts, "torch.int32", (n + 1,), "starts"), n, self.page_table.shape[1],
+            return _pack_kvbatch(_table(self.page_table, _T_I32, (n, None), "page_table"),
+                                 _table(self.lengths, _T_I32, (n,), "lengths"),
+                                 _table(self.starts, _T_I32, (n + 1,), "starts"), n, self.page_table.shape[1],
                                  self.tokens, self.max_new, self.max_length)
         except struct.error as e:
             _bad(f"batch: {e}")
@@ -423,8 +437,8 @@ class Rope:
         """The C struct's bytes."""
         if self.layout not in ROPE_LAYOUTS:
             _bad(f"rope layout must be one of {sorted(ROPE_LAYOUTS)}")
-        return _pack_rope(_table(self.table, "torch.float32", (None, self.rot_dim // 2, 2), "rope table"),
-                          _table(self.positions, "torch.int32", (tokens,), "positions"), self.table.shape[0], self.rot_dim,
+        return _pack_rope(_table(self.table, _T_F32, (None, self.rot_dim // 2, 2), "rope table"),
+                          _table(self.positions, _T_I32, (tokens,), "positions"), self.table.shape[0], self.rot_dim,
                           ROPE_LAYOUTS[self.layout], 0)
 
 
@@ -570,7 +584,7 @@ class Context:
             out = self._new((positions, rot_dim // 2, 2), torch.float32, torch.device("cuda", self.device), stream)
         p = _pack_rope_params(rot_dim, ROPE_SCALINGS[scaling], theta, factor, original_length, beta_fast, beta_slow,
                               attn_factor, low_turns, high_turns)
-        ptr = _table(out, "torch.float32", (positions, rot_dim // 2, 2), "out")
+        ptr = _table(out, _T_F32, (positions, rot_dim // 2, 2), "out")
         _check(self._lib.dyninfer_mi355x_rope_table(self._h, p, positions, ptr, self._stream(stream)))
         return out
 
@@ -617,8 +631,8 @@ class Context:
         packed = batch.pack()
         n = batch.lengths.shape[0]
         _check(self._lib.dyninfer_mi355x_kv_commit(
-            self._h, cache.pack(), packed, _table(path, "torch.int32", (n, None), "path"), path.shape[1],
-            _table(counts, "torch.int32", (n,), "counts"), self._stream(stream)))
+            self._h, cache.pack(), packed, _table(path, _T_I32, (n, None), "path"), path.shape[1],
+            _table(counts, _T_I32, (n,), "counts"), self._stream(stream)))
 
     def tree_attention(self, cache: KVCache, batch: KVBatch, q, mask=None, scale: Optional[float] = None, out=None,
                        lse=None, stream=None, workspace=None):
@@ -630,10 +644,10 @@ class Context:
         if out is None:
             out = self._new(q.shape, q.dtype, q.device, stream)
         qr, cb, bb = _rows(q, n, dim, "q"), cache.pack(), batch.pack()
-        mp = None if mask is None else _table(mask, "torch.int64", (n, None), "mask")
+        mp = None if mask is None else _table(mask, _T_I64, (n, None), "mask")
         if mask is not None and 64 * mask.shape[1] < batch.max_new:
             _bad("mask has fewer bits than max_new")
-        lp = None if lse is None else _table(lse, "torch.float32", (n, q.shape[1]), "lse")
+        lp = None if lse is None else _table(lse, _T_F32, (n, q.shape[1]), "lse")
         need = ctypes.c_uint64(0)
         if workspace is None:
             _check(self._lib.dyninfer_mi355x_tree_attention_workspace_bytes(cb, bb, q.shape[1], _dtype_code(q),
@@ -669,9 +683,9 @@ class Context:
             _bad("draft_probs must be a device tensor of the logits' shape whose last axis is contiguous")
         if not noise.is_cuda or noise.dtype != torch.float32 or noise.shape != (seqs, vocab) or noise.stride(1) != 1:
             _bad("noise must be a device tensor [sequences, vocab] of float32 whose last axis is contiguous")
-        sp = _table(starts, "torch.int32", (None,), "starts")
-        tp = None if temperature is None else _table(temperature, "torch.float32", (seqs,), "temperature")
-        pp = None if parents is None else _table(parents, "torch.int32", (n,), "parents")
+        sp = _table(starts, _T_I32, (None,), "starts")
+        tp = None if temperature is None else _table(temperature, _T_F32, (seqs,), "temperature")
+        pp = None if parents is None else _table(parents, _T_I32, (n,), "parents")
         path = self._new((seqs, max_new), torch.int32, logits.device, stream)
         counts = self._new((seqs,), torch.int32, logits.device, stream)
         token = self._new((seqs,), torch.int64, logits.device, stream)
@@ -681,8 +695,8 @@ class Context:
         args = _pack_verify(
             logits.data_ptr(), 0 if draft_probs is None else draft_probs.data_ptr(), _dtype_code(logits),
             0 if draft_probs is None else _dtype_code(draft_probs), logits.stride(0),
-            0 if draft_probs is None else draft_probs.stride(0), _table(draft_tokens, "torch.int64", (n,), "draft_tokens"),
-            pp or 0, sp, tp or 0, _table(uniform, "torch.float32", (n,), "uniform"), noise.data_ptr(), noise.stride(0),
+            0 if draft_probs is None else draft_probs.stride(0), _table(draft_tokens, _T_I64, (n,), "draft_tokens"),
+            pp or 0, sp, tp or 0, _table(uniform, _T_F32, (n,), "uniform"), noise.data_ptr(), noise.stride(0),
             vocab, seqs, n, max_new, path.data_ptr(), counts.data_ptr(), token.data_ptr())
         _check(self._lib.dyninfer_mi355x_draft_verify(self._h, args, wp, wn, self._stream(stream)))
         return path, counts, token

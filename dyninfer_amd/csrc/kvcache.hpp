@@ -119,9 +119,9 @@ struct VerifyArgs {
     int32_t* counts;
     int64_t* next;
 };
-// Workgroups a row of logits is cut into.
-uint32_t verify_pieces(uint32_t vocab);
-uint64_t verify_workspace_bytes(uint32_t seqs, uint32_t tokens, uint32_t vocab, uint32_t max_new);
+// Workgroups of its largest launch.
+uint64_t verify_blocks(uint32_t seqs, uint32_t tokens, uint32_t vocab);
+uint64_t verify_workspace_bytes(uint32_t seqs, uint32_t tokens, uint32_t vocab);
 hipError_t verify_launch(const VerifyArgs& a, uint8_t* work, hipStream_t st);
 
 }  // namespace dmx

@@ -2,7 +2,6 @@
 // positions, the quantized paged cache, attention of drafted tokens over it,
 // and their verification.  Checks here keep every kernel inside the buffers
 // described; what the host cannot see (device tables) the kernels check.
-#include <algorithm>
 #include <cmath>
 #include <utility>
 
@@ -385,7 +384,7 @@ int dyninfer_mi355x_draft_verify_workspace_bytes(uint32_t sequences, uint32_t to
     *out_bytes = 0;
     if (vocab == 0) return fail(BAD, "vocab must be above 0");
     if (max_new > tokens) return fail(BAD, "max_new must not be above tokens");
-    *out_bytes = dmx::verify_workspace_bytes(sequences, tokens, vocab, max_new);
+    *out_bytes = dmx::verify_workspace_bytes(sequences, tokens, vocab);
     return DYNINFER_MI355X_OK;
 }
 
@@ -415,9 +414,9 @@ int dyninfer_mi355x_draft_verify(dyninfer_mi355x_ctx_t* ctx, const dyninfer_veri
             (v->parents && !aligned(v->parents, 4)))
             return fail(BAD, "draft_tokens, uniform or parents are NULL or misaligned");
     }
-    const uint64_t need = dmx::verify_workspace_bytes(v->sequences, v->tokens, v->vocab, v->max_new);
+    const uint64_t need = dmx::verify_workspace_bytes(v->sequences, v->tokens, v->vocab);
     if (int rc = check_workspace(workspace, workspace_bytes, need, "draft_verify")) return rc;
-    if (int rc = check_grid((uint64_t)std::max(v->tokens, v->sequences) * dmx::verify_pieces(v->vocab))) return rc;
+    if (int rc = check_grid(dmx::verify_blocks(v->sequences, v->tokens, v->vocab))) return rc;
     dmx::VerifyArgs a = {};
     a.logits = v->logits;
     a.probs = v->draft_probs;
