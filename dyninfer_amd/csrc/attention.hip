@@ -68,10 +68,10 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
 // Rows beyond 16 share a pass in twos of tiles where the registers hold them.
 // Positions are split until some 768 workgroups are there, or one step of a
 // workgroup (256 positions) each is left.
-AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint32_t q_heads) {
+AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint32_t q_heads, bool bf16) {
     AttnPlan p = {};
     const uint64_t rows = (uint64_t)b.max_new * (q_heads / kv.heads);
-    p.tiles = rows <= 16 || kv.dim > 128 ? 1 : 2;
+    p.tiles = rows <= 16 || (kv.dim > 128 && !bf16) ? 1 : rows <= 32 || kv.dim > 128 || !bf16 ? 2 : 4;
     p.row_tiles = (uint32_t)((rows + 16 * p.tiles - 1) / (16 * p.tiles));
     const uint64_t step = kTile * kWaves;
     const uint64_t steps = max_length > step ? (max_length + step - 1) / step : 1;
@@ -88,8 +88,13 @@ AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint
     return p;
 }
 
+// Units of one part of one head of one sequence, to a multiple of the XCDs, times the row tiles.
+uint64_t attn_blocks(const AttnPlan& plan, uint32_t heads, uint32_t seqs) {
+    return ((uint64_t)heads * plan.splits * seqs + 7) / 8 * 8 * plan.row_tiles;
+}
+
 hipError_t attn_launch(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
-    const uint64_t grid = (uint64_t)plan.row_tiles * a.kv.heads * plan.splits * a.b.seqs;
+    const uint64_t grid = attn_blocks(plan, a.kv.heads, a.b.seqs);
     if (grid == 0) return hipSuccess;
     hipError_t e;
     if (a.kv.k_bits == 8)

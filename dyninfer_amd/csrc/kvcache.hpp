@@ -90,7 +90,8 @@ struct AttnPlan {
     uint32_t span;       // positions of each but the last
     uint64_t bytes;      // workspace
 };
-AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint32_t q_heads);
+AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint32_t q_heads, bool bf16);
+uint64_t attn_blocks(const AttnPlan& plan, uint32_t heads, uint32_t seqs);
 struct AttnArgs {
     KvView kv;
     KvBatch b;
