@@ -1,5 +1,5 @@
 // Attention over the quantized cache: how a call is cut into workgroups, and the
-// second launch that joins the parts of a row whose positions were split
+// second launch that joins the parts of a unit whose steps were split
 // (attention_impl.hpp holds the kernel itself).
 #include "attention_impl.hpp"
 
@@ -12,48 +12,68 @@ template <> hipError_t attend_launch<4, 4>(const AttnArgs&, uint32_t, uint64_t, 
 
 namespace {
 
-// One wave per (row, query head): the parts' maxima and sums, then the parts'
-// outputs, each brought to the common maximum.
+// One wave per (row, query head) whose unit was split: the parts' maxima and
+// sums, then the parts' outputs, each brought to the common maximum.
 template <int D>
-__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t rows_of_tile) {
     constexpr int W = D <= 128 ? 2 : 4;  // dims of a lane
     const uint32_t lane = threadIdx.x & 63u;
-    const uint64_t q_heads = (uint64_t)a.kv.heads * a.group;
+    const uint32_t q_heads = a.kv.heads * a.group;
     const uint64_t id = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const uint32_t h = (uint32_t)(id % q_heads);
     const uint64_t rest = id / q_heads;
-    const uint32_t i = (uint32_t)(rest % a.b.max_new);
+    const uint32_t i = (uint32_t)(rest % a.b.max_new), seq = (uint32_t)(rest / a.b.max_new);
     if (rest / a.b.max_new >= a.b.seqs) return;
-    const SeqRange r = seq_range(a.b, (uint32_t)(rest / a.b.max_new));
+    Share s = {};
+    s.seq = seq;
+    s.load(a, rows_of_tile);
+    const SeqRange r = seq_range(a.b, seq);
     if (i >= r.n) return;
-    const uint64_t token = r.row0 + i, total = (uint64_t)r.len + r.n;
-    const uint32_t parts = (uint32_t)min((uint64_t)a.splits, (total + a.span - 1) / a.span);
-    const uint64_t at = (token * q_heads + h) * a.splits;
-    const float* po = a.work + at * D;
-    const float* ml = a.work + (uint64_t)a.b.tokens * q_heads * a.splits * D + 2 * at;
+    const uint64_t all = a.where[2 * a.b.seqs], first = a.where[2 * seq], unit0 = a.where[2 * seq + 1];
+    const uint32_t row = i * a.group + h % a.group;
+    const uint32_t unit = h / a.group * s.row_tiles + row / rows_of_tile;
+    // the shares that hold the unit's first and last step: share w begins at floor(w all / shares)
+    const uint64_t x0 = first + (uint64_t)unit * (s.unit_steps + kUnitCost) + kUnitCost, x1 = x0 + s.unit_steps - 1;
+    const uint64_t n = shares_of(a, all), w0 = ((x0 + 1) * n - 1) / all, w1 = ((x1 + 1) * n - 1) / all;
+    const uint32_t parts = (uint32_t)(w1 - w0) + 1;
+    if (parts == 1) return;  // written by the first launch
+    const uint64_t at = (w0 + unit0 + unit) * rows_of_tile + row % rows_of_tile;
+    const float* po = a.parts + at * D;
+    const float* ml = a.stats + 2 * at;
+    const uint64_t pitch = rows_of_tile;  // rows from one part to the next
 
     float top = -__builtin_inff();
-    for (uint32_t s = lane; s < parts; s += 64) top = fmaxf(top, gptr<float>(ml)[2 * s]);
+    for (uint32_t p = lane; p < parts; p += 64) top = fmaxf(top, gptr<float>(ml)[2 * pitch * p]);
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
     const float ref = top == -__builtin_inff() ? 0.0f : top;
     float sum = 0.0f;
-    for (uint32_t s = lane; s < parts; s += 64) sum += gptr<float>(ml)[2 * s + 1] * exp2f(gptr<float>(ml)[2 * s] - ref);
+    for (uint32_t p = lane; p < parts; p += 64)
+        sum += gptr<float>(ml)[2 * pitch * p + 1] * exp2f(gptr<float>(ml)[2 * pitch * p] - ref);
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
 
-    const uint32_t d0 = W * lane;
     if (a.lse && lane == 0)
-        gptr_mut<float>(a.lse)[token * q_heads + h] = (top + log2f(sum)) * 0.69314718055994531f;
+        gptr_mut<float>(a.lse)[(r.row0 + (uint64_t)i) * q_heads + h] = (top + log2f(sum)) * 0.69314718055994531f;
+    const uint32_t d0 = W * lane;
     if (d0 >= D) return;
-    float o[W] = {};
-    for (uint32_t s = 0; s < parts; s++) {
-        const float f = exp2f(gptr<float>(ml)[2 * s] - ref);
+    typedef float vec __attribute__((ext_vector_type(W)));
+    vec o = {};
+    for (uint32_t p = 0; p < parts; p += 4) {  // four loads in flight
+        vec v[4];
+        float f[4];
 #pragma unroll
-        for (int j = 0; j < W; j++) o[j] += f * gptr<float>(po + (uint64_t)s * D)[d0 + j];
+        for (uint32_t k = 0; k < 4; k++) {
+            const uint64_t part = p + k < parts ? p + k : parts - 1;
+            v[k] = *gptr<vec>(po + part * pitch * D + d0);
+            f[k] = gptr<float>(ml)[2 * pitch * part];
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++)
+            if (p + k < parts) o += v[k] * exp2f(f[k] - ref);
     }
     const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : __builtin_nanf(""));
-    const int64_t e = (int64_t)token * a.out.ts + (int64_t)h * a.out.hs + d0;
+    const int64_t e = (r.row0 + (int64_t)i) * a.out.ts + (int64_t)h * a.out.hs + d0;
 #pragma unroll
     for (int j = 0; j < W; j++) {
         if (a.out.bf16)
@@ -65,50 +85,59 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
 
 }  // namespace
 
-// Rows beyond 16 share a pass in twos of tiles where the registers hold them.
-// Positions are split until some 768 workgroups are there, or one step of a
-// workgroup (256 positions) each is left.
+// Row tiles: one or two of 16 rows held by every wave, or four or eight held by
+// four waves (64 tokens x group 4 over 131k positions: 572 us with one, 382 with two,
+// 401 with four, 300 with eight; 8 x 4 over 4k in 32 sequences: 74, 70, 89, 98).
+// The steps of all units go in equal shares to as many workgroups as the CUs
+// hold at once (two each; one of 256 dims), or one step each if they are fewer:
+// sequences differ in length, and a share may end in the middle of a unit.
+// Units of one step, or so many that they fill the CUs several times over, are
+// a workgroup each, with no second launch.
 AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint32_t q_heads, bool bf16) {
     AttnPlan p = {};
     const uint64_t rows = (uint64_t)b.max_new * (q_heads / kv.heads);
-    p.tiles = rows <= 16 || (kv.dim > 128 && !bf16) ? 1 : rows <= 32 || kv.dim > 128 || !bf16 ? 2 : 4;
-    p.row_tiles = (uint32_t)((rows + 16 * p.tiles - 1) / (16 * p.tiles));
-    const uint64_t step = kTile * kWaves;
-    const uint64_t steps = max_length > step ? (max_length + step - 1) / step : 1;
+    // registers hold two tiles of at most 128 dims and bf16
+    const bool two = kv.dim <= 128 && bf16;
+    p.tiles = rows <= 16 || (rows <= 32 && !two) ? 1 : rows <= 32 ? 2 : rows <= 64 || !two ? 4 : 8;
+    const uint32_t tile = 16 * p.tiles;
+    p.row_tiles = (uint32_t)((rows + tile - 1) / tile);
+    const uint64_t steps = max_length > kStep ? (max_length + kStep - 1) / kStep : 1;
     const uint64_t units = (uint64_t)b.seqs * kv.heads * p.row_tiles;
-    uint64_t want = units ? (768 + units - 1) / units : 1;
-    if (want > steps) want = steps;
-    const uint64_t each = (steps + want - 1) / want;
-    uint64_t span = each * step;
-    if (span > 0x40000000u) span = 0x40000000u;
-    p.span = (uint32_t)span;
-    p.splits = (uint32_t)((steps * step + span - 1) / span);
-    if (p.splits < 1) p.splits = 1;
-    if (p.splits > 1) p.bytes = (uint64_t)b.tokens * q_heads * p.splits * (kv.dim + 2) * 4;
+    const uint64_t full = kv.dim > 128 ? 256 : 512;
+    if (steps == 1 || units >= 8 * full) {
+        p.grid = units;
+        return p;
+    }
+    const uint64_t places = units * (steps + kUnitCost);
+    p.shares = (uint32_t)(places < full ? places : full);
+    p.grid = p.shares;
+    const uint64_t slots = (units + p.shares) * tile;
+    p.stats = slots * kv.dim * 4;
+    p.where = p.stats + slots * 8;
+    p.bytes = p.where + (2 * (uint64_t)b.seqs + 1) * 8;
     return p;
 }
 
-// Units of one part of one head of one sequence, to a multiple of the XCDs, times the row tiles.
-uint64_t attn_blocks(const AttnPlan& plan, uint32_t heads, uint32_t seqs) {
-    return ((uint64_t)heads * plan.splits * seqs + 7) / 8 * 8 * plan.row_tiles;
-}
-
-hipError_t attn_launch(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
-    const uint64_t grid = attn_blocks(plan, a.kv.heads, a.b.seqs);
-    if (grid == 0) return hipSuccess;
+hipError_t attn_launch(AttnArgs a, const AttnPlan& plan, uint8_t* work, hipStream_t st) {
+    if (plan.grid == 0) return hipSuccess;
+    a.row_tiles = plan.row_tiles;
+    a.shares = plan.shares;
+    a.parts = reinterpret_cast<float*>(work);
+    a.stats = reinterpret_cast<float*>(work + plan.stats);
+    a.where = reinterpret_cast<uint64_t*>(work + plan.where);
     hipError_t e;
     if (a.kv.k_bits == 8)
-        e = a.kv.v_bits == 8 ? attend_launch<8, 8>(a, plan.tiles, grid, st) : attend_launch<8, 4>(a, plan.tiles, grid, st);
+        e = a.kv.v_bits == 8 ? attend_launch<8, 8>(a, plan.tiles, plan.grid, st) : attend_launch<8, 4>(a, plan.tiles, plan.grid, st);
     else
-        e = a.kv.v_bits == 8 ? attend_launch<4, 8>(a, plan.tiles, grid, st) : attend_launch<4, 4>(a, plan.tiles, grid, st);
-    if (e != hipSuccess || plan.splits == 1) return e;
+        e = a.kv.v_bits == 8 ? attend_launch<4, 8>(a, plan.tiles, plan.grid, st) : attend_launch<4, 4>(a, plan.tiles, plan.grid, st);
+    if (e != hipSuccess || plan.shares == 0) return e;
     const uint64_t waves = (uint64_t)a.b.seqs * a.b.max_new * a.kv.heads * a.group;
-    const uint32_t blocks = (uint32_t)((waves + 3) / 4);
+    const uint32_t blocks = (uint32_t)((waves + 3) / 4), tile = 16 * plan.tiles;
     switch (a.kv.dim) {
-    case 64: join_kernel<64><<<blocks, 256, 0, st>>>(a); break;
-    case 96: join_kernel<96><<<blocks, 256, 0, st>>>(a); break;
-    case 128: join_kernel<128><<<blocks, 256, 0, st>>>(a); break;
-    case 256: join_kernel<256><<<blocks, 256, 0, st>>>(a); break;
+    case 64: join_kernel<64><<<blocks, 256, 0, st>>>(a, tile); break;
+    case 96: join_kernel<96><<<blocks, 256, 0, st>>>(a, tile); break;
+    case 128: join_kernel<128><<<blocks, 256, 0, st>>>(a, tile); break;
+    case 256: join_kernel<256><<<blocks, 256, 0, st>>>(a, tile); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

@@ -5,15 +5,17 @@
 //   S[p, r] = scale q_r . k_p,  out_r = sum_p exp(S - max) v_p / sum_p exp(S - max)
 //
 // over the positions p that row r sees.  Rows of one kv head are the new tokens
-// times the query heads that share it, r = token * group + head: up to 32 of
+// times the query heads that share it, r = token * group + head: up to 128 of
 // them share one pass over the cache.
 //
-// One pass, online: a wave takes 64 positions at a time, keeps the running
-// maximum and sum of every row and the unnormalised output in registers, and
-// joins its state with the other three waves' in LDS at the end, and, when the
-// positions are split over workgroups, through the workspace and a second
-// small launch.  Few rows over a long context are bound by the cache's bytes;
-// from about 64 rows the vector instructions around the products are.
+// One pass, online: a step takes 32 positions; the running maximum and sum of
+// every row and the unnormalised output stay in registers.  Up to 32 rows every
+// wave of a workgroup holds all of them and takes its own positions, and the
+// four join in LDS at the end; beyond, every wave holds its own rows, all take
+// the same positions and share their decoding.  Where positions are split over
+// workgroups, the parts are joined through the workspace by a second small launch.
+// Few rows over a long context are bound by the cache's bytes; from about 64 rows
+// the vector instructions around the products are.
 //
 // The products are 16x16x32 MFMAs with the cache as the first operand, so that
 // a row of the output (a column of the second operand) belongs to lanes l with
@@ -22,8 +24,8 @@
 //   S (16 positions x 16 rows): lane l holds positions 4(l / 16) + i, i < 4
 //   P (32 positions x 16 rows): lane l holds positions 8(l / 16) + j, j < 8
 // The sum over positions may take them in any order if both operands agree, so
-// position 16g + 4s + i of a tile is row 4g + i of the s-th S: lane group g then
-// holds positions 16g..16g+15, which for one dim of V are 16 codes in a row.
+// lane group g's eight positions of a step, 4s + i of them being row 4g + i of
+// the s-th S, are eight in a row: for one dim of V eight codes in a row.
 //
 // Numerics: K codes are exact in f16 (0x6400 | byte is 1024 + byte; the offset
 // is taken off exactly), queries are scaled to a power of two that puts the
@@ -254,190 +256,298 @@ __device__ __forceinline__ void tiles_wait(uint32_t k) {
 // Half of a dword of bf16 pairs as f32.
 __device__ __forceinline__ float bf16_of(uint32_t w, int i) { return __uint_as_float(i ? w & 0xFFFF0000u : w << 16); }
 
-// Workgroups of four waves that a CU is to hold at once (the registers allow it).
-constexpr int resident(int d, int nq) { return d * nq <= 256 && d < 256 ? 2 : 1; }
+constexpr uint32_t kStep = kTile * kWaves;  // positions a workgroup takes at a time
 
-template <int D, int KB, int VB, int NQ, bool F32>
-__global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a) {
-    using T = TileLds<D, KB, VB>;
-    constexpr int NB = D / 32;            // blocks of a key
-    constexpr int DT = D / 16;            // 16-dim tiles of the output
-    constexpr int TERMS = F32 ? 3 : 2;    // bf16 terms of a probability
-    constexpr uint32_t R = T::STAGES;
-    constexpr uint32_t JOIN = NQ * DT * 1024;  // bytes of a wave's output
-    constexpr uint32_t LDS = kWaves * R * T::BYTES > 2 * JOIN ? kWaves * R * T::BYTES : 2 * JOIN;
-    __shared__ __align__(16) uint8_t lds[LDS];
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t g = lane >> 4, col = lane & 15u;
+// What beginning and ending a unit costs, in steps: 32 ragged sequences of up to
+// 4096 positions, a new one among them (units of one step), took 95.7 us with 0,
+// 67.4 with 2, 70.4 with 4.
+constexpr uint32_t kUnitCost = 2;
 
-    // Workgroups go round the eight XCDs; those that share a piece of the cache
-    // (row tiles of one part of one head) are eight apart, on one XCD and its L2.
-    const uint32_t rt = blockIdx.x / 8 % a.row_tiles;
-    uint32_t id = blockIdx.x / 8 / a.row_tiles * 8 + blockIdx.x % 8;
-    const uint32_t head = id % a.kv.heads;
-    id /= a.kv.heads;
-    const uint32_t split = id % a.splits, seq = id / a.splits;
-    if (seq >= a.b.seqs) return;
-    const SeqRange r = seq_range(a.b, seq);
-    const uint32_t rows = r.n * a.group;
-    if (rt * (16u * NQ) >= rows) return;
-    const uint64_t total = (uint64_t)r.len + r.n;
-    const uint64_t begin = (uint64_t)split * a.span;
-    if (begin >= total) return;
-    // a multiple of the tile, but for the sequence's own end, where sees() ends
-    const uint64_t end = split + 1 == a.splits ? total : min(total, begin + a.span);
+// The work of a call as a line: sequence after sequence, of each its units (head
+// after head, row tile after row tile), of each kUnitCost places and then its
+// steps along the positions.  A share is one of a.shares equal pieces of that line.
+struct Share {
+    uint64_t unit0;       // units before this sequence's
+    uint32_t share;       // which piece
+    uint32_t seq;
+    uint32_t unit;        // in the sequence
+    uint32_t row_tiles, units, unit_steps;  // of the sequence
+    uint32_t place;       // first place in the unit
+    uint32_t places;      // left in the share
 
-    // This wave's tiles: every fourth from the wave-th.
-    uint8_t* const mine = lds + wave * (R * T::BYTES);
-    const uint32_t tile0 = (uint32_t)(begin / kTile) + wave;
-    const uint32_t ends = (uint32_t)((end + kTile - 1) / kTile);
-    const uint32_t count = tile0 < ends ? (ends - tile0 + kWaves - 1) / kWaves : 0;
-    // Page ids of a tile's two chunks, all lanes alike (scalar loads).
-    const uint64_t table = (uint64_t)(a.b.table + (size_t)seq * a.b.table_pages);
-    auto page_of = [&](uint32_t chunk) -> int32_t {
-        const uint32_t i = chunk >> (a.kv.page_shift - 4u);
-        return i < a.b.table_pages ? *(const __attribute__((address_space(4))) int32_t*)(table + 4ull * i) : -1;
-    };
-    int32_t id0 = -1, id1 = -1;
-    auto look_up = [&](uint32_t k) {
-        const uint32_t c = 2 * (tile0 + kWaves * k);
-        id0 = page_of(c);
-        id1 = page_of(c + 1);
-    };
-    // Copies tile k, whose page ids are at hand, into its stage.  An absent chunk
-    // is copied from slot 0 and masked: two bits of `absent` for each tile held.
-    uint32_t absent = 0;
-    auto fetch = [&](uint32_t k, uint32_t place) {
-        const uint32_t c = 2 * (tile0 + kWaves * k);
-        const bool ok0 = id0 >= 0 && (uint64_t)(uint32_t)id0 < a.kv.pages, ok1 = id1 >= 0 && (uint64_t)(uint32_t)id1 < a.kv.pages;
-        absent |= ((ok0 ? 0u : 1u) | (ok1 ? 0u : 2u)) << (2 * place);
-        uint32_t ln = lane;
-        asm volatile("" : "+v"(ln));  // addresses are made here, not held in registers
-        copy_tile<D, KB, VB>(a.kv, ok0 ? chunk_slot(a.kv, id0, head, c) : 0, ok1 ? chunk_slot(a.kv, id1, head, c + 1) : 0, ln,
-                             mine + k % R * T::BYTES);
-    };
-    for (uint32_t k = 0; k < R - 1 && k < count; k++) {
-        look_up(k);
-        fetch(k, k);
+    __device__ __forceinline__ void load(const AttnArgs& a, uint32_t rows_of_tile) {
+        const SeqRange r = seq_range(a.b, seq);
+        row_tiles = (r.n * a.group + rows_of_tile - 1) / rows_of_tile;
+        units = row_tiles * a.kv.heads;
+        unit_steps = r.n ? (uint32_t)(((uint64_t)r.len + r.n + kStep - 1) / kStep) : 0;
     }
-    if (R - 1 < count) look_up(R - 1);
 
-    // this lane's rows (columns of the products), their queries as operands
+    // The share's steps of this unit: first one, and the one after the last.
+    __device__ __forceinline__ uint32_t first_step() const { return place > kUnitCost ? place - kUnitCost : 0; }
+    __device__ __forceinline__ uint32_t end_step() const {
+        const uint32_t e = min(place + places, unit_steps + kUnitCost);
+        return e > kUnitCost ? e - kUnitCost : 0;
+    }
+
+    // On to the next unit.
+    __device__ __forceinline__ void next(const AttnArgs& a, uint32_t rows_of_tile) {
+        places -= min(places, unit_steps + kUnitCost - place);
+        place = 0;
+        if (places == 0 || ++unit < units) return;
+        do {
+            unit0 += units;
+            unit = 0;
+            if (++seq >= a.b.seqs) {
+                places = 0;
+                return;
+            }
+            load(a, rows_of_tile);
+        } while (units == 0);
+    }
+};
+
+// Workgroups go round the eight XCDs; this numbering gives each XCD a run of
+// consecutive numbers, so that row tiles that read the same part of the cache
+// at the same time find it in one L2.
+__device__ __forceinline__ uint32_t by_xcd(uint32_t id, uint32_t n) {
+    const uint32_t each = n / 8, more = n % 8, x = id % 8;
+    return x * each + min(x, more) + id / 8;
+}
+
+// Shares in use: no share is empty.
+__device__ __forceinline__ uint32_t shares_of(const AttnArgs& a, uint64_t all) {
+    return (uint32_t)min((uint64_t)a.shares, all);
+}
+
+// Without shares: workgroup (sequence, head, row tile), all of its steps.
+__device__ __forceinline__ Share whole_unit(const AttnArgs& a, uint32_t rows_of_tile) {
+    Share s = {};
+    uint32_t id = by_xcd(blockIdx.x, gridDim.x);
+    const uint32_t rt = id % a.row_tiles;
+    id /= a.row_tiles;
+    s.seq = id / a.kv.heads;
+    s.load(a, rows_of_tile);
+    s.unit = id % a.kv.heads * s.row_tiles + rt;
+    s.places = rt < s.row_tiles ? s.unit_steps + kUnitCost : 0;
+    return s;
+}
+
+// Places and units of sequence s.
+__device__ __forceinline__ void seq_work(const AttnArgs& a, uint32_t rows_of_tile, uint32_t s, uint64_t& places, uint64_t& units) {
+    places = units = 0;
+    if (s >= a.b.seqs) return;
+    Share x = {};
+    x.seq = s;
+    x.load(a, rows_of_tile);
+    units = x.units;
+    places = x.units * (uint64_t)(x.unit_steps + kUnitCost);
+}
+
+// This workgroup's share.  The first workgroup also writes where each sequence's
+// places and units begin, for the second launch.  lds: 64 bytes and more.
+__device__ inline Share share_of(const AttnArgs& a, uint32_t rows_of_tile, uint8_t* lds) {
+    uint64_t* const sums = reinterpret_cast<uint64_t*>(lds);  // [2][4] of the waves
+    Share* const found = reinterpret_cast<Share*>(lds + 64);
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    uint32_t share = 0;
+    uint64_t all = 0;
+    uint64_t at = 0, to = 0;
+    uint64_t places = 0, units = 0;
+    for (int pass = 0; pass < 2; pass++) {  // how many places there are; whose the share's first is
+        uint64_t before = 0, units_before = 0;
+        for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 256) {
+            if (pass == 0 || a.b.seqs > 256) seq_work(a, rows_of_tile, s0 + threadIdx.x, places, units);
+            uint64_t x = places, y = units;  // inclusive sums
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const uint64_t u = __shfl_up((unsigned long long)x, d), v = __shfl_up((unsigned long long)y, d);
+                if (lane >= (uint32_t)d) x += u, y += v;
+            }
+            __syncthreads();
+            if (lane == 63) sums[wave] = x, sums[4 + wave] = y;
+            __syncthreads();
+            uint64_t tx = 0, ty = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < 4; w++) {
+                if (w == wave) x += tx, y += ty;
+                tx += sums[w];
+                ty += sums[4 + w];
+            }
+            const uint64_t first = before + x - places, unit0 = units_before + y - units;
+            if (pass == 1) {
+                if (at < to && first <= at && at < first + places) {
+                    Share f = {};
+                    f.unit0 = unit0;
+                    f.share = share;
+                    f.seq = s0 + threadIdx.x;
+                    f.load(a, rows_of_tile);
+                    f.unit = (uint32_t)((at - first) / (f.unit_steps + kUnitCost));
+                    f.place = (uint32_t)((at - first) % (f.unit_steps + kUnitCost));
+                    f.places = (uint32_t)(to - at);
+                    *found = f;
+                }
+                if (blockIdx.x == 0 && s0 + threadIdx.x < a.b.seqs) {
+                    a.where[2 * (s0 + threadIdx.x)] = first;
+                    a.where[2 * (s0 + threadIdx.x) + 1] = unit0;
+                }
+            }
+            before += tx;
+            units_before += ty;
+        }
+        if (pass == 0) {
+            all = before;
+            const uint32_t n = shares_of(a, all);
+            share = n < a.shares ? blockIdx.x : by_xcd(blockIdx.x, n);
+            if (share < n) {
+                at = share * all / n;
+                to = (share + 1ull) * all / n;
+            }
+        }
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.where[2 * a.b.seqs] = all;
+    __syncthreads();
+    Share f = {};
+    if (at < to) f = *found;
+    __syncthreads();
+    // the same in every lane
+    f.share = share;
+    f.seq = __builtin_amdgcn_readfirstlane(f.seq);
+    f.unit = __builtin_amdgcn_readfirstlane(f.unit);
+    f.row_tiles = __builtin_amdgcn_readfirstlane(f.row_tiles);
+    f.units = __builtin_amdgcn_readfirstlane(f.units);
+    f.unit_steps = __builtin_amdgcn_readfirstlane(f.unit_steps);
+    f.place = __builtin_amdgcn_readfirstlane(f.place);
+    f.places = __builtin_amdgcn_readfirstlane(f.places);
+    f.unit0 = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(f.unit0 >> 32)) << 32 |
+              (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)f.unit0);
+    return f;
+}
+
+// A wave's rows: NQ tiles of 16, their queries as operands, running statistics
+// and unnormalised outputs.  The two kernels differ in how the cache's codes come
+// to hold as operands; a step takes 32 positions, of which lane group g holds
+// eight in a row.
+template <int D, int KB, int VB, int NQ, bool F32>
+struct WaveRows {
+    static constexpr int NB = D / 32;          // blocks of a key
+    static constexpr int DT = D / 16;          // 16-dim tiles of the output
+    static constexpr int TERMS = F32 ? 3 : 2;  // bf16 terms of a probability
     f16x8 qf[NQ][NB], ql[F32 ? NQ : 1][F32 ? NB : 1];
     float factor[NQ], m[NQ], l[NQ];  // m: what exponents are taken from, about the largest so far (log2)
     uint32_t tok[NQ];
-    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;  // so that the largest score is that of the largest sum
-#pragma unroll
-    for (int t = 0; t < NQ; t++) {
-        const uint32_t row = rt * (16u * NQ) + 16u * t + col;
-        const bool live = row < rows;
-        tok[t] = live ? row / a.group : 0u;
-        const uint32_t h = head * a.group + (live ? row % a.group : 0u);
-        const int64_t at = (int64_t)(r.row0 + tok[t]) * a.q.ts + (int64_t)h * a.q.hs;
-        float x[NB][8], big = 0.0f;
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const int64_t e = at + 32 * b + 8 * g;
-            if (a.q.vec && !F32) {
-                const u32x4 w = *gptr<u32x4>(static_cast<const uint16_t*>(a.q.p) + e);
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[b][i] = bf16_of(w[i / 2], i & 1);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    x[b][i] = F32 ? gptr<float>(a.q.p)[e + i] : bf16_bits_to_f32(gptr<uint16_t>(a.q.p)[e + i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[b][i]));
-        }
-        big = rows_max(big);
-        // exponent e of the row's largest: 2^(14 - e) scales it into [2^14, 2^15)
-        int e = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
-        e = max(e, -100);
-        const float up = sign * __uint_as_float((uint32_t)(14 - e + 127) << 23);
-        factor[t] = sign * a.scale * 1.44269504088896341f * (KB == 4 ? 0.0625f : 1.0f);
-        factor[t] *= __uint_as_float((uint32_t)(e - 14 + 127) << 23);
-        factor[t] = fmaxf(factor[t], 1.2e-38f);  // a masked score is -inf also at scale 0
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float s = live ? x[b][i] * up : 0.0f;
-                qf[t][b][i] = (_Float16)s;
-                if constexpr (F32) ql[t][b][i] = (_Float16)(s - (float)qf[t][b][i]);
-            }
-        }
-        m[t] = -__builtin_inff();
-        l[t] = 0.0f;
-    }
-
     f32x4 o[NQ][DT];
-#pragma unroll
-    for (int t = 0; t < NQ; t++)
-#pragma unroll
-        for (int d = 0; d < DT; d++) o[t][d] = f32x4{0, 0, 0, 0};
 
-    for (uint32_t k = 0; k < count; k++) {
-        const uint32_t p0 = (tile0 + kWaves * k) * kTile;
-        const uint8_t* const tile = mine + k % R * T::BYTES;
-        // the stage of tile k - 1 is free: its last reads have been waited for
-        if (k + R - 1 < count) {
-            fetch(k + R - 1, R - 1);
-            if (k + R < count) look_up(k + R);
-        }
-        const uint32_t gone = absent & 3u;
-        absent >>= 2;
-        tiles_wait<T::DMA, R - 1>(count - 1 - k);
-        uint32_t ln = lane;
-        asm volatile("" : "+v"(ln));
-        const uint32_t g = ln >> 4, col = ln & 15u;
-
-        // S: 16 positions x 16 rows at a time
-        f32x4 sc[NQ][2];
+    // Rows first_row + 16 t + lane % 16 of the unit's.
+    __device__ __forceinline__ void load(const AttnArgs& a, const SeqRange& r, uint32_t head, uint32_t first_row,
+                                         uint32_t rows, uint32_t lane) {
+        const uint32_t g = lane >> 4, col = lane & 15u;
+        const float sign = a.scale < 0.0f ? -1.0f : 1.0f;  // so that the largest score is that of the largest sum
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-            uint32_t kw[D / 16 * KB / 8], ks[2 * NB];  // bf16 scales of four positions
-            read_k<D, KB, VB>(tile, s, col, g, kw);
-#pragma unroll
-            for (int i = 0; i < 2 * NB; i += 2) {
-                const u32x2 x = *reinterpret_cast<const u32x2*>(tile + T::KS0 + (8 * g + 4 * s) * (2 * NB) + 4 * i);
-                ks[i] = x.x, ks[i + 1] = x.y;
-            }
+        for (int t = 0; t < NQ; t++) {
+            const uint32_t row = first_row + 16u * t + col;
+            const bool live = row < rows;
+            tok[t] = live ? row / a.group : 0u;
+            const uint32_t h = head * a.group + (live ? row % a.group : 0u);
+            const int64_t at = (int64_t)(r.row0 + tok[t]) * a.q.ts + (int64_t)h * a.q.hs;
+            float x[NB][8], big = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                const f16x8 kf = k_block<D, KB>(kw, b);
+                const int64_t e = at + 32 * b + 8 * g;
+                if (a.q.vec && !F32) {
+                    const u32x4 w = *gptr<u32x4>(static_cast<const uint16_t*>(a.q.p) + e);
 #pragma unroll
-                for (int t = 0; t < NQ; t++) {
-                    f32x4 x = {0, 0, 0, 0};
-                    if constexpr (F32) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[t][b], x, 0, 0, 0);
-                    x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[t][b], x, 0, 0, 0);
+                    for (int i = 0; i < 8; i++) x[b][i] = bf16_of(w[i / 2], i & 1);
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int at = i * NB + b;
-                        const float w = bf16_of(ks[at / 2], at & 1);
-                        sc[t][s][i] = b == 0 ? x[i] * w : sc[t][s][i] + x[i] * w;
-                    }
+                    for (int i = 0; i < 8; i++)
+                        x[b][i] = F32 ? gptr<float>(a.q.p)[e + i] : bf16_bits_to_f32(gptr<uint16_t>(a.q.p)[e + i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[b][i]));
+            }
+            big = rows_max(big);
+            // exponent e of the row's largest: 2^(14 - e) scales it into [2^14, 2^15)
+            int e = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
+            e = max(e, -100);
+            const float up = sign * __uint_as_float((uint32_t)(14 - e + 127) << 23);
+            factor[t] = sign * a.scale * 1.44269504088896341f * (KB == 4 ? 0.0625f : 1.0f);
+            factor[t] *= __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+            factor[t] = fmaxf(factor[t], 1.2e-38f);  // a masked score is -inf also at scale 0
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float s = live ? x[b][i] * up : 0.0f;
+                    qf[t][b][i] = (_Float16)s;
+                    if constexpr (F32) ql[t][b][i] = (_Float16)(s - (float)qf[t][b][i]);
                 }
             }
-        }
-
-        const bool edge = gone != 0 || (uint64_t)p0 + kTile > r.len;
-        uint32_t vis[NQ];
-        if (edge) {
+            m[t] = -__builtin_inff();
+            l[t] = 0.0f;
 #pragma unroll
-            for (int t = 0; t < NQ; t++) {
-                vis[t] = gone >> (g >> 1) & 1u ? 0u
-                                               : sees(a.mask, a.mask_words, r.row0 + tok[t], tok[t], r.n,
-                                                      (int64_t)p0 + 8 * g - (int64_t)r.len);
+            for (int d = 0; d < DT; d++) o[t][d] = f32x4{0, 0, 0, 0};
+        }
+    }
+
+    // 32 positions.  In src, of the lane group's eight positions: key(s, f): f[b] =
+    // operand of block b of S number s (positions 4s..4s+3 of the eight);
+    // key_scales(s, w): w[position][block] of those four; value_scales(w): of the
+    // eight; raw(d): what value(x) makes the operand of dims 16d..16d+15 of.
+    // masked: vis[t] has a bit for each of the eight that row t sees; otherwise all
+    // are seen.  LDS reads are issued well before their use: two waves a SIMD do not
+    // hide them.
+    template <class Src>
+    __device__ __forceinline__ void step(const Src& src, bool masked, const uint32_t (&vis)[NQ]) {
+        constexpr int AHEAD = 2;  // operands of V read before they are needed
+        f32x4 sc[NQ][2];
+        f16x8 kf[NB];
+        float kw[4 * NB], vs[8];
+        typename Src::Raw vr[DT];
+        src.key(0, kf);
+        src.key_scales(0, kw);
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            // all products first: a sum is read well after it was begun
+            f32x4 x[NB][NQ];
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+#pragma unroll
+                for (int t = 0; t < NQ; t++) {
+                    x[b][t] = f32x4{0, 0, 0, 0};
+                    if constexpr (F32) x[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[b], ql[t][b], x[b][t], 0, 0, 0);
+                    x[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[b], qf[t][b], x[b][t], 0, 0, 0);
+                }
+            }
+            float w[4 * NB];
+#pragma unroll
+            for (int i = 0; i < 4 * NB; i++) w[i] = kw[i];
+            if (s == 0) {
+                src.key(1, kf);
+                src.key_scales(1, kw);
+            } else {
+                src.value_scales(vs);
+#pragma unroll
+                for (int d = 0; d < AHEAD; d++) vr[d] = src.raw(d);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int t = 0; t < NQ; t++)
+                        sc[t][s][i] = b == 0 ? x[b][t][i] * w[i * NB + b] : sc[t][s][i] + x[b][t][i] * w[i * NB + b];
+        }
+        if (masked) {
+#pragma unroll
+            for (int t = 0; t < NQ; t++)
 #pragma unroll
                 for (int i = 0; i < 8; i++) sc[t][i / 4][i % 4] = vis[t] >> i & 1u ? sc[t][i / 4][i % 4] : -__builtin_inff();
-            }
         }
 
         // Exponentials, from a reference that follows the row's largest score only when
-        // one is 2^8 above it: the sums are f32 either way, and most tiles then need
+        // one is 2^8 above it: the sums are f32 either way, and most steps then need
         // neither the maximum over lanes nor a rescaling.
-        const u32x4 vs = *reinterpret_cast<const u32x4*>(tile + T::VS0 + 16 * g);
         bf16x8 pf[NQ][TERMS];
 #pragma unroll
         for (int t = 0; t < NQ; t++) {
@@ -459,9 +569,9 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
             for (int i = 0; i < 8; i++) {
                 const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i / 4][i % 4], factor[t], -ref));
                 l[t] += e;
-                p[i] = e * bf16_of(vs[i / 2], i & 1);
+                p[i] = e * vs[i];
             }
-            if (edge) {  // a masked value's scale may be anything
+            if (masked) {  // a masked value's scale may be anything
 #pragma unroll
                 for (int i = 0; i < 8; i++) p[i] = vis[t] >> i & 1u ? p[i] : 0.0f;
             }
@@ -483,111 +593,484 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
         // the product with V
 #pragma unroll
         for (int d = 0; d < DT; d++) {
-            bf16x8 vf;
-            if constexpr (VB == 8) {
-                const u32x2 x = *reinterpret_cast<const u32x2*>(tile + T::V0 + 512 * d + 256 * (g >> 1) + 16 * col + 8 * (g & 1u));
-                vf = v_frag(x.x, x.y);
-            } else {  // nibbles as the high half of a byte: 16 code
-                const uint32_t x = *reinterpret_cast<const uint32_t*>(tile + T::V0 + 256 * d + 128 * (g >> 1) + 8 * col + 4 * (g & 1u));
-                vf = v_frag((x << 4) & 0xF0F0F0F0u, x & 0xF0F0F0F0u);
-            }
+            if (d + AHEAD < DT) vr[d + AHEAD] = src.raw(d + AHEAD);
+            const bf16x8 vf = src.value(vr[d]);
 #pragma unroll
             for (int n = TERMS - 1; n >= 0; n--)
 #pragma unroll
                 for (int t = 0; t < NQ; t++)
                     o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[t][n], o[t][d], 0, 0, 0);
         }
-        ring_wait<63>();  // the tile has been read
     }
 
-    // join the four waves: every wave brings its rows to the common maximum, then
-    // 2 and 3 hand theirs to 0 and 1, and 1 to 0
-    __shared__ float sm_m[kWaves][16 * NQ], sm_l[kWaves][16 * NQ];
+    // Writes the rows: the outputs where the unit is one workgroup's alone, the
+    // parts for the second launch otherwise.  m: log2 of what l is to be multiplied
+    // with; o still times 16 where V has 4 bits.
+    __device__ __forceinline__ void store(const AttnArgs& a, const Share& sh, const SeqRange& r, uint32_t head, uint32_t tile_row,
+                                          uint32_t first_row, uint32_t rows, uint32_t rows_of_tile, bool alone, uint32_t lane) {
+        const uint32_t g = lane >> 4, col = lane & 15u;
 #pragma unroll
-    for (int t = 0; t < NQ; t++) {
-        l[t] = rows_sum(l[t]);
-        if (g == 0) {
-            sm_m[wave][16 * t + col] = m[t];
-            sm_l[wave][16 * t + col] = l[t];
-        }
-    }
-    __syncthreads();
+        for (int t = 0; t < NQ; t++) {
+            const uint32_t row = first_row + 16u * t + col;
+            if (row >= rows) continue;
+            const uint32_t h = head * a.group + row % a.group;
+            const uint64_t token = r.row0 + row / a.group, q_heads = (uint64_t)a.kv.heads * a.group;
+            if (!alone) {
+                // parts of a unit are handed to the second launch; (share, unit) pairs climb a
+                // staircase, so share + unit numbers them without gaps
+                const uint64_t at = (sh.share + sh.unit0 + sh.unit) * rows_of_tile + (row - tile_row);
+                float* po = a.parts + at * D;
 #pragma unroll
-    for (int t = 0; t < NQ; t++) {
-        float top = -__builtin_inff(), sum = 0.0f;
+                for (int d = 0; d < DT; d++) *gptr_mut<f32x4>(po + 16 * d + 4 * g) = o[t][d] * (VB == 4 ? 0.0625f : 1.0f);
+                if (g == 0) {
+                    gptr_mut<float>(a.stats)[2 * at] = m[t];
+                    gptr_mut<float>(a.stats)[2 * at + 1] = l[t];
+                }
+            } else {
+                float inv = l[t] > 0.0f ? 1.0f / l[t] : (l[t] == 0.0f ? 0.0f : __builtin_nanf(""));
+                if (VB == 4) inv *= 0.0625f;
+                const int64_t at = (int64_t)token * a.out.ts + (int64_t)h * a.out.hs;
 #pragma unroll
-        for (uint32_t w = 0; w < kWaves; w++) top = fmaxf(top, sm_m[w][16 * t + col]);
-        // a wave that has seen no number yet has nothing to bring (or a NaN: times 1)
-        auto back = [&](float mw) { return mw == -__builtin_inff() ? 1.0f : exp2f(mw - top); };
+                for (int d = 0; d < DT; d++) {
+                    const f32x4 x = o[t][d] * inv;
+                    const int64_t e = at + 16 * d + 4 * g;
+                    if constexpr (F32) {
+                        if (a.out.vec) {
+                            *gptr_mut<f32x4>(static_cast<float*>(a.out.p) + e) = x;
+                        } else {
 #pragma unroll
-        for (uint32_t w = 0; w < kWaves; w++) sum += sm_l[w][16 * t + col] * back(sm_m[w][16 * t + col]);
-        const float own = back(m[t]) * (VB == 4 ? 0.0625f : 1.0f);
-        m[t] = sum == 0.0f ? -__builtin_inff() : top == -__builtin_inff() ? 0.0f : top;
-        l[t] = sum;
-#pragma unroll
-        for (int d = 0; d < DT; d++) o[t][d] *= own;
-    }
-    f32x4* const sm_o = reinterpret_cast<f32x4*>(lds);
-#pragma unroll
-    for (uint32_t half = 2; half >= 1; half /= 2) {
-        if (wave >= half && wave < 2 * half) {
-#pragma unroll
-            for (int t = 0; t < NQ; t++)
-#pragma unroll
-                for (int d = 0; d < DT; d++) sm_o[((wave - half) * NQ * DT + t * DT + d) * 64 + lane] = o[t][d];
-        }
-        __syncthreads();
-        if (wave < half) {
-#pragma unroll
-            for (int t = 0; t < NQ; t++)
-#pragma unroll
-                for (int d = 0; d < DT; d++) o[t][d] += sm_o[(wave * NQ * DT + t * DT + d) * 64 + lane];
-        }
-        __syncthreads();
-    }
-    if (wave != 0) return;
-#pragma unroll
-    for (int t = 0; t < NQ; t++) {
-        const uint32_t row = rt * (16u * NQ) + 16u * t + col;
-        if (row >= rows) continue;
-        const uint32_t h = head * a.group + row % a.group;
-        const uint64_t token = r.row0 + row / a.group, q_heads = (uint64_t)a.kv.heads * a.group;
-        if (a.splits > 1) {
-            const uint64_t at = (token * q_heads + h) * a.splits + split;
-            float* po = a.work + at * D;
-#pragma unroll
-            for (int d = 0; d < DT; d++) *gptr_mut<f32x4>(po + 16 * d + 4 * g) = o[t][d];
-            if (g == 0) {
-                float* ml = a.work + (uint64_t)a.b.tokens * q_heads * a.splits * D + 2 * at;
-                gptr_mut<float>(ml)[0] = m[t];
-                gptr_mut<float>(ml)[1] = l[t];
-            }
-        } else {
-            const float inv = l[t] > 0.0f ? 1.0f / l[t] : (l[t] == 0.0f ? 0.0f : __builtin_nanf(""));
-            const int64_t at = (int64_t)token * a.out.ts + (int64_t)h * a.out.hs;
-#pragma unroll
-            for (int d = 0; d < DT; d++) {
-                const f32x4 x = o[t][d] * inv;
-                const int64_t e = at + 16 * d + 4 * g;
-                if constexpr (F32) {
-                    if (a.out.vec) {
-                        *gptr_mut<f32x4>(static_cast<float*>(a.out.p) + e) = x;
+                            for (int i = 0; i < 4; i++) gptr_mut<float>(a.out.p)[e + i] = x[i];
+                        }
                     } else {
+                        const u32x2 w = {f32x2_to_bf16x2_bits(x[0], x[1]), f32x2_to_bf16x2_bits(x[2], x[3])};
+                        if (a.out.vec) {
+                            *gptr_mut<u32x2>(static_cast<uint16_t*>(a.out.p) + e) = w;
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) gptr_mut<float>(a.out.p)[e + i] = x[i];
+                            for (int i = 0; i < 4; i++)
+                                gptr_mut<uint16_t>(a.out.p)[e + i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+                        }
                     }
-                } else {
-                    const u32x2 w = {f32x2_to_bf16x2_bits(x[0], x[1]), f32x2_to_bf16x2_bits(x[2], x[3])};
-                    if (a.out.vec) {
-                        *gptr_mut<u32x2>(static_cast<uint16_t*>(a.out.p) + e) = w;
-                    } else {
+                }
+                if (a.lse && g == 0) gptr_mut<float>(a.lse)[token * q_heads + h] = (m[t] + log2f(l[t])) * 0.69314718055994531f;
+            }
+        }
+    }
+};
+
+// Page ids, all lanes alike (scalar loads).
+struct Pages {
+    uint64_t table;
+    uint32_t count, shift;
+    __device__ __forceinline__ Pages(const AttnArgs& a, uint32_t seq)
+        : table((uint64_t)(a.b.table + (size_t)seq * a.b.table_pages)), count(a.b.table_pages), shift(a.kv.page_shift - 4u) {}
+    __device__ __forceinline__ int32_t operator()(uint32_t chunk) const {
+        const uint32_t i = chunk >> shift;
+        return i < count ? *(const __attribute__((address_space(4))) int32_t*)(table + 4ull * i) : -1;
+    }
+};
+
+// bf16 scales as f32.
+template <int N>
+__device__ __forceinline__ void read_bf16(const uint8_t* p, float (&w)[N]) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            gptr_mut<uint16_t>(a.out.p)[e + i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+    for (int i = 0; i < N; i += 4) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(p + 2 * i);
+        w[i] = bf16_of(x.x, 0), w[i + 1] = bf16_of(x.x, 1), w[i + 2] = bf16_of(x.y, 0), w[i + 3] = bf16_of(x.y, 1);
+    }
+}
+
+// A tile in LDS as it was copied: codes, decoded as they are read.
+template <int D, int KB, int VB>
+struct CodeTile {
+    using T = TileLds<D, KB, VB>;
+    using Raw = u32x2;
+    static constexpr int NB = D / 32;
+    const uint8_t* tile;
+    uint32_t g, col;
+    __device__ __forceinline__ void key(int s, f16x8 (&f)[NB]) const {
+        uint32_t w[D / 16 * KB / 8];
+        read_k<D, KB, VB>(tile, s, col, g, w);
+#pragma unroll
+        for (int b = 0; b < NB; b++) f[b] = k_block<D, KB>(w, b);
+    }
+    __device__ __forceinline__ void key_scales(int s, float (&w)[4 * NB]) const {
+        read_bf16(tile + T::KS0 + (8 * g + 4 * s) * (2 * NB), w);
+    }
+    __device__ __forceinline__ void value_scales(float (&w)[8]) const { read_bf16(tile + T::VS0 + 16 * g, w); }
+    __device__ __forceinline__ Raw raw(int d) const {
+        if constexpr (VB == 8)
+            return *reinterpret_cast<const u32x2*>(tile + T::V0 + 512 * d + 256 * (g >> 1) + 16 * col + 8 * (g & 1u));
+        else
+            return u32x2{*reinterpret_cast<const uint32_t*>(tile + T::V0 + 256 * d + 128 * (g >> 1) + 8 * col + 4 * (g & 1u)), 0};
+    }
+    __device__ __forceinline__ bf16x8 value(Raw x) const {
+        if constexpr (VB == 8) return v_frag(x.x, x.y);
+        return v_frag((x.x << 4) & 0xF0F0F0F0u, x.x & 0xF0F0F0F0u);  // nibbles as the high half of a byte: 16 code
+    }
+};
+
+// Half of a tile in LDS that other waves have decoded: operands, scales in f32.
+template <int D>
+struct OperandTile {
+    using Raw = bf16x8;
+    static constexpr int NB = D / 32;
+    const f16x8* kf;
+    const bf16x8* vf;
+    const float* ks;
+    const float* vs;
+    __device__ __forceinline__ void key(int s, f16x8 (&f)[NB]) const {
+#pragma unroll
+        for (int b = 0; b < NB; b++) f[b] = kf[(s * NB + b) * 64];
+    }
+    __device__ __forceinline__ void key_scales(int s, float (&w)[4 * NB]) const {
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            const f32x4 x = reinterpret_cast<const f32x4*>(ks + 4 * s * NB)[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[4 * i + j] = x[j];
+        }
+    }
+    __device__ __forceinline__ void value_scales(float (&w)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const f32x4 x = reinterpret_cast<const f32x4*>(vs)[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[4 * i + j] = x[j];
+        }
+    }
+    __device__ __forceinline__ Raw raw(int d) const { return vf[d * 64]; }
+    __device__ __forceinline__ bf16x8 value(Raw x) const { return x; }
+};
+
+// Workgroups of four waves that a CU is to hold at once (the registers allow it).
+constexpr int resident(int d, int nq) { return d * nq <= 256 && d < 256 ? 2 : 1; }
+
+// Few rows (up to 16 NQ): every wave holds all of them and takes every fourth
+// tile of positions, copied straight into LDS and decoded as it is read.
+template <int D, int KB, int VB, int NQ, bool F32>
+__global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a) {
+    using T = TileLds<D, KB, VB>;
+    constexpr int DT = D / 16;
+    constexpr uint32_t R = T::STAGES, ROWS = 16u * NQ;
+    constexpr uint32_t JOIN = NQ * DT * 1024;  // bytes of a wave's output
+    constexpr uint32_t LDS = kWaves * R * T::BYTES > 2 * JOIN ? kWaves * R * T::BYTES : 2 * JOIN;
+    __shared__ __align__(16) uint8_t lds[LDS];
+    __shared__ float sm_m[kWaves][ROWS], sm_l[kWaves][ROWS];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    Share sh = a.shares == 0 ? whole_unit(a, ROWS) : share_of(a, ROWS, lds);
+    for (; sh.places != 0; sh.next(a, ROWS)) {
+        const uint32_t now0 = sh.first_step(), now1 = sh.end_step();  // steps of this unit
+        if (now0 >= now1) continue;
+        const uint32_t seq = sh.seq, head = sh.unit / sh.row_tiles, tile_row = sh.unit % sh.row_tiles * ROWS;
+        const SeqRange r = seq_range(a.b, seq);
+        const uint32_t rows = r.n * a.group;
+        const uint64_t total = (uint64_t)r.len + r.n;
+        const bool alone = now0 == 0 && now1 == sh.unit_steps;
+        const uint64_t begin = (uint64_t)now0 * kStep;
+        // a multiple of the tile, but for the sequence's own end, where sees() ends
+        const uint64_t end = min(total, (uint64_t)now1 * kStep);
+
+        // This wave's tiles: every fourth from the wave-th.
+        uint8_t* const mine = lds + wave * (R * T::BYTES);
+        const uint32_t tile0 = (uint32_t)(begin / kTile) + wave;
+        const uint32_t ends = (uint32_t)((end + kTile - 1) / kTile);
+        const uint32_t count = tile0 < ends ? (ends - tile0 + kWaves - 1) / kWaves : 0;
+        const Pages page_of(a, seq);
+        int32_t id0 = -1, id1 = -1;  // of the next tile to fetch
+        auto look_up = [&](uint32_t k) {
+            const uint32_t c = 2 * (tile0 + kWaves * k);
+            id0 = page_of(c);
+            id1 = page_of(c + 1);
+        };
+        // Copies tile k, whose page ids are at hand, into its stage.  An absent chunk
+        // is copied from slot 0 and masked: two bits of `absent` for each tile held.
+        uint32_t absent = 0;
+        auto fetch = [&](uint32_t k, uint32_t place) {
+            const uint32_t c = 2 * (tile0 + kWaves * k);
+            const bool ok0 = id0 >= 0 && (uint64_t)(uint32_t)id0 < a.kv.pages, ok1 = id1 >= 0 && (uint64_t)(uint32_t)id1 < a.kv.pages;
+            absent |= ((ok0 ? 0u : 1u) | (ok1 ? 0u : 2u)) << (2 * place);
+            uint32_t ln = lane;
+            asm volatile("" : "+v"(ln));  // addresses are made here, not held in registers
+            copy_tile<D, KB, VB>(a.kv, ok0 ? chunk_slot(a.kv, id0, head, c) : 0, ok1 ? chunk_slot(a.kv, id1, head, c + 1) : 0, ln,
+                                 mine + k % R * T::BYTES);
+        };
+        for (uint32_t k = 0; k < R - 1 && k < count; k++) {
+            look_up(k);
+            fetch(k, k);
+        }
+        if (R - 1 < count) look_up(R - 1);
+
+        WaveRows<D, KB, VB, NQ, F32> w;
+        w.load(a, r, head, tile_row, rows, lane);
+
+        for (uint32_t k = 0; k < count; k++) {
+            const uint32_t p0 = (tile0 + kWaves * k) * kTile;
+            const uint8_t* const tile = mine + k % R * T::BYTES;
+            // the stage of tile k - 1 is free: its last reads have been waited for
+            if (k + R - 1 < count) {
+                fetch(k + R - 1, R - 1);
+                if (k + R < count) look_up(k + R);
+            }
+            const uint32_t gone = absent & 3u;
+            absent >>= 2;
+            tiles_wait<T::DMA, R - 1>(count - 1 - k);
+            uint32_t ln = lane;
+            asm volatile("" : "+v"(ln));
+            const uint32_t g = ln >> 4, col = ln & 15u;
+            const bool masked = gone != 0 || (uint64_t)p0 + kTile > r.len;
+            uint32_t vis[NQ] = {};
+            if (masked) {
+#pragma unroll
+                for (int t = 0; t < NQ; t++)
+                    vis[t] = gone >> (g >> 1) & 1u ? 0u
+                                                   : sees(a.mask, a.mask_words, r.row0 + w.tok[t], w.tok[t], r.n,
+                                                          (int64_t)p0 + 8 * g - (int64_t)r.len);
+            }
+            w.step(CodeTile<D, KB, VB>{tile, g, col}, masked, vis);
+            ring_wait<63>();  // the tile has been read
+        }
+
+        // join the four waves: every wave brings its rows to the common maximum, then
+        // 2 and 3 hand theirs to 0 and 1, and 1 to 0
+        const uint32_t g = lane >> 4, col = lane & 15u;
+#pragma unroll
+        for (int t = 0; t < NQ; t++) {
+            w.l[t] = rows_sum(w.l[t]);
+            if (g == 0) {
+                sm_m[wave][16 * t + col] = w.m[t];
+                sm_l[wave][16 * t + col] = w.l[t];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NQ; t++) {
+            float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+            for (uint32_t v = 0; v < kWaves; v++) top = fmaxf(top, sm_m[v][16 * t + col]);
+            // a wave that has seen no number yet has nothing to bring (or a NaN: times 1)
+            auto back = [&](float mw) { return mw == -__builtin_inff() ? 1.0f : exp2f(mw - top); };
+#pragma unroll
+            for (uint32_t v = 0; v < kWaves; v++) sum += sm_l[v][16 * t + col] * back(sm_m[v][16 * t + col]);
+            const float own = back(w.m[t]);
+            w.m[t] = sum == 0.0f ? -__builtin_inff() : top == -__builtin_inff() ? 0.0f : top;
+            w.l[t] = sum;
+#pragma unroll
+            for (int d = 0; d < DT; d++) w.o[t][d] *= own;
+        }
+        f32x4* const sm_o = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+        for (uint32_t half = 2; half >= 1; half /= 2) {
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int t = 0; t < NQ; t++)
+#pragma unroll
+                    for (int d = 0; d < DT; d++) sm_o[((wave - half) * NQ * DT + t * DT + d) * 64 + lane] = w.o[t][d];
+            }
+            __syncthreads();
+            if (wave < half) {
+#pragma unroll
+                for (int t = 0; t < NQ; t++)
+#pragma unroll
+                    for (int d = 0; d < DT; d++) w.o[t][d] += sm_o[(wave * NQ * DT + t * DT + d) * 64 + lane];
+            }
+            __syncthreads();
+        }
+        if (wave == 0) w.store(a, sh, r, head, tile_row, tile_row, rows, ROWS, alone, lane);
+        __syncthreads();  // the LDS is the next unit's
+    }
+}
+
+// Many rows (64 NQ): every wave holds its own and all take the same positions, 64
+// at a time.  The waves decode a quarter of the tile each and leave the operands
+// in LDS for all, one tile ahead; the codes of the tile after that are on their
+// way into registers.  A step of few rows spends two fifths of its vector
+// instructions on decoding; here that is shared by four waves.
+constexpr uint32_t kWideTile = 64;
+
+template <int D, int KB, int VB, int NQ, bool F32>
+__global__ __launch_bounds__(256, D < 256 ? 2 : 1) void attend_wide_kernel(AttnArgs a) {
+    constexpr int NB = D / 32, DT = D / 16, PAIRS = D / 64, ODD = NB % 2;
+    constexpr uint32_t ROWS = 64u * NQ;
+    constexpr uint32_t RB = D * KB / 8;                  // bytes of a key
+    constexpr uint32_t KF = 0, VF = 4 * NB * 1024;       // operands: [S][block][lane], [half][dims][lane]
+    constexpr uint32_t KS = VF + 2 * DT * 1024, VS = KS + 64 * NB * 4, BUF = VS + 256;  // scales in f32
+    constexpr int KU = PAIRS, VU = (DT + 3) / 4;         // units of a wave: (S = wave, pair), 16 dims
+    __shared__ __align__(16) uint8_t lds[2 * BUF];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    Share sh = a.shares == 0 ? whole_unit(a, ROWS) : share_of(a, ROWS, lds);
+    for (; sh.places != 0; sh.next(a, ROWS)) {
+        const uint32_t now0 = sh.first_step(), now1 = sh.end_step();
+        if (now0 >= now1) continue;
+        const uint32_t seq = sh.seq, head = sh.unit / sh.row_tiles, tile_row = sh.unit % sh.row_tiles * ROWS;
+        const uint32_t first_row = tile_row + wave * (16u * NQ);
+        const SeqRange r = seq_range(a.b, seq);
+        const uint32_t rows = r.n * a.group;
+        const uint64_t total = (uint64_t)r.len + r.n;
+        const bool alone = now0 == 0 && now1 == sh.unit_steps;
+        const uint32_t tile0 = now0 * (kStep / kWideTile);
+        const uint32_t ends = (uint32_t)((min(total, (uint64_t)now1 * kStep) + kWideTile - 1) / kWideTile);
+        const uint32_t count = ends - tile0;
+        const Pages page_of(a, seq);
+
+        int32_t ids[4];  // of the next tile to load
+        auto look_up = [&](uint32_t k) {
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++) ids[c] = page_of(4 * (tile0 + k) + c);
+        };
+        // A tile's codes, this wave's quarter: keys of S number `wave` (row m of S number s
+        // is position 16 (m / 4) + 4 s + m % 4), values of 16 dims and all positions (lane
+        // group g holds 16g..16g+15), wave 0 the keys' scales, wave 1 the values'.
+        u32x4 kr[KU], vr[VU], sr;
+        u32x2 ko;
+        uint32_t absent_raw = 0;  // four bits: chunks of the tile in registers that are not there
+        auto load = [&](uint32_t k) {
+            uint32_t ln = lane;
+            asm volatile("" : "+v"(ln));
+            const uint32_t g = ln >> 4, col = ln & 15u;
+            uint64_t slot[4];
+            absent_raw = 0;
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++) {
+                const bool ok = ids[c] >= 0 && (uint64_t)(uint32_t)ids[c] < a.kv.pages;
+                slot[c] = ok ? chunk_slot(a.kv, ids[c], head, 4 * (tile0 + k) + c) : 0;
+                absent_raw |= ok ? 0u : 1u << c;
+            }
+            auto pick = [&](uint32_t i) {
+                const uint64_t x = i & 1u ? slot[1] : slot[0], y = i & 1u ? slot[3] : slot[2];
+                return i & 2u ? y : x;
+            };
+            const uint8_t* p = a.kv.k + (pick(col >> 2) + 4 * wave + (col & 3u)) * RB;
+#pragma unroll
+            for (int j = 0; j < KU; j++) {
+                if constexpr (KB == 8) {
+                    kr[j] = *gptr<u32x4>(p + 64 * j + 16 * g);
+                } else {
+                    const u32x2 x = *gptr<u32x2>(p + 32 * j + 8 * g);
+                    kr[j].x = x.x, kr[j].y = x.y;
+                }
+            }
+            if constexpr (ODD) {
+                if constexpr (KB == 8) ko = *gptr<u32x2>(p + 64 * PAIRS + 8 * g);
+                else ko.x = *gptr<uint32_t>(p + 32 * PAIRS + 4 * g);
+            }
+            const uint8_t* q = a.kv.v + pick(g) * (D * VB / 8) + col * (2 * VB);
+#pragma unroll
+            for (int j = 0; j < VU; j++) {
+                const uint32_t d = wave + 4 * j;
+                if (DT % 4 == 0 || d < (uint32_t)DT) {
+                    if constexpr (VB == 8) {
+                        vr[j] = *gptr<u32x4>(q + 256 * d);
+                    } else {
+                        const u32x2 x = *gptr<u32x2>(q + 128 * d);
+                        vr[j].x = x.x, vr[j].y = x.y;
                     }
                 }
             }
-            if (a.lse && g == 0) gptr_mut<float>(a.lse)[token * q_heads + h] = (m[t] + log2f(l[t])) * 0.69314718055994531f;
+            if (wave == 0) {
+                if (ln < 8u * NB)
+                    sr = *gptr<u32x4>(a.kv.k + a.kv.k_scales + pick(ln / (2 * NB)) * (2 * NB) + ln % (2 * NB) * 16);
+            } else if (wave == 1) {
+                if (ln < 8) sr = *gptr<u32x4>(a.kv.v + a.kv.v_scales + pick(ln >> 1) * 2 + 16 * (ln & 1u));
+            }
+        };
+        // those codes as operands into a buffer
+        auto decode = [&](uint8_t* buf) {
+            uint32_t ln = lane;
+            asm volatile("" : "+v"(ln));
+            f16x8* const kf = reinterpret_cast<f16x8*>(buf + KF + wave * (NB * 1024)) + ln;
+#pragma unroll
+            for (int j = 0; j < KU; j++) {
+                if constexpr (KB == 8) {
+                    kf[64 * (2 * j)] = k_frag(kr[j].x, kr[j].y);
+                    kf[64 * (2 * j + 1)] = k_frag(kr[j].z, kr[j].w);
+                } else {
+                    kf[64 * (2 * j)] = k_frag((kr[j].x << 4) & 0xF0F0F0F0u, kr[j].x & 0xF0F0F0F0u);
+                    kf[64 * (2 * j + 1)] = k_frag((kr[j].y << 4) & 0xF0F0F0F0u, kr[j].y & 0xF0F0F0F0u);
+                }
+            }
+            if constexpr (ODD) {
+                if constexpr (KB == 8) kf[64 * (NB - 1)] = k_frag(ko.x, ko.y);
+                else kf[64 * (NB - 1)] = k_frag((ko.x << 4) & 0xF0F0F0F0u, ko.x & 0xF0F0F0F0u);
+            }
+            bf16x8* const vf = reinterpret_cast<bf16x8*>(buf + VF) + ln;
+#pragma unroll
+            for (int j = 0; j < VU; j++) {
+                const uint32_t d = wave + 4 * j;
+                if (DT % 4 == 0 || d < (uint32_t)DT) {
+                    if constexpr (VB == 8) {
+                        vf[64 * d] = v_frag(vr[j].x, vr[j].y);
+                        vf[64 * (DT + d)] = v_frag(vr[j].z, vr[j].w);
+                    } else {
+                        vf[64 * d] = v_frag((vr[j].x << 4) & 0xF0F0F0F0u, vr[j].x & 0xF0F0F0F0u);
+                        vf[64 * (DT + d)] = v_frag((vr[j].y << 4) & 0xF0F0F0F0u, vr[j].y & 0xF0F0F0F0u);
+                    }
+                }
+            }
+            if (ln < (wave == 0 ? 8u * NB : wave == 1 ? 8u : 0u)) {
+                f32x4* const to = reinterpret_cast<f32x4*>(buf + (wave == 0 ? KS : VS) + 32 * ln);
+                to[0] = f32x4{bf16_of(sr.x, 0), bf16_of(sr.x, 1), bf16_of(sr.y, 0), bf16_of(sr.y, 1)};
+                to[1] = f32x4{bf16_of(sr.z, 0), bf16_of(sr.z, 1), bf16_of(sr.w, 0), bf16_of(sr.w, 1)};
+            }
+        };
+
+        look_up(0);
+        load(0);
+        if (1 < count) look_up(1);
+        WaveRows<D, KB, VB, NQ, F32> w;
+        w.load(a, r, head, first_row, rows, lane);
+        decode(lds);
+        uint32_t absent = absent_raw;  // of the tile being worked on
+        if (1 < count) {
+            load(1);
+            if (2 < count) look_up(2);
+        }
+        __syncthreads();
+        for (uint32_t k = 0; k < count; k++) {
+            const uint32_t p0 = (tile0 + k) * kWideTile;
+            const uint8_t* const buf = lds + (k & 1u) * BUF;
+            const uint32_t gone = absent;
+            if (k + 1 < count) {
+                decode(lds + ((k + 1) & 1u) * BUF);
+                absent = absent_raw;
+                if (k + 2 < count) {
+                    load(k + 2);
+                    if (k + 3 < count) look_up(k + 3);
+                }
+            }
+            if (first_row < rows) {
+#pragma unroll 1
+                for (uint32_t c = 0; c < 2; c++) {
+                    uint32_t ln = lane;
+                    asm volatile("" : "+v"(ln));
+                    const uint32_t g = ln >> 4;
+                    const bool masked = gone != 0 || (uint64_t)p0 + kWideTile > r.len;
+                    uint32_t vis[NQ] = {};
+                    if (masked) {
+#pragma unroll
+                        for (int t = 0; t < NQ; t++)
+                            vis[t] = gone >> g & 1u ? 0u
+                                                    : sees(a.mask, a.mask_words, r.row0 + w.tok[t], w.tok[t], r.n,
+                                                           (int64_t)p0 + 16 * g + 8 * c - (int64_t)r.len);
+                    }
+                    w.step(OperandTile<D>{reinterpret_cast<const f16x8*>(buf + KF) + 2 * c * NB * 64 + ln,
+                                          reinterpret_cast<const bf16x8*>(buf + VF) + c * DT * 64 + ln,
+                                          reinterpret_cast<const float*>(buf + KS) + (16 * g + 8 * c) * NB,
+                                          reinterpret_cast<const float*>(buf + VS) + 16 * g + 8 * c},
+                           masked, vis);
+                }
+            }
+            __syncthreads();
+        }
+        if (first_row < rows) {
+#pragma unroll
+            for (int t = 0; t < NQ; t++) {
+                w.l[t] = rows_sum(w.l[t]);
+                w.m[t] = w.l[t] == 0.0f ? -__builtin_inff() : w.m[t] == -__builtin_inff() ? 0.0f : w.m[t];
+            }
+            w.store(a, sh, r, head, tile_row, first_row, rows, ROWS, alone, lane);
         }
     }
 }
@@ -599,19 +1082,19 @@ hipError_t attend_launch(const AttnArgs& a, uint32_t tiles, uint64_t grid, hipSt
 template <int D, int KB, int VB>
 hipError_t attend_launch_dim(const AttnArgs& a, uint32_t tiles, uint64_t grid, hipStream_t st) {
     const dim3 gd((uint32_t)grid), bd(64 * kWaves);
-    if (!a.q.bf16) {
-        if (tiles == 1) {
-            attend_kernel<D, KB, VB, 1, true><<<gd, bd, 0, st>>>(a);
-        } else {
-            if constexpr (D <= 128) attend_kernel<D, KB, VB, 2, true><<<gd, bd, 0, st>>>(a);
+    if (tiles >= 4) {  // 64 or 128 rows
+        if (!a.q.bf16) attend_wide_kernel<D, KB, VB, 1, true><<<gd, bd, 0, st>>>(a);
+        else if (tiles == 4) attend_wide_kernel<D, KB, VB, 1, false><<<gd, bd, 0, st>>>(a);
+        else {
+            if constexpr (D <= 128) attend_wide_kernel<D, KB, VB, 2, false><<<gd, bd, 0, st>>>(a);
             else return hipErrorInvalidValue;
         }
+    } else if (!a.q.bf16) {
+        attend_kernel<D, KB, VB, 1, true><<<gd, bd, 0, st>>>(a);
     } else if (tiles == 1) {
         attend_kernel<D, KB, VB, 1, false><<<gd, bd, 0, st>>>(a);
-    } else if (tiles == 2) {
-        attend_kernel<D, KB, VB, 2, false><<<gd, bd, 0, st>>>(a);
     } else {
-        if constexpr (D <= 128) attend_kernel<D, KB, VB, 4, false><<<gd, bd, 0, st>>>(a);
+        if constexpr (D <= 128) attend_kernel<D, KB, VB, 2, false><<<gd, bd, 0, st>>>(a);
         else return hipErrorInvalidValue;
     }
     return hipGetLastError();

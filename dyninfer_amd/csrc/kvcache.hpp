@@ -84,25 +84,26 @@ hipError_t kv_commit_launch(const KvView& kv, const KvBatch& b, const int32_t* p
 
 // Attention: how a call is cut (host), its workspace and its launch.
 struct AttnPlan {
-    uint32_t tiles;      // 16-row tiles a workgroup holds (1, 2 or 4)
-    uint32_t row_tiles;  // workgroups along a sequence's rows
-    uint32_t splits;     // workgroups along its positions
-    uint32_t span;       // positions of each but the last
-    uint64_t bytes;      // workspace
+    uint32_t tiles;      // 16-row tiles a workgroup holds: 1 or 2 by every wave, 4 or 8 by four waves
+    uint32_t row_tiles;  // of the sequence with the most rows
+    uint32_t shares;     // equal pieces of all units' steps, a workgroup each; 0: a unit each
+    uint64_t grid;
+    uint64_t bytes, stats, where;  // workspace, and where its parts begin
 };
 AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint32_t q_heads, bool bf16);
-uint64_t attn_blocks(const AttnPlan& plan, uint32_t heads, uint32_t seqs);
 struct AttnArgs {
     KvView kv;
     KvBatch b;
     KvRows q, out;
     const int64_t* mask;
     float* lse;
-    float* work;
-    uint32_t mask_words, group, row_tiles, splits, span;
+    float* parts;     // [share + unit][row of the tile][dim], not yet over their sums
+    float* stats;     // [share + unit][row of the tile][2]: what exponents are from, sum
+    uint64_t* where;  // [sequence][2]: steps and units before it; then all steps
+    uint32_t mask_words, group, row_tiles, shares;
     float scale;
 };
-hipError_t attn_launch(const AttnArgs& a, const AttnPlan& plan, hipStream_t st);
+hipError_t attn_launch(AttnArgs a, const AttnPlan& plan, uint8_t* work, hipStream_t st);
 
 struct VerifyArgs {
     const void* logits;

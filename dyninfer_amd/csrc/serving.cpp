@@ -79,6 +79,7 @@ int check_batch(const dyninfer_kvbatch_t* b, bool tables, dmx::KvBatch& out) {
     }
     if (b->tokens > 0x7FFFFFFFu || b->max_new > b->tokens)
         return fail(BAD, "batch: max_new must not be above tokens, nor tokens above 2^31 - 1");
+    if (b->sequences > (1u << 24)) return fail(UNSUPPORTED, "batch: more than 2^24 sequences; split the call");
     if (b->max_length > 0x7FFFFFFFull) return fail(UNSUPPORTED, "batch: sequences are limited to 2^31 - 1 positions");
     out = {b->page_table, b->lengths, b->starts, b->sequences, b->table_pages, b->tokens, b->max_new};
     return 0;
@@ -360,22 +361,16 @@ int dyninfer_mi355x_tree_attention(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kv
     if ((uint64_t)a.b.max_new * a.group > 0x7FFFFFFFull) return fail(UNSUPPORTED, "too many rows of one kv head");
     const dmx::AttnPlan plan = dmx::attn_plan(a.kv, a.b, batch->max_length, q->heads, a.q.bf16);
     if (int rc = check_workspace(workspace, workspace_bytes, plan.bytes, "tree_attention")) return rc;
-    if ((uint64_t)a.b.seqs * plan.splits > kMaxGrid || (uint64_t)plan.row_tiles * a.kv.heads > kMaxGrid)
-        return check_grid(~0ull);
-    if (int rc = check_grid(dmx::attn_blocks(plan, a.kv.heads, a.b.seqs))) return rc;
+    if (int rc = check_grid(plan.grid)) return rc;
     if (int rc = check_grid((uint64_t)a.b.seqs * a.b.max_new / 4)) return rc;
     if (int rc = check_grid((uint64_t)a.b.seqs * a.b.max_new * q->heads / 4)) return rc;
     a.mask = mask;
     a.mask_words = mask_words;
     a.lse = lse;
-    a.work = static_cast<float*>(workspace);
-    a.row_tiles = plan.row_tiles;
-    a.splits = plan.splits;
-    a.span = plan.span;
     a.scale = scale;
     DeviceGuard g(ctx->device);
     if (g.err != hipSuccess) return hip_fail(g.err, "hipSetDevice");
-    return launched(dmx::attn_launch(a, plan, static_cast<hipStream_t>(stream)));
+    return launched(dmx::attn_launch(a, plan, static_cast<uint8_t*>(workspace), static_cast<hipStream_t>(stream)));
 }
 
 int dyninfer_mi355x_draft_verify_workspace_bytes(uint32_t sequences, uint32_t tokens, uint32_t vocab, uint32_t max_new,
