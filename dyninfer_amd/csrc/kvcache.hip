@@ -158,43 +158,56 @@ __global__ __launch_bounds__(256) void rope_kernel(KvRows x, KvRows y, uint32_t 
     rope_row<D>(x, y, (uint32_t)(i / heads), (uint32_t)(i % heads), threadIdx.x % L, rp);
 }
 
-// Largest value of the N lanes around this one (N a power of two, aligned).
+// Largest of the N lanes around this one (N a power of two, aligned), by moves
+// within rows of 16 lanes.
 template <int N>
-__device__ __forceinline__ float lanes_max(float x) {
-#pragma unroll
-    for (int m = 1; m < N; m *= 2) x = fmaxf(x, __shfl_xor(x, m));
+__device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, true));   // lane ^ 1
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true));   // lane ^ 2
+    if (N > 4) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xF, 0xF, true));  // mirrored in 8
+    if (N > 8) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xF, 0xF, true));  // mirrored in 16
+    if (N > 16) x = max(x, (uint32_t)__shfl_xor((int)x, 16));
     return x;
 }
 
 // A block's scale and this lane's eight codes of it.  N lanes hold the block;
-// a lane without dims passes zeros.
+// a lane without dims passes zeros.  Magnitudes are compared as the whole numbers
+// their bits are, which puts infinities and NaN on top.
 template <int BITS, int N>
 __device__ __forceinline__ uint16_t quantize(const float (&x)[8], int32_t (&c)[8]) {
-    float top = 0.0f, low = 0.0f;
-    uint32_t big = 0;
+    uint32_t top = 0, low = 0;  // of the positive and of the negative values (8 bits: of all)
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        top = fmaxf(top, x[i]);
-        low = fmaxf(low, -x[i]);
-        big = max(big, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+        const uint32_t u = __float_as_uint(x[i]);
+        if (BITS == 8) {
+            top = max(top, u & 0x7FFFFFFFu);
+        } else {
+            top = max(top, u >> 31 ? 0u : u);
+            low = max(low, u >> 31 ? u & 0x7FFFFFFFu : 0u);
+        }
     }
     top = lanes_max<N>(top);
-    low = lanes_max<N>(low);
-#pragma unroll
-    for (int m = 1; m < N; m *= 2) big = max(big, (uint32_t)__shfl_xor((int)big, m));
-    if (big >= 0x7F800000u) {  // an infinity or a NaN: the block reads back as NaN
+    if (BITS == 4) low = lanes_max<N>(low);
+    if (max(top, low) >= 0x7F800000u) {  // an infinity or a NaN: the block reads back as NaN
 #pragma unroll
         for (int i = 0; i < 8; i++) c[i] = 0;
         return 0x7FC0u;
     }
-    const float d = BITS == 8 ? fmaxf(top, low) / 127.0f : (top > low ? top : -low) / -8.0f;
+    const float d = BITS == 8 ? __uint_as_float(top) / 127.0f
+                              : (top > low ? __uint_as_float(top) : -__uint_as_float(low)) / -8.0f;
     const uint16_t bits = f32_to_bf16_bits(d);
     const float s = bf16_bits_to_f32(bits);
+    // x / s, correctly rounded: with r the correctly rounded reciprocal, one step from
+    // x r is (Markstein), as long as nothing leaves the range of normal numbers
+    const bool plain = fabsf(s) >= 0x1p-100f && fabsf(s) <= 0x1p100f;
+    const float r = 1.0f / (plain ? s : 1.0f);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
+        float q = x[i] * r;
+        q = __builtin_fmaf(__builtin_fmaf(-q, s, x[i]), r, q);
+        if (!plain) q = s == 0.0f ? 0.0f : x[i] / s;
         // the rounded scale may be a little small: the largest code is clamped
-        const float q = s == 0.0f ? 0.0f : rintf(x[i] / s);
-        c[i] = (int32_t)fminf(fmaxf(q, BITS == 8 ? -127.0f : -8.0f), BITS == 8 ? 127.0f : 7.0f);
+        c[i] = (int32_t)fminf(fmaxf(rintf(q), BITS == 8 ? -127.0f : -8.0f), BITS == 8 ? 127.0f : 7.0f);
     }
     return bits;
 }
@@ -205,43 +218,88 @@ __device__ __forceinline__ uint32_t k_place(uint32_t b, uint32_t t) {
     return (b / 2) * 64 + ((b | 1u) * 32 < D ? t * 16 + (b & 1) * 8 : t * 8);
 }
 
-// Grid: `kv_blocks` workgroups for the keys, one per (sequence, chunk of 16
-// positions, head), as many for the values, then the queries' rows.  A chunk is
-// one workgroup's alone, so values of 4 bits, two tokens to a byte, are merged
-// without atomics.
+// A workgroup of the append and read kernels takes a chunk of 16 positions of
+// some heads; a thread has 8 dims of 4 of its tokens, whose loads are in flight
+// together.  For values, which lie [dim][token], that is one dword a dim (8 bits),
+// turned in registers: through LDS, byte by byte, 8 x 16k tokens of 8 heads took
+// 192 us to read, with 4 heads a workgroup 282, this way 133 (a copy of their bytes: 140).
+template <int D>
+constexpr uint32_t kHeads = 64 / kLanes<D>;
+template <int D>
+constexpr uint32_t kKeyHeads = kLanes<D> == 8 ? 2 : 1;  // of the append's keys
+
+struct Chunk {
+    SeqRange r;
+    uint64_t pos0;      // of its token 0
+    int64_t page;       // -1: absent
+    uint64_t slot;      // of this thread's head and token 0
+    uint32_t c, h;      // chunk, head
+    uint32_t lo, hi;    // tokens lo..hi-1 are the call's
+    bool live;          // the head exists
+
+    __device__ __forceinline__ uint32_t row(uint32_t t) const { return r.row0 + (uint32_t)(pos0 + t - r.len); }
+    __device__ __forceinline__ bool has(uint32_t t) const { return live && t >= lo && t < hi; }
+    // a token of the call near t, for loads that need not be switched off
+    __device__ __forceinline__ uint32_t near(uint32_t t) const { return min(max(t, lo), hi - 1); }
+};
+
+// Workgroup blk of (sequence, chunk, HEADS heads), its head number `which`; false:
+// nothing of the call is there.
+template <uint32_t HEADS>
+__device__ __forceinline__ bool find_chunk(const KvView& kv, const KvBatch& b, uint32_t blk, uint32_t chunks, uint32_t which,
+                                           Chunk& c) {
+    const uint32_t groups = (kv.heads + HEADS - 1) / HEADS;
+    c.h = blk % groups * HEADS + which;
+    c.live = c.h < kv.heads;
+    const uint32_t rest = blk / groups, seq = rest / chunks;
+    c.r = seq_range(b, seq);
+    c.c = c.r.len / 16 + rest % chunks;
+    c.pos0 = 16ull * c.c;
+    if (c.r.n == 0 || c.pos0 >= (uint64_t)c.r.len + c.r.n) return false;
+    c.lo = c.r.len > c.pos0 ? (uint32_t)(c.r.len - c.pos0) : 0u;
+    c.hi = (uint32_t)min((uint64_t)16, (uint64_t)c.r.len + c.r.n - c.pos0);
+    c.page = chunk_page(kv, b, seq, c.c);
+    c.slot = c.page < 0 ? 0 : chunk_slot(kv, c.page, c.live ? c.h : 0, c.c);
+    return true;
+}
+
+// Bytes i of four dwords as one dword each: x[j] byte i -> x[i] byte j.
+__device__ __forceinline__ void turn4(uint32_t (&x)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), b = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
+    const uint32_t c = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u), d = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+    x[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+    x[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    x[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+    x[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+// Grid: `k_blocks` workgroups for the keys, one per (sequence, chunk, 256 / lanes
+// of a row / 16 heads), a thread 8 dims of one token; `v_blocks` for the values,
+// one per (sequence, chunk, kHeads heads); then the queries' rows.  A chunk of a
+// head's values is one wave's alone, so values of 4 bits, two tokens to a byte, are
+// merged without atomics.  (Keys by four tokens a thread: 220 registers, the whole
+// launch over 4 x 2048 tokens 86 us instead of 37.)
 template <int D, int KB, int VB>
 __global__ __launch_bounds__(256) void append_kernel(KvView kv, KvBatch b, KvRows k, KvRows v, RopeView rp, KvRows q,
-                                                     KvRows q_out, uint32_t q_heads, uint32_t chunks,
-                                                     uint32_t kv_blocks) {
+                                                     KvRows q_out, uint32_t q_heads, uint32_t chunks, uint32_t k_blocks,
+                                                     uint32_t v_blocks) {
     constexpr uint32_t L = kLanes<D>, ROWS = 256 / L;
-    const uint32_t lane = threadIdx.x % L, slot = threadIdx.x / L;
+    const uint32_t lane = threadIdx.x % L, d0 = 8 * lane;
     uint32_t blk = blockIdx.x;
-    if (blk >= 2 * kv_blocks) {
-        const uint64_t i = (uint64_t)(blk - 2 * kv_blocks) * ROWS + slot;
+    if (blk >= k_blocks + v_blocks) {
+        const uint64_t i = (uint64_t)(blk - k_blocks - v_blocks) * ROWS + threadIdx.x / L;
         if (i < (uint64_t)b.tokens * q_heads)
             rope_row<D>(q, q_out, (uint32_t)(i / q_heads), (uint32_t)(i % q_heads), lane, rp);
         return;
     }
-    const bool keys = blk < kv_blocks;
-    if (!keys) blk -= kv_blocks;
-    const uint32_t head = blk % kv.heads, rest = blk / kv.heads;
-    const uint32_t seq = rest / chunks;
-    const SeqRange r = seq_range(b, seq);
-    const uint32_t c = r.len / 16 + rest % chunks;
-    const uint64_t pos0 = 16ull * c;
-    if (r.n == 0 || pos0 >= (uint64_t)r.len + r.n) return;
-    const int64_t page = chunk_page(kv, b, seq, c);
-    if (page < 0) return;
-    const uint64_t s0 = chunk_slot(kv, page, head, c);
-    // the chunk's tokens lo..hi-1 are new; token t is row row0 + (pos0 + t - len)
-    const uint32_t lo = r.len > pos0 ? (uint32_t)(r.len - pos0) : 0u;
-    const uint32_t hi = (uint32_t)min((uint64_t)16, (uint64_t)r.len + r.n - pos0);
-    const uint32_t d0 = 8 * lane;
-    if (keys) {
-        for (uint32_t t = slot; t < 16; t += ROWS) {
-            if (t < lo || t >= hi) continue;  // whole rows leave together: the shuffles stay within a row
-            const uint32_t token = r.row0 + (uint32_t)(pos0 + t - r.len);
-            const int64_t row = (int64_t)token * k.ts + (int64_t)head * k.hs;
+    Chunk c;
+    if (blk < k_blocks) {
+        constexpr uint32_t HEADS = kKeyHeads<D>;
+        if (!find_chunk<HEADS>(kv, b, blk, chunks, threadIdx.x / L / 16, c) || c.page < 0) return;
+        for (uint32_t t = threadIdx.x / L % 16; t < 16; t += ROWS) {
+            if (!c.has(t)) continue;  // whole rows leave together: the shuffles stay within a row
+            const uint32_t token = c.row(t);
+            const int64_t row = (int64_t)token * k.ts + (int64_t)c.h * k.hs;
             float x[8] = {};
             if (d0 < D) {
                 load8(k, row + d0, x);
@@ -250,134 +308,140 @@ __global__ __launch_bounds__(256) void append_kernel(KvView kv, KvBatch b, KvRow
             int32_t code[8];
             const uint16_t sc = quantize<KB, 4>(x, code);
             if (d0 >= D) continue;
-            const uint32_t blk32 = lane / 4, part = lane % 4, at = k_place<D>(blk32, part);
+            const uint32_t blk32 = lane / 4, part = lane % 4, in_row = k_place<D>(blk32, part);
+            const uint64_t at = c.slot + t;
             if constexpr (KB == 8) {
                 u32x2 w = {0, 0};
 #pragma unroll
-                for (int i = 0; i < 8; i++) w[i / 4] |= (uint32_t)(code[i] + 128) << (8 * (i % 4));
-                *gptr_mut<u32x2>(kv.k + (s0 + t) * D + at) = w;
+                for (int j = 0; j < 8; j++) w[j / 4] |= (uint32_t)(code[j] + 128) << (8 * (j % 4));
+                *gptr_mut<u32x2>(kv.k + at * D + in_row) = w;
             } else {
                 uint32_t w = 0;
 #pragma unroll
-                for (int i = 0; i < 8; i++) w |= (uint32_t)(code[i] + 8) << (8 * (i % 4) + 4 * (i / 4));
-                *gptr_mut<uint32_t>(kv.k + (s0 + t) * (D / 2) + at / 2) = w;
+                for (int j = 0; j < 8; j++) w |= (uint32_t)(code[j] + 8) << (8 * (j % 4) + 4 * (j / 4));
+                *gptr_mut<uint32_t>(kv.k + at * (D / 2) + in_row / 2) = w;
             }
-            if (part == 0) gptr_mut<uint16_t>(kv.k + kv.k_scales)[(s0 + t) * (D / 32) + blk32] = sc;
+            if (part == 0) gptr_mut<uint16_t>(kv.k + kv.k_scales)[at * (D / 32) + blk32] = sc;
         }
         return;
     }
-    __shared__ uint8_t sm[D * 16];  // [dim][token]
-    for (uint32_t t = slot; t < 16; t += ROWS) {
-        if (t < lo || t >= hi) continue;
-        const uint32_t token = r.row0 + (uint32_t)(pos0 + t - r.len);
-        float x[8] = {};
-        if (d0 < D) load8(v, (int64_t)token * v.ts + (int64_t)head * v.hs + d0, x);
-        int32_t code[8];
-        const uint16_t sc = quantize<VB, (int)L>(x, code);
-        if (d0 < D) {
+    const uint32_t which = threadIdx.x / L, quad = which % 4, t0 = 4 * quad;
+    if (!find_chunk<kHeads<D>>(kv, b, blk - k_blocks, chunks, which / 4, c) || c.page < 0) return;
+    float x[4][8] = {};
+    if (d0 < D) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) sm[(d0 + i) * 16 + t] = (uint8_t)code[i];
-        }
-        if (lane == 0) gptr_mut<uint16_t>(kv.v + kv.v_scales)[s0 + t] = sc;
+        for (uint32_t t = 0; t < 4; t++)
+            load8(v, (int64_t)c.row(c.near(t0 + t)) * v.ts + (int64_t)(c.live ? c.h : 0) * v.hs + d0, x[t]);
     }
-    __syncthreads();
-    const uint32_t dim = threadIdx.x;
-    if (dim >= D) return;
-    const u32x4 w = *reinterpret_cast<const u32x4*>(sm + dim * 16);
-    if constexpr (VB == 8) {
-        uint8_t* dst = kv.v + s0 * D + dim * 16;
-        if (lo == 0 && hi == 16) {
-            *gptr_mut<u32x4>(dst) = w;
-        } else {
+    int32_t code[4][8];
+    uint16_t sc[4];
+    uint32_t mask = 0;  // bytes of the tokens that are the call's
 #pragma unroll
-            for (uint32_t t = 0; t < 16; t++)
-                if (t >= lo && t < hi) gptr_mut<uint8_t>(dst)[t] = (uint8_t)(w[t / 4] >> (8 * (t % 4)));
+    for (uint32_t t = 0; t < 4; t++) {
+        sc[t] = quantize<VB, (int)L>(x[t], code[t]);
+        if (!c.has(t0 + t)) continue;
+        mask |= 255u << (8 * t);
+        if (lane == 0) gptr_mut<uint16_t>(kv.v + kv.v_scales)[c.slot + t0 + t] = sc[t];
+    }
+    if constexpr (VB == 8) {
+        if (d0 >= D) return;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t w = (code[0][j] & 255u) | (code[1][j] & 255u) << 8 | (code[2][j] & 255u) << 16 | (uint32_t)code[3][j] << 24;
+            uint8_t* dst = kv.v + c.slot * D + (d0 + j) * 16 + t0;
+            if (mask == ~0u) {
+                *gptr_mut<uint32_t>(dst) = w;
+            } else {
+#pragma unroll
+                for (uint32_t t = 0; t < 4; t++)
+                    if (mask >> (8 * t) & 1u) gptr_mut<uint8_t>(dst)[t] = (uint8_t)(w >> (8 * t));
+            }
         }
     } else {
-        // dword j: tokens 8j..8j+3 in the low nibbles, 8j+4..8j+7 in the high ones
-        u32x2 x;
+        // even quads take the low nibbles of a dword, odd ones, L lanes on, the high
+        // ones; the even quad's lane writes both
+        const uint32_t other = __shfl_xor((int)mask, (int)L);
+        const uint32_t all = (mask & 0x0F0F0F0Fu) | (other & 0xF0F0F0F0u);
 #pragma unroll
-        for (int j = 0; j < 2; j++) x[j] = (w[2 * j] & 0x0F0F0F0Fu) | ((w[2 * j + 1] & 0x0F0F0F0Fu) << 4);
-        uint8_t* dst = kv.v + s0 * (D / 2) + dim * 8;
-        if (lo != 0 || hi != 16) {
-            const u32x2 old = *gptr<u32x2>(dst);
-            u32x2 m = {0, 0};
-#pragma unroll
-            for (uint32_t t = 0; t < 16; t++)
-                if (t >= lo && t < hi) m[t / 8] |= 15u << (8 * (t % 4) + 4 * (t % 8 / 4));
-            x = (x & m) | (old & ~m);
+        for (int j = 0; j < 8; j++) {
+            const uint32_t w = (code[0][j] & 15u) | (code[1][j] & 15u) << 8 | (code[2][j] & 15u) << 16 | (code[3][j] & 15u) << 24;
+            const uint32_t hi = __shfl_xor((int)w, (int)L);
+            if (d0 >= D || quad % 2 || all == 0) continue;
+            uint32_t* dst = reinterpret_cast<uint32_t*>(kv.v + c.slot * (D / 2) + (d0 + j) * 8 + t0 / 2);
+            uint32_t y = w | hi << 4;
+            if (all != ~0u) y = (y & all) | (*gptr<uint32_t>(dst) & ~all);
+            *gptr_mut<uint32_t>(dst) = y;
         }
-        *gptr_mut<u32x2>(dst) = x;
     }
 }
 
-// One workgroup per (sequence, chunk of 16 positions, head), keys then values.
+// One workgroup per (sequence, chunk, kHeads heads), keys then values.
 template <int D, int KB, int VB>
 __global__ __launch_bounds__(256) void read_kernel(KvView kv, KvBatch b, KvRows k, KvRows v, uint32_t chunks,
                                                    uint32_t kv_blocks) {
-    constexpr uint32_t L = kLanes<D>, ROWS = 256 / L;
-    const uint32_t lane = threadIdx.x % L, slot = threadIdx.x / L;
+    constexpr uint32_t L = kLanes<D>;
+    const uint32_t lane = threadIdx.x % L, d0 = 8 * lane;
     uint32_t blk = blockIdx.x;
     const bool keys = k.p != nullptr && blk < kv_blocks;
     if (k.p != nullptr && !keys) blk -= kv_blocks;
-    const uint32_t head = blk % kv.heads, rest = blk / kv.heads;
-    const uint32_t seq = rest / chunks;
-    const SeqRange r = seq_range(b, seq);
-    const uint32_t c = r.len / 16 + rest % chunks;
-    const uint64_t pos0 = 16ull * c;
-    if (r.n == 0 || pos0 >= (uint64_t)r.len + r.n) return;
-    const int64_t page = chunk_page(kv, b, seq, c);
-    const uint64_t s0 = page < 0 ? 0 : chunk_slot(kv, page, head, c);
-    const uint32_t lo = r.len > pos0 ? (uint32_t)(r.len - pos0) : 0u;
-    const uint32_t hi = (uint32_t)min((uint64_t)16, (uint64_t)r.len + r.n - pos0);
-    const uint32_t d0 = 8 * lane;
-    __shared__ uint8_t sm[D * 16];  // [dim][token]
-    if (!keys && page >= 0) {
-        const uint32_t dim = threadIdx.x;
-        if (dim < D) {
-            u32x4 w;
-            if constexpr (VB == 8) {
-                w = *gptr<u32x4>(kv.v + s0 * D + dim * 16);
-            } else {
-                const u32x2 x = *gptr<u32x2>(kv.v + s0 * (D / 2) + dim * 8);
+    const uint32_t which = threadIdx.x / L, quad = which % 4, t0 = 4 * quad;
+    Chunk c;
+    if (!find_chunk<kHeads<D>>(kv, b, blk, chunks, which / 4, c) || d0 >= D || !c.live) return;
+    float x[4][8], s[4];
+    if (c.page < 0) {
 #pragma unroll
-                for (int j = 0; j < 2; j++) {  // nibble n (signed) as a byte: (n ^ 8) - 8, bytewise
-                    const uint32_t a = x[j] & 0x0F0F0F0Fu, h = (x[j] >> 4) & 0x0F0F0F0Fu;
-                    w[2 * j] = a | ((a & 0x08080808u) * 30u);  // bit 3 set: bits 4..7 too
-                    w[2 * j + 1] = h | ((h & 0x08080808u) * 30u);
-                }
-            }
-            *reinterpret_cast<u32x4*>(sm + dim * 16) = w;
-        }
-        __syncthreads();
-    }
-    for (uint32_t t = slot; t < 16; t += ROWS) {
-        if (t < lo || t >= hi || d0 >= D) continue;
-        const uint32_t token = r.row0 + (uint32_t)(pos0 + t - r.len);
-        float x[8], s = __builtin_nanf("");
-        int32_t code[8] = {};
-        if (page >= 0 && keys) {
-            const uint32_t at = k_place<D>(lane / 4, lane % 4);
-            s = bf16_bits_to_f32(gptr<uint16_t>(kv.k + kv.k_scales)[(s0 + t) * (D / 32) + lane / 4]);
+        for (uint32_t t = 0; t < 4; t++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[t][j] = __builtin_nanf("");
+    } else if (keys) {
+        const uint32_t at = k_place<D>(lane / 4, lane % 4);
+        uint32_t w[4][KB / 4];
+#pragma unroll
+        for (uint32_t t = 0; t < 4; t++) {
+            const uint64_t row = c.slot + t0 + t;
+            s[t] = bf16_bits_to_f32(gptr<uint16_t>(kv.k + kv.k_scales)[row * (D / 32) + lane / 4]);
             if constexpr (KB == 8) {
-                const u32x2 w = *gptr<u32x2>(kv.k + (s0 + t) * D + at);
-#pragma unroll
-                for (int i = 0; i < 8; i++) code[i] = (int32_t)((w[i / 4] >> (8 * (i % 4))) & 255u) - 128;
+                const u32x2 y = *gptr<u32x2>(kv.k + row * D + at);
+                w[t][0] = y.x, w[t][1] = y.y;
             } else {
-                const uint32_t w = *gptr<uint32_t>(kv.k + (s0 + t) * (D / 2) + at / 2);
-#pragma unroll
-                for (int i = 0; i < 8; i++) code[i] = (int32_t)((w >> (8 * (i % 4) + 4 * (i / 4))) & 15u) - 8;
+                w[t][0] = *gptr<uint32_t>(kv.k + row * (D / 2) + at / 2);
             }
-        } else if (page >= 0) {
-            s = bf16_bits_to_f32(gptr<uint16_t>(kv.v + kv.v_scales)[s0 + t]);
-#pragma unroll
-            for (int i = 0; i < 8; i++) code[i] = (int8_t)sm[(d0 + i) * 16 + t];
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = (float)code[i] * s;
-        const KvRows& o = keys ? k : v;
-        store8(o, (int64_t)token * o.ts + (int64_t)head * o.hs + d0, x);
+        for (uint32_t t = 0; t < 4; t++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int32_t code = KB == 8 ? (int32_t)((w[t][j / 4 % (KB / 4)] >> (8 * (j % 4))) & 255u) - 128
+                                             : (int32_t)((w[t][0] >> (8 * (j % 4) + 4 * (j / 4))) & 15u) - 8;
+                x[t][j] = (float)code * s[t];
+            }
+    } else {
+        uint32_t w[2][4];  // [half of the dims][dim]: four tokens each
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            w[j / 4][j % 4] = VB == 8 ? *gptr<uint32_t>(kv.v + c.slot * D + (d0 + j) * 16 + t0)
+                                      : *gptr<uint32_t>(kv.v + c.slot * (D / 2) + (d0 + j) * 8 + 4 * (quad / 2));
+        const u32x2 sw = *gptr<u32x2>(kv.v + kv.v_scales + 2 * (c.slot + t0));
+#pragma unroll
+        for (uint32_t t = 0; t < 4; t++) s[t] = bf16_bits_to_f32(sw[t / 2] >> (16 * (t % 2)) & 0xFFFFu);
+        if constexpr (VB == 4) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {  // nibble n (signed) as a byte: bit 3 set, bits 4..7 too
+                const uint32_t n = (w[j / 4][j % 4] >> (4 * (quad % 2))) & 0x0F0F0F0Fu;
+                w[j / 4][j % 4] = n | ((n & 0x08080808u) * 30u);
+            }
+        }
+        turn4(w[0]);
+        turn4(w[1]);
+#pragma unroll
+        for (uint32_t t = 0; t < 4; t++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[t][j] = (float)(int8_t)(w[j / 4][t] >> (8 * (j % 4))) * s[t];
     }
+    const KvRows& o = keys ? k : v;
+#pragma unroll
+    for (uint32_t t = 0; t < 4; t++)
+        if (c.has(t0 + t)) store8(o, (int64_t)c.row(t0 + t) * o.ts + (int64_t)c.h * o.hs + d0, x[t]);
 }
 
 // One workgroup per (sequence, head, keys or values).  A thread owns the same
@@ -505,11 +569,12 @@ hipError_t kv_append_launch(const KvView& kv, const KvBatch& b, const KvRows& k,
         constexpr int D = decltype(d)::value;
         constexpr uint64_t rows = 256 / kLanes<D>;
         const uint32_t chunks = chunk_bound(b.max_new);
-        const uint32_t kv_blocks = b.seqs * chunks * kv.heads;
-        const uint64_t grid = 2ull * kv_blocks + ((uint64_t)b.tokens * q_heads + rows - 1) / rows;
+        const uint32_t k_blocks = b.seqs * chunks * ((kv.heads + kKeyHeads<D> - 1) / kKeyHeads<D>);
+        const uint32_t v_blocks = b.seqs * chunks * ((kv.heads + kHeads<D> - 1) / kHeads<D>);
+        const uint64_t grid = (uint64_t)k_blocks + v_blocks + ((uint64_t)b.tokens * q_heads + rows - 1) / rows;
         if (grid == 0) return hipSuccess;
         append_kernel<D, decltype(kb)::value, decltype(vb)::value>
-            <<<(uint32_t)grid, 256, 0, st>>>(kv, b, k, v, rope, q, q_out, q_heads, chunks, kv_blocks);
+            <<<(uint32_t)grid, 256, 0, st>>>(kv, b, k, v, rope, q, q_out, q_heads, chunks, k_blocks, v_blocks);
         return hipGetLastError();
     });
 }
@@ -518,7 +583,7 @@ hipError_t kv_read_launch(const KvView& kv, const KvBatch& b, const KvRows& k, c
     return by_cache(kv, [&](auto d, auto kb, auto vb) {
         constexpr int D = decltype(d)::value;
         const uint32_t chunks = chunk_bound(b.max_new);
-        const uint32_t kv_blocks = b.seqs * chunks * kv.heads;
+        const uint32_t kv_blocks = b.seqs * chunks * ((kv.heads + kHeads<D> - 1) / kHeads<D>);
         const uint32_t grid = kv_blocks * ((k.p != nullptr) + (v.p != nullptr));
         if (grid == 0) return hipSuccess;
         read_kernel<D, decltype(kb)::value, decltype(vb)::value><<<grid, 256, 0, st>>>(kv, b, k, v, chunks, kv_blocks);
