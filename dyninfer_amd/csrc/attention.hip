@@ -98,12 +98,12 @@ AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint
     const uint64_t rows = (uint64_t)b.max_new * (q_heads / kv.heads);
     // registers hold two tiles of at most 128 dims and bf16
     const bool two = kv.dim <= 128 && bf16;
-    p.tiles = rows <= 16 || (rows <= 32 && !two) ? 1 : rows <= 32 ? 2 : rows <= 64 || !two ? 4 : 8;
+    p.tiles = rows <= 16 || (rows <= 32 && !two) ? 1 : rows <= 32 ? 2 : rows <= 64 || !two ? 4 : rows <= 128 ? 8 : 16;
     const uint32_t tile = 16 * p.tiles;
     p.row_tiles = (uint32_t)((rows + tile - 1) / tile);
     const uint64_t steps = max_length > kStep ? (max_length + kStep - 1) / kStep : 1;
     const uint64_t units = (uint64_t)b.seqs * kv.heads * p.row_tiles;
-    const uint64_t full = kv.dim > 128 ? 256 : 512;
+    const uint64_t full = kv.dim > 128 || p.tiles == 16 ? 256 : 512;
     if (steps == 1 || units >= 8 * full) {
         p.grid = units;
         return p;

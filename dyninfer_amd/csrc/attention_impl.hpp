@@ -346,8 +346,8 @@ __device__ __forceinline__ void seq_work(const AttnArgs& a, uint32_t rows_of_til
 // This workgroup's share.  The first workgroup also writes where each sequence's
 // places and units begin, for the second launch.  lds: 64 bytes and more.
 __device__ inline Share share_of(const AttnArgs& a, uint32_t rows_of_tile, uint8_t* lds) {
-    uint64_t* const sums = reinterpret_cast<uint64_t*>(lds);  // [2][4] of the waves
-    Share* const found = reinterpret_cast<Share*>(lds + 64);
+    uint64_t* const sums = reinterpret_cast<uint64_t*>(lds);  // [2][8] of the waves
+    Share* const found = reinterpret_cast<Share*>(lds + 128);
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     uint32_t share = 0;
     uint64_t all = 0;
@@ -355,8 +355,8 @@ __device__ inline Share share_of(const AttnArgs& a, uint32_t rows_of_tile, uint8
     uint64_t places = 0, units = 0;
     for (int pass = 0; pass < 2; pass++) {  // how many places there are; whose the share's first is
         uint64_t before = 0, units_before = 0;
-        for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 256) {
-            if (pass == 0 || a.b.seqs > 256) seq_work(a, rows_of_tile, s0 + threadIdx.x, places, units);
+        for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += blockDim.x) {
+            if (pass == 0 || a.b.seqs > blockDim.x) seq_work(a, rows_of_tile, s0 + threadIdx.x, places, units);
             uint64_t x = places, y = units;  // inclusive sums
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) {
@@ -364,14 +364,14 @@ __device__ inline Share share_of(const AttnArgs& a, uint32_t rows_of_tile, uint8
                 if (lane >= (uint32_t)d) x += u, y += v;
             }
             __syncthreads();
-            if (lane == 63) sums[wave] = x, sums[4 + wave] = y;
+            if (lane == 63) sums[wave] = x, sums[8 + wave] = y;
             __syncthreads();
             uint64_t tx = 0, ty = 0;
 #pragma unroll
-            for (uint32_t w = 0; w < 4; w++) {
+            for (uint32_t w = 0; w < blockDim.x / 64; w++) {
                 if (w == wave) x += tx, y += ty;
                 tx += sums[w];
-                ty += sums[4 + w];
+                ty += sums[8 + w];
             }
             const uint64_t first = before + x - places, unit0 = units_before + y - units;
             if (pass == 1) {
@@ -882,21 +882,21 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
     }
 }
 
-// Many rows (64 NQ): every wave holds its own and all take the same positions, 64
-// at a time.  The waves decode a quarter of the tile each and leave the operands
-// in LDS for all, one tile ahead; the codes of the tile after that are on their
-// way into registers.  A step of few rows spends two fifths of its vector
-// instructions on decoding; here that is shared by four waves.
+// Many rows (16 NQ WAVES): every wave holds its own and all take the same
+// positions, 64 at a time.  The waves decode a part of the tile each and leave the
+// operands in LDS for all, one tile ahead; the codes of the tile after that are on
+// their way into registers.  A step of few rows spends two fifths of its vector
+// instructions on decoding; here that is shared by four or eight waves.
 constexpr uint32_t kWideTile = 64;
 
-template <int D, int KB, int VB, int NQ, bool F32>
-__global__ __launch_bounds__(256, D < 256 ? 2 : 1) void attend_wide_kernel(AttnArgs a) {
+template <int D, int KB, int VB, int NQ, bool F32, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, D < 256 ? 2 : 1) void attend_wide_kernel(AttnArgs a) {
     constexpr int NB = D / 32, DT = D / 16, PAIRS = D / 64, ODD = NB % 2;
-    constexpr uint32_t ROWS = 64u * NQ;
+    constexpr uint32_t ROWS = 16u * NQ * WAVES;
     constexpr uint32_t RB = D * KB / 8;                  // bytes of a key
     constexpr uint32_t KF = 0, VF = 4 * NB * 1024;       // operands: [S][block][lane], [half][dims][lane]
     constexpr uint32_t KS = VF + 2 * DT * 1024, VS = KS + 64 * NB * 4, BUF = VS + 256;  // scales in f32
-    constexpr int KU = PAIRS, VU = (DT + 3) / 4;         // units of a wave: (S = wave, pair), 16 dims
+    constexpr int KU = (4 * PAIRS + WAVES - 1) / WAVES, VU = (DT + WAVES - 1) / WAVES;  // units of a wave: (S, pair), 16 dims
     __shared__ __align__(16) uint8_t lds[2 * BUF];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -920,9 +920,10 @@ __global__ __launch_bounds__(256, D < 256 ? 2 : 1) void attend_wide_kernel(AttnA
 #pragma unroll
             for (uint32_t c = 0; c < 4; c++) ids[c] = page_of(4 * (tile0 + k) + c);
         };
-        // A tile's codes, this wave's quarter: keys of S number `wave` (row m of S number s
-        // is position 16 (m / 4) + 4 s + m % 4), values of 16 dims and all positions (lane
-        // group g holds 16g..16g+15), wave 0 the keys' scales, wave 1 the values'.
+        // A tile's codes, this wave's part: keys of an S and a pair of blocks (row m of S
+        // number s is position 16 (m / 4) + 4 s + m % 4), values of 16 dims and all positions
+        // (lane group g holds 16g..16g+15), wave 0 the keys' scales, wave 1 the values'.
+        // Unit u of the keys: S u % 4, pair u / 4.
         u32x4 kr[KU], vr[VU], sr;
         u32x2 ko;
         uint32_t absent_raw = 0;  // four bits: chunks of the tile in registers that are not there
@@ -942,25 +943,30 @@ __global__ __launch_bounds__(256, D < 256 ? 2 : 1) void attend_wide_kernel(AttnA
                 const uint64_t x = i & 1u ? slot[1] : slot[0], y = i & 1u ? slot[3] : slot[2];
                 return i & 2u ? y : x;
             };
-            const uint8_t* p = a.kv.k + (pick(col >> 2) + 4 * wave + (col & 3u)) * RB;
+            const uint8_t* p = a.kv.k + (pick(col >> 2) + 4 * (wave % 4) + (col & 3u)) * RB;
 #pragma unroll
             for (int j = 0; j < KU; j++) {
-                if constexpr (KB == 8) {
-                    kr[j] = *gptr<u32x4>(p + 64 * j + 16 * g);
-                } else {
-                    const u32x2 x = *gptr<u32x2>(p + 32 * j + 8 * g);
-                    kr[j].x = x.x, kr[j].y = x.y;
+                const uint32_t pair = (wave + WAVES * j) / 4;
+                if ((4 * PAIRS) % WAVES == 0 || pair < (uint32_t)PAIRS) {
+                    if constexpr (KB == 8) {
+                        kr[j] = *gptr<u32x4>(p + 64 * pair + 16 * g);
+                    } else {
+                        const u32x2 x = *gptr<u32x2>(p + 32 * pair + 8 * g);
+                        kr[j].x = x.x, kr[j].y = x.y;
+                    }
                 }
             }
             if constexpr (ODD) {
-                if constexpr (KB == 8) ko = *gptr<u32x2>(p + 64 * PAIRS + 8 * g);
-                else ko.x = *gptr<uint32_t>(p + 32 * PAIRS + 4 * g);
+                if (wave < 4) {
+                    if constexpr (KB == 8) ko = *gptr<u32x2>(p + 64 * PAIRS + 8 * g);
+                    else ko.x = *gptr<uint32_t>(p + 32 * PAIRS + 4 * g);
+                }
             }
             const uint8_t* q = a.kv.v + pick(g) * (D * VB / 8) + col * (2 * VB);
 #pragma unroll
             for (int j = 0; j < VU; j++) {
-                const uint32_t d = wave + 4 * j;
-                if (DT % 4 == 0 || d < (uint32_t)DT) {
+                const uint32_t d = wave + WAVES * j;
+                if (DT % WAVES == 0 || d < (uint32_t)DT) {
                     if constexpr (VB == 8) {
                         vr[j] = *gptr<u32x4>(q + 256 * d);
                     } else {
@@ -980,26 +986,31 @@ __global__ __launch_bounds__(256, D < 256 ? 2 : 1) void attend_wide_kernel(AttnA
         auto decode = [&](uint8_t* buf) {
             uint32_t ln = lane;
             asm volatile("" : "+v"(ln));
-            f16x8* const kf = reinterpret_cast<f16x8*>(buf + KF + wave * (NB * 1024)) + ln;
+            f16x8* const kf = reinterpret_cast<f16x8*>(buf + KF + wave % 4 * (NB * 1024)) + ln;
 #pragma unroll
             for (int j = 0; j < KU; j++) {
-                if constexpr (KB == 8) {
-                    kf[64 * (2 * j)] = k_frag(kr[j].x, kr[j].y);
-                    kf[64 * (2 * j + 1)] = k_frag(kr[j].z, kr[j].w);
-                } else {
-                    kf[64 * (2 * j)] = k_frag((kr[j].x << 4) & 0xF0F0F0F0u, kr[j].x & 0xF0F0F0F0u);
-                    kf[64 * (2 * j + 1)] = k_frag((kr[j].y << 4) & 0xF0F0F0F0u, kr[j].y & 0xF0F0F0F0u);
+                const uint32_t pair = (wave + WAVES * j) / 4;
+                if ((4 * PAIRS) % WAVES == 0 || pair < (uint32_t)PAIRS) {
+                    if constexpr (KB == 8) {
+                        kf[128 * pair] = k_frag(kr[j].x, kr[j].y);
+                        kf[128 * pair + 64] = k_frag(kr[j].z, kr[j].w);
+                    } else {
+                        kf[128 * pair] = k_frag((kr[j].x << 4) & 0xF0F0F0F0u, kr[j].x & 0xF0F0F0F0u);
+                        kf[128 * pair + 64] = k_frag((kr[j].y << 4) & 0xF0F0F0F0u, kr[j].y & 0xF0F0F0F0u);
+                    }
                 }
             }
             if constexpr (ODD) {
-                if constexpr (KB == 8) kf[64 * (NB - 1)] = k_frag(ko.x, ko.y);
-                else kf[64 * (NB - 1)] = k_frag((ko.x << 4) & 0xF0F0F0F0u, ko.x & 0xF0F0F0F0u);
+                if (wave < 4) {
+                    if constexpr (KB == 8) kf[64 * (NB - 1)] = k_frag(ko.x, ko.y);
+                    else kf[64 * (NB - 1)] = k_frag((ko.x << 4) & 0xF0F0F0F0u, ko.x & 0xF0F0F0F0u);
+                }
             }
             bf16x8* const vf = reinterpret_cast<bf16x8*>(buf + VF) + ln;
 #pragma unroll
             for (int j = 0; j < VU; j++) {
-                const uint32_t d = wave + 4 * j;
-                if (DT % 4 == 0 || d < (uint32_t)DT) {
+                const uint32_t d = wave + WAVES * j;
+                if (DT % WAVES == 0 || d < (uint32_t)DT) {
                     if constexpr (VB == 8) {
                         vf[64 * d] = v_frag(vr[j].x, vr[j].y);
                         vf[64 * (DT + d)] = v_frag(vr[j].z, vr[j].w);
@@ -1082,12 +1093,18 @@ hipError_t attend_launch(const AttnArgs& a, uint32_t tiles, uint64_t grid, hipSt
 template <int D, int KB, int VB>
 hipError_t attend_launch_dim(const AttnArgs& a, uint32_t tiles, uint64_t grid, hipStream_t st) {
     const dim3 gd((uint32_t)grid), bd(64 * kWaves);
-    if (tiles >= 4) {  // 64 or 128 rows
-        if (!a.q.bf16) attend_wide_kernel<D, KB, VB, 1, true><<<gd, bd, 0, st>>>(a);
-        else if (tiles == 4) attend_wide_kernel<D, KB, VB, 1, false><<<gd, bd, 0, st>>>(a);
-        else {
-            if constexpr (D <= 128) attend_wide_kernel<D, KB, VB, 2, false><<<gd, bd, 0, st>>>(a);
-            else return hipErrorInvalidValue;
+    if (tiles >= 4) {  // 64, 128 or 256 rows
+        if (!a.q.bf16) {
+            attend_wide_kernel<D, KB, VB, 1, true, 4><<<gd, bd, 0, st>>>(a);
+        } else if (tiles == 4) {
+            attend_wide_kernel<D, KB, VB, 1, false, 4><<<gd, bd, 0, st>>>(a);
+        } else {
+            if constexpr (D <= 128) {
+                if (tiles == 8) attend_wide_kernel<D, KB, VB, 2, false, 4><<<gd, bd, 0, st>>>(a);
+                else attend_wide_kernel<D, KB, VB, 2, false, 8><<<gd, dim3(512), 0, st>>>(a);
+            } else {
+                return hipErrorInvalidValue;
+            }
         }
     } else if (!a.q.bf16) {
         attend_kernel<D, KB, VB, 1, true><<<gd, bd, 0, st>>>(a);
