@@ -22,8 +22,9 @@ namespace {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // Logits of a workgroup of the statistics.  Few rows are cut finer, for the
-// latency of one pass: 5 rows of 151936 in 16384s took 9.3 us, in 4096s 6.1;
-// 493 rows 49.8 us either way.
+// latency of one pass: 5 bf16 rows of 151936 in 16384s took 9.3 us, in 4096s 5.4
+// (4.8 with four loads in flight); 493 f32 rows, 300 MB, take 38 us, 49.8 with one
+// load in flight and an accurate exponential of every element.
 constexpr uint32_t kPiece = 16384, kSmallPiece = 4096;
 constexpr uint32_t kManyPieces = 1024;  // workgroups from which the large pieces are taken
 constexpr uint32_t kDraw = 4096;        // logits of a workgroup of the draw
@@ -48,6 +49,7 @@ struct Left {
     unsigned long long best;
 };
 
+// NaN as -inf, +inf as the largest f32.
 __device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -__builtin_inff()), kFltMax); }
 
 __device__ __forceinline__ float at(const void* p, uint32_t bf16, int64_t i) {
@@ -99,6 +101,7 @@ __global__ __launch_bounds__(256) void stats_kernel(VerifyArgs a, Stat* out, uin
     // 16-byte steps from the first boundary at or after lo
     const uint32_t off = (uint32_t)((uintptr_t)(base + (size_t)lo * E) & 15u) / E;
     const uint32_t first = min(hi, lo + (off ? V - off : 0u));
+    const float scale = fminf(inv_t * 1.44269504f, kFltMax);
     Stat st = {-__builtin_inff(), 0.0f, ~0u, 0u};
     auto take = [&](const float (&x)[V], uint32_t i0, uint32_t n) {
         float m = -__builtin_inff();
@@ -112,10 +115,12 @@ __global__ __launch_bounds__(256) void stats_kernel(VerifyArgs a, Stat* out, uin
             for (int j = V - 1; j >= 0; j--)
                 if ((uint32_t)j < n && x[j] == m) st.i = i0 + j;
         }
-        if (!greedy) {
+        if (!greedy && st.m != -__builtin_inff()) {
+            // the sum is its largest terms', whose arguments are small: 2^y as the
+            // instruction gives it, of the one product
 #pragma unroll
             for (uint32_t j = 0; j < V; j++)
-                if (j < n) st.s += weight(x[j], st.m, inv_t);
+                if (j < n) st.s += __builtin_amdgcn_exp2f((x[j] - st.m) * scale);
         }
     };
     // the ends that are no whole step, by one thread each
@@ -127,19 +132,30 @@ __global__ __launch_bounds__(256) void stats_kernel(VerifyArgs a, Stat* out, uin
     };
     if (threadIdx.x == 0 && first > lo) ends(lo, first);
     const uint32_t steps = (hi - first) / V;
-    for (uint32_t i = threadIdx.x; i < steps; i += 256) {
-        const u32x4 ww = *gptr<u32x4>(base + ((size_t)first + (size_t)i * V) * E);
-        float x[V];
+    constexpr uint32_t N = 4;  // loads in flight
+    for (uint32_t i0 = threadIdx.x; i0 < steps; i0 += 256 * N) {
+        u32x4 ww[N];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if constexpr (BF16) {
-                x[2 * j] = clean(bf16_bits_to_f32(ww[j] & 0xFFFFu));
-                x[2 * j + 1] = clean(__uint_as_float(ww[j] & 0xFFFF0000u));
-            } else {
-                x[j] = clean(__uint_as_float(ww[j]));
-            }
+        for (uint32_t k = 0; k < N; k++) {
+            const uint32_t i = min(i0 + 256 * k, steps - 1);
+            ww[k] = *gptr<u32x4>(base + ((size_t)first + (size_t)i * V) * E);
         }
-        take(x, first + i * V, V);
+#pragma unroll
+        for (uint32_t k = 0; k < N; k++) {
+            const uint32_t i = i0 + 256 * k;
+            if (i >= steps) break;
+            float x[V];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if constexpr (BF16) {
+                    x[2 * j] = clean(bf16_bits_to_f32(ww[k][j] & 0xFFFFu));
+                    x[2 * j + 1] = clean(__uint_as_float(ww[k][j] & 0xFFFF0000u));
+                } else {
+                    x[j] = clean(__uint_as_float(ww[k][j]));
+                }
+            }
+            take(x, first + i * V, V);
+        }
     }
     if (threadIdx.x == 255 && first + steps * V < hi) ends(first + steps * V, hi);
 #pragma unroll
@@ -337,46 +353,53 @@ __device__ __forceinline__ unsigned long long pack(float left, float full, uint3
     return top ? ((unsigned long long)top << 32) | (0xFFFFFFFFu - v) : 0ull;
 }
 
-__global__ __launch_bounds__(256) void draw_kernel(VerifyArgs a, const int32_t* gone_list, Left* left, uint32_t pieces) {
+__global__ __launch_bounds__(512) void draw_kernel(VerifyArgs a, const int32_t* gone_list, Left* left, uint32_t pieces) {
     const uint32_t seq = blockIdx.x / pieces, piece = blockIdx.x % pieces;
+    const uint32_t lo = piece * kDraw + threadIdx.x;
+    constexpr uint32_t N = kDraw / 512;  // all loads of a thread in flight together
+    float x[N], z[N], q[N];
+#pragma unroll
+    for (uint32_t j = 0; j < N; j++) {
+        const uint32_t v = lo + 512 * j;
+        z[j] = v < a.vocab ? gptr<float>(a.noise)[(int64_t)seq * a.noise_stride + v] : 1.0f;
+    }
     const Left l = left[seq];
     if (l.row == ~0u) return;
     const int32_t r0 = a.starts[seq];
     const int32_t* gone = gone_list + (r0 < 0 ? 0 : r0);
-    const float as = l.a * l.s;
+    const float as = l.a * l.s, scale = fminf(l.inv_t * 1.44269504f, kFltMax);
     const bool minus = a.probs && as > 0.0f;
-    const uint32_t lo = piece * kDraw;
     const int64_t lr = (int64_t)l.row * a.logits_stride, pr = (int64_t)l.row * a.probs_stride;
-    constexpr uint32_t N = kDraw / 256;  // all loads of a thread in flight together
-    float x[N], z[N], q[N];
 #pragma unroll
     for (uint32_t j = 0; j < N; j++) {
-        const uint32_t v = lo + threadIdx.x + 256 * j;
+        const uint32_t v = lo + 512 * j;
         x[j] = v < a.vocab ? at(a.logits, a.logits_bf16, lr + v) : -__builtin_inff();
-        z[j] = v < a.vocab ? gptr<float>(a.noise)[(int64_t)seq * a.noise_stride + v] : 1.0f;
         q[j] = minus && v < a.vocab ? at(a.probs, a.probs_bf16, pr + v) : 0.0f;
     }
     unsigned long long best = 0;
 #pragma unroll
     for (uint32_t j = 0; j < N; j++) {
-        const uint32_t v = lo + threadIdx.x + 256 * j;
-        const float e = weight(clean(x[j]), l.m, l.inv_t);
+        const uint32_t v = lo + 512 * j;
+        const float y = clean(x[j]);
+        const float e = y == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((y - l.m) * scale);
         float r = minus ? e - as * q[j] : e;
         for (uint32_t g = 0; g < l.gone; g++)
             if (gone[g] == (int32_t)v) r = 0.0f;
-        best = max(best, pack(r / z[j], e / z[j], v));
+        const float inv = __builtin_amdgcn_rcpf(z[j]);
+        best = max(best, pack(r * inv, e * inv, v));
     }
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) best = max(best, (unsigned long long)__shfl_xor((long long)best, s));
-    __shared__ unsigned long long sm[4];
+    __shared__ unsigned long long sm[8];
     if ((threadIdx.x & 63u) == 0) sm[threadIdx.x >> 6] = best;
     __syncthreads();
     if (threadIdx.x != 0) return;
-    for (int w = 1; w < 4; w++) best = max(best, sm[w]);
+    for (int w = 1; w < 8; w++) best = max(best, sm[w]);
     // The largest does not depend on the order of these; the last workgroup reads it.
     // Only this number passes between workgroups, by an atomic that has returned
     // before the count goes up, so no cache need be written back: with release and
-    // acquire on the count 2400 workgroups took 40.4 us, without 17.6.
+    // acquire on the count 2400 workgroups took 40.4 us, without 17.6 (1216 of 512
+    // threads: 12.6).
     const unsigned long long old = __hip_atomic_fetch_max(&left[seq].best, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::"v"(old) : "memory");
     const uint32_t before = __hip_atomic_fetch_add(&left[seq].done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -427,7 +450,7 @@ hipError_t verify_launch(const VerifyArgs& a, uint8_t* work, hipStream_t st) {
             stats_kernel<false><<<a.tokens * pieces, 256, 0, st>>>(a, stats, pieces, size);
     }
     walk_kernel<<<a.seqs, 1024, 0, st>>>(a, stats, pieces, rows, gone, left);
-    draw_kernel<<<a.seqs * draws, 256, 0, st>>>(a, gone, left, draws);
+    draw_kernel<<<a.seqs * draws, 512, 0, st>>>(a, gone, left, draws);
     return hipGetLastError();
 }
 
