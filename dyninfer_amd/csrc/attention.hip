@@ -19,22 +19,23 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t rows_of_
     constexpr int W = D <= 128 ? 2 : 4;  // dims of a lane
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t q_heads = a.kv.heads * a.group;
-    const uint64_t id = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const uint32_t h = (uint32_t)(id % q_heads);
-    const uint64_t rest = id / q_heads;
-    const uint32_t i = (uint32_t)(rest % a.b.max_new), seq = (uint32_t)(rest / a.b.max_new);
-    if (rest / a.b.max_new >= a.b.seqs) return;
+    const uint64_t id = (uint64_t)blockIdx.x * 4 + scalar(threadIdx.x >> 6);
+    const uint64_t rest = divide(id, q_heads);
+    const uint32_t h = (uint32_t)(id - rest * q_heads);
+    const uint64_t seq_at = divide(rest, a.b.max_new);
+    if (seq_at >= a.b.seqs) return;
+    const uint32_t i = (uint32_t)(rest - seq_at * a.b.max_new), seq = (uint32_t)seq_at;
+    const uint64_t all = a.where[2 * a.b.seqs], first = a.where[2 * seq], unit0 = a.where[2 * seq + 1];
     Share s = {};
     s.seq = seq;
     s.load(a, rows_of_tile);
     const SeqRange r = seq_range(a.b, seq);
     if (i >= r.n) return;
-    const uint64_t all = a.where[2 * a.b.seqs], first = a.where[2 * seq], unit0 = a.where[2 * seq + 1];
-    const uint32_t row = i * a.group + h % a.group;
-    const uint32_t unit = h / a.group * s.row_tiles + row / rows_of_tile;
+    const uint32_t kv_head = h / a.group, row = i * a.group + (h - kv_head * a.group);
+    const uint32_t unit = kv_head * s.row_tiles + row / rows_of_tile;
     // the shares that hold the unit's first and last step: share w begins at floor(w all / shares)
     const uint64_t x0 = first + (uint64_t)unit * (s.unit_steps + kUnitCost) + kUnitCost, x1 = x0 + s.unit_steps - 1;
-    const uint64_t n = shares_of(a, all), w0 = ((x0 + 1) * n - 1) / all, w1 = ((x1 + 1) * n - 1) / all;
+    const uint64_t n = shares_of(a, all), w0 = divide((x0 + 1) * n - 1, all), w1 = divide((x1 + 1) * n - 1, all);
     const uint32_t parts = (uint32_t)(w1 - w0) + 1;
     if (parts == 1) return;  // written by the first launch
     const uint64_t at = (w0 + unit0 + unit) * rows_of_tile + row % rows_of_tile;

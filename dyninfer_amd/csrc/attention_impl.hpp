@@ -343,83 +343,85 @@ __device__ __forceinline__ void seq_work(const AttnArgs& a, uint32_t rows_of_til
     places = x.units * (uint64_t)(x.unit_steps + kUnitCost);
 }
 
-// This workgroup's share.  The first workgroup also writes where each sequence's
-// places and units begin, for the second launch.  lds: 64 bytes and more.
-__device__ inline Share share_of(const AttnArgs& a, uint32_t rows_of_tile, uint8_t* lds) {
-    uint64_t* const sums = reinterpret_cast<uint64_t*>(lds);  // [2][8] of the waves
-    Share* const found = reinterpret_cast<Share*>(lds + 128);
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+// A number that is the same in every lane, as a scalar.
+__device__ __forceinline__ uint32_t scalar(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint64_t scalar64(uint64_t x) {
+    return (uint64_t)scalar((uint32_t)(x >> 32)) << 32 | scalar((uint32_t)x);
+}
+
+// x / y, mostly of numbers below 2^32 (a division of 64 bits takes some hundred
+// instructions).
+__device__ __forceinline__ uint64_t divide(uint64_t x, uint64_t y) {
+    return (x | y) >> 32 ? x / y : (uint64_t)((uint32_t)x / (uint32_t)y);
+}
+
+// This workgroup's share.  Every wave finds it by itself, 64 sequences at a time, so
+// that no barrier stands before its first copies.  The first wave of the first
+// workgroup also writes where each sequence's places and units begin, for the
+// second launch.
+__device__ __forceinline__ Share share_of(const AttnArgs& a, uint32_t rows_of_tile) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const bool writes = blockIdx.x == 0 && scalar(threadIdx.x >> 6) == 0;
+    uint64_t places = 0, units = 0, at = 0, to = 0, all = 0;
     uint32_t share = 0;
-    uint64_t all = 0;
-    uint64_t at = 0, to = 0;
-    uint64_t places = 0, units = 0;
-    for (int pass = 0; pass < 2; pass++) {  // how many places there are; whose the share's first is
-        uint64_t before = 0, units_before = 0;
-        for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += blockDim.x) {
-            if (pass == 0 || a.b.seqs > blockDim.x) seq_work(a, rows_of_tile, s0 + threadIdx.x, places, units);
-            uint64_t x = places, y = units;  // inclusive sums
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const uint64_t u = __shfl_up((unsigned long long)x, d), v = __shfl_up((unsigned long long)y, d);
-                if (lane >= (uint32_t)d) x += u, y += v;
-            }
-            __syncthreads();
-            if (lane == 63) sums[wave] = x, sums[8 + wave] = y;
-            __syncthreads();
-            uint64_t tx = 0, ty = 0;
-#pragma unroll
-            for (uint32_t w = 0; w < blockDim.x / 64; w++) {
-                if (w == wave) x += tx, y += ty;
-                tx += sums[w];
-                ty += sums[8 + w];
-            }
-            const uint64_t first = before + x - places, unit0 = units_before + y - units;
-            if (pass == 1) {
-                if (at < to && first <= at && at < first + places) {
-                    Share f = {};
-                    f.unit0 = unit0;
-                    f.share = share;
-                    f.seq = s0 + threadIdx.x;
-                    f.load(a, rows_of_tile);
-                    f.unit = (uint32_t)((at - first) / (f.unit_steps + kUnitCost));
-                    f.place = (uint32_t)((at - first) % (f.unit_steps + kUnitCost));
-                    f.places = (uint32_t)(to - at);
-                    *found = f;
-                }
-                if (blockIdx.x == 0 && s0 + threadIdx.x < a.b.seqs) {
-                    a.where[2 * (s0 + threadIdx.x)] = first;
-                    a.where[2 * (s0 + threadIdx.x) + 1] = unit0;
-                }
-            }
-            before += tx;
-            units_before += ty;
+    if (a.b.seqs > 64) {  // how many places there are
+        for (uint32_t s = lane; s < a.b.seqs; s += 64) {
+            seq_work(a, rows_of_tile, s, places, units);
+            all += places;
         }
-        if (pass == 0) {
-            all = before;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) all += __shfl_xor((unsigned long long)all, d);
+        all = scalar64(all);
+    }
+    Share f = {};
+    uint64_t before = 0, units_before = 0;
+    for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 64) {
+        seq_work(a, rows_of_tile, s0 + lane, places, units);
+        uint64_t x = places, y = units;  // sums over the lanes up to this one
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint64_t u = __shfl_up((unsigned long long)x, d), v = __shfl_up((unsigned long long)y, d);
+            if (lane >= (uint32_t)d) x += u, y += v;
+        }
+        if (a.b.seqs <= 64) all = scalar64(__shfl((unsigned long long)x, 63));
+        if (s0 == 0) {
             const uint32_t n = shares_of(a, all);
             share = n < a.shares ? blockIdx.x : by_xcd(blockIdx.x, n);
             if (share < n) {
-                at = share * all / n;
-                to = (share + 1ull) * all / n;
+                at = divide(share * all, n);
+                to = divide((share + 1ull) * all, n);
             }
         }
+        const uint64_t first = before + x - places, unit0 = units_before + y - units;
+        if (writes && s0 + lane < a.b.seqs) {
+            a.where[2 * (s0 + lane)] = first;
+            a.where[2 * (s0 + lane) + 1] = unit0;
+        }
+        const unsigned long long who = __ballot(at < to && first <= at && at < first + places);
+        if (who) {  // the sequence of the share's first place
+            const int w = __builtin_ctzll(who);
+            const uint64_t in = scalar64(at - __shfl((unsigned long long)first, w));
+            f.share = share;
+            f.seq = s0 + (uint32_t)w;
+            f.load(a, rows_of_tile);
+            f.unit0 = __shfl((unsigned long long)unit0, w);
+            f.unit = (uint32_t)divide(in, f.unit_steps + kUnitCost);
+            f.place = (uint32_t)(in - (uint64_t)f.unit * (f.unit_steps + kUnitCost));
+            f.places = (uint32_t)(to - at);
+            if (!writes) break;
+        }
+        before += __shfl((unsigned long long)x, 63);
+        units_before += __shfl((unsigned long long)y, 63);
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.where[2 * a.b.seqs] = all;
-    __syncthreads();
-    Share f = {};
-    if (at < to) f = *found;
-    __syncthreads();
-    // the same in every lane
-    f.share = share;
-    f.seq = __builtin_amdgcn_readfirstlane(f.seq);
-    f.unit = __builtin_amdgcn_readfirstlane(f.unit);
-    f.row_tiles = __builtin_amdgcn_readfirstlane(f.row_tiles);
-    f.units = __builtin_amdgcn_readfirstlane(f.units);
-    f.unit_steps = __builtin_amdgcn_readfirstlane(f.unit_steps);
-    f.place = __builtin_amdgcn_readfirstlane(f.place);
-    f.places = __builtin_amdgcn_readfirstlane(f.places);
-    f.unit0 = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(f.unit0 >> 32)) << 32 |
-              (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)f.unit0);
+    if (writes && lane == 0) a.where[2 * a.b.seqs] = all;
+    f.seq = scalar(f.seq);
+    f.unit = scalar(f.unit);
+    f.row_tiles = scalar(f.row_tiles);
+    f.units = scalar(f.units);
+    f.unit_steps = scalar(f.unit_steps);
+    f.place = scalar(f.place);
+    f.places = scalar(f.places);
+    f.unit0 = scalar64(f.unit0);
     return f;
 }
 
@@ -437,34 +439,63 @@ struct WaveRows {
     uint32_t tok[NQ];
     f32x4 o[NQ][DT];
 
+    // The queries as they lie in memory, loaded before the first tile is asked for:
+    // loads come back in order.
+    struct Raw {
+        u32x4 w[NQ][NB][F32 ? 2 : 1];
+    };
+
     // Rows first_row + 16 t + lane % 16 of the unit's.
     __device__ __forceinline__ void load(const AttnArgs& a, const SeqRange& r, uint32_t head, uint32_t first_row,
-                                         uint32_t rows, uint32_t lane) {
+                                         uint32_t rows, uint32_t lane, Raw& raw) {
         const uint32_t g = lane >> 4, col = lane & 15u;
-        const float sign = a.scale < 0.0f ? -1.0f : 1.0f;  // so that the largest score is that of the largest sum
 #pragma unroll
         for (int t = 0; t < NQ; t++) {
             const uint32_t row = first_row + 16u * t + col;
             const bool live = row < rows;
             tok[t] = live ? row / a.group : 0u;
-            const uint32_t h = head * a.group + (live ? row % a.group : 0u);
-            const int64_t at = (int64_t)(r.row0 + tok[t]) * a.q.ts + (int64_t)h * a.q.hs;
-            float x[NB][8], big = 0.0f;
+            const uint32_t h = head * a.group + (live ? row - tok[t] * a.group : 0u);
+            const int64_t at = (int64_t)(r.row0 + tok[t]) * a.q.ts + (int64_t)h * a.q.hs + 8 * g;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                const int64_t e = at + 32 * b + 8 * g;
-                if (a.q.vec && !F32) {
-                    const u32x4 w = *gptr<u32x4>(static_cast<const uint16_t*>(a.q.p) + e);
+                if constexpr (F32) {
+                    const float* p = static_cast<const float*>(a.q.p) + at + 32 * b;
+                    if (a.q.vec) {
+                        raw.w[t][b][0] = *gptr<u32x4>(p);
+                        raw.w[t][b][1] = *gptr<u32x4>(p + 4);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[b][i] = bf16_of(w[i / 2], i & 1);
+                        for (int i = 0; i < 8; i++) raw.w[t][b][i / 4][i % 4] = gptr<uint32_t>(p)[i];
+                    }
                 } else {
+                    const uint16_t* p = static_cast<const uint16_t*>(a.q.p) + at + 32 * b;
+                    if (a.q.vec) {
+                        raw.w[t][b][0] = *gptr<u32x4>(p);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        x[b][i] = F32 ? gptr<float>(a.q.p)[e + i] : bf16_bits_to_f32(gptr<uint16_t>(a.q.p)[e + i]);
+                        for (int i = 0; i < 4; i++)
+                            raw.w[t][b][0][i] = gptr<uint16_t>(p)[2 * i] | (uint32_t)gptr<uint16_t>(p)[2 * i + 1] << 16;
+                    }
                 }
-#pragma unroll
-                for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[b][i]));
             }
+        }
+    }
+
+    // The operands and the rows' factors; statistics and outputs begin.
+    __device__ __forceinline__ void begin(const AttnArgs& a, const Raw& raw, uint32_t first_row, uint32_t rows, uint32_t lane) {
+        const float sign = a.scale < 0.0f ? -1.0f : 1.0f;  // so that the largest score is that of the largest sum
+#pragma unroll
+        for (int t = 0; t < NQ; t++) {
+            const bool live = first_row + 16u * t + (lane & 15u) < rows;
+            float x[NB][8], big = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if constexpr (F32) x[b][i] = __uint_as_float(raw.w[t][b][i / 4][i % 4]);
+                    else x[b][i] = bf16_of(raw.w[t][b][0][i / 2], i & 1);
+                    big = fmaxf(big, fabsf(x[b][i]));
+                }
             big = rows_max(big);
             // exponent e of the row's largest: 2^(14 - e) scales it into [2^14, 2^15)
             int e = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
@@ -759,7 +790,7 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
     __shared__ float sm_m[kWaves][ROWS], sm_l[kWaves][ROWS];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-    Share sh = a.shares == 0 ? whole_unit(a, ROWS) : share_of(a, ROWS, lds);
+    Share sh = a.shares == 0 ? whole_unit(a, ROWS) : share_of(a, ROWS);
     for (; sh.places != 0; sh.next(a, ROWS)) {
         const uint32_t now0 = sh.first_step(), now1 = sh.end_step();  // steps of this unit
         if (now0 >= now1) continue;
@@ -796,23 +827,20 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
             copy_tile<D, KB, VB>(a.kv, ok0 ? chunk_slot(a.kv, id0, head, c) : 0, ok1 ? chunk_slot(a.kv, id1, head, c + 1) : 0, ln,
                                  mine + k % R * T::BYTES);
         };
-        for (uint32_t k = 0; k < R - 1 && k < count; k++) {
+        using Rows = WaveRows<D, KB, VB, NQ, F32>;
+        Rows w;
+        typename Rows::Raw raw;
+        w.load(a, r, head, tile_row, rows, lane, raw);
+        for (uint32_t k = 0; k < R && k < count; k++) {
             look_up(k);
             fetch(k, k);
         }
-        if (R - 1 < count) look_up(R - 1);
-
-        WaveRows<D, KB, VB, NQ, F32> w;
-        w.load(a, r, head, tile_row, rows, lane);
+        if (R < count) look_up(R);
+        w.begin(a, raw, tile_row, rows, lane);
 
         for (uint32_t k = 0; k < count; k++) {
             const uint32_t p0 = (tile0 + kWaves * k) * kTile;
             const uint8_t* const tile = mine + k % R * T::BYTES;
-            // the stage of tile k - 1 is free: its last reads have been waited for
-            if (k + R - 1 < count) {
-                fetch(k + R - 1, R - 1);
-                if (k + R < count) look_up(k + R);
-            }
             const uint32_t gone = absent & 3u;
             absent >>= 2;
             tiles_wait<T::DMA, R - 1>(count - 1 - k);
@@ -829,7 +857,11 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
                                                           (int64_t)p0 + 8 * g - (int64_t)r.len);
             }
             w.step(CodeTile<D, KB, VB>{tile, g, col}, masked, vis);
-            ring_wait<63>();  // the tile has been read
+            ring_wait<63>();  // the tile has been read: its stage is free
+            if (k + R < count) {
+                fetch(k + R, R - 1);
+                if (k + R + 1 < count) look_up(k + R + 1);
+            }
         }
 
         // join the four waves: every wave brings its rows to the common maximum, then
@@ -900,7 +932,7 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 ? 2 : 1) void attend_wide_kerne
     __shared__ __align__(16) uint8_t lds[2 * BUF];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-    Share sh = a.shares == 0 ? whole_unit(a, ROWS) : share_of(a, ROWS, lds);
+    Share sh = a.shares == 0 ? whole_unit(a, ROWS) : share_of(a, ROWS);
     for (; sh.places != 0; sh.next(a, ROWS)) {
         const uint32_t now0 = sh.first_step(), now1 = sh.end_step();
         if (now0 >= now1) continue;
@@ -1027,11 +1059,14 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 ? 2 : 1) void attend_wide_kerne
             }
         };
 
+        using Rows = WaveRows<D, KB, VB, NQ, F32>;
+        Rows w;
+        typename Rows::Raw raw;
+        w.load(a, r, head, first_row, rows, lane, raw);
         look_up(0);
         load(0);
         if (1 < count) look_up(1);
-        WaveRows<D, KB, VB, NQ, F32> w;
-        w.load(a, r, head, first_row, rows, lane);
+        w.begin(a, raw, first_row, rows, lane);
         decode(lds);
         uint32_t absent = absent_raw;  // of the tile being worked on
         if (1 < count) {

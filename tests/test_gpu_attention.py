@@ -289,3 +289,13 @@ def test_refusals(ctx):
     need = ctx.tree_attention_workspace_bytes(c.cache, c.batch, 4)
     bad(lambda: ctx.tree_attention(c.cache, c.batch, q, workspace=torch.empty(need + 256, dtype=torch.uint8, device="cuda")[16:]))
     bad(lambda: ctx.tree_attention_workspace_bytes(c.cache, c.batch, 3))
+
+
+@pytest.mark.parametrize("count", [64, 65, 200])
+def test_many_sequences(ctx, count):
+    """Some without new tokens, one long: shares begin in the middle of the sequences."""
+    rng = np.random.default_rng(count)
+    news, lens = rng.integers(0, 3, count).tolist(), rng.integers(0, 90, count).tolist()
+    news[count - 2], lens[count - 2] = 2, 2500
+    c = Case(18, news, lens, 1, 64, 16, 8, 4)
+    check(ctx, c, "bf16", 2, chain(news, lens), None)
