@@ -92,8 +92,11 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t rows_of_
 // The steps of all units go in equal shares to as many workgroups as the CUs
 // hold at once (two each; one of 256 dims), or one step each if they are fewer:
 // sequences differ in length, and a share may end in the middle of a unit.
-// Units of one step, or so many that they fill the CUs several times over, are
-// a workgroup each, with no second launch.
+// Writing and joining parts costs as much as some steps, so units of few steps, and
+// units so many that they fill the CUs several times over, are a workgroup each:
+// 32 ragged sequences of up to 512, 1024 and 2048 positions with 8 rows took 19, 28
+// and 48 us that way and 29, 35 and 49 in shares, one sequence of 380 with one row 9.6
+// and 11.4, of 760 14.6 and 11.9, 100 of up to 8000 272 and 206.
 AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint32_t q_heads, bool bf16) {
     AttnPlan p = {};
     const uint64_t rows = (uint64_t)b.max_new * (q_heads / kv.heads);
@@ -105,7 +108,8 @@ AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint
     const uint64_t steps = max_length > kStep ? (max_length + kStep - 1) / kStep : 1;
     const uint64_t units = (uint64_t)b.seqs * kv.heads * p.row_tiles;
     const uint64_t full = kv.dim > 128 || p.tiles == 16 ? 256 : 512;
-    if (steps == 1 || units >= 8 * full) {
+    const uint64_t few = (p.tiles <= 2 ? 3 : 1) + units / 32;
+    if (steps <= (few < 12 ? few : 12) || units >= 8 * full) {
         p.grid = units;
         return p;
     }

@@ -84,7 +84,7 @@ hipError_t kv_commit_launch(const KvView& kv, const KvBatch& b, const int32_t* p
 
 // Attention: how a call is cut (host), its workspace and its launch.
 struct AttnPlan {
-    uint32_t tiles;      // 16-row tiles a workgroup holds: 1 or 2 by every wave, 4 or 8 by four waves
+    uint32_t tiles;      // 16-row tiles a workgroup holds: 1 or 2 by every wave, 4, 8 or 16 one or two a wave
     uint32_t row_tiles;  // of the sequence with the most rows
     uint32_t shares;     // equal pieces of all units' steps, a workgroup each; 0: a unit each
     uint64_t grid;
