@@ -43,6 +43,20 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t rows_of_
     const float* ml = a.stats + 2 * at;
     const uint64_t pitch = rows_of_tile;  // rows from one part to the next
 
+    const uint32_t d0 = W * lane;
+    typedef float vec __attribute__((ext_vector_type(W)));
+    vec v[4];
+    float f[4];
+    auto fetch = [&](uint32_t p) {  // four loads in flight, the first of them before the statistics
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+            const uint64_t part = p + k < parts ? p + k : parts - 1;
+            v[k] = *gptr<vec>(po + part * pitch * D + (d0 < D ? d0 : 0));
+            f[k] = gptr<float>(ml)[2 * pitch * part];
+        }
+    };
+    fetch(0);
+
     float top = -__builtin_inff();
     for (uint32_t p = lane; p < parts; p += 64) top = fmaxf(top, gptr<float>(ml)[2 * pitch * p]);
 #pragma unroll
@@ -56,22 +70,13 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t rows_of_
 
     if (a.lse && lane == 0)
         gptr_mut<float>(a.lse)[(r.row0 + (uint64_t)i) * q_heads + h] = (top + log2f(sum)) * 0.69314718055994531f;
-    const uint32_t d0 = W * lane;
     if (d0 >= D) return;
-    typedef float vec __attribute__((ext_vector_type(W)));
     vec o = {};
-    for (uint32_t p = 0; p < parts; p += 4) {  // four loads in flight
-        vec v[4];
-        float f[4];
-#pragma unroll
-        for (uint32_t k = 0; k < 4; k++) {
-            const uint64_t part = p + k < parts ? p + k : parts - 1;
-            v[k] = *gptr<vec>(po + part * pitch * D + d0);
-            f[k] = gptr<float>(ml)[2 * pitch * part];
-        }
+    for (uint32_t p = 0; p < parts; p += 4) {
 #pragma unroll
         for (uint32_t k = 0; k < 4; k++)
             if (p + k < parts) o += v[k] * exp2f(f[k] - ref);
+        if (p + 4 < parts) fetch(p + 4);
     }
     const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : __builtin_nanf(""));
     const int64_t e = (r.row0 + (int64_t)i) * a.out.ts + (int64_t)h * a.out.hs + d0;
