@@ -93,7 +93,9 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t rows_of_
 
 // Row tiles: one or two of 16 rows held by every wave, or four or eight held by
 // four waves (64 tokens x group 4 over 131k positions: 572 us with one, 382 with two,
-// 401 with four, 300 with eight; 8 x 4 over 4k in 32 sequences: 74, 70, 89, 98).
+// 401 with four, 300 with eight; 8 x 4 over 4k in 32 sequences: 74, 70, 89, 98).  33 to
+// 64 rows take two where there are units enough (16 x 4 over 1k and 4k in 32 sequences:
+// 33 and 94 with two, 43 and 97 with four; over 4k in one: 23 and 18).
 // The steps of all units go in equal shares to as many workgroups as the CUs
 // hold at once (two each; one of 256 dims), or one step each if they are fewer:
 // sequences differ in length, and a share may end in the middle of a unit.
@@ -107,7 +109,8 @@ AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint
     const uint64_t rows = (uint64_t)b.max_new * (q_heads / kv.heads);
     // registers hold two tiles of at most 128 dims and bf16
     const bool two = kv.dim <= 128 && bf16;
-    p.tiles = rows <= 16 || (rows <= 32 && !two) ? 1 : rows <= 32 ? 2 : rows <= 64 || !two ? 4 : rows <= 128 ? 8 : 16;
+    const uint64_t pair = (uint64_t)b.seqs * kv.heads >= 128 ? 64 : 32;
+    p.tiles = rows <= 16 || (rows <= 32 && !two) ? 1 : two && rows <= pair ? 2 : rows <= 64 || !two ? 4 : rows <= 128 ? 8 : 16;
     const uint32_t tile = 16 * p.tiles;
     p.row_tiles = (uint32_t)((rows + tile - 1) / tile);
     const uint64_t steps = max_length > kStep ? (max_length + kStep - 1) / kStep : 1;

@@ -299,3 +299,13 @@ def test_many_sequences(ctx, count):
     news[count - 2], lens[count - 2] = 2, 2500
     c = Case(18, news, lens, 1, 64, 16, 8, 4)
     check(ctx, c, "bf16", 2, chain(news, lens), None)
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("count,news,lens", [(130, (33, 65), 50), (300, (0, 3), 600)])
+def test_many_units(ctx, io, count, news, lens):
+    """Units of 33 to 64 rows, and units of few steps, in calls with very many of them."""
+    rng = np.random.default_rng(count)
+    news, lens = rng.integers(*news, count).tolist(), rng.integers(0, lens, count).tolist()
+    c = Case(19, news, lens, 1, 64, 16, 8, 8)
+    check(ctx, c, io, 1, chain(news, lens), None)
