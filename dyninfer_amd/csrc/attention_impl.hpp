@@ -425,6 +425,13 @@ __device__ __forceinline__ Share share_of(const AttnArgs& a, uint32_t rows_of_ti
     return f;
 }
 
+// x, opaque: what is computed from it stays in its branch.  (The tests of the mask's bits
+// were done in every step, a tenth of its vector instructions.)
+__device__ __forceinline__ uint32_t here(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // A wave's rows: NQ tiles of 16, their queries as operands, running statistics
 // and unnormalised outputs.  The two kernels differ in how the cache's codes come
 // to hold as operands; a step takes 32 positions, of which lane group g holds
@@ -571,9 +578,11 @@ struct WaveRows {
         }
         if (masked) {
 #pragma unroll
-            for (int t = 0; t < NQ; t++)
+            for (int t = 0; t < NQ; t++) {
+                const uint32_t see = here(vis[t]);
 #pragma unroll
-                for (int i = 0; i < 8; i++) sc[t][i / 4][i % 4] = vis[t] >> i & 1u ? sc[t][i / 4][i % 4] : -__builtin_inff();
+                for (int i = 0; i < 8; i++) sc[t][i / 4][i % 4] = see >> i & 1u ? sc[t][i / 4][i % 4] : -__builtin_inff();
+            }
         }
 
         // Exponentials, from a reference that follows the row's largest score only when
@@ -603,8 +612,9 @@ struct WaveRows {
                 p[i] = e * vs[i];
             }
             if (masked) {  // a masked value's scale may be anything
+                const uint32_t see = here(vis[t]);
 #pragma unroll
-                for (int i = 0; i < 8; i++) p[i] = vis[t] >> i & 1u ? p[i] : 0.0f;
+                for (int i = 0; i < 8; i++) p[i] = see >> i & 1u ? p[i] : 0.0f;
             }
 #pragma unroll
             for (int n = 0; n < TERMS; n++) {
