@@ -23,7 +23,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // Logits of a workgroup of the statistics.  Few rows are cut finer, for the
 // latency of one pass: 5 bf16 rows of 151936 in 16384s took 9.3 us, in 4096s 5.4
-// (4.8 with four loads in flight); 493 f32 rows, 300 MB, take 38 us, 49.8 with one
+// (4.8 with four loads in flight); 376 f32 rows, 228 MB, take 38 us, 49.8 with one
 // load in flight and an accurate exponential of every element.
 constexpr uint32_t kPiece = 16384, kSmallPiece = 4096;
 constexpr uint32_t kManyPieces = 1024;  // workgroups from which the large pieces are taken
