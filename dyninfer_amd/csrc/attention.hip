@@ -104,7 +104,10 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t rows_of_
 // 32 ragged sequences of up to 512, 1024 and 2048 positions with 8 rows took 19, 28
 // and 48 us that way and 29, 35 and 49 in shares, one sequence of 380 with one row 9.6
 // and 11.4, of 760 14.6 and 11.9, 100 of up to 8000 272 and 206.
-AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint32_t q_heads, bool bf16) {
+// Rows of a chain see only what lies before them, so a prompt's row tiles differ in
+// length, which only whole units make use of: taken where what is left out is worth
+// a unit a CU.
+AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint32_t q_heads, bool bf16, bool chain) {
     AttnPlan p = {};
     const uint64_t rows = (uint64_t)b.max_new * (q_heads / kv.heads);
     // registers hold two tiles of at most 128 dims and bf16
@@ -117,7 +120,8 @@ AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint
     const uint64_t units = (uint64_t)b.seqs * kv.heads * p.row_tiles;
     const uint64_t full = kv.dim > 128 || p.tiles == 16 ? 256 : 512;
     const uint64_t few = (p.tiles <= 2 ? 3 : 1) + units / 32;
-    if (steps <= (few < 12 ? few : 12) || units >= 8 * full) {
+    const bool prompt = chain && units * (double)b.max_new >= 2.0 * full * max_length;
+    if (steps <= (few < 12 ? few : 12) || units >= 8 * full || prompt) {
         p.grid = units;
         return p;
     }

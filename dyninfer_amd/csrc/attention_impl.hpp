@@ -319,11 +319,24 @@ __device__ __forceinline__ uint32_t shares_of(const AttnArgs& a, uint64_t all) {
     return (uint32_t)min((uint64_t)a.shares, all);
 }
 
-// Without shares: workgroup (sequence, head, row tile), all of its steps.
+// Positions that some of the rows first..end-1 of a unit's may see are below this: in a
+// chain those up to the last of their tokens, otherwise all.
+__device__ __forceinline__ uint64_t seen_by_some(const AttnArgs& a, const SeqRange& r, uint32_t end) {
+    return (uint64_t)r.len + (a.mask ? r.n : (end - 1) / a.group + 1);
+}
+
+// Tiles of TILE positions below this are seen whole by all rows from first on.
+template <uint32_t TILE>
+__device__ __forceinline__ uint32_t open_tiles(const AttnArgs& a, const SeqRange& r, uint32_t first) {
+    return (uint32_t)(((uint64_t)r.len + (a.mask ? 0u : first / a.group + 1)) / TILE);
+}
+
+// Without shares: workgroup (sequence, head, row tile), all of its steps; the last
+// row tile first, which has the most positions where rows form a chain.
 __device__ __forceinline__ Share whole_unit(const AttnArgs& a, uint32_t rows_of_tile) {
     Share s = {};
     uint32_t id = by_xcd(blockIdx.x, gridDim.x);
-    const uint32_t rt = id % a.row_tiles;
+    const uint32_t rt = a.row_tiles - 1 - id % a.row_tiles;
     id /= a.row_tiles;
     s.seq = id / a.kv.heads;
     s.load(a, rows_of_tile);
@@ -807,10 +820,11 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
         const uint32_t seq = sh.seq, head = sh.unit / sh.row_tiles, tile_row = sh.unit % sh.row_tiles * ROWS;
         const SeqRange r = seq_range(a.b, seq);
         const uint32_t rows = r.n * a.group;
-        const uint64_t total = (uint64_t)r.len + r.n;
+        const uint64_t total = seen_by_some(a, r, min(tile_row + ROWS, rows));
+        const uint32_t open = open_tiles<kTile>(a, r, tile_row);
         const bool alone = now0 == 0 && now1 == sh.unit_steps;
         const uint64_t begin = (uint64_t)now0 * kStep;
-        // a multiple of the tile, but for the sequence's own end, where sees() ends
+        // a multiple of the tile, but for the end of what the rows see, where sees() ends
         const uint64_t end = min(total, (uint64_t)now1 * kStep);
 
         // This wave's tiles: every fourth from the wave-th.
@@ -857,7 +871,7 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
             uint32_t ln = lane;
             asm volatile("" : "+v"(ln));
             const uint32_t g = ln >> 4, col = ln & 15u;
-            const bool masked = gone != 0 || (uint64_t)p0 + kTile > r.len;
+            const bool masked = gone != 0 || tile0 + kWaves * k >= open;
             uint32_t vis[NQ] = {};
             if (masked) {
 #pragma unroll
@@ -950,11 +964,12 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 ? 2 : 1) void attend_wide_kerne
         const uint32_t first_row = tile_row + wave * (16u * NQ);
         const SeqRange r = seq_range(a.b, seq);
         const uint32_t rows = r.n * a.group;
-        const uint64_t total = (uint64_t)r.len + r.n;
+        const uint64_t total = seen_by_some(a, r, min(tile_row + ROWS, rows));
+        const uint32_t open = scalar(open_tiles<kWideTile>(a, r, first_row));
         const bool alone = now0 == 0 && now1 == sh.unit_steps;
         const uint32_t tile0 = now0 * (kStep / kWideTile);
         const uint32_t ends = (uint32_t)((min(total, (uint64_t)now1 * kStep) + kWideTile - 1) / kWideTile);
-        const uint32_t count = ends - tile0;
+        const uint32_t count = tile0 < ends ? ends - tile0 : 0;
         const Pages page_of(a, seq);
 
         int32_t ids[4];  // of the next tile to load
@@ -1102,7 +1117,7 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 ? 2 : 1) void attend_wide_kerne
                     uint32_t ln = lane;
                     asm volatile("" : "+v"(ln));
                     const uint32_t g = ln >> 4;
-                    const bool masked = gone != 0 || (uint64_t)p0 + kWideTile > r.len;
+                    const bool masked = gone != 0 || tile0 + k >= open;
                     uint32_t vis[NQ] = {};
                     if (masked) {
 #pragma unroll
@@ -1126,7 +1141,9 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 ? 2 : 1) void attend_wide_kerne
                 w.l[t] = rows_sum(w.l[t]);
                 w.m[t] = w.l[t] == 0.0f ? -__builtin_inff() : w.m[t] == -__builtin_inff() ? 0.0f : w.m[t];
             }
-            w.store(a, sh, r, head, tile_row, first_row, rows, ROWS, alone, lane);
+            uint32_t ln = lane;
+            asm volatile("" : "+v"(ln));  // the places are made here, not held through the loop
+            w.store(a, sh, r, head, tile_row, first_row, rows, ROWS, alone, ln);
         }
     }
 }

@@ -90,7 +90,7 @@ struct AttnPlan {
     uint64_t grid;
     uint64_t bytes, stats, where;  // workspace, and where its parts begin
 };
-AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint32_t q_heads, bool bf16);
+AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint32_t q_heads, bool bf16, bool chain);
 struct AttnArgs {
     KvView kv;
     KvBatch b;

@@ -334,7 +334,7 @@ int dyninfer_mi355x_tree_attention_workspace_bytes(const dyninfer_kvcache_t* cac
     dmx::KvView kv = {};
     kv.heads = cache->kv_heads;
     kv.dim = cache->head_dim;
-    *out_bytes = dmx::attn_plan(kv, b, batch->max_length, q_heads, dtype == DYNINFER_DTYPE_BF16).bytes;
+    *out_bytes = dmx::attn_plan(kv, b, batch->max_length, q_heads, dtype == DYNINFER_DTYPE_BF16, false).bytes;
     return DYNINFER_MI355X_OK;
 }
 
@@ -359,7 +359,7 @@ int dyninfer_mi355x_tree_attention(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kv
     if (!std::isfinite(scale)) return fail(BAD, "scale must be finite");
     a.group = q->heads / a.kv.heads;
     if ((uint64_t)a.b.max_new * a.group > 0x7FFFFFFFull) return fail(UNSUPPORTED, "too many rows of one kv head");
-    const dmx::AttnPlan plan = dmx::attn_plan(a.kv, a.b, batch->max_length, q->heads, a.q.bf16);
+    const dmx::AttnPlan plan = dmx::attn_plan(a.kv, a.b, batch->max_length, q->heads, a.q.bf16, !mask);
     if (int rc = check_workspace(workspace, workspace_bytes, plan.bytes, "tree_attention")) return rc;
     if (int rc = check_grid(plan.grid)) return rc;
     if (int rc = check_grid((uint64_t)a.b.seqs * a.b.max_new / 4)) return rc;

@@ -309,3 +309,27 @@ def test_many_units(ctx, io, count, news, lens):
     news, lens = rng.integers(*news, count).tolist(), rng.integers(0, lens, count).tolist()
     c = Case(19, news, lens, 1, 64, 16, 8, 8)
     check(ctx, c, io, 1, chain(news, lens), None)
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,group,news,lens", [
+    (16, 1, [300] * 15 + [1, 257], [0] * 10 + [33] * 7),  # units of many row tiles, whole
+    (4, 4, [700, 130], [0, 500]), (8, 3, [1500, 0, 64], [0, 9, 2000])])
+def test_prompts(ctx, io, heads, group, news, lens):
+    """Long chains: a row tile stops at its last row's own position."""
+    c = Case(20, news, lens, heads, 64, 64, 8, 8)
+    check(ctx, c, io, heads * group, chain(news, lens), None)
+
+
+def test_a_prompt_in_whole_units(ctx):
+    """Row tiles many and long enough that they are not cut: the first and last rows of some."""
+    n, heads = 4500, 8
+    c = Case(21, [n], [0], heads, 64, 256, 8, 8)
+    assert ctx.tree_attention_workspace_bytes(c.cache, c.batch, heads, d.DTYPE_BF16) > 0
+    q, qf = rows(c.rng, n, heads, 64, torch.bfloat16, "plain")
+    got = ctx.tree_attention(c.cache, c.batch, q).float().cpu().numpy()
+    k, v = (c.ref.rows(c.table[0], 0, n, kind) for kind in "kv")
+    for i in (0, 1, 63, 64, 255, 256, 257, 1023, 1024, 2049, 4351, 4352, n - 1):
+        o, _, mag, dot = kvref.attend(qf[i:i + 1].astype(np.float64), k[:i + 1], v[:i + 1], np.ones((1, i + 1), bool), 0.125)
+        rel = 2 * dot * 2.0 ** -24 * (64 + 16) + 2.0 ** -16 + 2.0 ** -24 * (32 + n / 4)
+        assert (np.abs(got[i] - o[0]) <= rel[0][:, None] * mag[0] + 2.0 ** -8 * np.abs(o[0]) + 1e-30).all()
