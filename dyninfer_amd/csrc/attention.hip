@@ -91,11 +91,17 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t rows_of_
 
 }  // namespace
 
-// Row tiles: one or two of 16 rows held by every wave, or four or eight held by
-// four waves (64 tokens x group 4 over 131k positions: 572 us with one, 382 with two,
-// 401 with four, 300 with eight; 8 x 4 over 4k in 32 sequences: 74, 70, 89, 98).  33 to
-// 64 rows take two where there are units enough (16 x 4 over 1k and 4k in 32 sequences:
-// 33 and 94 with two, 43 and 97 with four; over 4k in one: 23 and 18).
+// Row tiles: one or two of 16 rows held by every wave, or four, eight or sixteen held
+// one or two a wave (four waves, eight of sixteen).  Larger ones decode a position for
+// more rows, smaller ones make more workgroups and leave out more of a prompt.  Times (us)
+// with 2, 4, 8 and 16, 4 rows a token, by `work`, the steps of all units of eight tiles:
+//   1 x 63 tokens after 500 (work 80): 17.2 15.6 19.3 23.8; after 4000 (528): 30.8 34.8 41.3
+//   40.5; 32 x 63 after 4000 (16896): 425 390 293 281; 1 x 16 after 4000 (128): 22.9 18.0,
+//   after 64000 (2000): 73 77 89; 32 x 16 after 1000 (1024): 33 43 58
+//   prompts: 1 x 512 (512): 18.7 23.2 30.8 42.9; 1 x 1024 (2048): 43.9 44.2 55.7 74.4; 4 x 2048
+//   (32768): 419 374 286 297; 1 x 512 after 8000: 193 207 156 151
+// f32 and 256 dims hold one row tile a wave: 32 x 8 after 4000 77 with one, 88 with four;
+// 32 x 16 126 and 100 (f32).
 // The steps of all units go in equal shares to as many workgroups as the CUs
 // hold at once (two each; one of 256 dims), or one step each if they are fewer:
 // sequences differ in length, and a share may end in the middle of a unit.
@@ -112,11 +118,18 @@ AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint
     const uint64_t rows = (uint64_t)b.max_new * (q_heads / kv.heads);
     // registers hold two tiles of at most 128 dims and bf16
     const bool two = kv.dim <= 128 && bf16;
-    const uint64_t pair = (uint64_t)b.seqs * kv.heads >= 128 ? 64 : 32;
-    p.tiles = rows <= 16 || (rows <= 32 && !two) ? 1 : two && rows <= pair ? 2 : rows <= 64 || !two ? 4 : rows <= 128 ? 8 : 16;
+    const uint64_t steps = max_length > kStep ? (max_length + kStep - 1) / kStep : 1;
+    const double heads = (double)b.seqs * kv.heads, eights = heads * (double)rows / 128, work = eights * (double)steps;
+    const bool fresh = chain && 2ull * b.max_new > max_length;  // mostly a prompt
+    if (rows <= 16) p.tiles = 1;
+    else if (!two) p.tiles = rows <= 32 ? 1 : 4;
+    else if (rows <= 32) p.tiles = 2;
+    else if (work <= 200) p.tiles = 4;
+    else if (work <= 1024 || rows <= 64) p.tiles = 2;
+    else if (fresh && eights <= 512 && steps <= 16) p.tiles = 4;
+    else p.tiles = rows <= 128 || fresh ? 8 : 16;
     const uint32_t tile = 16 * p.tiles;
     p.row_tiles = (uint32_t)((rows + tile - 1) / tile);
-    const uint64_t steps = max_length > kStep ? (max_length + kStep - 1) / kStep : 1;
     const uint64_t units = (uint64_t)b.seqs * kv.heads * p.row_tiles;
     const uint64_t full = kv.dim > 128 || p.tiles == 16 ? 256 : 512;
     const uint64_t few = (p.tiles <= 2 ? 3 : 1) + units / 32;

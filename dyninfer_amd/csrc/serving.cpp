@@ -2,6 +2,7 @@
 // positions, the quantized paged cache, attention of drafted tokens over it,
 // and their verification.  Checks here keep every kernel inside the buffers
 // described; what the host cannot see (device tables) the kernels check.
+#include <algorithm>
 #include <cmath>
 #include <utility>
 
@@ -334,7 +335,8 @@ int dyninfer_mi355x_tree_attention_workspace_bytes(const dyninfer_kvcache_t* cac
     dmx::KvView kv = {};
     kv.heads = cache->kv_heads;
     kv.dim = cache->head_dim;
-    *out_bytes = dmx::attn_plan(kv, b, batch->max_length, q_heads, dtype == DYNINFER_DTYPE_BF16, false).bytes;
+    for (bool chain : {false, true})  // enough with a mask and without
+        *out_bytes = std::max(*out_bytes, dmx::attn_plan(kv, b, batch->max_length, q_heads, dtype == DYNINFER_DTYPE_BF16, chain).bytes);
     return DYNINFER_MI355X_OK;
 }
 
