@@ -20,6 +20,7 @@ Reference correspondences:
 from __future__ import annotations
 
 import ctypes
+import functools
 import json
 import os
 import struct
@@ -322,6 +323,14 @@ def _bad(message: str):
 
 _T_F32, _T_I32, _T_I64 = 0, 1, 2
 _TABLE_DTYPES: list = []  # torch's dtypes of these codes, filled on first use
+
+
+@functools.lru_cache(maxsize=64)
+def _verify_workspace_bytes(seqs: int, tokens: int, vocab: int, max_new: int) -> int:
+    """dyninfer_mi355x_draft_verify_workspace_bytes, which depends on these numbers only."""
+    need = ctypes.c_uint64(0)
+    _check(library().dyninfer_mi355x_draft_verify_workspace_bytes(seqs, tokens, vocab, max_new, ctypes.byref(need)))
+    return need.value
 
 
 def _table(t, code: int, shape, what: str) -> int:
@@ -702,19 +711,20 @@ class Context:
             _bad("draft_probs must be a device tensor of the logits' shape whose last axis is contiguous")
         if not noise.is_cuda or noise.dtype != torch.float32 or noise.shape != (seqs, vocab) or noise.stride(1) != 1:
             _bad("noise must be a device tensor [sequences, vocab] of float32 whose last axis is contiguous")
-        sp = _table(starts, _T_I32, (None,), "starts")
+        sp, dp = _table(starts, _T_I32, (None,), "starts"), _table(draft_tokens, _T_I64, (n,), "draft_tokens")
         tp = None if temperature is None else _table(temperature, _T_F32, (seqs,), "temperature")
         pp = None if parents is None else _table(parents, _T_I32, (n,), "parents")
-        path = self._new((seqs, max_new), torch.int32, logits.device, stream)
-        counts = self._new((seqs,), torch.int32, logits.device, stream)
-        token = self._new((seqs,), torch.int64, logits.device, stream)
-        need = ctypes.c_uint64(0)
-        _check(self._lib.dyninfer_mi355x_draft_verify_workspace_bytes(seqs, n, vocab, max_new, ctypes.byref(need)))
-        wp, wn, _keep = self._work(need.value, workspace, logits.device, stream)
+        if stream is None:  # new_empty: 0.3 us less each than torch.empty
+            path, counts, token = starts.new_empty((seqs, max_new)), starts.new_empty((seqs,)), draft_tokens.new_empty((seqs,))
+        else:
+            path = self._new((seqs, max_new), torch.int32, logits.device, stream)
+            counts = self._new((seqs,), torch.int32, logits.device, stream)
+            token = self._new((seqs,), torch.int64, logits.device, stream)
+        wp, wn, _keep = self._work(_verify_workspace_bytes(seqs, n, vocab, max_new), workspace, logits.device, stream)
         args = _pack_verify(
             logits.data_ptr(), 0 if draft_probs is None else draft_probs.data_ptr(), _dtype_code(logits),
             0 if draft_probs is None else _dtype_code(draft_probs), logits.stride(0),
-            0 if draft_probs is None else draft_probs.stride(0), _table(draft_tokens, _T_I64, (n,), "draft_tokens"),
+            0 if draft_probs is None else draft_probs.stride(0), dp,
             pp or 0, sp, tp or 0, _table(uniform, _T_F32, (n,), "uniform"), noise.data_ptr(), noise.stride(0),
             vocab, seqs, n, max_new, path.data_ptr(), counts.data_ptr(), token.data_ptr())
         _check(self._lib.dyninfer_mi355x_draft_verify(self._h, args, wp, wn, self._on(stream)))
