@@ -15,30 +15,20 @@ namespace {
 // One wave per (row, query head) whose unit was split: the parts' maxima and
 // sums, then the parts' outputs, each brought to the common maximum.
 template <int D>
-__global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t rows_of_tile) {
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t tile_shift) {
     constexpr int W = D <= 128 ? 2 : 4;  // dims of a lane
     const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t q_heads = a.kv.heads * a.group;
-    const uint64_t id = (uint64_t)blockIdx.x * 4 + scalar(threadIdx.x >> 6);
-    const uint64_t rest = divide(id, q_heads);
-    const uint32_t h = (uint32_t)(id - rest * q_heads);
-    const uint64_t seq_at = divide(rest, a.b.max_new);
-    if (seq_at >= a.b.seqs) return;
-    const uint32_t i = (uint32_t)(rest - seq_at * a.b.max_new), seq = (uint32_t)seq_at;
-    const uint64_t all = a.where[2 * a.b.seqs], first = a.where[2 * seq], unit0 = a.where[2 * seq + 1];
-    Share s = {};
-    s.seq = seq;
-    s.load(a, rows_of_tile);
+    const uint32_t q_heads = a.kv.heads * a.group, seq = blockIdx.y, id = blockIdx.x * 4 + scalar(threadIdx.x >> 6);
+    const uint32_t i = id / q_heads, h = id - i * q_heads;
+    if (i >= a.b.max_new) return;
+    const uint32_t kv_head = h / a.group, row = i * a.group + (h - kv_head * a.group);
+    const uint32_t* const noted = a.where + 2 * ((seq * a.kv.heads + kv_head) * a.row_tiles + (row >> tile_shift));
     const SeqRange r = seq_range(a.b, seq);
     if (i >= r.n) return;
-    const uint32_t kv_head = h / a.group, row = i * a.group + (h - kv_head * a.group);
-    const uint32_t unit = kv_head * s.row_tiles + row / rows_of_tile;
-    // the shares that hold the unit's first and last step: share w begins at floor(w all / shares)
-    const uint64_t x0 = first + (uint64_t)unit * (s.unit_steps + kUnitCost) + kUnitCost, x1 = x0 + s.unit_steps - 1;
-    const uint64_t n = shares_of(a, all), w0 = divide((x0 + 1) * n - 1, all), w1 = divide((x1 + 1) * n - 1, all);
-    const uint32_t parts = (uint32_t)(w1 - w0) + 1;
+    const uint32_t parts = noted[1] - noted[0] + 1;
     if (parts == 1) return;  // written by the first launch
-    const uint64_t at = (w0 + unit0 + unit) * rows_of_tile + row % rows_of_tile;
+    const uint32_t rows_of_tile = 1u << tile_shift;
+    const uint64_t at = (uint64_t)noted[0] * rows_of_tile + (row & (rows_of_tile - 1));
     const float* po = a.parts + at * D;
     const float* ml = a.stats + 2 * at;
     const uint64_t pitch = rows_of_tile;  // rows from one part to the next
@@ -144,7 +134,7 @@ AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint
     const uint64_t slots = (units + p.shares) * tile;
     p.stats = slots * kv.dim * 4;
     p.where = p.stats + slots * 8;
-    p.bytes = p.where + (2 * (uint64_t)b.seqs + 1) * 8;
+    p.bytes = p.where + 8 * units;
     return p;
 }
 
@@ -154,20 +144,21 @@ hipError_t attn_launch(AttnArgs a, const AttnPlan& plan, uint8_t* work, hipStrea
     a.shares = plan.shares;
     a.parts = reinterpret_cast<float*>(work);
     a.stats = reinterpret_cast<float*>(work + plan.stats);
-    a.where = reinterpret_cast<uint64_t*>(work + plan.where);
+    a.where = reinterpret_cast<uint32_t*>(work + plan.where);
     hipError_t e;
     if (a.kv.k_bits == 8)
         e = a.kv.v_bits == 8 ? attend_launch<8, 8>(a, plan.tiles, plan.grid, st) : attend_launch<8, 4>(a, plan.tiles, plan.grid, st);
     else
         e = a.kv.v_bits == 8 ? attend_launch<4, 8>(a, plan.tiles, plan.grid, st) : attend_launch<4, 4>(a, plan.tiles, plan.grid, st);
     if (e != hipSuccess || plan.shares == 0) return e;
-    const uint64_t waves = (uint64_t)a.b.seqs * a.b.max_new * a.kv.heads * a.group;
-    const uint32_t blocks = (uint32_t)((waves + 3) / 4), tile = 16 * plan.tiles;
+    // with shares there are fewer units than the grid's second axis allows
+    const dim3 blocks((uint32_t)(((uint64_t)a.b.max_new * a.kv.heads * a.group + 3) / 4), a.b.seqs);
+    const uint32_t shift = (uint32_t)__builtin_ctz(16 * plan.tiles);
     switch (a.kv.dim) {
-    case 64: join_kernel<64><<<blocks, 256, 0, st>>>(a, tile); break;
-    case 96: join_kernel<96><<<blocks, 256, 0, st>>>(a, tile); break;
-    case 128: join_kernel<128><<<blocks, 256, 0, st>>>(a, tile); break;
-    case 256: join_kernel<256><<<blocks, 256, 0, st>>>(a, tile); break;
+    case 64: join_kernel<64><<<blocks, 256, 0, st>>>(a, shift); break;
+    case 96: join_kernel<96><<<blocks, 256, 0, st>>>(a, shift); break;
+    case 128: join_kernel<128><<<blocks, 256, 0, st>>>(a, shift); break;
+    case 256: join_kernel<256><<<blocks, 256, 0, st>>>(a, shift); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

@@ -331,6 +331,16 @@ __device__ __forceinline__ uint32_t open_tiles(const AttnArgs& a, const SeqRange
     return (uint32_t)(((uint64_t)r.len + (a.mask ? 0u : first / a.group + 1)) / TILE);
 }
 
+// Notes which parts a unit has, for the second launch: the share that has its first step
+// writes the first, the one that has its last step the last.
+__device__ __forceinline__ void note_parts(const AttnArgs& a, const Share& sh, uint32_t head, uint32_t now0, uint32_t now1) {
+    if (a.shares == 0 || threadIdx.x != 0) return;
+    uint32_t* const to = a.where + 2 * ((sh.seq * a.kv.heads + head) * a.row_tiles + (sh.unit - head * sh.row_tiles));
+    const uint32_t part = sh.share + (uint32_t)sh.unit0 + sh.unit;
+    if (now0 == 0) to[0] = part;
+    if (now1 == sh.unit_steps) to[1] = part;
+}
+
 // Without shares: workgroup (sequence, head, row tile), all of its steps; the last
 // row tile first, which has the most positions where rows form a chain.
 __device__ __forceinline__ Share whole_unit(const AttnArgs& a, uint32_t rows_of_tile) {
@@ -369,12 +379,9 @@ __device__ __forceinline__ uint64_t divide(uint64_t x, uint64_t y) {
 }
 
 // This workgroup's share.  Every wave finds it by itself, 64 sequences at a time, so
-// that no barrier stands before its first copies.  The first wave of the first
-// workgroup also writes where each sequence's places and units begin, for the
-// second launch.
+// that no barrier stands before its first copies.
 __device__ __forceinline__ Share share_of(const AttnArgs& a, uint32_t rows_of_tile) {
     const uint32_t lane = threadIdx.x & 63u;
-    const bool writes = blockIdx.x == 0 && scalar(threadIdx.x >> 6) == 0;
     uint64_t places = 0, units = 0, at = 0, to = 0, all = 0;
     uint32_t share = 0;
     if (a.b.seqs > 64) {  // how many places there are
@@ -406,10 +413,6 @@ __device__ __forceinline__ Share share_of(const AttnArgs& a, uint32_t rows_of_ti
             }
         }
         const uint64_t first = before + x - places, unit0 = units_before + y - units;
-        if (writes && s0 + lane < a.b.seqs) {
-            a.where[2 * (s0 + lane)] = first;
-            a.where[2 * (s0 + lane) + 1] = unit0;
-        }
         const unsigned long long who = __ballot(at < to && first <= at && at < first + places);
         if (who) {  // the sequence of the share's first place
             const int w = __builtin_ctzll(who);
@@ -421,12 +424,11 @@ __device__ __forceinline__ Share share_of(const AttnArgs& a, uint32_t rows_of_ti
             f.unit = (uint32_t)divide(in, f.unit_steps + kUnitCost);
             f.place = (uint32_t)(in - (uint64_t)f.unit * (f.unit_steps + kUnitCost));
             f.places = (uint32_t)(to - at);
-            if (!writes) break;
+            break;
         }
         before += __shfl((unsigned long long)x, 63);
         units_before += __shfl((unsigned long long)y, 63);
     }
-    if (writes && lane == 0) a.where[2 * a.b.seqs] = all;
     f.seq = scalar(f.seq);
     f.unit = scalar(f.unit);
     f.row_tiles = scalar(f.row_tiles);
@@ -934,6 +936,7 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
             __syncthreads();
         }
         if (wave == 0) w.store(a, sh, r, head, tile_row, tile_row, rows, ROWS, alone, lane);
+        note_parts(a, sh, head, now0, now1);
         __syncthreads();  // the LDS is the next unit's
     }
 }
@@ -1145,6 +1148,7 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 ? 2 : 1) void attend_wide_kerne
             asm volatile("" : "+v"(ln));  // the places are made here, not held through the loop
             w.store(a, sh, r, head, tile_row, first_row, rows, ROWS, alone, ln);
         }
+        note_parts(a, sh, head, now0, now1);
     }
 }
 

@@ -99,7 +99,7 @@ struct AttnArgs {
     float* lse;
     float* parts;     // [share + unit][row of the tile][dim], not yet over their sums
     float* stats;     // [share + unit][row of the tile][2]: what exponents are from, sum
-    uint64_t* where;  // [sequence][2]: steps and units before it; then all steps
+    uint32_t* where;  // [sequence][kv head][row tile][2]: its first and its last part
     uint32_t mask_words, group, row_tiles, shares;
     float scale;
 };
