@@ -564,8 +564,8 @@ class Context:
         return out
 
     # ---- around attention: rotary positions, the quantized cache, attention over it, verification
-    # Host time of a call (us, small sizes): rope 8.2, kv_append with queries 11.5, kv_read
-    # 11.5, tree_attention 15.5, draft_verify 22; of it the C entry, mostly its launches, 3.9 a launch,
+    # Host time of a call (us, small sizes): rope 8.1, kv_append with queries 11.0, kv_read
+    # 11.5, tree_attention 15.5, draft_verify 21; of it the C entry, mostly its launches, 3.9 a launch,
     # a new output or workspace 1.2 to 1.7, a checked descriptor 0.3 to 1.
     def _on(self, stream) -> int:
         """The raw stream: the given one, or the current one of the context's device."""
