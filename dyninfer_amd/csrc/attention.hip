@@ -13,7 +13,9 @@ template <> hipError_t attend_launch<4, 4>(const AttnArgs&, uint32_t, uint64_t, 
 namespace {
 
 // One wave per (row, query head) whose unit was split: the parts' maxima and
-// sums, then the parts' outputs, each brought to the common maximum.
+// sums, then the parts' outputs, each brought to the common maximum.  Bound by latency:
+// 5.4 us for 8192 rows of two or three parts (7.9 when every wave found its parts by
+// itself, with some 260 scalar instructions).
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t tile_shift) {
     constexpr int W = D <= 128 ? 2 : 4;  // dims of a lane

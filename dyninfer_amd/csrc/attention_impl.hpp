@@ -5,11 +5,11 @@
 //   S[p, r] = scale q_r . k_p,  out_r = sum_p exp(S - max) v_p / sum_p exp(S - max)
 //
 // over the positions p that row r sees.  Rows of one kv head are the new tokens
-// times the query heads that share it, r = token * group + head: up to 128 of
+// times the query heads that share it, r = token * group + head: up to 256 of
 // them share one pass over the cache.
 //
 // One pass, online: a step takes 32 positions; the running maximum and sum of
-// every row and the unnormalised output stay in registers.  Up to 32 rows every
+// every row and the unnormalised output stay in registers.  In tiles of up to 32 rows every
 // wave of a workgroup holds all of them and takes its own positions, and the
 // four join in LDS at the end; beyond, every wave holds its own rows, all take
 // the same positions and share their decoding.  Where positions are split over
@@ -803,7 +803,10 @@ struct OperandTile {
 constexpr int resident(int d, int nq) { return d * nq <= 256 && d < 256 ? 2 : 1; }
 
 // Few rows (up to 16 NQ): every wave holds all of them and takes every fourth
-// tile of positions, copied straight into LDS and decoded as it is read.
+// tile of positions, copied straight into LDS and decoded as it is read.  32 ragged
+// sequences of up to 4096 positions, 8 tokens of 32 / 8 heads of 128 dims: 48 us, 188 MB
+// at 3.9 TB/s, a wave issuing in 41% of its cycles and waiting in 34%; one token
+// over 700 positions 8.7 us, latency.
 template <int D, int KB, int VB, int NQ, bool F32>
 __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a) {
     using T = TileLds<D, KB, VB>;
@@ -945,7 +948,10 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
 // positions, 64 at a time.  The waves decode a part of the tile each and leave the
 // operands in LDS for all, one tile ahead; the codes of the tile after that are on
 // their way into registers.  A step of few rows spends two fifths of its vector
-// instructions on decoding; here that is shared by four or eight waves.
+// instructions on decoding; here that is shared by four or eight waves.  64 tokens over
+// 131071 positions of 8 heads, 256 rows each: 275 us, 137 GFLOP at 500 TFLOP/s (a third
+// more of products are the probabilities' second terms), bound by the issue of the vector
+// instructions around the products: 34% of the SIMDs' cycles are MFMAs.
 constexpr uint32_t kWideTile = 64;
 
 template <int D, int KB, int VB, int NQ, bool F32, int WAVES>

@@ -150,6 +150,8 @@ __device__ __forceinline__ void rope_row(const KvRows& x, const KvRows& y, uint3
     if (d0 < D) store8(y, (int64_t)token * y.ts + (int64_t)head * y.hs + d0, v);
 }
 
+// 4099 tokens of 40 heads of 128 dims in f32: 27.9 us, 6.2 TB/s.  (Four heads of a token by a
+// thread, which share its cosines: 29.4, one token 3.7 us instead of 2.2.)
 template <int D>
 __global__ __launch_bounds__(256) void rope_kernel(KvRows x, KvRows y, uint32_t tokens, uint32_t heads, RopeView rp) {
     constexpr uint32_t L = kLanes<D>;
@@ -278,7 +280,7 @@ __device__ __forceinline__ void turn4(uint32_t (&x)[4]) {
 // one per (sequence, chunk, kHeads heads); then the queries' rows.  A chunk of a
 // head's values is one wave's alone, so values of 4 bits, two tokens to a byte, are
 // merged without atomics.  (Keys by four tokens a thread: 220 registers, the whole
-// launch over 4 x 2048 tokens 86 us instead of 37.)
+// launch over 4 x 2048 tokens 86 us instead of 36, 146 MB at 4.1 TB/s.)
 template <int D, int KB, int VB>
 __global__ __launch_bounds__(256) void append_kernel(KvView kv, KvBatch b, KvRows k, KvRows v, RopeView rp, KvRows q,
                                                      KvRows q_out, uint32_t q_heads, uint32_t chunks, uint32_t k_blocks,
@@ -375,7 +377,8 @@ __global__ __launch_bounds__(256) void append_kernel(KvView kv, KvBatch b, KvRow
     }
 }
 
-// One workgroup per (sequence, chunk, kHeads heads), keys then values.
+// One workgroup per (sequence, chunk, kHeads heads), keys then values.  8 x 16k tokens of
+// 8 heads of 128 dims, 8 bits to bf16: 133 us, 5.2 TB/s, two thirds of it writes.
 template <int D, int KB, int VB>
 __global__ __launch_bounds__(256) void read_kernel(KvView kv, KvBatch b, KvRows k, KvRows v, uint32_t chunks,
                                                    uint32_t kv_blocks) {
@@ -447,6 +450,7 @@ __global__ __launch_bounds__(256) void read_kernel(KvView kv, KvBatch b, KvRows 
 // One workgroup per (sequence, head, keys or values).  A thread owns the same
 // bytes of every row (a dword of a key, a dim of a value), so its moves are in
 // order by themselves: a row's source lies at or after every row written so far.
+// Latency: 7.5 us for 16 trees of 24.
 template <int D, int KB, int VB>
 __global__ __launch_bounds__(256) void commit_kernel(KvView kv, KvBatch b, const int32_t* path, uint32_t path_stride,
                                                      const int32_t* counts) {
