@@ -92,8 +92,11 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t tile_shi
 //   after 64000 (2000): 73 77 89; 32 x 16 after 1000 (1024): 33 43 58
 //   prompts: 1 x 512 (512): 18.7 23.2 30.8 42.9; 1 x 1024 (2048): 43.9 44.2 55.7 74.4; 4 x 2048
 //   (32768): 419 374 286 297; 1 x 512 after 8000: 193 207 156 151
-// f32 and 256 dims hold one row tile a wave: 32 x 8 after 4000 77 with one, 88 with four;
-// 32 x 16 126 and 100 (f32).
+// f32, whose queries' second terms are in LDS where a wave holds two tiles: 1 x 8 after 500
+// 11.6 with one, 15.1 with two, after 60000 (938) 58.7 57.5, 32 x 8 after 4000 (2048)
+// 74.3 68.2 (88 with four); 32 x 16 after 4000 126 with one, 100 with four; 8 x 63 after 2000
+// (2016) 54.9 with four, 57.3 with sixteen, 32 x 63 after 1000 (4536) 130 115, 4 x 1024 as a
+// prompt 130 174.  256 dims: one tile a wave, 32 x 8 after 4000 160 with one, 211 with four.
 // The steps of all units go in equal shares to as many workgroups as the CUs
 // hold at once (two each; one of 256 dims), or one step each if they are fewer:
 // sequences differ in length, and a share may end in the middle of a unit.
@@ -108,13 +111,14 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t tile_shi
 AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint32_t q_heads, bool bf16, bool chain) {
     AttnPlan p = {};
     const uint64_t rows = (uint64_t)b.max_new * (q_heads / kv.heads);
-    // registers hold two tiles of at most 128 dims and bf16
-    const bool two = kv.dim <= 128 && bf16;
+    const bool two = kv.dim <= 128;  // registers hold two tiles of at most 128 dims
     const uint64_t steps = max_length > kStep ? (max_length + kStep - 1) / kStep : 1;
     const double heads = (double)b.seqs * kv.heads, eights = heads * (double)rows / 128, work = eights * (double)steps;
     const bool fresh = chain && 2ull * b.max_new > max_length;  // mostly a prompt
     if (rows <= 16) p.tiles = 1;
     else if (!two) p.tiles = rows <= 32 ? 1 : 4;
+    else if (!bf16 && rows <= 32) p.tiles = work <= 900 ? 1 : 2;
+    else if (!bf16) p.tiles = rows <= 128 || fresh || work <= 3000 ? 4 : 16;
     else if (rows <= 32) p.tiles = 2;
     else if (work <= 200) p.tiles = 4;
     else if (work <= 1024 || rows <= 64) p.tiles = 2;

@@ -456,7 +456,10 @@ struct WaveRows {
     static constexpr int NB = D / 32;          // blocks of a key
     static constexpr int DT = D / 16;          // 16-dim tiles of the output
     static constexpr int TERMS = F32 ? 3 : 2;  // bf16 terms of a probability
-    f16x8 qf[NQ][NB], ql[F32 ? NQ : 1][F32 ? NB : 1];
+    // second terms of f32 queries: in registers, with two tiles in LDS, a lane's NQ NB apart
+    static constexpr bool LOWS = F32 && NQ == 2;
+    f16x8 qf[NQ][NB], ql[F32 && !LOWS ? NQ : 1][F32 && !LOWS ? NB : 1];
+    f16x8* lows;
     float factor[NQ], m[NQ], l[NQ];  // m: what exponents are taken from, about the largest so far (log2)
     uint32_t tok[NQ];
     f32x4 o[NQ][DT];
@@ -528,12 +531,15 @@ struct WaveRows {
             factor[t] = fmaxf(factor[t], 1.2e-38f);  // a masked score is -inf also at scale 0
 #pragma unroll
             for (int b = 0; b < NB; b++) {
+                f16x8 low;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const float s = live ? x[b][i] * up : 0.0f;
                     qf[t][b][i] = (_Float16)s;
-                    if constexpr (F32) ql[t][b][i] = (_Float16)(s - (float)qf[t][b][i]);
+                    if constexpr (F32) low[i] = (_Float16)(s - (float)qf[t][b][i]);
                 }
+                if constexpr (LOWS) lows[(t * NB + b) * 64] = low;
+                else if constexpr (F32) ql[t][b] = low;
             }
             m[t] = -__builtin_inff();
             l[t] = 0.0f;
@@ -567,7 +573,9 @@ struct WaveRows {
 #pragma unroll
                 for (int t = 0; t < NQ; t++) {
                     x[b][t] = f32x4{0, 0, 0, 0};
-                    if constexpr (F32) x[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[b], ql[t][b], x[b][t], 0, 0, 0);
+                    if constexpr (F32)
+                        x[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[b], LOWS ? lows[(t * NB + b) * 64] : ql[LOWS ? 0 : t][LOWS ? 0 : b],
+                                                                         x[b][t], 0, 0, 0);
                     x[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[b], qf[t][b], x[b][t], 0, 0, 0);
                 }
             }
@@ -811,11 +819,14 @@ template <int D, int KB, int VB, int NQ, bool F32>
 __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a) {
     using T = TileLds<D, KB, VB>;
     constexpr int DT = D / 16;
-    constexpr uint32_t R = T::STAGES, ROWS = 16u * NQ;
+    constexpr uint32_t ROWS = 16u * NQ, LOWS = WaveRows<D, KB, VB, NQ, F32>::LOWS ? NQ * (D / 32) * 64 : 0;
+    // a stage less where the queries' second terms would leave one workgroup a CU
+    constexpr uint32_t R = T::STAGES - (LOWS != 0 && kWaves * T::STAGES * T::BYTES + LOWS * 16 + 2048 > 80 * 1024 ? 1 : 0);
     constexpr uint32_t JOIN = NQ * DT * 1024;  // bytes of a wave's output
     constexpr uint32_t LDS = kWaves * R * T::BYTES > 2 * JOIN ? kWaves * R * T::BYTES : 2 * JOIN;
     __shared__ __align__(16) uint8_t lds[LDS];
     __shared__ float sm_m[kWaves][ROWS], sm_l[kWaves][ROWS];
+    __shared__ f16x8 sm_low[LOWS ? LOWS : 1];  // every wave writes the same
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     Share sh = a.shares == 0 ? whole_unit(a, ROWS) : share_of(a, ROWS);
@@ -858,6 +869,7 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
         };
         using Rows = WaveRows<D, KB, VB, NQ, F32>;
         Rows w;
+        w.lows = sm_low + lane;
         typename Rows::Raw raw;
         w.load(a, r, head, tile_row, rows, lane, raw);
         for (uint32_t k = 0; k < R && k < count; k++) {
@@ -949,8 +961,8 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
 // operands in LDS for all, one tile ahead; the codes of the tile after that are on
 // their way into registers.  A step of few rows spends two fifths of its vector
 // instructions on decoding; here that is shared by four or eight waves.  64 tokens over
-// 131071 positions of 8 heads, 256 rows each: 275 us, 137 GFLOP at 500 TFLOP/s (a third
-// more of products are the probabilities' second terms), bound by the issue of the vector
+// 131071 positions of 8 heads, 256 rows each: 275 us, 137 GFLOP at 500 TFLOP/s (and half
+// as many products again for the probabilities' second terms), bound by the issue of the vector
 // instructions around the products: 34% of the SIMDs' cycles are MFMAs.
 constexpr uint32_t kWideTile = 64;
 
@@ -962,7 +974,9 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 ? 2 : 1) void attend_wide_kerne
     constexpr uint32_t KF = 0, VF = 4 * NB * 1024;       // operands: [S][block][lane], [half][dims][lane]
     constexpr uint32_t KS = VF + 2 * DT * 1024, VS = KS + 64 * NB * 4, BUF = VS + 256;  // scales in f32
     constexpr int KU = (4 * PAIRS + WAVES - 1) / WAVES, VU = (DT + WAVES - 1) / WAVES;  // units of a wave: (S, pair), 16 dims
+    constexpr uint32_t LOWS = WaveRows<D, KB, VB, NQ, F32>::LOWS ? NQ * NB * 64 : 0;
     __shared__ __align__(16) uint8_t lds[2 * BUF];
+    __shared__ f16x8 sm_low[LOWS ? WAVES * LOWS : 1];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     Share sh = a.shares == 0 ? whole_unit(a, ROWS) : share_of(a, ROWS);
@@ -1095,6 +1109,7 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 ? 2 : 1) void attend_wide_kerne
 
         using Rows = WaveRows<D, KB, VB, NQ, F32>;
         Rows w;
+        w.lows = sm_low + wave * LOWS + lane;
         typename Rows::Raw raw;
         w.load(a, r, head, first_row, rows, lane, raw);
         look_up(0);
@@ -1166,25 +1181,28 @@ template <int D, int KB, int VB>
 hipError_t attend_launch_dim(const AttnArgs& a, uint32_t tiles, uint64_t grid, hipStream_t st) {
     const dim3 gd((uint32_t)grid), bd(64 * kWaves);
     if (tiles >= 4) {  // 64, 128 or 256 rows
-        if (!a.q.bf16) {
-            attend_wide_kernel<D, KB, VB, 1, true, 4><<<gd, bd, 0, st>>>(a);
-        } else if (tiles == 4) {
-            attend_wide_kernel<D, KB, VB, 1, false, 4><<<gd, bd, 0, st>>>(a);
+        if (tiles == 4) {
+            if (a.q.bf16) attend_wide_kernel<D, KB, VB, 1, false, 4><<<gd, bd, 0, st>>>(a);
+            else attend_wide_kernel<D, KB, VB, 1, true, 4><<<gd, bd, 0, st>>>(a);
         } else {
             if constexpr (D <= 128) {
-                if (tiles == 8) attend_wide_kernel<D, KB, VB, 2, false, 4><<<gd, bd, 0, st>>>(a);
+                if (!a.q.bf16) attend_wide_kernel<D, KB, VB, 2, true, 8><<<gd, dim3(512), 0, st>>>(a);
+                else if (tiles == 8) attend_wide_kernel<D, KB, VB, 2, false, 4><<<gd, bd, 0, st>>>(a);
                 else attend_wide_kernel<D, KB, VB, 2, false, 8><<<gd, dim3(512), 0, st>>>(a);
             } else {
                 return hipErrorInvalidValue;
             }
         }
-    } else if (!a.q.bf16) {
-        attend_kernel<D, KB, VB, 1, true><<<gd, bd, 0, st>>>(a);
     } else if (tiles == 1) {
-        attend_kernel<D, KB, VB, 1, false><<<gd, bd, 0, st>>>(a);
+        if (a.q.bf16) attend_kernel<D, KB, VB, 1, false><<<gd, bd, 0, st>>>(a);
+        else attend_kernel<D, KB, VB, 1, true><<<gd, bd, 0, st>>>(a);
     } else {
-        if constexpr (D <= 128) attend_kernel<D, KB, VB, 2, false><<<gd, bd, 0, st>>>(a);
-        else return hipErrorInvalidValue;
+        if constexpr (D <= 128) {
+            if (a.q.bf16) attend_kernel<D, KB, VB, 2, false><<<gd, bd, 0, st>>>(a);
+            else attend_kernel<D, KB, VB, 2, true><<<gd, bd, 0, st>>>(a);
+        } else {
+            return hipErrorInvalidValue;
+        }
     }
     return hipGetLastError();
 }

@@ -333,3 +333,18 @@ def test_a_prompt_in_whole_units(ctx):
         o, _, mag, dot = kvref.attend(qf[i:i + 1].astype(np.float64), k[:i + 1], v[:i + 1], np.ones((1, i + 1), bool), 0.125)
         rel = 2 * dot * 2.0 ** -24 * (64 + 16) + 2.0 ** -16 + 2.0 ** -24 * (32 + n / 4)
         assert (np.abs(got[i] - o[0]) <= rel[0][:, None] * mag[0] + 2.0 ** -8 * np.abs(o[0]) + 1e-30).all()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("kb,vb", [(8, 8), (8, 4), (4, 8), (4, 4)])
+@pytest.mark.parametrize("group,news,lens,told", [
+    (4, [6, 5, 8], [300, 0, 700], 200000), (6, [5, 0, 3], [90, 7, 400], 300000),
+    (4, [40, 33, 1], [200, 0, 513], 200000), (5, [70, 9, 64], [0, 300, 150], 100000)])
+def test_tiles_of_long_calls(ctx, io, dim, kb, vb, group, news, lens, told):
+    """The row tiles that calls of much work take, on small data by a longest length that is told."""
+    c = Case(dim + kb + vb, news, lens, 2, dim, 32, kb, vb)
+    c.batch.max_length = told
+    trees = [seen_rows(random_tree(c.rng, n))[:n, :n] for n in news]
+    sees = [np.concatenate([np.ones((n, l), bool), t], 1) for n, l, t in zip(news, lens, trees)]
+    check(ctx, c, io, 2 * group, sees, dev(np.concatenate([words(t, 2) for t in trees])))
