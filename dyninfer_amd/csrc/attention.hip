@@ -12,15 +12,16 @@ template <> hipError_t attend_launch<4, 4>(const AttnArgs&, uint32_t, uint64_t, 
 
 namespace {
 
-// One wave per (row, query head) whose unit was split: the parts' maxima and
-// sums, then the parts' outputs, each brought to the common maximum.  Bound by latency:
+// SPLIT waves per (row, query head) whose unit was split: the parts' maxima and
+// sums, then the parts' outputs, each brought to the common maximum; of SPLIT waves
+// every one takes four parts of each 4 SPLIT.  Bound by latency:
 // 5.4 us for 8192 rows of two or three parts (7.9 when every wave found its parts by
 // itself, with some 260 scalar instructions).
-template <int D>
-__global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t tile_shift) {
+template <int D, int SPLIT>
+__global__ __launch_bounds__(SPLIT == 1 ? 256 : 64 * SPLIT) void join_kernel(AttnArgs a, uint32_t tile_shift) {
     constexpr int W = D <= 128 ? 2 : 4;  // dims of a lane
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t q_heads = a.kv.heads * a.group, seq = blockIdx.y, id = blockIdx.x * 4 + scalar(threadIdx.x >> 6);
+    const uint32_t lane = threadIdx.x & 63u, wave = scalar(threadIdx.x >> 6), p0 = SPLIT == 1 ? 0 : 4 * wave;
+    const uint32_t q_heads = a.kv.heads * a.group, seq = blockIdx.y, id = SPLIT == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
     const uint32_t i = id / q_heads, h = id - i * q_heads;
     if (i >= a.b.max_new) return;
     const uint32_t kv_head = h / a.group, row = i * a.group + (h - kv_head * a.group);
@@ -42,12 +43,12 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t tile_shi
     auto fetch = [&](uint32_t p) {  // four loads in flight, the first of them before the statistics
 #pragma unroll
         for (uint32_t k = 0; k < 4; k++) {
-            const uint64_t part = p + k < parts ? p + k : parts - 1;
+            const uint64_t part = min(p + k, parts - 1);
             v[k] = *gptr<vec>(po + part * pitch * D + (d0 < D ? d0 : 0));
             f[k] = gptr<float>(ml)[2 * pitch * part];
         }
     };
-    fetch(0);
+    fetch(p0);
 
     float top = -__builtin_inff();
     for (uint32_t p = lane; p < parts; p += 64) top = fmaxf(top, gptr<float>(ml)[2 * pitch * p]);
@@ -60,16 +61,24 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t tile_shi
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
 
-    if (a.lse && lane == 0)
+    if (a.lse && threadIdx.x % (64 * SPLIT) == 0)
         gptr_mut<float>(a.lse)[(r.row0 + (uint64_t)i) * q_heads + h] = (top + log2f(sum)) * 0.69314718055994531f;
-    if (d0 >= D) return;
     vec o = {};
-    for (uint32_t p = 0; p < parts; p += 4) {
+    for (uint32_t p = p0; p < parts; p += 4 * SPLIT) {
 #pragma unroll
         for (uint32_t k = 0; k < 4; k++)
             if (p + k < parts) o += v[k] * exp2f(f[k] - ref);
-        if (p + 4 < parts) fetch(p + 4);
+        if (p + 4 * SPLIT < parts) fetch(p + 4 * SPLIT);
     }
+    if constexpr (SPLIT > 1) {
+        __shared__ vec sm[SPLIT][64];
+        sm[wave][lane] = o;
+        __syncthreads();
+        if (wave != 0) return;
+#pragma unroll
+        for (int w = 1; w < SPLIT; w++) o += sm[w][lane];
+    }
+    if (d0 >= D) return;
     const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : __builtin_nanf(""));
     const int64_t e = (r.row0 + (int64_t)i) * a.out.ts + (int64_t)h * a.out.hs + d0;
 #pragma unroll
@@ -79,6 +88,17 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t tile_shi
         else
             gptr_mut<float>(a.out.p)[e + j] = o[j] * inv;
     }
+}
+
+// Eight waves a row for few rows of many parts (whole calls, one wave and eight: one
+// row of 8 heads after 16000, 64 parts, 26.5 and 20.0 us, of one head after 100000, 512 parts,
+// 87.8 and 35.5; 2016 rows after 2000, 42 parts, 22.9 and 29.2).
+template <int D>
+void join_launch(const AttnArgs& a, uint32_t shift, uint32_t parts, hipStream_t st) {
+    const uint64_t rows = (uint64_t)a.b.max_new * a.kv.heads * a.group;
+    // with shares there are fewer sequences than the grid's second axis allows
+    if (parts >= 8 && rows * a.b.seqs <= 1024) join_kernel<D, 8><<<dim3((uint32_t)rows, a.b.seqs), 512, 0, st>>>(a, shift);
+    else join_kernel<D, 1><<<dim3((uint32_t)((rows + 3) / 4), a.b.seqs), 256, 0, st>>>(a, shift);
 }
 
 }  // namespace
@@ -137,6 +157,7 @@ AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint
     const uint64_t places = units * (steps + kUnitCost);
     p.shares = (uint32_t)(places < full ? places : full);
     p.grid = p.shares;
+    p.parts = (uint32_t)(p.shares / units);
     const uint64_t slots = (units + p.shares) * tile;
     p.stats = slots * kv.dim * 4;
     p.where = p.stats + slots * 8;
@@ -157,14 +178,12 @@ hipError_t attn_launch(AttnArgs a, const AttnPlan& plan, uint8_t* work, hipStrea
     else
         e = a.kv.v_bits == 8 ? attend_launch<4, 8>(a, plan.tiles, plan.grid, st) : attend_launch<4, 4>(a, plan.tiles, plan.grid, st);
     if (e != hipSuccess || plan.shares == 0) return e;
-    // with shares there are fewer units than the grid's second axis allows
-    const dim3 blocks((uint32_t)(((uint64_t)a.b.max_new * a.kv.heads * a.group + 3) / 4), a.b.seqs);
     const uint32_t shift = (uint32_t)__builtin_ctz(16 * plan.tiles);
     switch (a.kv.dim) {
-    case 64: join_kernel<64><<<blocks, 256, 0, st>>>(a, shift); break;
-    case 96: join_kernel<96><<<blocks, 256, 0, st>>>(a, shift); break;
-    case 128: join_kernel<128><<<blocks, 256, 0, st>>>(a, shift); break;
-    case 256: join_kernel<256><<<blocks, 256, 0, st>>>(a, shift); break;
+    case 64: join_launch<64>(a, shift, plan.parts, st); break;
+    case 96: join_launch<96>(a, shift, plan.parts, st); break;
+    case 128: join_launch<128>(a, shift, plan.parts, st); break;
+    case 256: join_launch<256>(a, shift, plan.parts, st); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

@@ -87,6 +87,7 @@ struct AttnPlan {
     uint32_t tiles;      // 16-row tiles a workgroup holds: 1 or 2 by every wave, 4, 8 or 16 one or two a wave
     uint32_t row_tiles;  // of the sequence with the most rows
     uint32_t shares;     // equal pieces of all units' steps, a workgroup each; 0: a unit each
+    uint32_t parts;      // of a unit, about
     uint64_t grid;
     uint64_t bytes, stats, where;  // workspace, and where its parts begin
 };
