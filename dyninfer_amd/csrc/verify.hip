@@ -89,12 +89,15 @@ __device__ __forceinline__ float temperature(const VerifyArgs& a, uint32_t seq) 
     return a.temperature ? gptr<float>(a.temperature)[seq] : 1.0f;
 }
 
+// 1 / t of a positive temperature, neither infinite nor 0: -inf times it is -inf.
+__device__ __forceinline__ float inverse(float t) { return fmaxf(fminf(1.0f / t, kFltMax), 1.2e-38f); }
+
 template <bool BF16>
 __global__ __launch_bounds__(256) void stats_kernel(VerifyArgs a, Stat* out, uint32_t pieces, uint32_t size) {
     const uint32_t piece = blockIdx.x % pieces, row = blockIdx.x / pieces;
     const float t = temperature(a, seq_of(a.starts, a.seqs, row));
     const bool greedy = !(t > 0.0f);
-    const float inv_t = greedy ? 0.0f : fminf(1.0f / t, kFltMax);
+    const float inv_t = greedy ? 0.0f : inverse(t);
     const uint32_t lo = piece * size, hi = min(a.vocab, lo + size);
     constexpr uint32_t E = BF16 ? 2 : 4, V = 16 / E;  // elements of a 16-byte load
     const uint8_t* base = static_cast<const uint8_t*>(a.logits) + (int64_t)row * a.logits_stride * (int64_t)E;
@@ -280,7 +283,7 @@ __global__ __launch_bounds__(1024) void walk_kernel(VerifyArgs a, const Stat* st
     }
     const float t = temperature(a, seq);
     const bool greedy = !(t > 0.0f);
-    const float inv_t = greedy ? 0.0f : fminf(1.0f / t, kFltMax);
+    const float inv_t = greedy ? 0.0f : inverse(t);
     int32_t* gone = gone_list + row0;  // the rejected tokens of the current node
 
     // a row's statistics from its pieces', a wave a row

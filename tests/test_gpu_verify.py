@@ -209,3 +209,23 @@ def test_refusals(ctx):
     bad(lambda: run(draft_probs=kw["draft_probs"].half()), 2)
     bad(lambda: run(workspace=torch.empty(16, dtype=torch.uint8, device="cuda")))
     torch.cuda.synchronize()
+
+
+def test_infinite_temperature(ctx):
+    """Every token of a logit above -inf is as likely: the smallest noise among them is drawn."""
+    c = Draft(70, [1] * 40, 1003, False)
+    c.logits[c.rng.random(c.logits.shape) < 0.5] = -np.inf
+    c.temperature[:] = np.inf
+    _, _, token = c.run(ctx)
+    want = np.where(np.isinf(c.logits), np.inf, c.noise).argmin(-1)
+    assert (token.cpu().numpy() == want).all()
+
+
+@pytest.mark.parametrize("vocab", [4096, 4099, 20008])
+@pytest.mark.parametrize("dtype,pdtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32),
+                                          (torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16)])
+def test_siblings_after_rejections(ctx, vocab, dtype, pdtype):
+    """Drafts far from the target, so that rejections at a node sum its row, of whole eights and not."""
+    c = Draft(71 + vocab, [16, 9, 1, 16, 12, 16], vocab, True, near=2.5)
+    c.temperature[:] = 1.0
+    c.check(ctx, dtype, pdtype)
