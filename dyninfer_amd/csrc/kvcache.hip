@@ -134,13 +134,80 @@ __device__ __forceinline__ void rotate8(const KvRows& r, int64_t row, uint32_t t
     }
 }
 
-// One head of one token: loads, rotates, stores.  In place is safe: a head's
-// lanes are one wave's, which has loaded all of it before its first store.
+// Four elements from element offset `at`, a multiple of four.
+__device__ __forceinline__ void load4(const KvRows& r, int64_t at, float (&x)[4]) {
+    if (r.bf16 && r.vec) {
+        const u32x2 w = *gptr<u32x2>(static_cast<const uint16_t*>(r.p) + at);
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    } else if (r.vec) {
+        const f32x4 w = *gptr<f32x4>(static_cast<const float*>(r.p) + at);
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = w[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = load1(r, at + i);
+    }
+}
+__device__ __forceinline__ void store4(const KvRows& r, int64_t at, const float (&x)[4]) {
+    if (r.bf16) {
+        const u32x2 w = {f32x2_to_bf16x2_bits(x[0], x[1]), f32x2_to_bf16x2_bits(x[2], x[3])};
+        uint16_t* p = static_cast<uint16_t*>(r.p) + at;
+        if (r.vec) {
+            *gptr_mut<u32x2>(p) = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) gptr_mut<uint16_t>(p)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        }
+    } else {
+        float* p = static_cast<float*>(r.p) + at;
+        if (r.vec) {
+            *gptr_mut<f32x4>(p) = f32x4{x[0], x[1], x[2], x[3]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) gptr_mut<float>(p)[i] = x[i];
+        }
+    }
+}
+
+// One head of one token: loads, rotates, stores.  Halves of whole fours: a lane takes four
+// pairs (with eight dims of one half it loads their partners as well and twice the cosines:
+// append over 4 x 2048 tokens 36.0 us instead of 30.7, one token 2.2 instead of 1.8).  Otherwise in place is safe as well: a head's lanes are one
+// wave's, which has loaded all of it before its first store.
 template <int D>
 __device__ __forceinline__ void rope_row(const KvRows& x, const KvRows& y, uint32_t token, uint32_t head, uint32_t lane,
                                          const RopeView& rp) {
     const uint32_t d0 = 8 * lane;
     const int64_t row = (int64_t)token * x.ts + (int64_t)head * x.hs;
+    if (rp.half && rp.rot % 8 == 0 && d0 < rp.rot) {
+        const int64_t to = (int64_t)token * y.ts + (int64_t)head * y.hs;
+        const uint32_t i0 = 4 * lane, i1 = i0 + rp.rot / 2;
+        const int32_t pos = gptr<int32_t>(rp.positions)[token];
+        float a[4], b[4], p[4], q[4];
+        load4(x, row + i0, a);
+        load4(x, row + i1, b);
+        const bool in = pos >= 0 && (uint32_t)pos < rp.table_positions;
+        f32x4 cs[2] = {};
+        if (in) {
+            const float* t = rp.table + (size_t)pos * rp.rot + 2 * i0;
+            cs[0] = *gptr<f32x4>(t);
+            cs[1] = *gptr<f32x4>(t + 4);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const f32x4 w = cs[i];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int e = 2 * i + j;
+                const float c = w[2 * j], s = w[2 * j + 1];
+                p[e] = in ? a[e] * c - b[e] * s : __builtin_nanf("");
+                q[e] = in ? a[e] * s + b[e] * c : __builtin_nanf("");
+            }
+        }
+        store4(y, to + i0, p);
+        store4(y, to + i1, q);
+        return;
+    }
     float v[8];
     if (d0 < D) {
         load8(x, row + d0, v);
@@ -150,8 +217,8 @@ __device__ __forceinline__ void rope_row(const KvRows& x, const KvRows& y, uint3
     if (d0 < D) store8(y, (int64_t)token * y.ts + (int64_t)head * y.hs + d0, v);
 }
 
-// 4099 tokens of 40 heads of 128 dims in f32: 27.9 us, 6.2 TB/s.  (Four heads of a token by a
-// thread, which share its cosines: 29.4, one token 3.7 us instead of 2.2.)
+// 4099 tokens of 40 heads of 128 dims in f32: 27.9 us, 6.2 TB/s; one token 1.8 us.  (Four
+// heads of a token by a thread, which share its cosines: 29.4 and 3.7.)
 template <int D>
 __global__ __launch_bounds__(256) void rope_kernel(KvRows x, KvRows y, uint32_t tokens, uint32_t heads, RopeView rp) {
     constexpr uint32_t L = kLanes<D>;
@@ -280,7 +347,7 @@ __device__ __forceinline__ void turn4(uint32_t (&x)[4]) {
 // one per (sequence, chunk, kHeads heads); then the queries' rows.  A chunk of a
 // head's values is one wave's alone, so values of 4 bits, two tokens to a byte, are
 // merged without atomics.  (Keys by four tokens a thread: 220 registers, the whole
-// launch over 4 x 2048 tokens 86 us instead of 36, 146 MB at 4.1 TB/s.)
+// launch over 4 x 2048 tokens, 146 MB in 30.7 us, 4.8 TB/s now, 86 us instead of 37 then.)
 template <int D, int KB, int VB>
 __global__ __launch_bounds__(256) void append_kernel(KvView kv, KvBatch b, KvRows k, KvRows v, RopeView rp, KvRows q,
                                                      KvRows q_out, uint32_t q_heads, uint32_t chunks, uint32_t k_blocks,
