@@ -397,8 +397,9 @@ int dyninfer_mi355x_draft_verify(dyninfer_mi355x_ctx_t* ctx, const dyninfer_veri
     if (!float_type(v->logits_dtype) || (v->draft_probs && !float_type(v->probs_dtype)))
         return fail(UNSUPPORTED, "logits and draft_probs must be f32 or bf16");
     auto size = [](uint32_t t) { return t == DYNINFER_DTYPE_BF16 ? 2u : 4u; };
-    if (!v->starts || !aligned(v->starts, 4) || !v->path || !aligned(v->path, 4) || !v->counts || !aligned(v->counts, 4) ||
-        !v->next_token || !aligned(v->next_token, 8) || (v->temperature && !aligned(v->temperature, 4)))
+    // without rows (max_new 0) path has no elements
+    if (!v->starts || !aligned(v->starts, 4) || (v->max_new && !v->path) || !aligned(v->path, 4) || !v->counts ||
+        !aligned(v->counts, 4) || !v->next_token || !aligned(v->next_token, 8) || (v->temperature && !aligned(v->temperature, 4)))
         return fail(BAD, "starts, temperature or an output is NULL or misaligned");
     if (!v->noise || !aligned(v->noise, 4)) return fail(BAD, "noise is NULL or misaligned");
     if (v->noise_stride < (int64_t)v->vocab && v->sequences > 1) return fail(BAD, "noise rows overlap");

@@ -458,7 +458,7 @@ typedef struct dyninfer_verify {
     const float* noise;          /* [sequences, vocab], > 0, rows noise_stride apart */
     int64_t noise_stride;
     uint32_t vocab, sequences, tokens, max_new;
-    int32_t* path;       /* out [sequences, max_new]: the accepted nodes, 0 first, then -1 */
+    int32_t* path;       /* out [sequences, max_new]: the accepted nodes, 0 first, then -1 (max_new 0: may be NULL) */
     int32_t* counts;     /* out [sequences]: how many (0 for a sequence without rows) */
     int64_t* next_token; /* out [sequences] */
 } dyninfer_verify_t;

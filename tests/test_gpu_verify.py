@@ -229,3 +229,16 @@ def test_siblings_after_rejections(ctx, vocab, dtype, pdtype):
     c = Draft(71 + vocab, [16, 9, 1, 16, 12, 16], vocab, True, near=2.5)
     c.temperature[:] = 1.0
     c.check(ctx, dtype, pdtype)
+
+
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("tokens", [0, 3])
+def test_rounds_without_rows(ctx, tokens, probs):
+    """Sequences of which none has rows in the call (or may have any): count 0 and no token."""
+    vocab = 40
+    logits = torch.zeros((tokens, vocab), device="cuda")
+    path, counts, token = ctx.draft_verify(
+        logits, torch.zeros(tokens, dtype=torch.int64, device="cuda"), None, i32([0, 0, tokens, tokens]), 0,
+        uniform=torch.zeros(tokens, device="cuda"), noise=torch.ones((3, vocab), device="cuda"),
+        temperature=torch.tensor([1.0, 0.0, 1.0], device="cuda"), draft_probs=logits if probs else None)
+    assert path.shape == (3, 0) and counts.tolist() == [0, 0, 0] and token.tolist() == [-1, -1, -1]
