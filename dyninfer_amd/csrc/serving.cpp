@@ -315,7 +315,8 @@ int dyninfer_mi355x_kv_commit(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache
     if (int rc = check_cache(cache, kv)) return rc;
     if (int rc = check_batch(batch, true, b)) return rc;
     if (b.tokens == 0 || b.seqs == 0) return DYNINFER_MI355X_OK;
-    if (!path || !counts || !aligned(path, 4) || !aligned(counts, 4)) return fail(BAD, "path / counts are NULL or misaligned");
+    if ((path_stride && !path) || !counts || !aligned(path, 4) || !aligned(counts, 4))
+        return fail(BAD, "path / counts are NULL or misaligned");
     if (int rc = check_grid(2ull * b.seqs * kv.heads)) return rc;
     DeviceGuard g(ctx->device);
     if (g.err != hipSuccess) return hip_fail(g.err, "hipSetDevice");

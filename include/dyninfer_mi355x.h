@@ -400,7 +400,8 @@ int dyninfer_mi355x_kv_read(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache_t
  * Keeps an accepted path of each sequence's rows: for j < counts[b], the codes and scales at
  * position lengths[b] + path[b * path_stride + j] move to lengths[b] + j, unchanged.  A path
  * ascends (path[j] >= j); an entry that does not (or lies outside the sequence's rows) is left
- * out.  path and counts as dyninfer_mi355x_draft_verify writes them (device int32).
+ * out.  path and counts as dyninfer_mi355x_draft_verify writes them (device int32; path_stride 0:
+ * nothing moves, and path may be NULL).
  */
 int dyninfer_mi355x_kv_commit(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache_t* cache,
                               const dyninfer_kvbatch_t* batch, const int32_t* path, uint32_t path_stride,

@@ -365,3 +365,11 @@ def test_rope_outside_the_table(ctx, rot):
         assert torch.equal(y[:, :, rot:], x[:, :, rot:])
         assert torch.isnan(y[:, :, :rot]).all(-1).all(-1).tolist() == [False, True, False, True, True]
         assert not torch.isnan(y[[0, 2]]).any()
+
+
+def test_commit_of_paths_without_entries(ctx):
+    """What verification returns where no sequence may have rows: paths of width 0 move nothing."""
+    c = Case(30, [5, 3], [7, 20], 2, 64, 16, 8, 4)
+    for counts in ([0, 0], [2, 1]):
+        ctx.kv_commit(c.cache, c.batch, torch.empty((2, 0), dtype=torch.int32, device="cuda"), i32(counts))
+    assert c.same_bytes()
