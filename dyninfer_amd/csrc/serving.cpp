@@ -74,7 +74,7 @@ int check_cache(const dyninfer_kvcache_t* c, dmx::KvView& kv) {
 int check_batch(const dyninfer_kvbatch_t* b, bool tables, dmx::KvBatch& out) {
     if (!b) return fail(BAD, "batch is NULL");
     if (tables && b->sequences) {
-        if (!b->page_table || !b->lengths || !b->starts) return fail(BAD, "batch tables are NULL");
+        if ((b->table_pages && !b->page_table) || !b->lengths || !b->starts) return fail(BAD, "batch tables are NULL");
         if (!aligned(b->page_table, 4) || !aligned(b->lengths, 4) || !aligned(b->starts, 4))
             return fail(BAD, "batch tables must be 4-byte aligned");
     }

@@ -317,7 +317,7 @@ typedef struct dyninfer_kvcache {
  * are dropped, reads give NaN, attention does not see it.  A negative length counts as 0.
  */
 typedef struct dyninfer_kvbatch {
-    const int32_t* page_table; /* [sequences, table_pages] */
+    const int32_t* page_table; /* [sequences, table_pages]; table_pages 0 (may be NULL): every position is absent */
     const int32_t* lengths;    /* [sequences] */
     const int32_t* starts;     /* [sequences + 1] */
     uint32_t sequences, table_pages;

@@ -373,3 +373,22 @@ def test_commit_of_paths_without_entries(ctx):
     for counts in ([0, 0], [2, 1]):
         ctx.kv_commit(c.cache, c.batch, torch.empty((2, 0), dtype=torch.int32, device="cuda"), i32(counts))
     assert c.same_bytes()
+
+
+def test_sequences_without_pages(ctx):
+    """A page table of no columns: every position is absent."""
+    c = Case(31, [2, 1], [0, 5], 2, 64, 16, 8, 8)
+    batch = d.KVBatch(torch.empty((2, 0), dtype=torch.int32, device="cuda"), c.batch.lengths, c.batch.starts, 3, 2, 6)
+    k, v, q = (torch.randn((3, h, 64), device="cuda") for h in (2, 2, 4))
+    table = ctx.rope_table(8, 64)
+    pos = i32([0, 1, 5])
+    got = ctx.kv_append(c.cache, batch, k, v, rope=d.Rope(table, pos, 64), q=q)
+    assert torch.equal(got, ctx.rope(q, d.Rope(table, pos, 64))) and c.same_bytes()
+    assert all(torch.isnan(x).all() for x in ctx.kv_read(c.cache, batch))
+    lse = torch.zeros((3, 4), device="cuda")
+    assert (ctx.tree_attention(c.cache, batch, q, lse=lse) == 0).all() and (lse == -float("inf")).all()
+    ctx.kv_commit(c.cache, batch, i32([[0, 1], [0, -1]]), i32([2, 1]))
+    assert c.same_bytes()
+    none = d.KVBatch(batch.page_table, batch.lengths, i32([0, 0, 0]), 0, 0, 5)  # nor rows
+    ctx.kv_append(c.cache, none, k[:0], v[:0])
+    assert all(x.shape == (0, 2, 64) for x in ctx.kv_read(c.cache, none))
