@@ -167,6 +167,8 @@ AttnPlan attn_plan(const KvView& kv, const KvBatch& b, uint64_t max_length, uint
 
 hipError_t attn_launch(AttnArgs a, const AttnPlan& plan, uint8_t* work, hipStream_t st) {
     if (plan.grid == 0) return hipSuccess;
+    // sixteen tiles: eight waves.  A call in shares has few rows, its second launch always fits
+    if (!launchable(plan.grid, plan.tiles == 16 ? 512 : 256)) return kTooManyThreads;
     a.row_tiles = plan.row_tiles;
     a.shares = plan.shares;
     a.parts = reinterpret_cast<float*>(work);

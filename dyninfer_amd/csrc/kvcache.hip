@@ -618,6 +618,7 @@ hipError_t rope_table_launch(uint32_t rot, uint32_t scaling, double theta, doubl
                              double hi, double attn, uint32_t positions, float* out, hipStream_t st) {
     const uint64_t n = (uint64_t)positions * (rot / 2);
     if (n == 0) return hipSuccess;
+    if (!launchable((n + 255) / 256, 256)) return kTooManyThreads;
     rope_table_kernel<<<(uint32_t)((n + 255) / 256), 256, 0, st>>>(rot, scaling, theta, factor, original, lo, hi, attn,
                                                                    positions, out);
     return hipGetLastError();
@@ -629,7 +630,9 @@ hipError_t rope_launch(const KvRows& x, const KvRows& y, uint32_t tokens, uint32
     return by_dim(dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
         constexpr uint64_t rows = 256 / kLanes<D>;
-        rope_kernel<D><<<(uint32_t)(((uint64_t)tokens * heads + rows - 1) / rows), 256, 0, st>>>(x, y, tokens, heads, rope);
+        const uint64_t grid = ((uint64_t)tokens * heads + rows - 1) / rows;
+        if (!launchable(grid, 256)) return kTooManyThreads;
+        rope_kernel<D><<<(uint32_t)grid, 256, 0, st>>>(x, y, tokens, heads, rope);
         return hipGetLastError();
     });
 }
@@ -640,12 +643,14 @@ hipError_t kv_append_launch(const KvView& kv, const KvBatch& b, const KvRows& k,
         constexpr int D = decltype(d)::value;
         constexpr uint64_t rows = 256 / kLanes<D>;
         const uint32_t chunks = chunk_bound(b.max_new);
-        const uint32_t k_blocks = b.seqs * chunks * ((kv.heads + kKeyHeads<D> - 1) / kKeyHeads<D>);
-        const uint32_t v_blocks = b.seqs * chunks * ((kv.heads + kHeads<D> - 1) / kHeads<D>);
-        const uint64_t grid = (uint64_t)k_blocks + v_blocks + ((uint64_t)b.tokens * q_heads + rows - 1) / rows;
+        // below 2^64: at most 2^24 sequences, 2^27 + 1 chunks, 2^12 heads (values: half of them)
+        const uint64_t k_blocks = (uint64_t)b.seqs * chunks * ((kv.heads + kKeyHeads<D> - 1) / kKeyHeads<D>);
+        const uint64_t v_blocks = (uint64_t)b.seqs * chunks * ((kv.heads + kHeads<D> - 1) / kHeads<D>);
+        const uint64_t grid = k_blocks + v_blocks + ((uint64_t)b.tokens * q_heads + rows - 1) / rows;
         if (grid == 0) return hipSuccess;
-        append_kernel<D, decltype(kb)::value, decltype(vb)::value>
-            <<<(uint32_t)grid, 256, 0, st>>>(kv, b, k, v, rope, q, q_out, q_heads, chunks, k_blocks, v_blocks);
+        if (!launchable(grid, 256)) return kTooManyThreads;
+        append_kernel<D, decltype(kb)::value, decltype(vb)::value><<<(uint32_t)grid, 256, 0, st>>>(
+            kv, b, k, v, rope, q, q_out, q_heads, chunks, (uint32_t)k_blocks, (uint32_t)v_blocks);
         return hipGetLastError();
     });
 }
@@ -654,10 +659,12 @@ hipError_t kv_read_launch(const KvView& kv, const KvBatch& b, const KvRows& k, c
     return by_cache(kv, [&](auto d, auto kb, auto vb) {
         constexpr int D = decltype(d)::value;
         const uint32_t chunks = chunk_bound(b.max_new);
-        const uint32_t kv_blocks = b.seqs * chunks * ((kv.heads + kHeads<D> - 1) / kHeads<D>);
-        const uint32_t grid = kv_blocks * ((k.p != nullptr) + (v.p != nullptr));
+        const uint64_t kv_blocks = (uint64_t)b.seqs * chunks * ((kv.heads + kHeads<D> - 1) / kHeads<D>);
+        const uint64_t grid = kv_blocks * ((k.p != nullptr) + (v.p != nullptr));
         if (grid == 0) return hipSuccess;
-        read_kernel<D, decltype(kb)::value, decltype(vb)::value><<<grid, 256, 0, st>>>(kv, b, k, v, chunks, kv_blocks);
+        if (!launchable(grid, 256)) return kTooManyThreads;
+        read_kernel<D, decltype(kb)::value, decltype(vb)::value>
+            <<<(uint32_t)grid, 256, 0, st>>>(kv, b, k, v, chunks, (uint32_t)kv_blocks);
         return hipGetLastError();
     });
 }
@@ -666,10 +673,11 @@ hipError_t kv_commit_launch(const KvView& kv, const KvBatch& b, const int32_t* p
                             const int32_t* counts, hipStream_t st) {
     return by_cache(kv, [&](auto d, auto kb, auto vb) {
         constexpr int D = decltype(d)::value;
-        const uint32_t grid = 2 * b.seqs * kv.heads;
+        const uint64_t grid = 2ull * b.seqs * kv.heads;
         if (grid == 0) return hipSuccess;
+        if (!launchable(grid, 256)) return kTooManyThreads;
         commit_kernel<D, decltype(kb)::value, decltype(vb)::value>
-            <<<grid, 256, 0, st>>>(kv, b, path, path_stride, counts);
+            <<<(uint32_t)grid, 256, 0, st>>>(kv, b, path, path_stride, counts);
         return hipGetLastError();
     });
 }

@@ -70,6 +70,11 @@ __device__ __forceinline__ uint64_t chunk_slot(const KvView& kv, int64_t p, uint
     return (((uint64_t)p * kv.heads + h) << kv.page_shift) + 16u * in_page;
 }
 
+// A launch's threads are counted in 32 bits.  The launches below return kTooManyThreads, and
+// enqueue nothing, for calls that would need more.
+constexpr hipError_t kTooManyThreads = hipErrorInvalidConfiguration;
+inline bool launchable(uint64_t blocks, uint32_t threads) { return blocks <= 0xFFFFFFFFull / threads; }
+
 hipError_t rope_table_launch(uint32_t rot, uint32_t scaling, double theta, double factor, double original, double lo,
                              double hi, double attn, uint32_t positions, float* out, hipStream_t st);
 hipError_t rope_launch(const KvRows& x, const KvRows& y, uint32_t tokens, uint32_t heads, uint32_t dim,
@@ -122,8 +127,6 @@ struct VerifyArgs {
     int32_t* counts;
     int64_t* next;
 };
-// Workgroups of its largest launch.
-uint64_t verify_blocks(uint32_t seqs, uint32_t tokens, uint32_t vocab);
 uint64_t verify_workspace_bytes(uint32_t seqs, uint32_t tokens, uint32_t vocab);
 hipError_t verify_launch(const VerifyArgs& a, uint8_t* work, hipStream_t st);
 

@@ -19,7 +19,6 @@ namespace {
 
 constexpr int BAD = DYNINFER_MI355X_ERR_INVALID_ARGUMENT;
 constexpr int UNSUPPORTED = DYNINFER_MI355X_ERR_UNSUPPORTED;
-constexpr uint64_t kMaxGrid = 0x40000000u;  // workgroups of a launch
 
 bool dim_ok(uint32_t d) { return d == 64 || d == 96 || d == 128 || d == 256; }
 
@@ -123,17 +122,6 @@ int check_rope(const dyninfer_rope_t* r, uint32_t dim, uint32_t tokens, dmx::Rop
     return 0;
 }
 
-int check_grid(uint64_t blocks) {
-    return blocks <= kMaxGrid ? 0 : fail(UNSUPPORTED, "the call needs more than 2^30 workgroups; split it");
-}
-
-// Workgroups of a launch over the chunks of 16 positions that new rows touch.
-uint64_t chunk_blocks(const dmx::KvView& kv, const dmx::KvBatch& b) {
-    const uint64_t chunks = b.max_new ? ((uint64_t)b.max_new + 14) / 16 + 1 : 0;
-    const uint64_t n = (uint64_t)b.seqs * chunks;  // below 2^60
-    return n > kMaxGrid ? n : n * kv.heads;
-}
-
 int same_place(const dyninfer_rows_t* a, const dyninfer_rows_t* b) {
     return a->data == b->data && a->token_stride == b->token_stride && a->head_stride == b->head_stride;
 }
@@ -177,7 +165,11 @@ int check_workspace(const void* p, uint64_t bytes, uint64_t need, const char* wh
     return 0;
 }
 
-int launched(hipError_t e) { return e == hipSuccess ? DYNINFER_MI355X_OK : hip_fail(e, "kernel launch"); }
+int launched(hipError_t e) {
+    if (e == dmx::kTooManyThreads)
+        return fail(UNSUPPORTED, "the call needs 2^32 threads or more in a launch; split it");
+    return e == hipSuccess ? DYNINFER_MI355X_OK : hip_fail(e, "kernel launch");
+}
 
 }  // namespace
 
@@ -212,7 +204,6 @@ int dyninfer_mi355x_rope_table(dyninfer_mi355x_ctx_t* ctx, const dyninfer_rope_p
     }
     if (positions == 0) return DYNINFER_MI355X_OK;
     if (!table || !aligned(table, 16)) return fail(BAD, "rope table is NULL or not 16-byte aligned");
-    if (int rc = check_grid((uint64_t)positions * (p->rot_dim / 2) / 256)) return rc;
     DeviceGuard g(ctx->device);
     if (g.err != hipSuccess) return hip_fail(g.err, "hipSetDevice");
     return launched(dmx::rope_table_launch(p->rot_dim, p->scaling, p->theta, p->factor, p->original_length, lo, hi, attn,
@@ -231,7 +222,6 @@ int dyninfer_mi355x_rope(dyninfer_mi355x_ctx_t* ctx, const dyninfer_rows_t* x, c
     if (int rc = check_out(y, head_dim, tokens, "y", out)) return rc;
     if (x->dtype != y->dtype || x->heads != y->heads) return fail(BAD, "x and y must share dtype and heads");
     if (int rc = check_apart(x, y, tokens, head_dim, "y")) return rc;
-    if (int rc = check_grid((uint64_t)tokens * x->heads / 8)) return rc;
     DeviceGuard g(ctx->device);
     if (g.err != hipSuccess) return hip_fail(g.err, "hipSetDevice");
     return launched(dmx::rope_launch(in, out, tokens, x->heads, head_dim, rp, static_cast<hipStream_t>(stream)));
@@ -266,7 +256,6 @@ int dyninfer_mi355x_kv_append(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache
     if (int rc = check_rows(v, kv.dim, "v", vr)) return rc;
     if (k->heads != kv.heads || v->heads != kv.heads) return fail(BAD, "k and v must have the cache's heads");
     if (k->dtype != v->dtype) return fail(BAD, "k and v must share a dtype");
-    uint64_t grid = 2 * chunk_blocks(kv, b);
     if (q) {
         if (int rc = check_rows(q, kv.dim, "q", qr)) return rc;
         if (int rc = check_out(q_out, kv.dim, b.tokens, "q_out", qo)) return rc;
@@ -276,9 +265,7 @@ int dyninfer_mi355x_kv_append(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache
         if ((meet(q_out, k, b.tokens, kv.dim) && !interleaved(q_out, k, kv.dim)) ||
             (meet(q_out, v, b.tokens, kv.dim) && !interleaved(q_out, v, kv.dim)))
             return fail(BAD, "q_out overlaps k or v");
-        grid += (uint64_t)b.tokens * q->heads / 8;
     }
-    if (int rc = check_grid(grid)) return rc;
     DeviceGuard g(ctx->device);
     if (g.err != hipSuccess) return hip_fail(g.err, "hipSetDevice");
     return launched(dmx::kv_append_launch(kv, b, kr, vr, rp, qr, qo, q ? q->heads : 0, static_cast<hipStream_t>(stream)));
@@ -300,7 +287,6 @@ int dyninfer_mi355x_kv_read(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache_t
         if (int rc = check_out(v, kv.dim, b.tokens, "v", vr)) return rc;
     if ((k && k->heads != kv.heads) || (v && v->heads != kv.heads)) return fail(BAD, "k and v must have the cache's heads");
     if (k && v && meet(k, v, b.tokens, kv.dim) && !interleaved(k, v, kv.dim)) return fail(BAD, "k and v overlap");
-    if (int rc = check_grid(2 * chunk_blocks(kv, b))) return rc;
     DeviceGuard g(ctx->device);
     if (g.err != hipSuccess) return hip_fail(g.err, "hipSetDevice");
     return launched(dmx::kv_read_launch(kv, b, kr, vr, static_cast<hipStream_t>(stream)));
@@ -317,7 +303,6 @@ int dyninfer_mi355x_kv_commit(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache
     if (b.tokens == 0 || b.seqs == 0) return DYNINFER_MI355X_OK;
     if ((path_stride && !path) || !counts || !aligned(path, 4) || !aligned(counts, 4))
         return fail(BAD, "path / counts are NULL or misaligned");
-    if (int rc = check_grid(2ull * b.seqs * kv.heads)) return rc;
     DeviceGuard g(ctx->device);
     if (g.err != hipSuccess) return hip_fail(g.err, "hipSetDevice");
     return launched(dmx::kv_commit_launch(kv, b, path, path_stride, counts, static_cast<hipStream_t>(stream)));
@@ -364,9 +349,6 @@ int dyninfer_mi355x_tree_attention(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kv
     if ((uint64_t)a.b.max_new * a.group > 0x7FFFFFFFull) return fail(UNSUPPORTED, "too many rows of one kv head");
     const dmx::AttnPlan plan = dmx::attn_plan(a.kv, a.b, batch->max_length, q->heads, a.q.bf16, !mask);
     if (int rc = check_workspace(workspace, workspace_bytes, plan.bytes, "tree_attention")) return rc;
-    if (int rc = check_grid(plan.grid)) return rc;
-    if (int rc = check_grid((uint64_t)a.b.seqs * a.b.max_new / 4)) return rc;
-    if (int rc = check_grid((uint64_t)a.b.seqs * a.b.max_new * q->heads / 4)) return rc;
     a.mask = mask;
     a.mask_words = mask_words;
     a.lse = lse;
@@ -415,7 +397,6 @@ int dyninfer_mi355x_draft_verify(dyninfer_mi355x_ctx_t* ctx, const dyninfer_veri
     }
     const uint64_t need = dmx::verify_workspace_bytes(v->sequences, v->tokens, v->vocab);
     if (int rc = check_workspace(workspace, workspace_bytes, need, "draft_verify")) return rc;
-    if (int rc = check_grid(dmx::verify_blocks(v->sequences, v->tokens, v->vocab))) return rc;
     dmx::VerifyArgs a = {};
     a.logits = v->logits;
     a.probs = v->draft_probs;

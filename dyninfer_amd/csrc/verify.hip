@@ -470,11 +470,6 @@ uint64_t round256(uint64_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
 
-uint64_t verify_blocks(uint32_t seqs, uint32_t tokens, uint32_t vocab) {
-    const uint64_t a = (uint64_t)tokens * piece_count(tokens, vocab), b = (uint64_t)seqs * ((vocab + kDraw - 1) / kDraw);
-    return a > b ? a : b;
-}
-
 uint64_t verify_workspace_bytes(uint32_t seqs, uint32_t tokens, uint32_t vocab) {
     return round256((uint64_t)tokens * piece_count(tokens, vocab) * sizeof(Stat)) + round256((uint64_t)tokens * sizeof(Stat)) +
            round256((uint64_t)tokens * 4) + (uint64_t)seqs * sizeof(Left);
@@ -484,6 +479,9 @@ hipError_t verify_launch(const VerifyArgs& a, uint8_t* work, hipStream_t st) {
     if (a.seqs == 0) return hipSuccess;
     const uint32_t size = piece_size(a.tokens, a.vocab), pieces = piece_count(a.tokens, a.vocab);
     const uint32_t draws = (a.vocab + kDraw - 1) / kDraw;
+    if (!launchable((uint64_t)a.tokens * pieces, 256) || !launchable(a.seqs, 1024) ||
+        !launchable((uint64_t)a.seqs * draws, 512))
+        return kTooManyThreads;
     Stat* stats = reinterpret_cast<Stat*>(work);
     work += round256((uint64_t)a.tokens * pieces * sizeof(Stat));
     Stat* rows = reinterpret_cast<Stat*>(work);

@@ -392,3 +392,32 @@ def test_sequences_without_pages(ctx):
     none = d.KVBatch(batch.page_table, batch.lengths, i32([0, 0, 0]), 0, 0, 5)  # nor rows
     ctx.kv_append(c.cache, none, k[:0], v[:0])
     assert all(x.shape == (0, 2, 64) for x in ctx.kv_read(c.cache, none))
+
+
+@pytest.mark.parametrize("call", ["append", "read", "commit", "attend"])
+def test_calls_of_too_many_threads(ctx, call):
+    """A launch's threads are counted in 32 bits: calls that need more are refused as such, smaller ones run."""
+    n = 1 << 20
+    zero = torch.zeros((n, 1), dtype=torch.int32, device="cuda")
+    starts = torch.zeros(n + 1, dtype=torch.int32, device="cuda")
+    starts[-1] = 1  # the last sequence has a row
+    batch = d.KVBatch(zero, zero[:, 0].contiguous(), starts, 1, 1, 1)
+
+    def run(heads):
+        cache = d.KVCache.empty(1, heads, 64, 16)
+        x = torch.randn((1, heads, 64), device="cuda")
+        ctx.kv_append(cache, d.KVBatch(zero[:1], zero[0], i32([0, 1]), 1, 1, 1), x, x)
+        if call == "append":
+            ctx.kv_append(cache, batch, x, x)
+        elif call == "read":
+            return ctx.kv_read(cache, batch)[1], x
+        elif call == "commit":
+            ctx.kv_commit(cache, batch, zero, zero[:, 0].contiguous())
+        else:
+            return ctx.tree_attention(cache, batch, x), x
+        return ctx.kv_read(cache, d.KVBatch(zero[:1], zero[0], i32([0, 1]), 1, 1, 1))[1], x
+
+    bad(lambda: run(64), d.ERR_UNSUPPORTED)
+    got, x = run(1)
+    # a value's code is at most half a scale off, the scale that of the largest / 127, rounded to 8 bits
+    assert (got - x).abs().max() <= x.abs().max() * (0.5 / 127 + 2 ** -8) * 1.01

@@ -242,3 +242,11 @@ def test_rounds_without_rows(ctx, tokens, probs):
         uniform=torch.zeros(tokens, device="cuda"), noise=torch.ones((3, vocab), device="cuda"),
         temperature=torch.tensor([1.0, 0.0, 1.0], device="cuda"), draft_probs=logits if probs else None)
     assert path.shape == (3, 0) and counts.tolist() == [0, 0, 0] and token.tolist() == [-1, -1, -1]
+
+
+def test_too_many_sequences(ctx):
+    """A launch's threads are counted in 32 bits."""
+    n = 1 << 22
+    bad(lambda: ctx.draft_verify(torch.zeros((1, 1), device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda"), None,
+                                 torch.zeros(n + 1, dtype=torch.int32, device="cuda"), 1,
+                                 uniform=torch.zeros(1, device="cuda"), noise=torch.ones((n, 1), device="cuda")), 2)
