@@ -250,3 +250,124 @@ def test_too_many_sequences(ctx):
     bad(lambda: ctx.draft_verify(torch.zeros((1, 1), device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda"), None,
                                  torch.zeros(n + 1, dtype=torch.int32, device="cuda"), 1,
                                  uniform=torch.zeros(1, device="cuda"), noise=torch.ones((n, 1), device="cuda")), 2)
+
+
+def decidable(dr, dtype=torch.float32, pdtype=torch.float32):
+    """How far the closest decision of a Draft is from a tie, in 64 bits: the smallest of the
+    differences u q - R(c) at the children tried and of the largest two scores at the end, each
+    over what its f32 error scales with.  R_k = max(p - a q, 0) / w: p and a q are rounded on their own,
+    and w, a sum of such, is off by a part of 1."""
+    cast = lambda a, t: torch.from_numpy(a).to(t).double().numpy()
+    logits = cast(dr.logits, dtype)
+    probs = None if dr.probs is None else cast(dr.probs, pdtype)
+    least = np.inf
+    for b, n in enumerate(dr.news):
+        t = float(dr.temperature[b])
+        if n == 0 or not t > 0:
+            continue
+        r0, cur, a, w, gone = dr.starts[b], 0, 0.0, 1.0, []
+
+        def p_of(node):
+            e = np.exp((logits[r0 + node] - logits[r0 + node].max()) / t)
+            return e / e.sum()
+
+        def rest():
+            if probs is not None:
+                return np.maximum(p - a * probs[r0 + cur], 0)
+            left = p.copy()
+            left[gone] = 0
+            return left
+
+        p = p_of(0)
+        for i in range(1, n):
+            if dr.parents[r0 + i] != cur:
+                continue
+            tok, u = dr.tokens[r0 + i], float(dr.uniform[r0 + i])
+            q = 1.0 if probs is None else probs[r0 + cur, tok]
+            side = rest()[tok] / w
+            err = (p[tok] + (0 if probs is None else a * q)) / w + side / w + u * q
+            least = min(least, abs(u * q - side) / err if u * q or side else 1.0)
+            if u * q < side:
+                cur, a, w, gone, p = i, 0.0, 1.0, [], p_of(i)
+            elif probs is not None:
+                a += w
+                w = rest().sum()
+                assert w > 0  # a case of its own
+            else:
+                gone.append(tok)
+                w = rest().sum()
+        aq = 0 if probs is None else a * probs[r0 + cur]
+        score, err = rest() / dr.noise[b], (p + aq) / dr.noise[b]
+        top = score.argmax()
+        others = np.arange(dr.vocab) != top
+        if others.any():
+            least = min(least, ((score[top] - score) / (err[top] + err))[others].min())
+    return least
+
+
+def check_decidable(dr, ctx, dtype=torch.float32, pdtype=torch.float32):
+    assert decidable(dr, dtype, pdtype) > 2.0 ** -16
+    return dr.check(ctx, dtype, pdtype)
+
+
+LARGE_TREES = [(64, False, 200), (64, True, 210), (64, True, 220), (300, False, 200), (300, True, 205), (300, True, 210)]
+
+
+def large_trees(vocab, probs, seed):
+    """Trees of more nodes than the walk holds at a time, whose nodes have children far behind them."""
+    dr = Draft(seed, [600, 257, 256, 1, 513], vocab, probs, near=1.5)
+    for b, n in enumerate(dr.news):
+        for i in range(1, n):
+            # some hang on the root, before the boundary and behind it, the others on any node
+            up = 0 if dr.rng.random() < (1 / 30 if i < 256 else 1 / 8) else int(dr.rng.integers(0, i))
+            dr.parents[dr.starts[b] + i] = up
+            p = (dr.probs if probs else np.exp(dr.logits))[dr.starts[b] + up].astype(np.float64)
+            dr.tokens[dr.starts[b] + i] = dr.rng.choice(vocab, p=p / p.sum())
+            u = dr.uniform[dr.starts[b] + i]
+            dr.uniform[dr.starts[b] + i] = 0.97 + 0.03 * u if i < 256 else 0.2 * u  # mostly rejected, mostly accepted
+    dr.temperature[:] = 1
+    return dr
+
+
+@pytest.mark.parametrize("vocab,probs,seed", LARGE_TREES)
+def test_trees_of_more_nodes_than_the_walk_holds(ctx, vocab, probs, seed):
+    """Rejections at a node before the boundary go on to its children behind it."""
+    dr = large_trees(vocab, probs, seed)
+    path, counts, _ = check_decidable(dr, ctx)
+    assert any((p[:c] > 256).any() for p, c in zip(path, counts))  # from one group of nodes to the next
+
+
+def long_chains(probs):
+    """Chains that are accepted past the boundary."""
+    dr = Draft(300, [700, 300, 257], 40, probs, tree=False, near=0.05)
+    dr.uniform *= 0.3
+    dr.temperature[:] = [1, 0, 1]
+    n0, n1 = dr.starts[1], dr.starts[2]
+    best = dr.logits.argmax(-1)
+    dr.tokens[n0 + 1:n1] = best[n0:n1 - 1]  # greedy: all accepted
+    for b in (0, 2):
+        dr.tokens[dr.starts[b] + 1:dr.starts[b + 1]] = best[dr.starts[b]:dr.starts[b + 1] - 1]
+        if not probs:
+            dr.logits[np.arange(dr.starts[b], dr.starts[b + 1]), best[dr.starts[b]:dr.starts[b + 1]]] += 4
+    return dr
+
+
+@pytest.mark.parametrize("probs", [False, True])
+def test_chains_of_more_nodes_than_the_walk_holds(ctx, probs):
+    dr = long_chains(probs)
+    _, counts, _ = check_decidable(dr, ctx)
+    assert counts[1] == 300
+
+
+LARGE_PIECES = [(20001, torch.float32, 400), (32768, torch.bfloat16, 401), (40001, torch.float32, 402), (40001, torch.bfloat16, 403)]
+
+
+def large_pieces(vocab, probs, seed):
+    return Draft(seed, [8] * 60 + [1, 37, 0, 6], vocab, probs)
+
+
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("vocab,dtype,seed", LARGE_PIECES)
+def test_many_rows_of_several_pieces(ctx, vocab, dtype, seed, probs):
+    """Rows so many that the statistics take them 16384 logits at a time, the last piece shorter."""
+    check_decidable(large_pieces(vocab, probs, seed), ctx, dtype)
