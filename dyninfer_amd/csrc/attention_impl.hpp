@@ -88,6 +88,14 @@ __device__ __forceinline__ float rows_sum(float x) {
     return x + __shfl_xor(x, 32);
 }
 
+// A row's sum at the end.  Exponents are exact differences from m, which is the largest score
+// rounded to 24 bits; beyond 2^31 that alone may lie outside the exponential's range, the sum be 0 or
+// infinite: NaN, so that the row is not taken for one that sees nothing.
+__device__ __forceinline__ float row_sum(float l, float m) {
+    l = rows_sum(l);
+    return m == -__builtin_inff() || (l > 0.0f && l < __builtin_inff()) ? l : __builtin_nanf("");
+}
+
 // How a tile of the cache (two chunks of 16 positions) lies in a wave's LDS, in
 // 16-byte units, each copied by one lane straight from memory.  The order is the
 // one in which lanes read it back, so that a wave's reads are consecutive.
@@ -910,7 +918,7 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
         const uint32_t g = lane >> 4, col = lane & 15u;
 #pragma unroll
         for (int t = 0; t < NQ; t++) {
-            w.l[t] = rows_sum(w.l[t]);
+            w.l[t] = row_sum(w.l[t], w.m[t]);
             if (g == 0) {
                 sm_m[wave][16 * t + col] = w.m[t];
                 sm_l[wave][16 * t + col] = w.l[t];
@@ -1162,7 +1170,7 @@ __global__ __launch_bounds__(64 * WAVES, D < 256 ? 2 : 1) void attend_wide_kerne
         if (first_row < rows) {
 #pragma unroll
             for (int t = 0; t < NQ; t++) {
-                w.l[t] = rows_sum(w.l[t]);
+                w.l[t] = row_sum(w.l[t], w.m[t]);
                 w.m[t] = w.l[t] == 0.0f ? -__builtin_inff() : w.m[t] == -__builtin_inff() ? 0.0f : w.m[t];
             }
             uint32_t ln = lane;

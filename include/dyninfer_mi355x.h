@@ -416,6 +416,8 @@ int dyninfer_mi355x_kv_commit(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache
  * lse -inf.  q and out share a dtype (f32 or bf16); group = heads / kv_heads, any whole number.
  * lse: f32 [tokens, heads], the natural logarithm of the sum of exponentials, or NULL.
  * What is masked has no influence, whatever it holds (NaN scales included).
+ * Scores up to 2^30 in magnitude are resolved; a row whose largest score is beyond gives what it should
+ * or NaN.  Sums of scaled codes are f32, so that keys' scales beyond 2^98 may overflow.
  * Rounding: scores as from exact products with f32 sums (f32 queries: to 22 bits of a row's
  * largest); a probability times its value's scale is rounded to 16 bits of mantissa (f32: 24).
  * workspace: device memory of dyninfer_mi355x_tree_attention_workspace_bytes, 256-byte aligned

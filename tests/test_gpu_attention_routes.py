@@ -241,3 +241,32 @@ def test_pages_beyond_32_bits(ctx):
     ds = dot * 2.0 ** -24 * (dim + 16) + kvref.attend(flat, np.abs(k64), v64, sees, dim ** -0.5)[3] * 2.0 ** -22
     tol = (2 * ds + 2.0 ** -23 + 2.0 ** -24 * (32 + n / 4))[..., None] * mag + 2.0 ** -24 * np.abs(o) + 1e-30
     assert (np.abs(ctx.tree_attention(cache, batch, dev(q)).cpu().numpy() - o) <= tol).all()
+
+
+@pytest.mark.parametrize("io,news,told", [("bf16", 2, None), ("f32", 2, None), ("bf16", 2, 3000), ("f32", 2, 3000),
+                                          ("bf16", 40, None), ("f32", 40, None), ("bf16", 40, 200000), ("f32", 40, 200000)])
+def test_scores_beyond_the_exponentials_range(ctx, io, news, told):
+    """One key that every row's queries agree with, the others 0: each row gets that key's value, or,
+    from scores of 2^30 on, NaN; never 0 as if it saw nothing.  The weights are exactly 1 and 0, so
+    that the value is rounded to its terms and to the output's type only."""
+    c = Case(47, [news], [700], 1, 64, 16, 8, 8)
+    if told:
+        c.batch.max_length = told
+    c.ref.kc[...] = 0
+    p, slot = c.table[0][333 // 16], 333 % 16
+    c.ref.kc[p, 0, slot], c.ref.ks[p, 0, slot] = 127, 1
+    c.ref.vc[p, 0, slot] = 1 + c.rng.integers(0, 127, 64)
+    kb, vb = c.ref.buffers()
+    c.cache.k.copy_(dev(kb)), c.cache.v.copy_(dev(vb))
+    q = c.rng.uniform(0.5, 1, (news, 4, 64)) * np.exp2(c.rng.uniform(6, 60, (news, 4, 1)))
+    q = dev(q.astype(np.float32), DT[io])
+    lse = torch.zeros((news, 4), device="cuda")
+    got = ctx.tree_attention(c.cache, c.batch, q, lse=lse).double().cpu().numpy()
+    score = q.double().sum(-1).cpu().numpy() * 127 / 8
+    assert (score < 2.0 ** 29).any() and (score > 2.0 ** 33).any()
+    v = c.ref.row(p, slot, "v")[0]
+    right = (np.abs(got - v) <= np.abs(v) * (2.0 ** -22 if io == "f32" else 2.0 ** -8 + 2.0 ** -16)).all(-1)
+    lost = np.isnan(got).all(-1)
+    assert (right | lost).all() and not lost[score < 2.0 ** 30].any()
+    lse = lse.cpu().numpy().astype(np.float64)
+    assert (np.isnan(lse) == lost).all() and (np.abs(lse - score) <= score * 2.0 ** -16)[right].all()
