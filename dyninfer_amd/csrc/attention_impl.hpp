@@ -118,7 +118,7 @@ struct TileLds {
     static_assert(KMAIN % 64 == 0 && V % 32 == 0 && KS + VS <= 64, "whole copies");
     // Tiles a wave holds: one is worked on while the others are on their way.  Two
     // of 8-bit codes and 128 dims make some 70 KB a workgroup, two of them a CU.
-    static constexpr uint32_t STAGES = BYTES > 9216 ? 2 : BYTES > 6656 ? 2 : BYTES > 4608 ? 3 : 4;
+    static constexpr uint32_t STAGES = BYTES > 6656 ? 2 : BYTES > 4608 ? 3 : 4;
 };
 
 // 16 bytes a lane from src + OFF to dst + 16 lane.  OFF is the instruction's own

@@ -85,7 +85,7 @@ int check_batch(const dyninfer_kvbatch_t* b, bool tables, dmx::KvBatch& out) {
     return 0;
 }
 
-int check_rows(const dyninfer_rows_t* r, uint32_t dim, const char* what, dmx::KvRows& out) {
+int check_rows(const dyninfer_rows_t* r, const char* what, dmx::KvRows& out) {
     const std::string w(what);
     if (!r || !r->data) return fail(BAD, w + " is NULL");
     if (r->dtype != DYNINFER_DTYPE_F32 && r->dtype != DYNINFER_DTYPE_BF16) return fail(UNSUPPORTED, w + " must be f32 or bf16");
@@ -98,13 +98,12 @@ int check_rows(const dyninfer_rows_t* r, uint32_t dim, const char* what, dmx::Kv
     out.hs = r->head_stride;
     out.bf16 = e == 2;
     out.vec = aligned(r->data, 16) && r->token_stride * e % 16 == 0 && (r->heads == 1 || r->head_stride * e % 16 == 0);
-    (void)dim;
     return 0;
 }
 
 // Rows that are written: no two heads or tokens may share an element.
 int check_out(const dyninfer_rows_t* r, uint32_t dim, uint32_t tokens, const char* what, dmx::KvRows& out) {
-    if (int rc = check_rows(r, dim, what, out)) return rc;
+    if (int rc = check_rows(r, what, out)) return rc;
     const int64_t d = dim, h = r->heads, n = tokens;
     const bool token_major = (h <= 1 || r->head_stride >= d) && (n <= 1 || r->token_stride >= (h > 1 ? (h - 1) * r->head_stride + d : d));
     const bool head_major = (n <= 1 || r->token_stride >= d) && (h <= 1 || r->head_stride >= (n > 1 ? (n - 1) * r->token_stride + d : d));
@@ -218,7 +217,7 @@ int dyninfer_mi355x_rope(dyninfer_mi355x_ctx_t* ctx, const dyninfer_rows_t* x, c
     if (int rc = check_rope(rope, head_dim, tokens, rp)) return rc;
     if (tokens == 0) return DYNINFER_MI355X_OK;
     dmx::KvRows in, out;
-    if (int rc = check_rows(x, head_dim, "x", in)) return rc;
+    if (int rc = check_rows(x, "x", in)) return rc;
     if (int rc = check_out(y, head_dim, tokens, "y", out)) return rc;
     if (x->dtype != y->dtype || x->heads != y->heads) return fail(BAD, "x and y must share dtype and heads");
     if (int rc = check_apart(x, y, tokens, head_dim, "y")) return rc;
@@ -252,12 +251,12 @@ int dyninfer_mi355x_kv_append(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache
         if (int rc = check_rope(rope, kv.dim, b.tokens, rp)) return rc;
     if (b.tokens == 0 || b.seqs == 0) return DYNINFER_MI355X_OK;
     dmx::KvRows kr, vr, qr = {}, qo = {};
-    if (int rc = check_rows(k, kv.dim, "k", kr)) return rc;
-    if (int rc = check_rows(v, kv.dim, "v", vr)) return rc;
+    if (int rc = check_rows(k, "k", kr)) return rc;
+    if (int rc = check_rows(v, "v", vr)) return rc;
     if (k->heads != kv.heads || v->heads != kv.heads) return fail(BAD, "k and v must have the cache's heads");
     if (k->dtype != v->dtype) return fail(BAD, "k and v must share a dtype");
     if (q) {
-        if (int rc = check_rows(q, kv.dim, "q", qr)) return rc;
+        if (int rc = check_rows(q, "q", qr)) return rc;
         if (int rc = check_out(q_out, kv.dim, b.tokens, "q_out", qo)) return rc;
         if (q->dtype != q_out->dtype || q->heads != q_out->heads) return fail(BAD, "q and q_out must share dtype and heads");
         if (int rc = check_apart(q, q_out, b.tokens, kv.dim, "q_out")) return rc;
@@ -335,7 +334,7 @@ int dyninfer_mi355x_tree_attention(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kv
     if (int rc = check_cache(cache, a.kv)) return rc;
     if (int rc = check_batch(batch, true, a.b)) return rc;
     if (a.b.tokens == 0 || a.b.seqs == 0 || a.b.max_new == 0) return DYNINFER_MI355X_OK;
-    if (int rc = check_rows(q, a.kv.dim, "q", a.q)) return rc;
+    if (int rc = check_rows(q, "q", a.q)) return rc;
     if (int rc = check_out(out, a.kv.dim, a.b.tokens, "out", a.out)) return rc;
     if (q->dtype != out->dtype || q->heads != out->heads) return fail(BAD, "q and out must share dtype and heads");
     if (meet(q, out, a.b.tokens, a.kv.dim) && !interleaved(q, out, a.kv.dim)) return fail(BAD, "out overlaps q");

@@ -41,11 +41,11 @@ struct Stat {
 
 // What the draw needs of a sequence, written by the walk.
 struct Left {
-    uint32_t row;    // of the logits; ~0: no rows
+    uint32_t row;    // of the logits; ~0: nothing to draw (greedy, or no rows)
     uint32_t gone;   // rejected tokens (no draft probabilities), in the list of row0 + j
     float m, inv_t;  // p = exp((x - m) inv_t) / s
     float s, a;      // scores (e - a s q) / noise
-    uint32_t greedy, done;
+    uint32_t done;   // workgroups of the draw that have brought their best
     unsigned long long best;
 };
 
