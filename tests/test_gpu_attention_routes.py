@@ -270,3 +270,20 @@ def test_scores_beyond_the_exponentials_range(ctx, io, news, told):
     assert (right | lost).all() and not lost[score < 2.0 ** 30].any()
     lse = lse.cpu().numpy().astype(np.float64)
     assert (np.isnan(lse) == lost).all() and (np.abs(lse - score) <= score * 2.0 ** -16)[right].all()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("kb", [8, 4])
+@pytest.mark.parametrize("news,power", [(2, 97), (40, 97), (2, -110), (40, -110)])
+def test_keys_and_queries_far_from_one(ctx, io, kb, news, power):
+    """Keys' scales near 2^98, up to where sums of scaled codes stay finite, and very small ones, with
+    queries that bring the scores back to ordinary sizes."""
+    c = Case(48, [news], [300], 1, 64, 16, kb, 8)
+    c.ref.ks[...] = kvref.bf16(c.rng.uniform(0.5, 1, c.ref.ks.shape) * 2.0 ** power)
+    kbuf, vbuf = c.ref.buffers()
+    c.cache.k.copy_(dev(kbuf)), c.cache.v.copy_(dev(vbuf))
+    q = dev((c.rng.normal(0, 1, (news, 4, 64)) * 2.0 ** -(power + 3)).astype(np.float32), DT[io])
+    lse = torch.zeros((news, 4), device="cuda")
+    got = ctx.tree_attention(c.cache, c.batch, q, lse=lse).double().cpu().numpy()
+    out, want, tol, ltol = expect(c, q.float().cpu().numpy(), chain([news], [300]), 0.125, io == "f32")
+    assert (np.abs(got - out) <= tol).all() and (np.abs(lse.cpu().numpy() - want) <= ltol).all()
