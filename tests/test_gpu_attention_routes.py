@@ -33,7 +33,8 @@ def tree_masks(c, count):
 ROUTES = [  # dims, type, group, new rows, lengths, told longest length, tiles
     ((64, 96, 128, 256), "bf16", 2, [3, 5, 1], [300, 0, 700], 3000, 1),
     ((64, 96, 128, 256), "f32", 2, [3, 5, 1], [300, 0, 700], 3000, 1),
-    ((256,), "bf16", 4, [6, 5, 8], [300, 0, 700], 200000, 1),       # two row tiles of 16
+    ((64, 96, 128), "f32", 4, [6, 5, 8], [300, 0, 700], 2500, 1),   # two row tiles of 16, as are the next
+    ((256,), "bf16", 4, [6, 5, 8], [300, 0, 700], 200000, 1),
     ((256,), "f32", 4, [6, 5, 8], [300, 0, 700], 200000, 1),
     ((64, 96, 128), "bf16", 4, [12, 9, 1], [300, 0, 513], 200000, 2),
     ((64, 96, 128), "bf16", 4, [12, 9, 1], [300, 0, 513], 2500, 4),
