@@ -564,9 +564,9 @@ class Context:
         return out
 
     # ---- around attention: rotary positions, the quantized cache, attention over it, verification
-    # Host time of a call (us, small sizes): rope 8.1, kv_append with queries 11.0, kv_read
-    # 11.5, tree_attention 15.5, draft_verify 21; of it the C entry, mostly its launches, 3.9 a launch,
-    # a new output or workspace 1.2 to 1.7, a checked descriptor 0.3 to 1.
+    # Host time of a call (us, small sizes): rope 7.9, kv_append with queries 11.2, kv_read 10.9,
+    # kv_commit 7.8, tree_attention 10.6 with one launch and 15.6 with two, draft_verify 20; of it the C entry,
+    # mostly its launches, 3.9 a launch, a new output or workspace 1.2 to 1.7, a checked descriptor 0.3 to 1.
     def _on(self, stream) -> int:
         """The raw stream: the given one, or the current one of the context's device."""
         if stream is None:

@@ -15,7 +15,7 @@ namespace {
 // SPLIT waves per (row, query head) whose unit was split: the parts' maxima and
 // sums, then the parts' outputs, each brought to the common maximum; of SPLIT waves
 // every one takes four parts of each 4 SPLIT.  Bound by latency:
-// 5.4 us for 8192 rows of two or three parts (7.9 when every wave found its parts by
+// 5.3 us for 8192 rows of two or three parts (7.9 when every wave found its parts by
 // itself, with some 260 scalar instructions).
 template <int D, int SPLIT>
 __global__ __launch_bounds__(SPLIT == 1 ? 256 : 64 * SPLIT) void join_kernel(AttnArgs a, uint32_t tile_shift) {
@@ -105,26 +105,35 @@ void join_launch(const AttnArgs& a, uint32_t shift, uint32_t parts, hipStream_t 
 
 // Row tiles: one or two of 16 rows held by every wave, or four, eight or sixteen held
 // one or two a wave (four waves, eight of sixteen).  Larger ones decode a position for
-// more rows, smaller ones make more workgroups and leave out more of a prompt.  Times (us)
-// with 2, 4, 8 and 16, 4 rows a token, by `work`, the steps of all units of eight tiles:
-//   1 x 63 tokens after 500 (work 80): 17.2 15.6 19.3 23.8; after 4000 (528): 30.8 34.8 41.3
-//   40.5; 32 x 63 after 4000 (16896): 425 390 293 281; 1 x 16 after 4000 (128): 22.9 18.0,
-//   after 64000 (2000): 73 77 89; 32 x 16 after 1000 (1024): 33 43 58
-//   prompts: 1 x 512 (512): 18.7 23.2 30.8 42.9; 1 x 1024 (2048): 43.9 44.2 55.7 74.4; 4 x 2048
-//   (32768): 419 374 286 297; 1 x 512 after 8000: 193 207 156 151
-// f32, whose queries' second terms are in LDS where a wave holds two tiles: 1 x 8 after 500
-// 11.6 with one, 15.1 with two, after 60000 (938) 58.7 57.5, 32 x 8 after 4000 (2048)
-// 74.3 68.2 (88 with four); 32 x 16 after 4000 126 with one, 100 with four; 8 x 63 after 2000
-// (2016) 54.9 with four, 57.3 with sixteen, 32 x 63 after 1000 (4536) 130 115, 4 x 1024 as a
-// prompt 130 174.  256 dims: one tile a wave, 32 x 8 after 4000 160 with one, 211 with four.
+// more rows, smaller ones make more workgroups and leave out more of a prompt.  Times (us, ten
+// calls in a graph) of 32 query over 8 kv heads, 8 bits, 128 dims [64 dims], with 2, 4, 8 and 16
+// tiles, by `work`, the steps of all units of eight tiles:
+//   1 x 63 tokens after 500 (80): 18.0 15.2 18.6 23.3 [14.1 13.2 15.7 18.2]; after 4000 (504):
+//   30.4 32.3 37.2 38.5 [22.4 24.7 27.8 29.1]; 32 x 63 after 4000 (16128): 409 385 274 263
+//   [268 284 204 200]; 1 x 16 after 4000 (128): 24.4 19.4 21.4 27.2 [18.0 15.1 16.7 21.6], after
+//   64000 (2004): 65 63 77 103 [45 47 60 87]; 32 x 16 after 1000 (1024): 36 43 55 53 [25 34 44 45]
+//   prompts: 1 x 512 (512): 18.6 23.6 31.2 38.3 [13.0 18.9 24.9 30.0]; 1 x 1024 (2048): 44.2 43.6
+//   55.1 66.2 [30.8 33.2 43.1 52.5]; 4 x 2048 (32768): 429 391 291 307 [294 208 186 225]; 1 x 512
+//   after 8000 (8576): 189 211 154 151 [131 157 116 116]
+// f32, whose queries' second terms are in LDS where a wave holds two tiles, with 1, 2, 4 and 16:
+//   1 x 8 after 500: 12.0 15.7 14.1 20.1 [10.4 12.9 12.6 16.0], after 60000 (940): 54 49 61 136
+//   [37 35 48 92]; 32 x 8 after 4000 (2048): 102 87 115 271 [66 57 88 179]; 32 x 16 after 4000: 189
+//   134 130 280 [118 88 94 183]; 8 x 63 after 2000 (2142): 97 73 79 79 [68 52 61 55]; 32 x 63 after
+//   1000 (4536): 195 149 121 109 [129 99 72 70]; 4 x 1024 as a prompt: 233 185 131 177 [154 123 82 112]
+// 256 dims, with 1 and 4: 1 x 63 after 4000 63 53, 32 x 16 after 1000 121 71, 1 x 16 after 4000 29 36,
+// f32 32 x 8 after 4000 248 280.  96 dims and 4 bits order themselves alike, most times within a tenth.
+// The rule misses the best by more than a tenth in three places: f32 from 33 rows over contexts that are
+// not long (two tiles: 52 for 61 and 88 for 94 above, at 64 dims), f32 prompts of 512 (22.6 for 26.1),
+// 256 dims of 64 rows over a short context (29 for 36).
 // The steps of all units go in equal shares to as many workgroups as the CUs
 // hold at once (two each; one of 256 dims), or one step each if they are fewer:
 // sequences differ in length, and a share may end in the middle of a unit.
 // Writing and joining parts costs as much as some steps, so units of few steps, and
-// units so many that they fill the CUs several times over, are a workgroup each:
-// 32 ragged sequences of up to 512, 1024 and 2048 positions with 8 rows took 19, 28
-// and 48 us that way and 29, 35 and 49 in shares, one sequence of 380 with one row 9.6
-// and 11.4, of 760 14.6 and 11.9, 100 of up to 8000 272 and 206.
+// units so many that they fill the CUs several times over, are a workgroup each.  In shares and
+// whole: one row over 380 positions 11.3 10.5 [10.2 8.7], over 760 11.8 15.7 [10.8 12.5]; 32 ragged
+// sequences with 8 rows of up to 500 26.4 18.7 [20.2 13.1], 1000 30.9 27.5 [24.5 19.8], 2000 38.4
+// 44.1 [30.9 31.3]; 100 of up to 1500 76.3 76.3 [52.6 50.1], of up to 8000 242 294 [160 207].  256 dims
+// 14.0 15.8, 14.5 24.0, 41 37, 53 54, 83 98, 190 226 (taken whole, the rule's loss there), 736 848.
 // Rows of a chain see only what lies before them, so a prompt's row tiles differ in
 // length, which only whole units make use of: taken where what is left out is worth
 // a unit a CU.

@@ -33,7 +33,10 @@
 // queries: a second f16 holds what the first leaves), each block's sum is
 // multiplied by its f32 scale.  V codes are exact in bf16; p times the value's
 // scale, of unknown range, is split into bf16 terms: two (16 bits) for bf16
-// outputs, three (24 bits) for f32 ones.
+// outputs, three (24 bits) for f32 ones.  A third term for bf16 took 295 us instead of 261 for
+// 64 tokens over 131071 positions and 4.26 ms instead of 3.72 for a prompt of 16384; of the first's outputs
+// 0.25% are not the 64-bit value rounded to bf16 with two terms and 0.07% with three, 0.28% where
+// the same is computed in f32 throughout.
 #pragma once
 #include <type_traits>
 
@@ -820,9 +823,9 @@ constexpr int resident(int d, int nq) { return d * nq <= 256 && d < 256 ? 2 : 1;
 
 // Few rows (up to 16 NQ): every wave holds all of them and takes every fourth
 // tile of positions, copied straight into LDS and decoded as it is read.  32 ragged
-// sequences of up to 4096 positions, 8 tokens of 32 / 8 heads of 128 dims: 48 us, 188 MB
-// at 3.9 TB/s, a wave issuing in 41% of its cycles and waiting in 34%; one token
-// over 700 positions 8.7 us, latency.
+// sequences of up to 4096 positions, 8 tokens of 32 / 8 heads of 128 dims: 53 us, 188 MB
+// at 3.5 TB/s, a wave issuing in 41% of its cycles and waiting in 34%; one token
+// over 700 positions 8.8 us, latency.
 template <int D, int KB, int VB, int NQ, bool F32>
 __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a) {
     using T = TileLds<D, KB, VB>;
@@ -969,7 +972,7 @@ __global__ __launch_bounds__(256, resident(D, NQ)) void attend_kernel(AttnArgs a
 // operands in LDS for all, one tile ahead; the codes of the tile after that are on
 // their way into registers.  A step of few rows spends two fifths of its vector
 // instructions on decoding; here that is shared by four or eight waves.  64 tokens over
-// 131071 positions of 8 heads, 256 rows each: 275 us, 137 GFLOP at 500 TFLOP/s (and half
+// 131071 positions of 8 heads, 256 rows each: 252 us, 137 GFLOP at 545 TFLOP/s (and half
 // as many products again for the probabilities' second terms), bound by the issue of the vector
 // instructions around the products: 34% of the SIMDs' cycles are MFMAs.
 constexpr uint32_t kWideTile = 64;

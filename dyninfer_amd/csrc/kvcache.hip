@@ -172,8 +172,9 @@ __device__ __forceinline__ void store4(const KvRows& r, int64_t at, const float 
 
 // One head of one token: loads, rotates, stores.  Halves of whole fours: a lane takes four
 // pairs (with eight dims of one half it loads their partners as well and twice the cosines:
-// append over 4 x 2048 tokens 36.0 us instead of 30.7, one token 2.2 instead of 1.8).  Otherwise in place is safe as well: a head's lanes are one
-// wave's, which has loaded all of it before its first store.
+// append over 4 x 2048 tokens 36.0 us instead of 30.7, one token 2.2 instead of 1.8).  Otherwise
+// in place is safe as well: a head's lanes are one wave's, which has loaded all of it before its
+// first store.
 template <int D>
 __device__ __forceinline__ void rope_row(const KvRows& x, const KvRows& y, uint32_t token, uint32_t head, uint32_t lane,
                                          const RopeView& rp) {
@@ -217,7 +218,7 @@ __device__ __forceinline__ void rope_row(const KvRows& x, const KvRows& y, uint3
     if (d0 < D) store8(y, (int64_t)token * y.ts + (int64_t)head * y.hs + d0, v);
 }
 
-// 4099 tokens of 40 heads of 128 dims in f32: 27.9 us, 6.2 TB/s; one token 1.8 us.  (Four
+// 4099 tokens of 40 heads of 128 dims in f32: 28.9 us, 6.0 TB/s; one token 1.8 us.  (Four
 // heads of a token by a thread, which share its cosines: 29.4 and 3.7.)
 template <int D>
 __global__ __launch_bounds__(256) void rope_kernel(KvRows x, KvRows y, uint32_t tokens, uint32_t heads, RopeView rp) {
@@ -517,7 +518,8 @@ __global__ __launch_bounds__(256) void read_kernel(KvView kv, KvBatch b, KvRows 
 // One workgroup per (sequence, head, keys or values).  A thread owns the same
 // bytes of every row (a dword of a key, a dim of a value), so its moves are in
 // order by themselves: a row's source lies at or after every row written so far.
-// Latency: 7.5 us for 16 trees of 24.
+// Latency, some four dependent loads a move, one move after another: 7.6 us for 16 paths out of trees of 24,
+// 9.0 for 16 paths of ten, 43 for 16 of 64.
 template <int D, int KB, int VB>
 __global__ __launch_bounds__(256) void commit_kernel(KvView kv, KvBatch b, const int32_t* path, uint32_t path_stride,
                                                      const int32_t* counts) {

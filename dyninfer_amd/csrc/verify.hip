@@ -23,7 +23,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // Logits of a workgroup of the statistics.  Few rows are cut finer, for the
 // latency of one pass: 5 bf16 rows of 151936 in 16384s took 9.3 us, in 4096s 5.4
-// (4.8 with four loads in flight); 376 f32 rows, 228 MB, take 38 us, 49.8 with one
+// (4.8 with four loads in flight); 376 f32 rows, 228 MB, take 38 to 43 us, 49.8 with one
 // load in flight and an accurate exponential of every element.
 constexpr uint32_t kPiece = 16384, kSmallPiece = 4096;
 constexpr uint32_t kManyPieces = 1024;  // workgroups from which the large pieces are taken
@@ -212,9 +212,10 @@ __device__ __forceinline__ void eight(const void* p, uint32_t bf16, int64_t i, f
 }
 
 // This thread's share of sum max(p - aq q, 0) over a row, or, without q, of what the
-// rejected tokens leave of p.  One workgroup reads the row, bound by its instructions: calls
-// of 8 trees of 8 with f32 and bf16 probabilities over 151936 tokens took 181 and 240 us with
-// loads of one element and an accurate exponential, so 78 and 84.
+// rejected tokens leave of p.  One workgroup reads the row, bound by its instructions, some 17 us
+// for 151936 tokens: 15 siblings that all miss, 14 such sums, take 246 us of a call's 271 with f32
+// probabilities, 258 of 285 with bf16.  (Calls of 8 trees of 8 took 181 and 240 us with loads of one
+// element and an accurate exponential, so 78 and 84 on the same drafts.)
 __device__ float left_of_row(const VerifyArgs& a, uint32_t row, const Stat& st, float inv_t, float aq, const int32_t* gone,
                              uint32_t rejected) {
     if (st.m == -__builtin_inff()) return 0.0f;
