@@ -25,7 +25,7 @@ import json
 import os
 import struct
 from dataclasses import dataclass
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 __all__ = [
     "LIB_PATH", "DyninferError", "QWeight", "Context", "library", "candidates", "registry_select",
@@ -69,7 +69,8 @@ EXPORTED_SYMBOLS = (
     "dyninfer_mi355x_rope_table", "dyninfer_mi355x_rope", "dyninfer_mi355x_kv_cache_bytes", "dyninfer_mi355x_kv_append",
     "dyninfer_mi355x_kv_read", "dyninfer_mi355x_kv_commit", "dyninfer_mi355x_tree_attention",
     "dyninfer_mi355x_tree_attention_workspace_bytes", "dyninfer_mi355x_draft_verify",
-    "dyninfer_mi355x_draft_verify_workspace_bytes",
+    "dyninfer_mi355x_draft_verify_workspace_bytes", "dyninfer_mi355x_qk_norm_rope", "dyninfer_mi355x_kv_append_normed",
+    "dyninfer_mi355x_token_logprobs", "dyninfer_mi355x_token_logprobs_workspace_bytes",
 )
 
 
@@ -98,7 +99,9 @@ _pack_kvcache = struct.Struct("@6I5Q").pack
 _pack_kvbatch = struct.Struct("@3Q4IQ").pack
 _pack_rows = struct.Struct("@Q2I2q").pack
 _pack_rope = struct.Struct("@2Q4I").pack
+_pack_head_norm = struct.Struct("@QI2fI").pack
 _pack_rope_params = struct.Struct("@2I8d").pack
+_pack_logprobs = struct.Struct("@Qq2Q4I5Q").pack
 _pack_verify = struct.Struct("@2Q2I2q6Qq4I3Q").pack
 
 _lib: Optional[ctypes.CDLL] = None
@@ -165,10 +168,14 @@ def library() -> ctypes.CDLL:
         "dyninfer_mi355x_rope": (I, [P, P, P, U32, U32, P, P]),
         "dyninfer_mi355x_kv_cache_bytes": (I, [P, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)]),
         "dyninfer_mi355x_kv_append": (I, [P, P, P, P, P, P, P, P, P]),
+        "dyninfer_mi355x_qk_norm_rope": (I, [P, P, P, P, P, P, P, U32, U32, P, P]),
+        "dyninfer_mi355x_kv_append_normed": (I, [P, P, P, P, P, P, P, P, P, P, P]),
         "dyninfer_mi355x_kv_read": (I, [P, P, P, P, P, P]),
         "dyninfer_mi355x_kv_commit": (I, [P, P, P, P, U32, P, P]),
         "dyninfer_mi355x_tree_attention": (I, [P, P, P, P, P, U32, ctypes.c_float, P, P, P, ctypes.c_uint64, P]),
         "dyninfer_mi355x_tree_attention_workspace_bytes": (I, [P, P, U32, U32, ctypes.POINTER(ctypes.c_uint64)]),
+        "dyninfer_mi355x_token_logprobs": (I, [P, P, P, ctypes.c_uint64, P]),
+        "dyninfer_mi355x_token_logprobs_workspace_bytes": (I, [U32, U32, U32, U32, ctypes.POINTER(ctypes.c_uint64)]),
         "dyninfer_mi355x_draft_verify": (I, [P, P, P, ctypes.c_uint64, P]),
         "dyninfer_mi355x_draft_verify_workspace_bytes": (I, [U32, U32, U32, U32, ctypes.POINTER(ctypes.c_uint64)]),
     }
@@ -333,6 +340,14 @@ def _verify_workspace_bytes(seqs: int, tokens: int, vocab: int, max_new: int) ->
     return need.value
 
 
+@functools.lru_cache(maxsize=64)
+def _logprobs_workspace_bytes(rows: int, vocab: int, top: int, dtype: int) -> int:
+    """dyninfer_mi355x_token_logprobs_workspace_bytes, which depends on these numbers only."""
+    need = ctypes.c_uint64(0)
+    _check(library().dyninfer_mi355x_token_logprobs_workspace_bytes(rows, vocab, top, dtype, ctypes.byref(need)))
+    return need.value
+
+
 def _table(t, code: int, shape, what: str) -> int:
     """Address of a contiguous device tensor of that type and shape (None: any length)."""
     if not _TABLE_DTYPES:
@@ -451,6 +466,26 @@ class Rope:
                               _table(self.positions, _T_I32, (tokens,), "positions"), n, rot, layout, 0)
         except struct.error as e:
             _bad(f"rope: {e}")
+
+
+@dataclass
+class HeadNorm:
+    """The norm of a head (dyninfer_head_norm_t): x / sqrt(mean(x^2) + eps) * (weight + offset).
+    ``weight``: device tensor [head_dim], f32 or bf16, or None (ones)."""
+    weight: object = None
+    eps: float = 1e-6
+    offset: float = 0.0
+
+    def pack(self, dim: int) -> bytes:
+        """The C struct's bytes."""
+        w = self.weight
+        if w is not None and (not w.is_cuda or w.shape != (dim,) or not w.is_contiguous()):
+            _bad(f"the norm's weight must be a contiguous device tensor [{dim}]")
+        try:
+            return _pack_head_norm(0 if w is None else w.data_ptr(), DTYPE_F32 if w is None else _dtype_code(w), self.eps,
+                                   self.offset, 0)
+        except (struct.error, OverflowError) as e:
+            _bad(f"norm: {e}")
 
 
 class Context:
@@ -626,18 +661,43 @@ class Context:
                                               rope.pack(n), self._on(stream)))
         return out
 
+    def qk_norm_rope(self, q, k=None, rope: Optional[Rope] = None, q_norm: Optional[HeadNorm] = None,
+                     k_norm: Optional[HeadNorm] = None, q_out=None, k_out=None, stream=None):
+        """q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] with each head by its norm,
+        then rotated, in one launch: (q_out, k_out) (dyninfer_mi355x_qk_norm_rope).  Either norm, or
+        ``rope``, may be None; q_out may be q, k_out may be k."""
+        if q_out is None:
+            q_out = self._like(q, stream)
+        if k is not None and k_out is None:
+            k_out = self._like(k, stream)
+        n, _, dim = q.shape if q.dim() == 3 else (0, 0, 0)
+        _check(self._lib.dyninfer_mi355x_qk_norm_rope(
+            self._h, _rows(q, n, dim, "q"), None if q_norm is None else q_norm.pack(dim), _rows(q_out, n, dim, "q_out"),
+            None if k is None else _rows(k, n, dim, "k"), None if k_norm is None else k_norm.pack(dim),
+            None if k_out is None else _rows(k_out, n, dim, "k_out"), n, dim, None if rope is None else rope.pack(n),
+            self._on(stream)))
+        return q_out, k_out
+
     def kv_append(self, cache: KVCache, batch: KVBatch, k, v, rope: Optional[Rope] = None, q=None, q_out=None,
-                  stream=None):
+                  stream=None, q_norm: Optional[HeadNorm] = None, k_norm: Optional[HeadNorm] = None):
         """Quantizes the rows k, v [tokens, kv_heads, head_dim] into the cache, k rotated first if
         ``rope`` is given; then q [tokens, heads, head_dim] is rotated by the same launch and
-        returned (dyninfer_mi355x_kv_append)."""
+        returned (dyninfer_mi355x_kv_append).  With ``k_norm`` or ``q_norm`` heads take their norm
+        before the rotation (dyninfer_mi355x_kv_append_normed)."""
         n, dim = batch.tokens, cache.head_dim
         if q is not None and q_out is None:
             q_out = self._like(q, stream)
-        _check(self._lib.dyninfer_mi355x_kv_append(
-            self._h, cache.pack(), batch.pack(), _rows(k, n, dim, "k"), _rows(v, n, dim, "v"),
-            None if rope is None else rope.pack(n), None if q is None else _rows(q, n, dim, "q"),
-            None if q_out is None else _rows(q_out, n, dim, "q_out"), self._on(stream)))
+        if q_norm is None and k_norm is None:
+            _check(self._lib.dyninfer_mi355x_kv_append(
+                self._h, cache.pack(), batch.pack(), _rows(k, n, dim, "k"), _rows(v, n, dim, "v"),
+                None if rope is None else rope.pack(n), None if q is None else _rows(q, n, dim, "q"),
+                None if q_out is None else _rows(q_out, n, dim, "q_out"), self._on(stream)))
+            return q_out
+        _check(self._lib.dyninfer_mi355x_kv_append_normed(
+            self._h, cache.pack(), batch.pack(), _rows(k, n, dim, "k"), None if k_norm is None else k_norm.pack(dim),
+            _rows(v, n, dim, "v"), None if rope is None else rope.pack(n), None if q is None else _rows(q, n, dim, "q"),
+            None if q_norm is None else q_norm.pack(dim), None if q_out is None else _rows(q_out, n, dim, "q_out"),
+            self._on(stream)))
         return q_out
 
     def kv_read(self, cache: KVCache, batch: KVBatch, dtype=None, k_out=None, v_out=None, stream=None):
@@ -729,6 +789,42 @@ class Context:
             vocab, seqs, n, max_new, path.data_ptr(), counts.data_ptr(), token.data_ptr())
         _check(self._lib.dyninfer_mi355x_draft_verify(self._h, args, wp, wn, self._on(stream)))
         return path, counts, token
+
+    def token_logprobs(self, logits, tokens=None, top: int = 0, temperature=None, stream=None, workspace=None):
+        """Of logits [rows, vocab]: ``TokenLogprobs`` with the log probabilities of ``tokens`` (int64
+        [rows]), their ranks, the entropy, and the ``top`` likeliest tokens with their log probabilities
+        (dyninfer_mi355x_token_logprobs).  ``temperature`` f32 [rows] (0: greedy) or None (1).  What is not
+        asked for is None."""
+        import torch
+        if not logits.is_cuda or logits.dim() != 2 or logits.stride(1) != 1:
+            _bad("logits must be a device tensor [rows, vocab] whose last axis is contiguous")
+        n, vocab = logits.shape
+        if not isinstance(top, int) or top < 0:
+            _bad("top must be a number of tokens")
+        code = _dtype_code(logits)
+        kp = 0 if tokens is None else _table(tokens, _T_I64, (n,), "tokens")
+        tp = 0 if temperature is None else _table(temperature, _T_F32, (n,), "temperature")
+        wp, wn, _keep = self._work(_logprobs_workspace_bytes(n, vocab, top, code), workspace, logits.device, stream)
+        new = lambda shape, dtype: self._new(shape, dtype, logits.device, stream)
+        entropy = new((n,), torch.float32)
+        logprobs = None if tokens is None else new((n,), torch.float32)
+        ranks = None if tokens is None else new((n,), torch.int32)
+        top_tokens = new((n, top), torch.int64) if top else None
+        top_logprobs = new((n, top), torch.float32) if top else None
+        ptr = lambda t: 0 if t is None else t.data_ptr()
+        args = _pack_logprobs(logits.data_ptr(), logits.stride(0), kp, tp, code, n, vocab, top, ptr(logprobs), ptr(ranks),
+                              ptr(entropy), ptr(top_tokens), ptr(top_logprobs))
+        _check(self._lib.dyninfer_mi355x_token_logprobs(self._h, args, wp, wn, self._on(stream)))
+        return TokenLogprobs(logprobs, ranks, entropy, top_tokens, top_logprobs)
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``Context.token_logprobs`` returns."""
+    logprobs: object      # f32 [rows], or None without tokens
+    ranks: object         # int32 [rows], or None without tokens
+    entropy: object       # f32 [rows]
+    top_tokens: object    # int64 [rows, top], or None
+    top_logprobs: object  # f32 [rows, top], or None
 
 
 def candidates() -> list:

@@ -1,4 +1,4 @@
-// Rotary positions and the quantized paged cache: writing, reading back, and
+// Norms of heads, rotary positions and the quantized paged cache: writing, reading back, and
 // keeping an accepted path.  All are bound by memory (large calls) or by the
 // latency of one launch (small ones); the arithmetic is small beside either.
 //
@@ -76,11 +76,97 @@ __device__ __forceinline__ void store8(const KvRows& r, int64_t at, const float 
     }
 }
 
-// x: dims d0..d0+7 of the row at element offset `row`; rotated in place.  The
+// What a row's values are multiplied by before they are rotated: nothing, or ..
+struct NoNorm {
+    __device__ __forceinline__ void apply(uint32_t, float (&)[8]) const {}
+    __device__ __forceinline__ void apply(uint32_t, float (&)[4]) const {}
+    __device__ __forceinline__ float one(uint32_t, float x) const { return x; }
+};
+
+// .. its root mean square's inverse and the weight of the dim: (x f) r (w + offset), where f is
+// 1, or 2^-72 for a row whose squares would leave f32.
+struct HeadNorm {
+    const NormView& n;
+    float f, r;
+
+    __device__ __forceinline__ float one(uint32_t d, float x) const {
+        x = x * f * r;
+        if (!n.weight) return x * (1.0f + n.offset);
+        return x * ((n.bf16 ? bf16_bits_to_f32(gptr<uint16_t>(n.weight)[d]) : gptr<float>(n.weight)[d]) + n.offset);
+    }
+    template <int N>
+    __device__ __forceinline__ void apply(uint32_t d0, float (&x)[N]) const {
+        float w[N];
+        if (!n.weight) {
+#pragma unroll
+            for (int i = 0; i < N; i++) w[i] = 1.0f;
+        } else if (n.vec && n.bf16) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                const u32x2 a = *gptr<u32x2>(static_cast<const uint16_t*>(n.weight) + d0 + i);
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[i + j] = __uint_as_float(j & 1 ? a[j / 2] & 0xFFFF0000u : a[j / 2] << 16);
+            }
+        } else if (n.vec) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                const f32x4 a = *gptr<f32x4>(static_cast<const float*>(n.weight) + d0 + i);
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[i + j] = a[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                w[i] = n.bf16 ? bf16_bits_to_f32(gptr<uint16_t>(n.weight)[d0 + i]) : gptr<float>(n.weight)[d0 + i];
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = x[i] * f * r * (w[i] + n.offset);
+    }
+};
+
+// Sum over the N lanes around this one (N a power of two, 8 to 32, aligned), the same in all of them.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float x) {
+    auto moved = [](float v, auto ctrl) {
+        return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), decltype(ctrl)::value, 0xF, 0xF, true));
+    };
+    x += moved(x, std::integral_constant<int, 0xB1>());   // lane ^ 1
+    x += moved(x, std::integral_constant<int, 0x4E>());   // lane ^ 2
+    x += moved(x, std::integral_constant<int, 0x141>());  // mirrored in 8
+    if constexpr (N > 8) x += moved(x, std::integral_constant<int, 0x140>());  // mirrored in 16
+    if constexpr (N > 16) x += __shfl_xor(x, 16);
+    return x;
+}
+
+// The norm of the head whose D dims the kLanes<D> lanes around this one hold, eight in each
+// (zeros in lanes without dims; the lanes of a head come here together).  v_rsq_f32 is off by
+// one ulp at most, beside the two roundings of the product.  Rows of 1e19 and more, whose squares
+// overflow, are summed again at 2^-72 of their size; eps is then far below the mean.  A NaN
+// makes the head NaN, an infinity its own dim (the others become 0).
+template <int D>
+__device__ __forceinline__ HeadNorm head_norm(const NormView& n, const float (&x)[8]) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) s += x[i] * x[i];
+    s = lanes_sum<kLanes<D>>(s);
+    float f = 1.0f, e = n.eps;
+    if (!(s <= 3.0e38f)) {
+        f = 0x1p-72f;
+        e = n.eps * 0x1p-72f * 0x1p-72f;
+        s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) s += x[i] * f * (x[i] * f);
+        s = lanes_sum<kLanes<D>>(s);
+    }
+    return {n, f, __builtin_amdgcn_rsqf(s * (1.0f / D) + e)};
+}
+
+// x: dims d0..d0+7 of the row at element offset `row`, after `norm`; rotated in place.  The
 // wide forms need the pairs of the eight dims to be eight dims or eight pairs
 // of floats in a row: rot / 2 (half) a multiple of 8, rot (interleaved) too.
+template <class N>
 __device__ __forceinline__ void rotate8(const KvRows& r, int64_t row, uint32_t token, uint32_t d0, const RopeView& rp,
-                                        float (&x)[8]) {
+                                        const N& norm, float (&x)[8]) {
     if (d0 >= rp.rot) return;
     const uint32_t h = rp.rot / 2;
     const int32_t pos = gptr<int32_t>(rp.positions)[token];
@@ -95,6 +181,7 @@ __device__ __forceinline__ void rotate8(const KvRows& r, int64_t row, uint32_t t
         const bool first = d0 < h;
         float y[8];
         load8(r, row + (first ? d0 + h : d0 - h), y);
+        norm.apply(first ? d0 + h : d0 - h, y);
         const f32x4* cs = reinterpret_cast<const f32x4*>(t + 2 * (first ? d0 : d0 - h));
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -127,8 +214,9 @@ __device__ __forceinline__ void rotate8(const KvRows& r, int64_t row, uint32_t t
             if (d >= rp.rot) continue;
             const uint32_t f = rp.half ? (d < h ? d : d - h) : d / 2;
             const bool first = rp.half ? d < h : d % 2 == 0;
-            const float y = load1(r, row + (rp.half ? (first ? d + h : d - h) : (d ^ 1u)));
-            const float c = gptr<float>(t)[2 * f], s = gptr<float>(t)[2 * f + 1], a = load1(r, row + d);
+            const uint32_t e = rp.half ? (first ? d + h : d - h) : (d ^ 1u);
+            const float y = norm.one(e, load1(r, row + e));
+            const float c = gptr<float>(t)[2 * f], s = gptr<float>(t)[2 * f + 1], a = x[i];
             x[i] = first ? a * c - y * s : y * s + a * c;
         }
     }
@@ -170,52 +258,71 @@ __device__ __forceinline__ void store4(const KvRows& r, int64_t at, const float 
     }
 }
 
-// One head of one token: loads, rotates, stores.  Halves of whole fours: a lane takes four
+// One head of one token: loads, takes its norm (NORM), rotates, stores.  Halves of whole fours: a lane takes four
 // pairs (with eight dims of one half it loads their partners as well and twice the cosines:
 // append over 4 x 2048 tokens 36.0 us instead of 30.7, one token 2.2 instead of 1.8).  Otherwise
 // in place is safe as well: a head's lanes are one wave's, which has loaded all of it before its
 // first store.
-template <int D>
+template <int D, bool NORM>
 __device__ __forceinline__ void rope_row(const KvRows& x, const KvRows& y, uint32_t token, uint32_t head, uint32_t lane,
-                                         const RopeView& rp) {
+                                         const RopeView& rp, const NormView& nv) {
     const uint32_t d0 = 8 * lane;
     const int64_t row = (int64_t)token * x.ts + (int64_t)head * x.hs;
-    if (rp.half && rp.rot % 8 == 0 && d0 < rp.rot) {
-        const int64_t to = (int64_t)token * y.ts + (int64_t)head * y.hs;
-        const uint32_t i0 = 4 * lane, i1 = i0 + rp.rot / 2;
-        const int32_t pos = gptr<int32_t>(rp.positions)[token];
-        float a[4], b[4], p[4], q[4];
+    const int64_t to = (int64_t)token * y.ts + (int64_t)head * y.hs;
+    const bool pairs = rp.half && rp.rot % 8 == 0 && d0 < rp.rot;
+    const uint32_t i0 = 4 * lane, i1 = i0 + rp.rot / 2;
+    float v[8] = {};  // eight dims, or four pairs: first all of the one side
+    if (pairs) {
+        float a[4], b[4];
         load4(x, row + i0, a);
         load4(x, row + i1, b);
-        const bool in = pos >= 0 && (uint32_t)pos < rp.table_positions;
-        f32x4 cs[2] = {};
-        if (in) {
-            const float* t = rp.table + (size_t)pos * rp.rot + 2 * i0;
-            cs[0] = *gptr<f32x4>(t);
-            cs[1] = *gptr<f32x4>(t + 4);
-        }
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const f32x4 w = cs[i];
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int e = 2 * i + j;
-                const float c = w[2 * j], s = w[2 * j + 1];
-                p[e] = in ? a[e] * c - b[e] * s : __builtin_nanf("");
-                q[e] = in ? a[e] * s + b[e] * c : __builtin_nanf("");
-            }
-        }
-        store4(y, to + i0, p);
-        store4(y, to + i1, q);
-        return;
-    }
-    float v[8];
-    if (d0 < D) {
+        for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+    } else if (d0 < D) {
         load8(x, row + d0, v);
-        rotate8(x, row, token, d0, rp, v);
     }
-    __builtin_amdgcn_wave_barrier();
-    if (d0 < D) store8(y, (int64_t)token * y.ts + (int64_t)head * y.hs + d0, v);
+    auto finish = [&](const auto& norm) {
+        if (pairs) {
+            const int32_t pos = gptr<int32_t>(rp.positions)[token];
+            float a[4], b[4], p[4], q[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) a[i] = v[i], b[i] = v[4 + i];
+            const bool in = pos >= 0 && (uint32_t)pos < rp.table_positions;
+            f32x4 cs[2] = {};
+            if (in) {
+                const float* t = rp.table + (size_t)pos * rp.rot + 2 * i0;
+                cs[0] = *gptr<f32x4>(t);
+                cs[1] = *gptr<f32x4>(t + 4);
+            }
+            norm.apply(i0, a);
+            norm.apply(i1, b);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const f32x4 w = cs[i];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int e = 2 * i + j;
+                    const float c = w[2 * j], s = w[2 * j + 1];
+                    p[e] = in ? a[e] * c - b[e] * s : __builtin_nanf("");
+                    q[e] = in ? a[e] * s + b[e] * c : __builtin_nanf("");
+                }
+            }
+            store4(y, to + i0, p);
+            store4(y, to + i1, q);
+            return;
+        }
+        if (d0 < D) {
+            norm.apply(d0, v);
+            rotate8(x, row, token, d0, rp, norm, v);
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (d0 < D) store8(y, to + d0, v);
+    };
+    if constexpr (NORM) {
+        finish(head_norm<D>(nv, v));
+    } else {
+        finish(NoNorm());
+    }
 }
 
 // 4099 tokens of 40 heads of 128 dims in f32: 28.9 us, 6.0 TB/s; one token 1.8 us.  (Four
@@ -225,7 +332,27 @@ __global__ __launch_bounds__(256) void rope_kernel(KvRows x, KvRows y, uint32_t 
     constexpr uint32_t L = kLanes<D>;
     const uint64_t i = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
     if (i >= (uint64_t)tokens * heads) return;
-    rope_row<D>(x, y, (uint32_t)(i / heads), (uint32_t)(i % heads), threadIdx.x % L, rp);
+    rope_row<D, false>(x, y, (uint32_t)(i / heads), (uint32_t)(i % heads), threadIdx.x % L, rp, NormView{});
+}
+
+// Queries in the first q_blocks workgroups, then keys.  A head is read once: its squares are
+// summed over its lanes, and the rotation takes the products from registers.
+template <int D>
+__global__ __launch_bounds__(256) void norm_rope_kernel(KvRows q, KvRows q_out, uint32_t q_heads, NormView q_norm, KvRows k,
+                                                        KvRows k_out, uint32_t k_heads, NormView k_norm, uint32_t tokens,
+                                                        uint32_t q_blocks, RopeView rp) {
+    constexpr uint32_t L = kLanes<D>;
+    const bool keys = blockIdx.x >= q_blocks;
+    const uint32_t heads = keys ? k_heads : q_heads;
+    const uint64_t i = (uint64_t)(blockIdx.x - (keys ? q_blocks : 0u)) * (256 / L) + threadIdx.x / L;
+    if (i >= (uint64_t)tokens * heads) return;
+    const uint32_t token = (uint32_t)(i / heads), head = (uint32_t)(i % heads), lane = threadIdx.x % L;
+    const KvRows x = keys ? k : q, y = keys ? k_out : q_out;
+    const NormView n = keys ? k_norm : q_norm;
+    if (n.on)
+        rope_row<D, true>(x, y, token, head, lane, rp, n);
+    else
+        rope_row<D, false>(x, y, token, head, lane, rp, n);
 }
 
 // Largest of the N lanes around this one (N a power of two, aligned), by moves
@@ -349,17 +476,22 @@ __device__ __forceinline__ void turn4(uint32_t (&x)[4]) {
 // head's values is one wave's alone, so values of 4 bits, two tokens to a byte, are
 // merged without atomics.  (Keys by four tokens a thread: 220 registers, the whole
 // launch over 4 x 2048 tokens, 146 MB in 30.7 us, 4.8 TB/s now, 86 us instead of 37 then.)
-template <int D, int KB, int VB>
-__global__ __launch_bounds__(256) void append_kernel(KvView kv, KvBatch b, KvRows k, KvRows v, RopeView rp, KvRows q,
-                                                     KvRows q_out, uint32_t q_heads, uint32_t chunks, uint32_t k_blocks,
-                                                     uint32_t v_blocks) {
+// NORM: keys and queries by their norms first.
+template <int D, int KB, int VB, bool NORM>
+__global__ __launch_bounds__(256) void append_kernel(KvView kv, KvBatch b, KvRows k, NormView k_norm, KvRows v, RopeView rp,
+                                                     KvRows q, NormView q_norm, KvRows q_out, uint32_t q_heads,
+                                                     uint32_t chunks, uint32_t k_blocks, uint32_t v_blocks) {
     constexpr uint32_t L = kLanes<D>, ROWS = 256 / L;
     const uint32_t lane = threadIdx.x % L, d0 = 8 * lane;
     uint32_t blk = blockIdx.x;
     if (blk >= k_blocks + v_blocks) {
         const uint64_t i = (uint64_t)(blk - k_blocks - v_blocks) * ROWS + threadIdx.x / L;
-        if (i < (uint64_t)b.tokens * q_heads)
-            rope_row<D>(q, q_out, (uint32_t)(i / q_heads), (uint32_t)(i % q_heads), lane, rp);
+        if (i >= (uint64_t)b.tokens * q_heads) return;
+        const uint32_t token = (uint32_t)(i / q_heads), head = (uint32_t)(i % q_heads);
+        if (NORM && q_norm.on)
+            rope_row<D, true>(q, q_out, token, head, lane, rp, q_norm);
+        else
+            rope_row<D, false>(q, q_out, token, head, lane, rp, q_norm);
         return;
     }
     Chunk c;
@@ -371,9 +503,15 @@ __global__ __launch_bounds__(256) void append_kernel(KvView kv, KvBatch b, KvRow
             const uint32_t token = c.row(t);
             const int64_t row = (int64_t)token * k.ts + (int64_t)c.h * k.hs;
             float x[8] = {};
-            if (d0 < D) {
-                load8(k, row + d0, x);
-                if (rp.table) rotate8(k, row, token, d0, rp, x);
+            if (d0 < D) load8(k, row + d0, x);
+            if (NORM && k_norm.on) {
+                const HeadNorm norm = head_norm<D>(k_norm, x);
+                if (d0 < D) {
+                    norm.apply(d0, x);
+                    if (rp.table) rotate8(k, row, token, d0, rp, norm, x);
+                }
+            } else if (d0 < D && rp.table) {
+                rotate8(k, row, token, d0, rp, NoNorm(), x);
             }
             int32_t code[8];
             const uint16_t sc = quantize<KB, 4>(x, code);
@@ -639,8 +777,25 @@ hipError_t rope_launch(const KvRows& x, const KvRows& y, uint32_t tokens, uint32
     });
 }
 
-hipError_t kv_append_launch(const KvView& kv, const KvBatch& b, const KvRows& k, const KvRows& v, const RopeView& rope,
-                            const KvRows& q, const KvRows& q_out, uint32_t q_heads, hipStream_t st) {
+hipError_t qk_norm_rope_launch(const KvRows& q, const KvRows& q_out, uint32_t q_heads, const NormView& q_norm,
+                               const KvRows& k, const KvRows& k_out, uint32_t k_heads, const NormView& k_norm,
+                               uint32_t tokens, uint32_t dim, const RopeView& rope, hipStream_t st) {
+    if (tokens == 0) return hipSuccess;
+    return by_dim(dim, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        constexpr uint64_t rows = 256 / kLanes<D>;
+        const uint64_t q_blocks = ((uint64_t)tokens * q_heads + rows - 1) / rows;
+        const uint64_t grid = q_blocks + ((uint64_t)tokens * k_heads + rows - 1) / rows;
+        if (!launchable(grid, 256)) return kTooManyThreads;
+        norm_rope_kernel<D><<<(uint32_t)grid, 256, 0, st>>>(q, q_out, q_heads, q_norm, k, k_out, k_heads, k_norm, tokens,
+                                                            (uint32_t)q_blocks, rope);
+        return hipGetLastError();
+    });
+}
+
+hipError_t kv_append_launch(const KvView& kv, const KvBatch& b, const KvRows& k, const NormView& k_norm, const KvRows& v,
+                            const RopeView& rope, const KvRows& q, const NormView& q_norm, const KvRows& q_out,
+                            uint32_t q_heads, hipStream_t st) {
     return by_cache(kv, [&](auto d, auto kb, auto vb) {
         constexpr int D = decltype(d)::value;
         constexpr uint64_t rows = 256 / kLanes<D>;
@@ -651,9 +806,12 @@ hipError_t kv_append_launch(const KvView& kv, const KvBatch& b, const KvRows& k,
         const uint64_t grid = k_blocks + v_blocks + ((uint64_t)b.tokens * q_heads + rows - 1) / rows;
         if (grid == 0) return hipSuccess;
         if (!launchable(grid, 256)) return kTooManyThreads;
-        append_kernel<D, decltype(kb)::value, decltype(vb)::value><<<(uint32_t)grid, 256, 0, st>>>(
-            kv, b, k, v, rope, q, q_out, q_heads, chunks, (uint32_t)k_blocks, (uint32_t)v_blocks);
-        return hipGetLastError();
+        auto go = [&](auto norm) {
+            append_kernel<D, decltype(kb)::value, decltype(vb)::value, decltype(norm)::value><<<(uint32_t)grid, 256, 0, st>>>(
+                kv, b, k, k_norm, v, rope, q, q_norm, q_out, q_heads, chunks, (uint32_t)k_blocks, (uint32_t)v_blocks);
+            return hipGetLastError();
+        };
+        return k_norm.on || q_norm.on ? go(std::true_type()) : go(std::false_type());
     });
 }
 

@@ -1,6 +1,6 @@
 // The quantized paged cache as kernels see it, and the launches of the cache,
 // rotary, attention and verification kernels (kvcache.hip, attention*.hip,
-// verify.hip).  The byte layout is stated in include/dyninfer_mi355x.h.
+// verify.hip, prompt.hip, logprobs.hip).  The byte layout is stated in include/dyninfer_mi355x.h.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -41,6 +41,15 @@ struct RopeView {
     uint32_t table_positions, rot, half;  // half: layout (i, i + rot / 2), else interleaved
 };
 
+// The norm of a head before its rotation: x / sqrt(mean(x^2) + eps) * (weight + offset).
+struct NormView {
+    const void* weight;  // [dim], or NULL: ones
+    float eps, offset;
+    uint32_t bf16;       // the weight's type
+    uint32_t vec;        // 1: the weight starts at a 16-byte boundary
+    uint32_t on;         // 0: no norm
+};
+
 // A sequence's rows in the call and its committed length.
 struct SeqRange {
     uint32_t row0, n;
@@ -79,9 +88,14 @@ hipError_t rope_table_launch(uint32_t rot, uint32_t scaling, double theta, doubl
                              double hi, double attn, uint32_t positions, float* out, hipStream_t st);
 hipError_t rope_launch(const KvRows& x, const KvRows& y, uint32_t tokens, uint32_t heads, uint32_t dim,
                        const RopeView& rope, hipStream_t st);
+// Norm, then rotation of the rows of q and of k; k_heads 0: no keys; rope.table NULL: no rotation.
+hipError_t qk_norm_rope_launch(const KvRows& q, const KvRows& q_out, uint32_t q_heads, const NormView& q_norm,
+                               const KvRows& k, const KvRows& k_out, uint32_t k_heads, const NormView& k_norm,
+                               uint32_t tokens, uint32_t dim, const RopeView& rope, hipStream_t st);
 // rope.table NULL: no rotation; q_heads 0: no queries.
-hipError_t kv_append_launch(const KvView& kv, const KvBatch& b, const KvRows& k, const KvRows& v, const RopeView& rope,
-                            const KvRows& q, const KvRows& q_out, uint32_t q_heads, hipStream_t st);
+hipError_t kv_append_launch(const KvView& kv, const KvBatch& b, const KvRows& k, const NormView& k_norm, const KvRows& v,
+                            const RopeView& rope, const KvRows& q, const NormView& q_norm, const KvRows& q_out,
+                            uint32_t q_heads, hipStream_t st);
 // k.p / v.p NULL: not read.
 hipError_t kv_read_launch(const KvView& kv, const KvBatch& b, const KvRows& k, const KvRows& v, hipStream_t st);
 hipError_t kv_commit_launch(const KvView& kv, const KvBatch& b, const int32_t* path, uint32_t path_stride,
@@ -127,6 +141,29 @@ struct VerifyArgs {
     int32_t* counts;
     int64_t* next;
 };
+// Log probabilities (logprobs.hip).
+constexpr uint32_t kMostTop = 64;  // alternatives of a row
+struct LogprobArgs {
+    const void* logits;
+    int64_t stride;
+    const int64_t* tokens;
+    const float* temperature;
+    float* stats;              // [row][piece][4]
+    unsigned long long* keys;  // [row][piece][top]
+    float* logprobs;
+    int32_t* ranks;
+    float* entropy;
+    int64_t* top_tokens;
+    float* top_logprobs;
+    uint32_t bf16, rows, vocab, top;
+};
+struct LogprobPlan {
+    uint32_t pieces;          // of a row
+    uint64_t keys_at, bytes;  // workspace
+};
+LogprobPlan logprob_plan(uint32_t rows, uint32_t vocab, uint32_t top, bool bf16);
+hipError_t logprob_launch(LogprobArgs a, const LogprobPlan& plan, uint8_t* work, hipStream_t st);
+
 uint64_t verify_workspace_bytes(uint32_t seqs, uint32_t tokens, uint32_t vocab);
 hipError_t verify_launch(const VerifyArgs& a, uint8_t* work, hipStream_t st);
 

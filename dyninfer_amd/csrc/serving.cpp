@@ -1,9 +1,10 @@
 // C ABI of the calls around attention (include/dyninfer_mi355x.h): rotary
-// positions, the quantized paged cache, attention of drafted tokens over it,
-// and their verification.  Checks here keep every kernel inside the buffers
+// positions and norms of heads, the quantized paged cache, attention of drafted
+// tokens over it and of prompts, verification of drafts, and log probabilities.  Checks here keep every kernel inside the buffers
 // described; what the host cannot see (device tables) the kernels check.
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <utility>
 
 #include "capi_common.hpp"
@@ -121,6 +122,22 @@ int check_rope(const dyninfer_rope_t* r, uint32_t dim, uint32_t tokens, dmx::Rop
     return 0;
 }
 
+int check_norm(const dyninfer_head_norm_t* n, const char* what, dmx::NormView& out) {
+    out = {};
+    if (!n) return 0;
+    const std::string w(what);
+    if (n->weight) {
+        if (n->dtype != DYNINFER_DTYPE_F32 && n->dtype != DYNINFER_DTYPE_BF16)
+            return fail(UNSUPPORTED, w + ": weight must be f32 or bf16");
+        if (!aligned(n->weight, n->dtype == DYNINFER_DTYPE_BF16 ? 2 : 4)) return fail(BAD, w + ": weight is misaligned");
+    }
+    if (!(n->eps >= std::numeric_limits<float>::min()) || !std::isfinite(n->eps))
+        return fail(BAD, w + ": eps must be a normal number above 0");
+    if (!std::isfinite(n->offset)) return fail(BAD, w + ": offset must be finite");
+    out = {n->weight, n->eps, n->offset, n->dtype == DYNINFER_DTYPE_BF16, aligned(n->weight, 16), 1};
+    return 0;
+}
+
 int same_place(const dyninfer_rows_t* a, const dyninfer_rows_t* b) {
     return a->data == b->data && a->token_stride == b->token_stride && a->head_stride == b->head_stride;
 }
@@ -162,6 +179,12 @@ int check_workspace(const void* p, uint64_t bytes, uint64_t need, const char* wh
                              (p ? std::to_string(bytes) + " bytes" : std::string("NULL")) + ")");
     if (!aligned(p, 256)) return fail(BAD, std::string("the workspace of ") + what + " must be 256-byte aligned");
     return 0;
+}
+
+// Rows that are written while others are read.
+int check_clear(const dyninfer_rows_t* out, const dyninfer_rows_t* in, uint32_t tokens, uint32_t dim, const char* what) {
+    if (!meet(out, in, tokens, dim) || interleaved(out, in, dim)) return 0;
+    return fail(BAD, what);
 }
 
 int launched(hipError_t e) {
@@ -235,20 +258,62 @@ int dyninfer_mi355x_kv_cache_bytes(const dyninfer_kvcache_t* cache, uint64_t* k_
     return DYNINFER_MI355X_OK;
 }
 
-int dyninfer_mi355x_kv_append(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache_t* cache,
-                              const dyninfer_kvbatch_t* batch, const dyninfer_rows_t* k, const dyninfer_rows_t* v,
-                              const dyninfer_rope_t* rope, const dyninfer_rows_t* q, const dyninfer_rows_t* q_out,
-                              void* stream) {
+int dyninfer_mi355x_qk_norm_rope(dyninfer_mi355x_ctx_t* ctx, const dyninfer_rows_t* q, const dyninfer_head_norm_t* q_norm,
+                                 const dyninfer_rows_t* q_out, const dyninfer_rows_t* k,
+                                 const dyninfer_head_norm_t* k_norm, const dyninfer_rows_t* k_out, uint32_t tokens,
+                                 uint32_t head_dim, const dyninfer_rope_t* rope, void* stream) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (int rc = check_dim(head_dim)) return rc;
+    if (tokens > 0x7FFFFFFFu) return fail(BAD, "more than 2^31 - 1 tokens");
+    if (!k != !k_out) return fail(BAD, "k and k_out go together");
+    if (k_norm && !k) return fail(BAD, "a norm of keys is given but no keys");
+    if (!rope && (!q_norm || (k && !k_norm))) return fail(BAD, "rows have neither a norm nor a rope");
+    dmx::RopeView rp = {};
+    if (rope)
+        if (int rc = check_rope(rope, head_dim, tokens, rp)) return rc;
+    dmx::NormView qn, kn;
+    if (int rc = check_norm(q_norm, "q_norm", qn)) return rc;
+    if (int rc = check_norm(k_norm, "k_norm", kn)) return rc;
+    if (tokens == 0) return DYNINFER_MI355X_OK;
+    dmx::KvRows qr, qo, kr = {}, ko = {};
+    if (int rc = check_rows(q, "q", qr)) return rc;
+    if (int rc = check_out(q_out, head_dim, tokens, "q_out", qo)) return rc;
+    if (q->dtype != q_out->dtype || q->heads != q_out->heads) return fail(BAD, "q and q_out must share dtype and heads");
+    if (int rc = check_apart(q, q_out, tokens, head_dim, "q_out")) return rc;
+    if (k) {
+        if (int rc = check_rows(k, "k", kr)) return rc;
+        if (int rc = check_out(k_out, head_dim, tokens, "k_out", ko)) return rc;
+        if (k->dtype != k_out->dtype || k->heads != k_out->heads) return fail(BAD, "k and k_out must share dtype and heads");
+        if (int rc = check_apart(k, k_out, tokens, head_dim, "k_out")) return rc;
+        if (int rc = check_clear(q_out, k, tokens, head_dim, "q_out overlaps k")) return rc;
+        if (int rc = check_clear(k_out, q, tokens, head_dim, "k_out overlaps q")) return rc;
+        if (int rc = check_clear(q_out, k_out, tokens, head_dim, "q_out overlaps k_out")) return rc;
+    }
+    DeviceGuard g(ctx->device);
+    if (g.err != hipSuccess) return hip_fail(g.err, "hipSetDevice");
+    return launched(dmx::qk_norm_rope_launch(qr, qo, q->heads, qn, kr, ko, k ? k->heads : 0, kn, tokens, head_dim, rp,
+                                             static_cast<hipStream_t>(stream)));
+}
+
+int dyninfer_mi355x_kv_append_normed(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache_t* cache,
+                                     const dyninfer_kvbatch_t* batch, const dyninfer_rows_t* k,
+                                     const dyninfer_head_norm_t* k_norm, const dyninfer_rows_t* v,
+                                     const dyninfer_rope_t* rope, const dyninfer_rows_t* q,
+                                     const dyninfer_head_norm_t* q_norm, const dyninfer_rows_t* q_out, void* stream) {
     if (int rc = check_ctx(ctx)) return rc;
     dmx::KvView kv;
     dmx::KvBatch b;
     if (int rc = check_cache(cache, kv)) return rc;
     if (int rc = check_batch(batch, true, b)) return rc;
-    if ((q || q_out) && !rope) return fail(BAD, "queries are given but no rope to rotate them by");
+    if ((q || q_out) && !rope && !q_norm) return fail(BAD, "queries are given but no rope to rotate them by");
     if (!q != !q_out) return fail(BAD, "q and q_out go together");
+    if (q_norm && !q) return fail(BAD, "a norm of queries is given but no queries");
     dmx::RopeView rp = {};
     if (rope)
         if (int rc = check_rope(rope, kv.dim, b.tokens, rp)) return rc;
+    dmx::NormView qn, kn;
+    if (int rc = check_norm(q_norm, "q_norm", qn)) return rc;
+    if (int rc = check_norm(k_norm, "k_norm", kn)) return rc;
     if (b.tokens == 0 || b.seqs == 0) return DYNINFER_MI355X_OK;
     dmx::KvRows kr, vr, qr = {}, qo = {};
     if (int rc = check_rows(k, "k", kr)) return rc;
@@ -261,13 +326,19 @@ int dyninfer_mi355x_kv_append(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache
         if (q->dtype != q_out->dtype || q->heads != q_out->heads) return fail(BAD, "q and q_out must share dtype and heads");
         if (int rc = check_apart(q, q_out, b.tokens, kv.dim, "q_out")) return rc;
         // its rows are written while k and v are read
-        if ((meet(q_out, k, b.tokens, kv.dim) && !interleaved(q_out, k, kv.dim)) ||
-            (meet(q_out, v, b.tokens, kv.dim) && !interleaved(q_out, v, kv.dim)))
-            return fail(BAD, "q_out overlaps k or v");
+        if (int rc = check_clear(q_out, k, b.tokens, kv.dim, "q_out overlaps k or v")) return rc;
+        if (int rc = check_clear(q_out, v, b.tokens, kv.dim, "q_out overlaps k or v")) return rc;
     }
     DeviceGuard g(ctx->device);
     if (g.err != hipSuccess) return hip_fail(g.err, "hipSetDevice");
-    return launched(dmx::kv_append_launch(kv, b, kr, vr, rp, qr, qo, q ? q->heads : 0, static_cast<hipStream_t>(stream)));
+    return launched(dmx::kv_append_launch(kv, b, kr, kn, vr, rp, qr, qn, qo, q ? q->heads : 0, static_cast<hipStream_t>(stream)));
+}
+
+int dyninfer_mi355x_kv_append(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache_t* cache,
+                              const dyninfer_kvbatch_t* batch, const dyninfer_rows_t* k, const dyninfer_rows_t* v,
+                              const dyninfer_rope_t* rope, const dyninfer_rows_t* q, const dyninfer_rows_t* q_out,
+                              void* stream) {
+    return dyninfer_mi355x_kv_append_normed(ctx, cache, batch, k, nullptr, v, rope, q, nullptr, q_out, stream);
 }
 
 int dyninfer_mi355x_kv_read(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache_t* cache,
@@ -420,6 +491,56 @@ int dyninfer_mi355x_draft_verify(dyninfer_mi355x_ctx_t* ctx, const dyninfer_veri
     DeviceGuard g(ctx->device);
     if (g.err != hipSuccess) return hip_fail(g.err, "hipSetDevice");
     return launched(dmx::verify_launch(a, static_cast<uint8_t*>(workspace), static_cast<hipStream_t>(stream)));
+}
+
+int dyninfer_mi355x_token_logprobs_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t top, uint32_t dtype,
+                                                   uint64_t* out_bytes) {
+    if (!out_bytes) return fail(BAD, "out_bytes is NULL");
+    *out_bytes = 0;
+    if (vocab == 0 || vocab > 0x7FFFFFFFu) return fail(BAD, "vocab must be 1..2^31 - 1");
+    if (top > dmx::kMostTop) return fail(UNSUPPORTED, "more than " + std::to_string(dmx::kMostTop) + " alternatives");
+    if (dtype != DYNINFER_DTYPE_F32 && dtype != DYNINFER_DTYPE_BF16) return fail(UNSUPPORTED, "logits must be f32 or bf16");
+    *out_bytes = dmx::logprob_plan(rows, vocab, top, dtype == DYNINFER_DTYPE_BF16).bytes;
+    return DYNINFER_MI355X_OK;
+}
+
+int dyninfer_mi355x_token_logprobs(dyninfer_mi355x_ctx_t* ctx, const dyninfer_logprobs_t* p, void* workspace,
+                                   uint64_t workspace_bytes, void* stream) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (!p) return fail(BAD, "arguments are NULL");
+    if (p->vocab == 0 || p->vocab > 0x7FFFFFFFu) return fail(BAD, "vocab must be 1..2^31 - 1");
+    if (p->top > dmx::kMostTop) return fail(UNSUPPORTED, "more than " + std::to_string(dmx::kMostTop) + " alternatives");
+    if (p->logits_dtype != DYNINFER_DTYPE_F32 && p->logits_dtype != DYNINFER_DTYPE_BF16)
+        return fail(UNSUPPORTED, "logits must be f32 or bf16");
+    if ((p->logprobs || p->ranks) && !p->tokens) return fail(BAD, "logprobs or ranks are asked for but no tokens are given");
+    if (p->rows == 0) return DYNINFER_MI355X_OK;
+    if (!p->logits || !aligned(p->logits, p->logits_dtype == DYNINFER_DTYPE_BF16 ? 2 : 4))
+        return fail(BAD, "logits are NULL or misaligned");
+    if (p->rows > 1 && p->logits_stride < (int64_t)p->vocab) return fail(BAD, "rows of logits overlap");
+    if (!aligned(p->tokens, 8) || !aligned(p->temperature, 4)) return fail(BAD, "tokens or temperature are misaligned");
+    if (!aligned(p->logprobs, 4) || !aligned(p->ranks, 4) || !aligned(p->entropy, 4)) return fail(BAD, "an output is misaligned");
+    if (p->top && (!p->top_tokens || !aligned(p->top_tokens, 8) || !p->top_logprobs || !aligned(p->top_logprobs, 4)))
+        return fail(BAD, "top_tokens or top_logprobs are NULL or misaligned");
+    const bool bf16 = p->logits_dtype == DYNINFER_DTYPE_BF16;
+    const dmx::LogprobPlan plan = dmx::logprob_plan(p->rows, p->vocab, p->top, bf16);
+    if (int rc = check_workspace(workspace, workspace_bytes, plan.bytes, "token_logprobs")) return rc;
+    dmx::LogprobArgs a = {};
+    a.logits = p->logits;
+    a.stride = p->rows > 1 ? p->logits_stride : 0;
+    a.tokens = p->tokens;
+    a.temperature = p->temperature;
+    a.logprobs = p->logprobs;
+    a.ranks = p->ranks;
+    a.entropy = p->entropy;
+    a.top_tokens = p->top_tokens;
+    a.top_logprobs = p->top_logprobs;
+    a.bf16 = bf16;
+    a.rows = p->rows;
+    a.vocab = p->vocab;
+    a.top = p->top;
+    DeviceGuard g(ctx->device);
+    if (g.err != hipSuccess) return hip_fail(g.err, "hipSetDevice");
+    return launched(dmx::logprob_launch(a, plan, static_cast<uint8_t*>(workspace), static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

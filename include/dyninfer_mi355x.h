@@ -375,6 +375,29 @@ typedef struct dyninfer_rope {
 int dyninfer_mi355x_rope(dyninfer_mi355x_ctx_t* ctx, const dyninfer_rows_t* x, const dyninfer_rows_t* y,
                          uint32_t tokens, uint32_t head_dim, const dyninfer_rope_t* rope, void* stream);
 
+/* The norm of a head: x / sqrt(mean(x^2) + eps) * (weight + offset) over its head_dim values. */
+typedef struct dyninfer_head_norm {
+    const void* weight; /* [head_dim], device; NULL: ones */
+    uint32_t dtype;     /* of weight: f32 or bf16 */
+    float eps;          /* a normal number above 0 */
+    float offset;       /* 1 where weights are kept as differences from one, else 0 */
+    uint32_t reserved;
+} dyninfer_head_norm_t;
+
+/*
+ * q_out = the heads of q [tokens, heads, head_dim] by their norm, then rotated as
+ * dyninfer_mi355x_rope does, in one pass, and k_out of k by k_norm in the same launch.  In f32
+ * between the two, rounded once to q_out's type (that of q).  Either norm may be NULL (that tensor
+ * is rotated only), rope too (norms only), but not both for a tensor that is given; k, k_norm and
+ * k_out may be NULL together.  q_out may be q itself, k_out k itself (same pointer and strides), but outputs must not
+ * overlap inputs or each other otherwise.  Heads of any finite magnitude; a NaN makes its head NaN,
+ * an infinity its own value and what it is rotated with (the rest becomes 0).
+ */
+int dyninfer_mi355x_qk_norm_rope(dyninfer_mi355x_ctx_t* ctx, const dyninfer_rows_t* q, const dyninfer_head_norm_t* q_norm,
+                                 const dyninfer_rows_t* q_out, const dyninfer_rows_t* k,
+                                 const dyninfer_head_norm_t* k_norm, const dyninfer_rows_t* k_out, uint32_t tokens,
+                                 uint32_t head_dim, const dyninfer_rope_t* rope, void* stream);
+
 /* Bytes of a cache's k and v buffers (from its encodings, heads, head_dim, page_size and pages). */
 int dyninfer_mi355x_kv_cache_bytes(const dyninfer_kvcache_t* cache, uint64_t* k_bytes, uint64_t* v_bytes);
 
@@ -389,6 +412,14 @@ int dyninfer_mi355x_kv_append(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache
                               const dyninfer_kvbatch_t* batch, const dyninfer_rows_t* k, const dyninfer_rows_t* v,
                               const dyninfer_rope_t* rope, const dyninfer_rows_t* q, const dyninfer_rows_t* q_out,
                               void* stream);
+
+/* The same with norms before the rotation, in that launch: keys by k_norm, queries by q_norm
+ * (either NULL: none), as dyninfer_mi355x_qk_norm_rope does; q needs q_norm or rope. */
+int dyninfer_mi355x_kv_append_normed(dyninfer_mi355x_ctx_t* ctx, const dyninfer_kvcache_t* cache,
+                                     const dyninfer_kvbatch_t* batch, const dyninfer_rows_t* k,
+                                     const dyninfer_head_norm_t* k_norm, const dyninfer_rows_t* v,
+                                     const dyninfer_rope_t* rope, const dyninfer_rows_t* q,
+                                     const dyninfer_head_norm_t* q_norm, const dyninfer_rows_t* q_out, void* stream);
 
 /* Reads the batch's rows back: k and v [tokens, kv_heads, head_dim], f32 (code * scale, exact) or
  * bf16 (rounded once).  Either may be NULL. */
@@ -470,6 +501,36 @@ int dyninfer_mi355x_draft_verify(dyninfer_mi355x_ctx_t* ctx, const dyninfer_veri
                                  uint64_t workspace_bytes, void* stream);
 int dyninfer_mi355x_draft_verify_workspace_bytes(uint32_t sequences, uint32_t tokens, uint32_t vocab, uint32_t max_new,
                                                  uint64_t* out_bytes);
+
+/*
+ * Of logits [rows, vocab], p = softmax(logits / temperature): logprobs[r] = ln p of tokens[r], ranks[r]
+ * = how many tokens come before it in the order of logits (0: the likeliest; ties: the lower token
+ * first), entropy[r] = -sum p ln p in nats, and the `top` likeliest tokens in that order with their
+ * logarithms.  temperature[r] <= 0: p is 1 at the largest logit.  Temperatures from 1.5e-36 to 1e36 are
+ * resolved, those beyond count as the nearest; a NaN gives NaN.  A NaN logit counts as -inf, +inf as the
+ * largest f32.  A token outside the vocabulary (a padded batch's) has logarithm -inf and rank -1.
+ * Alternatives are tokens of logits above -inf; where there are fewer, the rest are token -1 with
+ * -inf.  A row of -inf only: logarithms -inf, entropy 0.  Sums are f32.
+ */
+typedef struct dyninfer_logprobs {
+    const void* logits; /* f32 or bf16, rows logits_stride elements apart */
+    int64_t logits_stride;
+    const int64_t* tokens;    /* [rows]; NULL: none (then neither logprobs nor ranks) */
+    const float* temperature; /* [rows]; NULL: all 1 */
+    uint32_t logits_dtype, rows, vocab;
+    uint32_t top;        /* 0..64 */
+    float* logprobs;     /* out [rows]; these three may each be NULL */
+    int32_t* ranks;      /* out [rows] */
+    float* entropy;      /* out [rows] */
+    int64_t* top_tokens; /* out [rows, top]; top 0: may be NULL, as the next */
+    float* top_logprobs; /* out [rows, top] */
+} dyninfer_logprobs_t;
+
+/* workspace: of dyninfer_mi355x_token_logprobs_workspace_bytes, 256-byte aligned. */
+int dyninfer_mi355x_token_logprobs(dyninfer_mi355x_ctx_t* ctx, const dyninfer_logprobs_t* args, void* workspace,
+                                   uint64_t workspace_bytes, void* stream);
+int dyninfer_mi355x_token_logprobs_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t top, uint32_t dtype,
+                                                   uint64_t* out_bytes);
 
 /*
  * GGUF container index: the exact byte range of every tensor of a GGUF file, so a
