@@ -70,6 +70,7 @@ EXPORTED_SYMBOLS = (
     "dyninfer_mi355x_kv_read", "dyninfer_mi355x_kv_commit", "dyninfer_mi355x_tree_attention",
     "dyninfer_mi355x_tree_attention_workspace_bytes", "dyninfer_mi355x_draft_verify",
     "dyninfer_mi355x_draft_verify_workspace_bytes", "dyninfer_mi355x_qk_norm_rope", "dyninfer_mi355x_kv_append_normed",
+    "dyninfer_mi355x_prompt_attention", "dyninfer_mi355x_prompt_attention_workspace_bytes",
     "dyninfer_mi355x_token_logprobs", "dyninfer_mi355x_token_logprobs_workspace_bytes",
 )
 
@@ -99,6 +100,7 @@ _pack_kvcache = struct.Struct("@6I5Q").pack
 _pack_kvbatch = struct.Struct("@3Q4IQ").pack
 _pack_rows = struct.Struct("@Q2I2q").pack
 _pack_rope = struct.Struct("@2Q4I").pack
+_pack_prompts = struct.Struct("@2Q6I").pack
 _pack_head_norm = struct.Struct("@QI2fI").pack
 _pack_rope_params = struct.Struct("@2I8d").pack
 _pack_logprobs = struct.Struct("@Qq2Q4I5Q").pack
@@ -174,6 +176,8 @@ def library() -> ctypes.CDLL:
         "dyninfer_mi355x_kv_commit": (I, [P, P, P, P, U32, P, P]),
         "dyninfer_mi355x_tree_attention": (I, [P, P, P, P, P, U32, ctypes.c_float, P, P, P, ctypes.c_uint64, P]),
         "dyninfer_mi355x_tree_attention_workspace_bytes": (I, [P, P, U32, U32, ctypes.POINTER(ctypes.c_uint64)]),
+        "dyninfer_mi355x_prompt_attention": (I, [P, P, P, P, P, U32, ctypes.c_float, P, P, P, ctypes.c_uint64, P]),
+        "dyninfer_mi355x_prompt_attention_workspace_bytes": (I, [P, U32, U32, U32, U32, ctypes.POINTER(ctypes.c_uint64)]),
         "dyninfer_mi355x_token_logprobs": (I, [P, P, P, ctypes.c_uint64, P]),
         "dyninfer_mi355x_token_logprobs_workspace_bytes": (I, [U32, U32, U32, U32, ctypes.POINTER(ctypes.c_uint64)]),
         "dyninfer_mi355x_draft_verify": (I, [P, P, P, ctypes.c_uint64, P]),
@@ -469,6 +473,31 @@ class Rope:
 
 
 @dataclass
+class PromptBatch:
+    """Prompts packed one after the other (dyninfer_prompts_t): rows starts[b] .. starts[b+1] - 1 of
+    the queries, int32 [sequences + 1] on the device; ``key_starts`` the same of the keys where
+    sequences have more keys than rows (None: as many).  ``max_new`` the most rows of a sequence,
+    ``max_keys`` the most keys (without ``key_starts`` those are max_new)."""
+    starts: object
+    max_new: int
+    key_starts: object = None
+    max_keys: int = 0
+
+    def pack(self, tokens: int, keys: int) -> bytes:
+        """The C struct's bytes."""
+        starts, key_starts = self.starts, self.key_starts
+        n = starts.shape[0] - 1 if starts.dim() == 1 else -1
+        if n < 0:
+            _bad("starts must have an element more than there are sequences")
+        try:
+            return _pack_prompts(_table(starts, _T_I32, (n + 1,), "starts"),
+                                 0 if key_starts is None else _table(key_starts, _T_I32, (n + 1,), "key_starts"), n,
+                                 tokens, self.max_new, keys, self.max_new if key_starts is None else self.max_keys, 0)
+        except struct.error as e:
+            _bad(f"batch: {e}")
+
+
+@dataclass
 class HeadNorm:
     """The norm of a head (dyninfer_head_norm_t): x / sqrt(mean(x^2) + eps) * (weight + offset).
     ``weight``: device tensor [head_dim], f32 or bf16, or None (ones)."""
@@ -753,6 +782,38 @@ class Context:
         need = ctypes.c_uint64(0)
         _check(self._lib.dyninfer_mi355x_tree_attention_workspace_bytes(cache.pack(), batch.pack(), q_heads, dtype,
                                                                         ctypes.byref(need)))
+        return need.value
+
+    def prompt_attention(self, q, k, v, batch: PromptBatch, scale: Optional[float] = None, out=None, lse=None, stream=None,
+                         workspace=None):
+        """Causal attention of q [tokens, heads, head_dim] over k, v [keys, kv_heads, head_dim] of the
+        same prompts (dyninfer_mi355x_prompt_attention).  ``scale``: head_dim ** -0.5 unless given.
+        ``lse``: f32 [tokens, heads] to write the log-sum-exp to."""
+        if out is None:
+            out = self._like(q, stream)
+        n, heads, dim = q.shape if q.dim() == 3 else (0, 0, 0)
+        m, kv_heads = (k.shape[0], k.shape[1]) if k.dim() == 3 else (0, 0)
+        qr, kr, vr = _rows(q, n, dim, "q"), _rows(k, m, dim, "k"), _rows(v, m, dim, "v")
+        bb = batch.pack(n, m)
+        lp = None if lse is None else _table(lse, _T_F32, (n, heads), "lse")
+        if workspace is None:
+            need = ctypes.c_uint64(0)
+            _check(self._lib.dyninfer_mi355x_prompt_attention_workspace_bytes(bb, heads, kv_heads, dim, _dtype_code(q),
+                                                                              ctypes.byref(need)))
+            wp, wn, _keep = self._work(need.value, None, q.device, stream)
+        else:
+            wp, wn = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        _check(self._lib.dyninfer_mi355x_prompt_attention(
+            self._h, bb, qr, kr, vr, dim, dim ** -0.5 if scale is None else scale, _rows(out, n, dim, "out"), lp, wp, wn,
+            self._on(stream)))
+        return out
+
+    def prompt_attention_workspace_bytes(self, batch: PromptBatch, tokens: int, keys: int, q_heads: int, kv_heads: int,
+                                         head_dim: int, dtype: int = DTYPE_F32) -> int:
+        """Device workspace bytes of a prompt_attention call (dyninfer_mi355x_prompt_attention_workspace_bytes)."""
+        need = ctypes.c_uint64(0)
+        _check(self._lib.dyninfer_mi355x_prompt_attention_workspace_bytes(batch.pack(tokens, keys), q_heads, kv_heads, head_dim,
+                                                                          dtype, ctypes.byref(need)))
         return need.value
 
     def draft_verify(self, logits, draft_tokens, parents, starts, max_new: int, *, uniform, noise, draft_probs=None,

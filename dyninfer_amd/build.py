@@ -23,7 +23,7 @@ SOURCES = [
     "gemm_q6_k.hip", "gemm_q5_k.hip", "gemm_iq4_xs.hip", "gemm_q4_k.hip", "gemm_q8_0.hip", "gemm_mlx_u4.hip",
     "gemm_q4_0.hip", "gemm_q4_1.hip",
     "attention_k8v8.hip", "attention_k8v4.hip", "attention_k4v8.hip", "attention_k4v4.hip", "attention.hip",
-    "kvcache.hip", "verify.hip", "logprobs.hip",
+    "prompt_bf16.hip", "prompt_f32.hip", "prompt.hip", "kvcache.hip", "verify.hip", "logprobs.hip",
     "gemv.hip", "gemv_mfma.hip", "gemm.hip", "xprep.hip", "dequant.hip", "embedding.hip",
     "capi.cpp", "serving.cpp", "registry.cpp", "gguf.cpp", "safetensors.cpp",
 ]

@@ -141,6 +141,28 @@ struct VerifyArgs {
     int32_t* counts;
     int64_t* next;
 };
+// Attention of prompts (prompt.hip): rows and keys of sequences packed one after the other.
+struct PromptPlan {
+    uint32_t waves;      // of a workgroup, 32 rows each
+    uint32_t row_tiles;  // of the sequence with the most rows
+    uint32_t parts;      // into which the keys of a row tile are split
+    uint64_t grid;
+    uint64_t bytes, stats;  // workspace, and where the parts' statistics begin in it
+};
+PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint32_t heads, uint32_t group, uint32_t dim,
+                       bool f32);
+struct PromptArgs {
+    KvRows q, k, v, out;
+    const int32_t* q_starts;
+    const int32_t* k_starts;
+    float* lse;
+    float* part_o;  // [row tile][sequence][kv head][part][row][dim], not yet over their sums
+    float* stats;   // [..][row][2]: what exponents are from, sum
+    uint32_t seqs, tokens, keys, max_new, heads, group, dim, row_tiles, parts;
+    float scale;
+};
+hipError_t prompt_launch(PromptArgs a, const PromptPlan& plan, uint8_t* work, hipStream_t st);
+
 // Log probabilities (logprobs.hip).
 constexpr uint32_t kMostTop = 64;  // alternatives of a row
 struct LogprobArgs {

@@ -143,14 +143,17 @@ int same_place(const dyninfer_rows_t* a, const dyninfer_rows_t* b) {
 }
 
 // First and last byte of rows, and whether two sets of rows may meet.
-bool meet(const dyninfer_rows_t* a, const dyninfer_rows_t* b, uint32_t tokens, uint32_t dim) {
-    if (!tokens) return false;
-    auto span = [&](const dyninfer_rows_t* r) {
+bool meet(const dyninfer_rows_t* a, uint32_t a_tokens, const dyninfer_rows_t* b, uint32_t b_tokens, uint32_t dim) {
+    if (!a_tokens || !b_tokens) return false;
+    auto span = [&](const dyninfer_rows_t* r, uint32_t tokens) {
         const uint64_t e = r->dtype == DYNINFER_DTYPE_BF16 ? 2 : 4;
         return e * ((uint64_t)(tokens - 1) * (uint64_t)r->token_stride + (uint64_t)(r->heads - 1) * (uint64_t)r->head_stride + dim);
     };
     const uintptr_t x = (uintptr_t)a->data, y = (uintptr_t)b->data;
-    return x < y + span(b) && y < x + span(a);
+    return x < y + span(b, b_tokens) && y < x + span(a, a_tokens);
+}
+bool meet(const dyninfer_rows_t* a, const dyninfer_rows_t* b, uint32_t tokens, uint32_t dim) {
+    return meet(a, tokens, b, tokens, dim);
 }
 
 // Whether the elements of two sets of rows lie apart although their spans meet:
@@ -181,10 +184,38 @@ int check_workspace(const void* p, uint64_t bytes, uint64_t need, const char* wh
     return 0;
 }
 
+bool clear_of(const dyninfer_rows_t* out, uint32_t out_tokens, const dyninfer_rows_t* in, uint32_t in_tokens, uint32_t dim) {
+    return !meet(out, out_tokens, in, in_tokens, dim) || interleaved(out, in, dim);
+}
+
 // Rows that are written while others are read.
 int check_clear(const dyninfer_rows_t* out, const dyninfer_rows_t* in, uint32_t tokens, uint32_t dim, const char* what) {
-    if (!meet(out, in, tokens, dim) || interleaved(out, in, dim)) return 0;
-    return fail(BAD, what);
+    return clear_of(out, tokens, in, tokens, dim) ? 0 : fail(BAD, what);
+}
+
+// `tables`: the device tables are needed (not for a size query).
+int check_prompts(const dyninfer_prompts_t* b, bool tables) {
+    if (!b) return fail(BAD, "batch is NULL");
+    if (tables && b->sequences && (!b->starts || !aligned(b->starts, 4) || !aligned(b->key_starts, 4)))
+        return fail(BAD, "batch: starts are NULL or misaligned");
+    if (b->tokens > 0x7FFFFFFFu || b->max_new > b->tokens)
+        return fail(BAD, "batch: max_new must not be above tokens, nor tokens above 2^31 - 1");
+    if (b->keys > 0x7FFFFFFFu || b->max_keys > b->keys)
+        return fail(BAD, "batch: max_keys must not be above keys, nor keys above 2^31 - 1");
+    if (!b->key_starts && b->keys != b->tokens) return fail(BAD, "batch: without key_starts there are as many keys as tokens");
+    if (b->sequences > (1u << 24)) return fail(UNSUPPORTED, "batch: more than 2^24 sequences; split the call");
+    return 0;
+}
+
+int check_groups(const dyninfer_prompts_t* b, uint32_t q_heads, uint32_t kv_heads) {
+    if (q_heads == 0 || kv_heads == 0 || q_heads % kv_heads) return fail(BAD, "query heads must be a multiple of the kv heads");
+    if (q_heads > 65535) return fail(UNSUPPORTED, "more than 65535 query heads");
+    if ((uint64_t)b->max_new * (q_heads / kv_heads) > 0x7FFFFFFFull) return fail(UNSUPPORTED, "too many rows of one kv head");
+    return 0;
+}
+
+dmx::PromptPlan plan_prompts(const dyninfer_prompts_t* b, uint32_t q_heads, uint32_t kv_heads, uint32_t dim, uint32_t dtype) {
+    return dmx::prompt_plan(b->sequences, b->max_new, b->max_keys, kv_heads, q_heads / kv_heads, dim, dtype == DYNINFER_DTYPE_F32);
 }
 
 int launched(hipError_t e) {
@@ -491,6 +522,62 @@ int dyninfer_mi355x_draft_verify(dyninfer_mi355x_ctx_t* ctx, const dyninfer_veri
     DeviceGuard g(ctx->device);
     if (g.err != hipSuccess) return hip_fail(g.err, "hipSetDevice");
     return launched(dmx::verify_launch(a, static_cast<uint8_t*>(workspace), static_cast<hipStream_t>(stream)));
+}
+
+int dyninfer_mi355x_prompt_attention_workspace_bytes(const dyninfer_prompts_t* batch, uint32_t q_heads, uint32_t kv_heads,
+                                                     uint32_t head_dim, uint32_t dtype, uint64_t* out_bytes) {
+    if (!out_bytes) return fail(BAD, "out_bytes is NULL");
+    *out_bytes = 0;
+    if (int rc = check_prompts(batch, false)) return rc;
+    if (int rc = check_dim(head_dim)) return rc;
+    if (dtype != DYNINFER_DTYPE_F32 && dtype != DYNINFER_DTYPE_BF16) return fail(UNSUPPORTED, "q must be f32 or bf16");
+    if (int rc = check_groups(batch, q_heads, kv_heads)) return rc;
+    *out_bytes = plan_prompts(batch, q_heads, kv_heads, head_dim, dtype).bytes;
+    return DYNINFER_MI355X_OK;
+}
+
+int dyninfer_mi355x_prompt_attention(dyninfer_mi355x_ctx_t* ctx, const dyninfer_prompts_t* batch, const dyninfer_rows_t* q,
+                                     const dyninfer_rows_t* k, const dyninfer_rows_t* v, uint32_t head_dim, float scale,
+                                     const dyninfer_rows_t* out, float* lse, void* workspace, uint64_t workspace_bytes,
+                                     void* stream) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (int rc = check_prompts(batch, true)) return rc;
+    if (int rc = check_dim(head_dim)) return rc;
+    if (!std::isfinite(scale)) return fail(BAD, "scale must be finite");
+    if (lse && !aligned(lse, 4)) return fail(BAD, "lse must be 4-byte aligned");
+    if (batch->tokens == 0 || batch->sequences == 0 || batch->max_new == 0) return DYNINFER_MI355X_OK;
+    dmx::PromptArgs a = {};
+    if (int rc = check_rows(q, "q", a.q)) return rc;
+    if (int rc = check_out(out, head_dim, batch->tokens, "out", a.out)) return rc;
+    if (q->dtype != out->dtype || q->heads != out->heads) return fail(BAD, "q and out must share dtype and heads");
+    if (int rc = check_clear(out, q, batch->tokens, head_dim, "out overlaps q")) return rc;
+    uint32_t kv_heads = 1;
+    if (batch->keys) {
+        if (int rc = check_rows(k, "k", a.k)) return rc;
+        if (int rc = check_rows(v, "v", a.v)) return rc;
+        if (k->heads != v->heads) return fail(BAD, "k and v must share their heads");
+        if (k->dtype != q->dtype || v->dtype != q->dtype) return fail(BAD, "q, k and v must share a dtype");
+        kv_heads = k->heads;
+        if (!clear_of(out, batch->tokens, k, batch->keys, head_dim) || !clear_of(out, batch->tokens, v, batch->keys, head_dim))
+            return fail(BAD, "out overlaps k or v");
+    }
+    if (int rc = check_groups(batch, q->heads, kv_heads)) return rc;
+    const dmx::PromptPlan plan = plan_prompts(batch, q->heads, kv_heads, head_dim, q->dtype);
+    if (int rc = check_workspace(workspace, workspace_bytes, plan.bytes, "prompt_attention")) return rc;
+    a.q_starts = batch->starts;
+    a.k_starts = batch->key_starts ? batch->key_starts : batch->starts;
+    a.lse = lse;
+    a.seqs = batch->sequences;
+    a.tokens = batch->tokens;
+    a.keys = batch->keys;
+    a.max_new = batch->max_new;
+    a.heads = kv_heads;
+    a.group = q->heads / kv_heads;
+    a.dim = head_dim;
+    a.scale = scale;
+    DeviceGuard g(ctx->device);
+    if (g.err != hipSuccess) return hip_fail(g.err, "hipSetDevice");
+    return launched(dmx::prompt_launch(a, plan, static_cast<uint8_t*>(workspace), static_cast<hipStream_t>(stream)));
 }
 
 int dyninfer_mi355x_token_logprobs_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t top, uint32_t dtype,

@@ -464,6 +464,43 @@ int dyninfer_mi355x_tree_attention_workspace_bytes(const dyninfer_kvcache_t* cac
                                                    uint32_t q_heads, uint32_t dtype, uint64_t* out_bytes);
 
 /*
+ * Prompts packed one after the other: rows starts[b] .. starts[b+1] - 1 of q are sequence b's,
+ * rows key_starts[b] .. of k and v its keys and values (key_starts NULL: starts).  A sequence has as
+ * many keys as rows, or more: its rows are then the last ones (a piece of a prompt whose first
+ * part was read before).  Device int32, 4-byte aligned.  max_new: the most rows of any sequence (rows
+ * past it are left out); max_keys: the most keys, which only shapes the launches (any number is handled).
+ */
+typedef struct dyninfer_prompts {
+    const int32_t* starts;     /* [sequences + 1] */
+    const int32_t* key_starts; /* [sequences + 1] or NULL */
+    uint32_t sequences;
+    uint32_t tokens, max_new; /* rows of q and out */
+    uint32_t keys, max_keys;  /* rows of k and v; without key_starts as many as tokens */
+    uint32_t reserved;
+} dyninfer_prompts_t;
+
+/*
+ * out[r, h] = sum_j softmax_j(scale * q[r, h] . k[j, h / group]) v[j, h / group] over the keys j <= i +
+ * (keys of the sequence - its rows) of row i = r - starts[b]: causal attention on the activations
+ * themselves, without a cache.  All of one dtype (f32 or bf16); group = heads of q / heads of k, any whole number;
+ * head_dim 64, 96, 128 or 256.  A row that sees nothing (fewer keys than rows) gives 0 and lse -inf.  Rows of
+ * out behind the last sequence are left as they were.  lse: f32 [tokens, heads], the natural logarithm of the sum
+ * of exponentials, or NULL.  What is masked has no influence, whatever it holds.
+ * Rounding: scores and outputs are sums in f32 (f32: of exact products); exponentials are f32, in
+ * bf16 rounded once before the product with v.  Scores up to 2^30 in magnitude are resolved.
+ * workspace: device memory of dyninfer_mi355x_prompt_attention_workspace_bytes, 256-byte aligned (NULL when that is 0),
+ * under the rules of dyninfer_mi355x_qlinear's.
+ */
+int dyninfer_mi355x_prompt_attention(dyninfer_mi355x_ctx_t* ctx, const dyninfer_prompts_t* batch, const dyninfer_rows_t* q,
+                                     const dyninfer_rows_t* k, const dyninfer_rows_t* v, uint32_t head_dim, float scale,
+                                     const dyninfer_rows_t* out, float* lse, void* workspace, uint64_t workspace_bytes,
+                                     void* stream);
+
+/* Host-only; reads the batch's numbers, no device memory. */
+int dyninfer_mi355x_prompt_attention_workspace_bytes(const dyninfer_prompts_t* batch, uint32_t q_heads, uint32_t kv_heads,
+                                                     uint32_t head_dim, uint32_t dtype, uint64_t* out_bytes);
+
+/*
  * Checks drafted tokens against the target model's logits.  Rows as in dyninfer_kvbatch_t: rows
  * starts[b].. are the nodes of sequence b's tree, node 0 its root (the last token known), every
  * other node a drafted token with a parent of smaller index.  Of the current node (first the
