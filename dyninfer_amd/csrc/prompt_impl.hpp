@@ -31,6 +31,26 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kNone = -__builtin_inff();
 
+// A number that is the same in every lane, as a scalar.
+__device__ __forceinline__ uint32_t scalar(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+__device__ __forceinline__ uint64_t scalar64(uint64_t x) {
+    return (uint64_t)scalar((uint32_t)(x >> 32)) << 32 | scalar((uint32_t)x);
+}
+
+// 16 bytes a lane from base + off (base wave-uniform) to LDS offset `to` + 16 lane.  In assembly, because
+// the compiler, which cannot tell one stage of the tiles from the other, puts a wait for
+// all copies in flight before every read of LDS behind the builtin; ring_barrier waits for these.
+// No register is loaded, and the compiler's own counts of what is in flight only become stricter.
+// Five wait states lie between a vector instruction that writes the address's scalars (v_readfirstlane)
+// and the copy, one between m0 and the copy.
+__device__ __forceinline__ void copy16(uint64_t base, uint32_t off, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base)
+                 : "memory");
+}
+__device__ __forceinline__ void copy16(const uint8_t* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+}
+
 // A sequence's rows and keys in the call.
 struct PromptRange {
     uint32_t row0, n;   // rows that the call takes
@@ -39,7 +59,7 @@ struct PromptRange {
 };
 
 __device__ __forceinline__ PromptRange prompt_range(const PromptArgs& a, uint32_t s) {
-    auto clip = [](int32_t x, uint32_t top) { return x < 0 ? 0u : min((uint32_t)x, top); };
+    auto clip = [](int32_t x, uint32_t top) { return scalar(x < 0 ? 0u : min((uint32_t)x, top)); };
     const uint32_t r0 = clip(a.q_starts[s], a.tokens), r1 = clip(a.q_starts[s + 1], a.tokens);
     const uint32_t k0 = clip(a.k_starts[s], a.keys), k1 = clip(a.k_starts[s + 1], a.keys);
     PromptRange r;
@@ -53,8 +73,9 @@ __device__ __forceinline__ PromptRange prompt_range(const PromptArgs& a, uint32_
 }
 
 // How a tile of KT keys (or values) lies in LDS: rows of RS units of 16 bytes (a power of two),
-// unit c of row k at c ^ (k & 7), so that the eight lanes of a read that begin at one dim
-// of consecutive keys, or the rows that a turned read takes together, are on different banks.
+// unit c of row k at c ^ mix(k).  LDS has 64 banks, 256 bytes: sixteen lanes that read one unit of
+// consecutive keys, and the rows that one read of the values takes together (bf16: 64 bytes of four
+// keys; f32: 128 bytes of two, four keys apart), are on different ones.
 template <int D, bool F32>
 struct TileShape {
     static constexpr uint32_t E = F32 ? 4 : 2, CH = D * E / 16;  // bytes of an element, units of a row
@@ -62,6 +83,11 @@ struct TileShape {
     static constexpr uint32_t RSB = RS * 16;
     static constexpr uint32_t KT = RS <= 16 ? 64 : 32;
     static constexpr uint32_t BYTES = KT * RSB;  // of K or of V
+    // Linear in the bits of k: mix(a ^ b) = mix(a) ^ mix(b).
+    static constexpr __device__ uint32_t mix(uint32_t k) {
+        if (F32) return (k >> 2 & 1u) << 3 | (k >> 3 & 1u) << 2 | (k & 3u);
+        return RS == 8 ? (k >> 1 & 1u) << 2 | (k >> 2 & 3u) : (k & 3u) << 2 | (k >> 2 & 3u);
+    }
 };
 
 template <int D, bool F32, int WAVES>
@@ -75,20 +101,25 @@ struct PromptWave {
     float m, l;        // what exponents are from (in powers of two; kNone: nothing seen yet), sum of this lane's
     float c;           // scale in powers of two
     int64_t pos;       // the last key that this lane's row sees, -1: none
-    uint32_t k_at[4], v_at[F32 ? 4 : 2];  // this lane's places in a tile
+    static constexpr uint32_t KA = T::RS == 8 ? 4 : 8, VA = F32 ? 4 : T::RS == 8 ? 2 : 4;
+    uint32_t k_at[KA], v_at[F32 ? 1 : 2][VA];  // this lane's places in a tile
 
     __device__ __forceinline__ void places(uint32_t lane) {
         const uint32_t col = lane & 31u, g = lane >> 5;
 #pragma unroll
-        for (uint32_t s = 0; s < 4; s++) k_at[s] = col * T::RSB + (((2 * s + g) ^ (col & 7u)) << 4);
+        for (uint32_t t = 0; t < KA; t++) k_at[t] = col * T::RSB + (((2 * t + g) ^ T::mix(col)) << 4);
         if constexpr (F32) {
 #pragma unroll
-            for (uint32_t b = 0; b < 4; b++) v_at[b] = (4 * g + b) * T::RSB + (((col / 4) ^ (4 * g + b)) << 4) + 4 * (col & 3u);
+            for (uint32_t b = 0; b < 4; b++) v_at[0][b] = (4 * g + b) * T::RSB + (((col / 4) ^ T::mix(4 * g + b)) << 4) + 4 * (col & 3u);
         } else {
-            const uint32_t i = lane & 15u, row = 4 * g + i / 4, half = (lane >> 4) & 1u;
+            const uint32_t i = lane & 15u, half = (lane >> 4) & 1u;
 #pragma unroll
-            for (uint32_t p = 0; p < 2; p++)
-                v_at[p] = row * T::RSB + (((4 * p + 2 * half + (i & 3u) / 2) ^ row) << 4) + 8 * (i & 1u);
+            for (uint32_t e = 0; e < 2; e++)
+#pragma unroll
+                for (uint32_t p = 0; p < VA; p++) {
+                    const uint32_t row = 8 * e + 4 * g + i / 4;
+                    v_at[e][p] = row * T::RSB + (((4 * p + 2 * half + (i & 3u) / 2) ^ T::mix(row)) << 4) + 8 * (i & 1u);
+                }
         }
     }
 
@@ -102,7 +133,7 @@ struct PromptWave {
         f32x16 s = {};
 #pragma unroll
         for (uint32_t t = 0; t < QN; t++) {
-            const Frag k = *reinterpret_cast<const Frag*>(kt + k_at[t & 3u] + (sub * 32 * T::RSB + (t >> 2) * 128));
+            const Frag k = *reinterpret_cast<const Frag*>(kt + k_at[t % KA] + (sub * 32 * T::RSB + t / KA * KA * 32));
             if constexpr (F32) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], q[t][j], s, 0, 0, 0);
@@ -120,13 +151,14 @@ struct PromptWave {
 #pragma unroll
         for (uint32_t e = 0; e < 2; e++)
             x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds4*)(vt + v_at[dt & 1u] + ((16 * s + 8 * e) * T::RSB + (dt >> 1) * 128)));
+                (lds4*)(vt + v_at[e][dt % VA] + (16 * s * T::RSB + dt / VA * VA * 64)));
         const u32x2 a = __builtin_bit_cast(u32x2, x[0]), b = __builtin_bit_cast(u32x2, x[1]);
         return __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
     }
     // (f32): one dim of the value of key number i of 32.
     __device__ __forceinline__ float value(const uint8_t* vt, uint32_t sub, uint32_t i, uint32_t dt) const {
-        return *reinterpret_cast<const float*>(vt + v_at[i & 3u] + ((32 * sub + 8 * (i >> 2)) * T::RSB + dt * 128));
+        const uint32_t at = v_at[0][i & 3u] ^ ((i >> 2 & 1u) << 6 | (dt & 1u) << 7);  // mix of key 8 (i / 4), and an odd dt
+        return *reinterpret_cast<const float*>(vt + at + ((32 * sub + 8 * (i >> 2)) * T::RSB + (dt >> 1) * 256));
     }
 
     // P V added to the output.  bf16: the exponentials are rounded to 8 bits of mantissa, an error of the
@@ -162,6 +194,7 @@ struct PromptWave {
 #pragma unroll
         for (uint32_t sub = 0; sub < SUB; sub++) p[sub] = scores(kt, sub);
         if (masked) {
+            asm volatile("");  // a branch, not a selection in every step
 #pragma unroll
             for (uint32_t sub = 0; sub < SUB; sub++) {
                 const int32_t sees = seen_of(k0, sub, lane);
@@ -338,39 +371,42 @@ __global__ __launch_bounds__(64 * WAVES, (TileShape<D, F32>::RS <= 16 ? 2 : 1)) 
     }
 
     // Copies tile t into a stage: unit blk * 64 + lane of K and of V, blk = wave + WAVES j, its key
-    // key0 + STEP j with the bits of STEP j beside those of key0 % 8.  Whole tiles go
+    // key0 + STEP j, where key0 < STEP, a power of two.  Whole tiles go
     // straight from memory, addresses a uniform one and 32 bits of the lane's; keys behind the end are the last one.
     constexpr uint32_t STEP = WAVES * PER;
     const uint8_t* const kb = static_cast<const uint8_t*>(a.k.p) + ((int64_t)r.key0 * a.k.ts + (int64_t)head * a.k.hs) * T::E;
     const uint8_t* const vb = static_cast<const uint8_t*>(a.v.p) + ((int64_t)r.key0 * a.v.ts + (int64_t)head * a.v.hs) * T::E;
-    const uint32_t key0 = wave * PER + lane / T::RS, chunk0 = (lane % T::RS) ^ (key0 & 7u);
+    const uint32_t key0 = wave * PER + lane / T::RS, chunk0 = (lane % T::RS) ^ T::mix(key0);
     const bool vec = a.k.vec && a.v.vec, near = vec && max(a.k.ts, a.v.ts) * (int64_t)T::E < (1 << 26);
     const uint32_t k_row = key0 * (uint32_t)a.k.ts * T::E, v_row = key0 * (uint32_t)a.v.ts * T::E;  // if near
+    uint64_t k_step = (uint32_t)a.k.ts * T::E * STEP, v_step = (uint32_t)a.v.ts * T::E * STEP;
+    uint64_t k_base = scalar64((uint64_t)(uintptr_t)kb), v_base = scalar64((uint64_t)(uintptr_t)vb);
+    asm volatile("" : "+s"(k_step), "+s"(v_step), "+s"(k_base), "+s"(v_base));  // kept as scalars
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
     auto copy = [&](uint32_t t, uint32_t stage) {
-        uint8_t* const to = lds + stage * STAGE + wave * 1024;
+        const uint32_t to = lds0 + stage * STAGE + wave * 1024;
         const uint32_t k0 = t * T::KT;
         if (near && (uint64_t)k0 + T::KT <= r.nk) {
-            const uint8_t* const ks = kb + (int64_t)k0 * a.k.ts * T::E;
-            const uint8_t* const vs = vb + (int64_t)k0 * a.v.ts * T::E;
+            uint64_t ks = k_base + t * (k_step * COPIES), vs = v_base + t * (v_step * COPIES);
 #pragma unroll
-            for (uint32_t j = 0; j < COPIES; j++) {
-                const uint32_t chunk = chunk0 ^ (STEP * j & 7u);
+            for (uint32_t j = 0; j < COPIES; j++, ks += k_step, vs += v_step) {
+                const uint32_t chunk = chunk0 ^ T::mix(STEP * j);
                 if (T::CH < T::RS && chunk >= T::CH) continue;
-                dma16(ks + (int64_t)(STEP * j) * a.k.ts * T::E + (k_row + 16 * chunk), to + WAVES * j * 1024);
-                dma16(vs + (int64_t)(STEP * j) * a.v.ts * T::E + (v_row + 16 * chunk), to + T::BYTES + WAVES * j * 1024);
+                copy16(ks, k_row + 16 * chunk, to + WAVES * j * 1024);
+                copy16(vs, v_row + 16 * chunk, to + T::BYTES + WAVES * j * 1024);
             }
             return;
         }
 #pragma unroll 1
         for (uint32_t j = 0; j < COPIES; j++) {
-            const uint32_t chunk = chunk0 ^ (STEP * j & 7u);
+            const uint32_t chunk = chunk0 ^ T::mix(STEP * j);
             const int64_t at = (int64_t)min((uint64_t)k0 + key0 + STEP * j, (uint64_t)r.nk - 1);
             const uint8_t* const from[2] = {kb + at * a.k.ts * T::E + 16 * chunk, vb + at * a.v.ts * T::E + 16 * chunk};
             if (T::CH < T::RS && chunk >= T::CH) continue;
 #pragma unroll
             for (uint32_t i = 0; i < 2; i++) {
                 if (vec) {
-                    dma16(from[i], to + i * T::BYTES + WAVES * j * 1024);
+                    copy16(from[i], to + i * T::BYTES + WAVES * j * 1024);
                     continue;
                 }
                 u32x4 x;
@@ -381,7 +417,7 @@ __global__ __launch_bounds__(64 * WAVES, (TileShape<D, F32>::RS <= 16 ? 2 : 1)) 
                     else
                         x[e] = gptr<uint16_t>(from[i])[2 * e] | (uint32_t)gptr<uint16_t>(from[i])[2 * e + 1] << 16;
                 }
-                *reinterpret_cast<u32x4*>(to + i * T::BYTES + WAVES * j * 1024 + 16 * lane) = x;
+                *reinterpret_cast<u32x4*>(lds + stage * STAGE + i * T::BYTES + (wave + WAVES * j) * 1024 + 16 * lane) = x;
             }
         }
     };
