@@ -9,49 +9,91 @@ namespace dmx {
 
 namespace {
 
-// A wave per (row, query head): its parts brought to the common maximum.
+// Lanes of a row: four dims each, a power of two of them.
 template <int D>
-__global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t rows_of_tile) {
-    constexpr int W = D <= 128 ? 2 : 4;  // dims of a lane
-    typedef float vec __attribute__((ext_vector_type(W)));
-    const uint32_t lane = threadIdx.x & 63u, q_heads = a.heads * a.group;
-    const uint64_t id = (uint64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+constexpr uint32_t kJoinLanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;
+
+// A row (token, query head) by kJoinLanes<D> * groups threads: each group brings every groups-th
+// part to its own maximum, then the groups are joined in LDS.  Bound by latency where rows are
+// few: one token of 32 heads after 16000, 62 parts, by one group took 34 us.
+template <int D>
+__global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t rows_of_tile, uint32_t groups) {
+    constexpr uint32_t L = kJoinLanes<D>;
+    typedef float vec __attribute__((ext_vector_type(4)));
+    __shared__ vec sm_o[256];
+    __shared__ float sm_m[256 / L], sm_l[256 / L];
+    const uint32_t q_heads = a.heads * a.group, lane = threadIdx.x % L, group = threadIdx.x / L % groups;
+    const uint64_t id = (uint64_t)blockIdx.x * (256 / L / groups) + threadIdx.x / L / groups;
     const uint64_t per = (uint64_t)a.max_new * q_heads;
-    if (id >= per * a.seqs) return;
-    const uint32_t seq = (uint32_t)(id / per), i = (uint32_t)(id % per / q_heads), h = (uint32_t)(id % q_heads);
+    const uint32_t seq = (uint32_t)min(id / per, (uint64_t)a.seqs - 1), i = (uint32_t)(id % per / q_heads), h = (uint32_t)(id % q_heads);
     auto clip = [&](int32_t x) { return x < 0 ? 0u : min((uint32_t)x, a.tokens); };
     const uint32_t r0 = clip(a.q_starts[seq]), r1 = clip(a.q_starts[seq + 1]);
-    if (r1 <= r0 || i >= r1 - r0) return;
-    const uint32_t head = h / a.group;
-    const uint64_t row = (uint64_t)i * a.group + (h - head * a.group);
-    const uint64_t unit = (row / rows_of_tile * a.seqs + seq) * a.heads + head;
-    const uint64_t at = unit * a.parts * rows_of_tile + row % rows_of_tile;  // of part 0; parts are rows_of_tile apart
-    const uint32_t d0 = W * lane, from = d0 < D ? d0 : 0;
-    float top = -__builtin_inff();
-    for (uint32_t p = 0; p < a.parts; p++) top = fmaxf(top, gptr<float>(a.stats)[2 * (at + (uint64_t)p * rows_of_tile)]);
-    const float ref = top == -__builtin_inff() ? 0.0f : top;
-    float sum = 0.0f;
+    const bool live = id < per * a.seqs && r1 > r0 && i < r1 - r0;
+    const uint32_t head = h / a.group, d0 = 4 * lane, from = d0 < D ? d0 : 0;
+    float m = -__builtin_inff(), l = 0.0f;
     vec o = {};
-    for (uint32_t p = 0; p < a.parts; p++) {
-        const uint64_t slot = at + (uint64_t)p * rows_of_tile;
-        const float pm = gptr<float>(a.stats)[2 * slot];
-        if (pm == -__builtin_inff()) continue;  // saw nothing
-        const float f = __builtin_amdgcn_exp2f(pm - ref);
-        sum += gptr<float>(a.stats)[2 * slot + 1] * f;
-        o += *gptr<vec>(a.part_o + slot * D + from) * f;
+    if (live) {
+        const uint64_t row = (uint64_t)i * a.group + (h - head * a.group);
+        const uint64_t unit = (row / rows_of_tile * a.seqs + seq) * a.heads + head;
+        const uint64_t at = unit * a.parts * rows_of_tile + row % rows_of_tile;  // of part 0; parts are rows_of_tile apart
+        for (uint32_t p0 = group; p0 < a.parts; p0 += 4 * groups) {  // four loads in flight
+            float pm[4], pl[4];
+            vec po[4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) {
+                const uint32_t p = p0 + k * groups;
+                const uint64_t slot = at + (uint64_t)min(p, a.parts - 1) * rows_of_tile;
+                pm[k] = p < a.parts ? gptr<float>(a.stats)[2 * slot] : -__builtin_inff();
+                pl[k] = gptr<float>(a.stats)[2 * slot + 1];
+                po[k] = *gptr<vec>(a.part_o + slot * D + from);
+            }
+            const float now = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m);
+            if (now == -__builtin_inff()) continue;  // saw nothing
+            const float f = __builtin_amdgcn_exp2f(m - now);
+            l *= f;
+            o *= f;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) {
+                if (pm[k] == -__builtin_inff()) continue;
+                const float g = __builtin_amdgcn_exp2f(pm[k] - now);
+                l += pl[k] * g;
+                o += po[k] * g;
+            }
+            m = now;
+        }
     }
-    const bool none = top == -__builtin_inff();
+    if (groups > 1) {
+        sm_o[threadIdx.x] = o;
+        if (lane == 0) sm_m[threadIdx.x / L] = m, sm_l[threadIdx.x / L] = l;
+        __syncthreads();
+        if (group != 0) return;
+        const uint32_t t0 = threadIdx.x / L;
+        float top = m, sum = 0.0f;
+        for (uint32_t g = 1; g < groups; g++) top = fmaxf(top, sm_m[t0 + g]);
+        o = vec{};
+        for (uint32_t g = 0; g < groups; g++) {
+            if (sm_m[t0 + g] == -__builtin_inff()) continue;
+            const float f = __builtin_amdgcn_exp2f(sm_m[t0 + g] - top);
+            sum += sm_l[t0 + g] * f;
+            o += sm_o[threadIdx.x + g * L] * f;
+        }
+        m = top;
+        l = sum;
+    }
+    if (!live) return;
+    const bool none = m == -__builtin_inff();
     if (a.lse && lane == 0)
-        gptr_mut<float>(a.lse)[(r0 + (uint64_t)i) * q_heads + h] = none ? top : (top + log2f(sum)) * 0.69314718055994531f;
+        gptr_mut<float>(a.lse)[(r0 + (uint64_t)i) * q_heads + h] = none ? m : (m + log2f(l)) * 0.69314718055994531f;
     if (d0 >= D) return;
-    const float inv = none ? 0.0f : 1.0f / sum;
+    const float inv = none ? 0.0f : 1.0f / l;
     const int64_t e = (int64_t)(r0 + (uint64_t)i) * a.out.ts + (int64_t)h * a.out.hs + d0;
 #pragma unroll
-    for (int j = 0; j < W; j++) {
+    for (int j = 0; j < 4; j++) {
+        const float y = none ? 0.0f : o[j] * inv;
         if (a.out.bf16)
-            gptr_mut<uint16_t>(a.out.p)[e + j] = f32_to_bf16_bits(o[j] * inv);
+            gptr_mut<uint16_t>(a.out.p)[e + j] = f32_to_bf16_bits(y);
         else
-            gptr_mut<float>(a.out.p)[e + j] = o[j] * inv;
+            gptr_mut<float>(a.out.p)[e + j] = y;
     }
 }
 
@@ -90,9 +132,14 @@ hipError_t prompt_launch(PromptArgs a, const PromptPlan& plan, uint8_t* work, hi
     a.stats = reinterpret_cast<float*>(work + plan.stats);
     const hipError_t e = a.q.bf16 ? prompt_launch_typed<false>(a, plan, st) : prompt_launch_typed<true>(a, plan, st);
     if (e != hipSuccess || plan.parts == 1) return e;
-    const uint64_t waves = (uint64_t)a.seqs * a.max_new * a.heads * a.group;
+    const uint64_t rows = (uint64_t)a.seqs * a.max_new * a.heads * a.group;
     auto join = [&](auto d) {
-        prompt_join_kernel<decltype(d)::value><<<(uint32_t)((waves + 3) / 4), 256, 0, st>>>(a, 32 * plan.waves);
+        constexpr int D = decltype(d)::value;
+        uint32_t groups = 1;  // about four parts each
+        while (groups < 256 / kJoinLanes<D> && 4 * groups < plan.parts) groups *= 2;
+        const uint64_t per = 256 / kJoinLanes<D> / groups, grid = (rows + per - 1) / per;
+        if (!launchable(grid, 256)) return kTooManyThreads;
+        prompt_join_kernel<D><<<(uint32_t)grid, 256, 0, st>>>(a, 32 * plan.waves, groups);
         return hipGetLastError();
     };
     switch (a.dim) {
