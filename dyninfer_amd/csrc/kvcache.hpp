@@ -182,6 +182,7 @@ struct LogprobArgs {
 };
 struct LogprobPlan {
     uint32_t pieces;          // of a row
+    bool small;               // a row is one wave's
     uint64_t keys_at, bytes;  // workspace
 };
 LogprobPlan logprob_plan(uint32_t rows, uint32_t vocab, uint32_t top, bool bf16);
