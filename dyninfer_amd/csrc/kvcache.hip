@@ -355,6 +355,86 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(KvRows q, KvRows q_out, 
         rope_row<D, false>(x, y, token, head, lane, rp, n);
 }
 
+// The same where every row and weight begins at 16 bytes and rot is whole eights (or none): a lane takes two
+// groups of four dims, four pairs of halves or eight in a row, and the eight floats of the table that
+// belong to them are at 8 lane in both layouts.  Bound by memory: two bytes of traffic for each byte of a row
+// and about forty operations for eight elements.  All loads are issued before the first is used, and the
+// types are the kernel's: 8191 tokens of 40 heads of 128 dims in bf16 take 37 us (172 MB, 4.7 TB/s; a copy
+// reaches 5.1), and 49 us through the general form, whose loads wait for each other's branches.
+template <int D, bool BF16, bool WBF16>
+__global__ __launch_bounds__(256) void norm_rope_wide_kernel(KvRows q, KvRows q_out, uint32_t q_heads, NormView q_norm, KvRows k,
+                                                             KvRows k_out, uint32_t k_heads, NormView k_norm, uint32_t tokens,
+                                                             uint32_t q_blocks, RopeView rp) {
+    constexpr uint32_t L = kLanes<D>;
+    const bool keys = blockIdx.x >= q_blocks;
+    const uint32_t heads = keys ? k_heads : q_heads, lane = threadIdx.x % L, d0 = 8 * lane;
+    const uint32_t i = (blockIdx.x - (keys ? q_blocks : 0u)) * (256 / L) + threadIdx.x / L;  // below 2^32: of a launch's threads
+    const uint32_t token = i / heads, head = i - token * heads;
+    if (token >= tokens) return;
+    const KvRows x = keys ? k : q, y = keys ? k_out : q_out;
+    const NormView n = keys ? k_norm : q_norm;
+    const int32_t pos = rp.rot ? gptr<int32_t>(rp.positions)[token] : 0;
+    const bool turned = d0 < rp.rot, pairs = turned && rp.half;
+    const uint32_t i0 = pairs ? 4 * lane : d0 < D ? d0 : 0u, i1 = pairs ? 4 * lane + rp.rot / 2 : i0 + 4;
+    const int64_t from = (int64_t)token * x.ts + (int64_t)head * x.hs, to = (int64_t)token * y.ts + (int64_t)head * y.hs;
+    typedef std::conditional_t<BF16, u32x2, f32x4> X;
+    typedef std::conditional_t<WBF16, u32x2, f32x4> WT;
+    constexpr uint32_t E = BF16 ? 2 : 4, WE = WBF16 ? 2 : 4;
+    const X xa = *gptr<X>(static_cast<const char*>(x.p) + (from + i0) * E), xb = *gptr<X>(static_cast<const char*>(x.p) + (from + i1) * E);
+    const WT wa = *gptr<WT>(static_cast<const char*>(n.weight) + i0 * WE), wb = *gptr<WT>(static_cast<const char*>(n.weight) + i1 * WE);
+    const bool in = pos >= 0 && (uint32_t)pos < rp.table_positions;
+    f32x4 c0 = {}, c1 = {};
+    if (turned && in) {
+        const float* t = rp.table + (size_t)pos * rp.rot + 8 * lane;
+        c0 = *gptr<f32x4>(t);
+        c1 = *gptr<f32x4>(t + 4);
+    }
+    auto four = [](auto v, float (&f)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if constexpr (sizeof(v) == 8)
+                f[j] = __uint_as_float(j & 1 ? v[j / 2] & 0xFFFF0000u : v[j / 2] << 16);
+            else
+                f[j] = v[j];
+        }
+    };
+    float a[4], b[4], u[4], v[4];
+    four(xa, a), four(xb, b), four(wa, u), four(wb, v);
+    float all[8];
+#pragma unroll
+    for (int j = 0; j < 4; j++) all[j] = d0 < D ? a[j] : 0.0f, all[4 + j] = d0 < D ? b[j] : 0.0f;
+    const HeadNorm norm = head_norm<D>(n, all);
+#pragma unroll
+    for (int j = 0; j < 4; j++) a[j] = a[j] * norm.f * norm.r * (u[j] + n.offset), b[j] = b[j] * norm.f * norm.r * (v[j] + n.offset);
+    if (turned) {
+        float p[4], r[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            // halves: pair j is (a[j], b[j]); otherwise pairs 0, 1 are a's and 2, 3 b's
+            const float c = j < 2 ? c0[2 * j] : c1[2 * j - 4], s = j < 2 ? c0[2 * j + 1] : c1[2 * j - 3];
+            const float g = rp.half ? a[j] : j < 2 ? a[2 * j] : b[2 * j - 4], h = rp.half ? b[j] : j < 2 ? a[2 * j + 1] : b[2 * j - 3];
+            p[j] = in ? g * c - h * s : __builtin_nanf("");
+            r[j] = in ? g * s + h * c : __builtin_nanf("");
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            a[j] = rp.half ? p[j] : j & 1 ? r[j / 2] : p[j / 2];
+            b[j] = rp.half ? r[j] : j & 1 ? r[2 + j / 2] : p[2 + j / 2];
+        }
+    }
+    if (d0 >= D) return;
+    auto store = [&](uint32_t at, const float (&f)[4]) {
+        X z;
+        if constexpr (BF16)
+            z = u32x2{f32x2_to_bf16x2_bits(f[0], f[1]), f32x2_to_bf16x2_bits(f[2], f[3])};
+        else
+            z = f32x4{f[0], f[1], f[2], f[3]};
+        *gptr_mut<X>(static_cast<char*>(y.p) + (to + at) * E) = z;
+    };
+    store(i0, a);
+    store(i1, b);
+}
+
 // Largest of the N lanes around this one (N a power of two, aligned), by moves
 // within rows of 16 lanes.
 template <int N>
@@ -787,6 +867,21 @@ hipError_t qk_norm_rope_launch(const KvRows& q, const KvRows& q_out, uint32_t q_
         const uint64_t q_blocks = ((uint64_t)tokens * q_heads + rows - 1) / rows;
         const uint64_t grid = q_blocks + ((uint64_t)tokens * k_heads + rows - 1) / rows;
         if (!launchable(grid, 256)) return kTooManyThreads;
+        const bool both = k_heads != 0;
+        const bool wide = q.vec && q_out.vec && q_norm.on && q_norm.weight && q_norm.vec && rope.rot % 8 == 0 &&
+                          (!both || (k.vec && k_out.vec && k_norm.on && k_norm.weight && k_norm.vec && k.bf16 == q.bf16 &&
+                                     k_norm.bf16 == q_norm.bf16));
+        if (wide) {
+            auto go = [&](auto io, auto wt) {
+                norm_rope_wide_kernel<D, decltype(io)::value, decltype(wt)::value><<<(uint32_t)grid, 256, 0, st>>>(
+                    q, q_out, q_heads, q_norm, k, k_out, k_heads, k_norm, tokens, (uint32_t)q_blocks, rope);
+                return hipGetLastError();
+            };
+            using Y = std::true_type;
+            using N = std::false_type;
+            if (q.bf16) return q_norm.bf16 ? go(Y(), Y()) : go(Y(), N());
+            return q_norm.bf16 ? go(N(), Y()) : go(N(), N());
+        }
         norm_rope_kernel<D><<<(uint32_t)grid, 256, 0, st>>>(q, q_out, q_heads, q_norm, k, k_out, k_heads, k_norm, tokens,
                                                             (uint32_t)q_blocks, rope);
         return hipGetLastError();
