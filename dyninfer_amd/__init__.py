@@ -31,7 +31,7 @@ __all__ = [
     "LIB_PATH", "DyninferError", "QWeight", "Context", "library", "candidates", "registry_select",
     "registry_require", "precision_check", "supports", "ENC_Q4_0", "ENC_Q4_1", "ENC_Q8_0", "ENC_Q6_K", "ENC_Q4_K", "ENC_Q5_K", "ENC_IQ4_XS", "ENC_MLX_U4",
     "DTYPE_F32", "DTYPE_F16", "DTYPE_BF16", "block_geometry", "weight_bytes", "prefill_workspace_bytes",
-    "KV_Q8", "KV_Q4", "KVCache", "KVBatch", "Rope", "ROPE_INTERLEAVED", "ROPE_HALF", "ROPE_SCALINGS",
+    "KV_Q8", "KV_Q4", "KVCache", "KVBatch", "Rope", "HeadNorm", "PromptBatch", "TokenLogprobs", "ROPE_INTERLEAVED", "ROPE_HALF", "ROPE_SCALINGS",
     "ERR_INVALID_ARGUMENT",
     "ERR_UNSUPPORTED", "ERR_HIP", "ERR_DEVICE", "ERR_BUFFER_TOO_SMALL",
 ]
@@ -860,7 +860,7 @@ class Context:
         if not logits.is_cuda or logits.dim() != 2 or logits.stride(1) != 1:
             _bad("logits must be a device tensor [rows, vocab] whose last axis is contiguous")
         n, vocab = logits.shape
-        if not isinstance(top, int) or top < 0:
+        if not isinstance(top, int) or not 0 <= top < 1 << 32:
             _bad("top must be a number of tokens")
         code = _dtype_code(logits)
         kp = 0 if tokens is None else _table(tokens, _T_I64, (n,), "tokens")

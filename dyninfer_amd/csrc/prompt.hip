@@ -148,8 +148,7 @@ hipError_t prompt_launch(PromptArgs a, const PromptPlan& plan, uint8_t* work, hi
         constexpr int D = decltype(d)::value;
         uint32_t groups = 1;  // about four parts each
         while (groups < 256 / kJoinLanes<D> && 4 * groups < plan.parts) groups *= 2;
-        const uint64_t per = 256 / kJoinLanes<D> / groups, grid = (rows + per - 1) / per;
-        if (!launchable(grid, 256)) return kTooManyThreads;
+        const uint64_t per = 256 / kJoinLanes<D> / groups, grid = (rows + per - 1) / per;  // split: below 2^17 rows in all
         prompt_join_kernel<D><<<(uint32_t)grid, 256, 0, st>>>(a, 32 * plan.waves, groups);
         return hipGetLastError();
     };

@@ -397,7 +397,7 @@ __global__ __launch_bounds__(64 * WAVES * (WAVES > 1 && D > 128 ? 2 : 1), (WAVES
     // this wave's rows; a negative scale turns their signs, a scale of 0 makes them 0
     const float scale = fabsf(a.scale);
     w.c = scale == 0.0f ? 1.0f : scale * 1.4426950408889634f;
-    {
+    auto load_rows = [&] {  // behind the first tile's copies: one latency for both
         const int64_t at = (int64_t)(r.row0 + token) * a.q.ts + (int64_t)q_head * a.q.hs + half * (D / HALVES);
         const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
 #pragma unroll
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(64 * WAVES * (WAVES > 1 && D > 128 ? 2 : 1), (WAVES
                     w.q[t] = f32x4{x[0], x[1], x[2], x[3]};
             }
         }
-    }
+    };
     w.m = kNone;
     w.l = 0.0f;
 #pragma unroll
@@ -497,6 +497,7 @@ __global__ __launch_bounds__(64 * WAVES * (WAVES > 1 && D > 128 ? 2 : 1), (WAVES
             }
         };
         if (t0 < t1) load(t0);
+        load_rows();
         for (uint32_t t = t0; t < t1; t++) {
             ring_barrier<63>();  // the tile before has been read
 #pragma unroll
@@ -570,6 +571,7 @@ __global__ __launch_bounds__(64 * WAVES * (WAVES > 1 && D > 128 ? 2 : 1), (WAVES
             }
         };
         if (t0 < t1) fetch(t0);
+        load_rows();
         for (uint32_t t = t0; t < t1; t++) {
             ring_barrier<0>();  // tile t has landed, and the other stage has been read
             if (t + 1 < t1) fetch(t + 1);
