@@ -543,7 +543,7 @@ int dyninfer_mi355x_prompt_attention(dyninfer_mi355x_ctx_t* ctx, const dyninfer_
     if (int rc = check_ctx(ctx)) return rc;
     if (int rc = check_prompts(batch, true)) return rc;
     if (int rc = check_dim(head_dim)) return rc;
-    if (!std::isfinite(scale)) return fail(BAD, "scale must be finite");
+    if (!std::isfinite(scale * 1.4426950408889634f)) return fail(BAD, "scale must be finite, also times log2(e)");
     if (lse && !aligned(lse, 4)) return fail(BAD, "lse must be 4-byte aligned");
     if (batch->tokens == 0 || batch->sequences == 0 || batch->max_new == 0) return DYNINFER_MI355X_OK;
     dmx::PromptArgs a = {};

@@ -467,7 +467,8 @@ int dyninfer_mi355x_tree_attention_workspace_bytes(const dyninfer_kvcache_t* cac
  * Prompts packed one after the other: rows starts[b] .. starts[b+1] - 1 of q are sequence b's,
  * rows key_starts[b] .. of k and v its keys and values (key_starts NULL: starts).  A sequence has as
  * many keys as rows, or more: its rows are then the last ones (a piece of a prompt whose first
- * part was read before).  Device int32, 4-byte aligned.  max_new: the most rows of any sequence (rows
+ * part was read before).  Device int32, 4-byte aligned; a start outside the rows there are counts as the
+ * nearest, and a sequence that ends before it starts has none.  max_new: the most rows of any sequence (rows
  * past it are left out); max_keys: the most keys, which only shapes the launches (any number is handled).
  */
 typedef struct dyninfer_prompts {
@@ -486,8 +487,10 @@ typedef struct dyninfer_prompts {
  * head_dim 64, 96, 128 or 256.  A row that sees nothing (fewer keys than rows) gives 0 and lse -inf.  Rows of
  * out behind the last sequence are left as they were.  lse: f32 [tokens, heads], the natural logarithm of the sum
  * of exponentials, or NULL.  What is masked has no influence, whatever it holds.
- * Rounding: scores and outputs are sums in f32 (f32: of exact products); exponentials are f32, in
- * bf16 rounded once before the product with v.  Scores up to 2^30 in magnitude are resolved.
+ * scale is finite, also times log2(e).
+ * Rounding: scores and outputs are sums in f32, of exact products in bf16 and of products to 23 bits in f32.
+ * Exponentials are f32; in bf16 they are rounded once to bf16 before the product with v, and to 16 bits
+ * of mantissa where max_new * group <= 32.  Scores up to 2^30 in magnitude are resolved.
  * workspace: device memory of dyninfer_mi355x_prompt_attention_workspace_bytes, 256-byte aligned (NULL when that is 0),
  * under the rules of dyninfer_mi355x_qlinear's.
  */

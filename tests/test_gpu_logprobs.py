@@ -218,3 +218,15 @@ def test_rows_beyond_32_bits(ctx):
     t.copy_(torch.randn(3, vocab, device="cuda"))
     tokens = torch.tensor([0, 999, 5], device="cuda")
     check(ctx.token_logprobs(t, tokens, top=5), t.float().cpu().numpy(), [0, 999, 5], 5)
+
+
+def test_refused(ctx):
+    x, t = torch.zeros(3, 9000, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    good = dict(logits=x, tokens=t, top=2)
+    ctx.token_logprobs(**good)
+    for bad in (dict(logits=x[0]), dict(logits=x.cpu()), dict(logits=x.half()), dict(logits=x[:, ::2]), dict(logits=x.double()[:, :9]),
+                dict(logits=x[:1].expand(3, 9000)), dict(logits=x[:, :0]), dict(tokens=t[:2]), dict(tokens=t.int()), dict(tokens=t.cpu()),
+                dict(top=65), dict(top=-1), dict(top=1 << 40), dict(top=1.5), dict(temperature=torch.ones(2, device="cuda")),
+                dict(temperature=torch.ones(3, device="cuda").double()), dict(workspace=torch.empty(16, device="cuda"))):
+        with pytest.raises((d.DyninferError, TypeError)):
+            ctx.token_logprobs(**{**good, **bad})

@@ -188,3 +188,18 @@ def test_nothing_to_do(ctx):
     x = torch.empty(0, 4, 64, device="cuda")
     out = ctx.qk_norm_rope(x, x, q_norm=d.HeadNorm(), k_norm=d.HeadNorm())
     assert out[0].shape == (0, 4, 64) and out[1].shape == (0, 4, 64)
+
+
+def test_refused(ctx):
+    q, k, w = torch.ones(6, 4, 64, device="cuda"), torch.ones(6, 2, 64, device="cuda"), torch.ones(64, device="cuda")
+    rope = d.Rope(ctx.rope_table(16, 64), i32(range(6)), 64)
+    good = dict(q=q, k=k, rope=rope, q_norm=d.HeadNorm(w), k_norm=d.HeadNorm(w))
+    ctx.qk_norm_rope(**good)
+    for bad in (dict(q=q[0]), dict(q=q.cpu(), q_out=q), dict(q=q.half()), dict(k=k[:5]), dict(k=k[:, :, :32]), dict(k=None),
+                dict(q_norm=d.HeadNorm(w[:32])), dict(q_norm=d.HeadNorm(w.cpu())), dict(q_norm=d.HeadNorm(w.half())),
+                dict(q_norm=d.HeadNorm(torch.ones(128, device="cuda")[::2])), dict(k_norm=d.HeadNorm(w, eps=0.0)),
+                dict(k_norm=d.HeadNorm(w, offset=float("inf"))), dict(q_norm=d.HeadNorm(w, eps=1e300)), dict(q_out=q[:, :2]),
+                dict(q_out=q[:, :1].expand(6, 4, 64)), dict(k_out=q[:, 1:3]), dict(rope=None, k_norm=None),
+                dict(rope=d.Rope(rope.table, rope.positions[:5], 64)), dict(rope=d.Rope(rope.table, rope.positions, 128))):
+        with pytest.raises(d.DyninferError):
+            ctx.qk_norm_rope(**{**good, **bad})

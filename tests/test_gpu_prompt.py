@@ -125,7 +125,7 @@ def test_many_sequences(ctx, io):
     rng = np.random.default_rng(5)
     news = rng.integers(0, 90, 150).tolist()
     p = Prompts(1, news, [0] * 150, 2, 2, 64, io, 1)
-    assert io == "f32" or ctx.prompt_attention_workspace_bytes(p.batch(), sum(news), sum(news), 4, 2, 64, d._dtype_code(p.q)) == 0
+    assert ctx.prompt_attention_workspace_bytes(p.batch(), sum(news), sum(news), 4, 2, 64, d._dtype_code(p.q)) == 0
     p.check(p.run(ctx))
 
 
@@ -278,3 +278,46 @@ def test_nothing_to_do(ctx):
     assert (out == 2.0).all()
     k = torch.empty(0, 2, 64, device="cuda")
     assert (ctx.prompt_attention(q, k, k, d.PromptBatch(i32([0, 3]), 3, i32([0, 0]), 0)) == 0).all()
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("news,priors,told", [([9], [9000], 3000), ([9], [9000], 0), ([200, 3], [700, 2500], 64), ([40], [0], 1)])
+def test_more_keys_than_told(ctx, io, news, priors, told):
+    """max_keys shapes the launch only: parts grow, and none is lost."""
+    for dim in (64, 256):
+        p = Prompts(25, news, priors, 1, 4, dim, io)
+        p.check(p.run(ctx, batch=d.PromptBatch(i32(p.starts), max(news), i32(p.key_starts), told)))
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+def test_starts_outside(ctx, io):
+    """Starts outside the rows count as the nearest; a sequence that ends before it starts has no rows."""
+    p = Prompts(27, [60, 40], [0, 0], 1, 2, 64, io)
+    p.starts[-1] = p.key_starts[-1] = 100
+    want = p.run(ctx)
+    p.check(want)
+    for starts in ([-7, 60, 100], [0, 60, 2**31 - 1], [-2**31, 60, 101]):
+        got = p.run(ctx, batch=d.PromptBatch(i32(starts), 60))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    out = torch.full_like(p.q, 5.0)
+    got = p.run(ctx, out=out, batch=d.PromptBatch(i32([60, 0, 60]), 60))
+    assert torch.equal(got[0][:60], want[0][:60]) and (out[60:] == 5.0).all() and (got[1][60:] == 7.0).all()
+
+
+def test_refused(ctx):
+    q, k = torch.ones(6, 4, 64, device="cuda"), torch.ones(9, 2, 64, device="cuda")
+    batch = d.PromptBatch(i32([0, 6]), 6, i32([0, 9]), 9)
+    good = dict(q=q, k=k, v=k, batch=batch)
+    assert torch.equal(ctx.prompt_attention(**good), torch.ones_like(q))
+    for bad in (dict(q=q[0]), dict(q=q.cpu()), dict(q=q.transpose(0, 2)), dict(k=k.half()), dict(v=k[:8]), dict(v=k[:, :1]),
+                dict(k=k.bfloat16()), dict(k=k[:, :, :32]), dict(batch=d.PromptBatch(i32([0, 6]), 6)),
+                dict(batch=d.PromptBatch(i32([0, 6]).long(), 6, i32([0, 9]), 9)), dict(batch=d.PromptBatch(i32([]), 6, i32([]), 9)),
+                dict(batch=d.PromptBatch(i32([0, 6]), 7, i32([0, 9]), 9)), dict(batch=d.PromptBatch(i32([0, 6]), -1, i32([0, 9]), 9)),
+                dict(batch=d.PromptBatch(i32([0, 6]), 6, i32([0, 9, 9]), 9)), dict(batch=d.PromptBatch(i32([0, 6]), 6, i32([0, 9]), 10)),
+                dict(lse=torch.empty(6, 3, device="cuda")), dict(lse=torch.empty(6, 4, device="cuda").double()),
+                dict(out=q), dict(out=q.bfloat16()), dict(out=torch.empty(5, 4, 64, device="cuda")), dict(scale=float("nan"))):
+        with pytest.raises(d.DyninferError):
+            ctx.prompt_attention(**{**good, **bad})
+    long = torch.ones(5000, 2, 64, device="cuda")
+    with pytest.raises(d.DyninferError):  # parts, and no room for them
+        ctx.prompt_attention(q, long, long, d.PromptBatch(i32([0, 6]), 6, i32([0, 5000]), 5000), workspace=torch.empty(256, device="cuda"))

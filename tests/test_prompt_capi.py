@@ -113,7 +113,7 @@ LONG = prompts(key_starts=E + 4096, seqs=1, tokens=4, max_new=4, keys=30000, max
     (dict(batch=prompts(tokens=1 << 31, keys=1 << 31)), BAD, "tokens"),
     (dict(batch=prompts(key_starts=E + 4096, keys=1 << 31)), BAD, "keys"),
     (dict(batch=prompts(seqs=(1 << 24) + 1)), UNSUPPORTED, "sequences"), (dict(dim=48), UNSUPPORTED, "head"),
-    (dict(scale=NAN), BAD, "scale"), (dict(scale=-INF), BAD, "scale"), (dict(lse=ctypes.c_void_p(G + 2)), BAD, "lse"),
+    (dict(scale=NAN), BAD, "scale"), (dict(scale=-INF), BAD, "scale"), (dict(scale=3e38), BAD, "scale"), (dict(lse=ctypes.c_void_p(G + 2)), BAD, "lse"),
     (dict(q=None), BAD, "q is NULL"), (dict(out=None), BAD, "out is NULL"), (dict(k=None), BAD, "k is NULL"), (dict(v=None), BAD, "v is NULL"),
     (dict(q=rows(A, heads=5), out=rows(D, heads=5)), BAD, "multiple"), (dict(k=rows(B, heads=3), v=rows(C, heads=3)), BAD, "multiple"),
     (dict(v=rows(C, heads=4)), BAD, "share their heads"), (dict(k=rows(B, heads=2, dtype=F32)), BAD, "share a dtype"),
