@@ -143,15 +143,13 @@ struct VerifyArgs {
 };
 // Attention of prompts (prompt.hip): rows and keys of sequences packed one after the other.
 struct PromptPlan {
-    uint32_t waves;      // of a workgroup, 32 rows each
     uint32_t row_tiles;  // of the sequence with the most rows
     uint32_t parts;      // into which the keys of a row tile are split, at most
     uint32_t each;       // steps of 64 keys of a part
     uint64_t grid;
     uint64_t bytes, stats;  // workspace, and where the parts' statistics begin in it
 };
-PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint32_t heads, uint32_t group, uint32_t dim,
-                       bool f32);
+PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint32_t heads, uint32_t group, uint32_t dim);
 struct PromptArgs {
     KvRows q, k, v, out;
     const int32_t* q_starts;

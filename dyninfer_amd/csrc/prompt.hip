@@ -18,7 +18,7 @@ constexpr uint32_t kJoinLanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;
 // part to its own maximum, then the groups are joined in LDS.  Bound by latency where rows are
 // few: one token of 32 heads after 16000, 62 parts, by one group took 34 us.
 template <int D>
-__global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t rows_of_tile, uint32_t groups) {
+__global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t groups) {
     constexpr uint32_t L = kJoinLanes<D>;
     typedef float vec __attribute__((ext_vector_type(4)));
     __shared__ vec sm_o[256];
@@ -29,8 +29,8 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t
     const uint32_t seq = (uint32_t)min(id / per, (uint64_t)a.seqs - 1), i = (uint32_t)(id % per / q_heads), h = (uint32_t)(id % q_heads);
     const PromptRange r = prompt_range(a, seq);
     const uint32_t r0 = r.row0, head = h / a.group;
-    const uint64_t row = (uint64_t)i * a.group + (h - head * a.group), tile = row / rows_of_tile;
-    const uint64_t last_row = min((tile + 1) * rows_of_tile, (uint64_t)r.n * a.group) - 1;
+    const uint64_t row = (uint64_t)i * a.group + (h - head * a.group), tile = row / kPromptRows;
+    const uint64_t last_row = min((tile + 1) * kPromptRows, (uint64_t)r.n * a.group) - 1;
     const uint32_t parts = i < r.n ? prompt_cut(a, prompt_keys(a, r, last_row)).parts : 1u;
     const bool live = id < per * a.seqs && parts > 1;  // the others are written
     const uint32_t d0 = 4 * lane, from = d0 < D ? d0 : 0;
@@ -38,14 +38,14 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t
     vec o = {};
     if (live) {
         const uint64_t unit = (tile * a.seqs + seq) * a.heads + head;
-        const uint64_t at = unit * a.parts * rows_of_tile + row % rows_of_tile;  // of part 0; parts are rows_of_tile apart
+        const uint64_t at = unit * a.parts * kPromptRows + row % kPromptRows;  // of part 0; parts are kPromptRows apart
         for (uint32_t p0 = group; p0 < parts; p0 += 4 * groups) {  // four loads in flight
             float pm[4], pl[4];
             vec po[4];
 #pragma unroll
             for (uint32_t k = 0; k < 4; k++) {
                 const uint32_t p = p0 + k * groups;
-                const uint64_t slot = at + (uint64_t)min(p, parts - 1) * rows_of_tile;
+                const uint64_t slot = at + (uint64_t)min(p, parts - 1) * kPromptRows;
                 pm[k] = p < parts ? gptr<float>(a.stats)[2 * slot] : -__builtin_inff();
                 pl[k] = gptr<float>(a.stats)[2 * slot + 1];
                 po[k] = *gptr<vec>(a.part_o + slot * D + from);
@@ -102,15 +102,12 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t
 
 }  // namespace
 
-PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint32_t heads, uint32_t group, uint32_t dim,
-                       bool f32) {
+PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint32_t heads, uint32_t group, uint32_t dim) {
     PromptPlan p = {};
     const uint64_t rows = (uint64_t)max_new * group;
-    p.waves = rows <= 32 ? 1 : 4;
-    const uint32_t tile = 32 * p.waves;
-    p.row_tiles = (uint32_t)((rows + tile - 1) / tile);
+    p.row_tiles = (uint32_t)((rows + kPromptRows - 1) / kPromptRows);
     const uint64_t units = (uint64_t)seqs * heads * p.row_tiles;
-    const double full = p.waves == 1 ? 1024 : dim > 128 ? 256 : 512;  // workgroups at a time
+    const double full = dim > 128 ? 256 : 512;  // workgroups at a time
     const uint64_t steps = ((uint64_t)max_keys + 63) / 64;
     const double load = units * (steps - std::min(max_new, max_keys) / 128.0) / full;  // steps that a place for a workgroup gets
     const double each = std::max(std::ceil(load), 4.0);
@@ -122,8 +119,8 @@ PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint3
     }
     p.grid = units * p.parts;
     if (p.parts > 1) {
-        p.stats = p.grid * tile * dim * 4;
-        p.bytes = (p.stats + p.grid * tile * 8 + 255) / 256 * 256;
+        p.stats = p.grid * kPromptRows * dim * 4;
+        p.bytes = (p.stats + p.grid * kPromptRows * 8 + 255) / 256 * 256;
     }
     return p;
 }
@@ -135,7 +132,7 @@ extern template hipError_t prompt_launch_typed<true>(const PromptArgs&, const Pr
 
 hipError_t prompt_launch(PromptArgs a, const PromptPlan& plan, uint8_t* work, hipStream_t st) {
     if (plan.grid == 0) return hipSuccess;
-    if (!launchable(plan.grid, plan.waves == 1 ? 64 : a.dim > 128 ? 512 : 256)) return kTooManyThreads;
+    if (!launchable(plan.grid, a.dim > 128 ? 512 : 256)) return kTooManyThreads;
     a.row_tiles = plan.row_tiles;
     a.parts = plan.parts;
     a.each = plan.each;
@@ -149,7 +146,7 @@ hipError_t prompt_launch(PromptArgs a, const PromptPlan& plan, uint8_t* work, hi
         uint32_t groups = 1;  // about four parts each
         while (groups < 256 / kJoinLanes<D> && 4 * groups < plan.parts) groups *= 2;
         const uint64_t per = 256 / kJoinLanes<D> / groups, grid = (rows + per - 1) / per;  // split: below 2^17 rows in all
-        prompt_join_kernel<D><<<(uint32_t)grid, 256, 0, st>>>(a, 32 * plan.waves, groups);
+        prompt_join_kernel<D><<<(uint32_t)grid, 256, 0, st>>>(a, groups);
         return hipGetLastError();
     };
     switch (a.dim) {

@@ -6,6 +6,8 @@ namespace dmx {
 
 namespace {
 
+constexpr uint32_t kPromptRows = 128;  // of a row tile: four waves (of 256 dims four pairs) of 32
+
 // A number that is the same in every lane, as a scalar.
 __device__ __forceinline__ uint32_t scalar(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 __device__ __forceinline__ uint64_t scalar64(uint64_t x) {

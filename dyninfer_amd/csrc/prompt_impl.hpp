@@ -60,9 +60,6 @@ __device__ __forceinline__ PromptArgs late_args() {
     return __builtin_bit_cast(PromptArgs, x);
 }
 
-// bf16; f32 by f32 matrix instructions; f32 by bf16 ones in three terms.
-enum PromptKind { kBf16, kF32, kSplit };
-
 // f32 in three bf16 terms, x = hi + mid + lo to 2^-24: hi cut off (so that no finite number
 // becomes infinite), the others rounded.  Products of terms below 2^-23 of the whole are left out, so six
 // matrix instructions take the place of sixteen times their cost in f32 ones.
@@ -99,58 +96,51 @@ __device__ __forceinline__ f32x16 mfma_terms(const Terms& a, const Terms& b, f32
 }
 
 // How a tile of KT keys (or values) lies in LDS: rows of RS units of 16 bytes (a power of two),
-// unit c of row k at c ^ mix(k).  LDS has 64 banks, 256 bytes: sixteen lanes that read one unit of
-// consecutive keys, and the rows that one read of the values takes together (bf16: 64 bytes of four
-// keys; f32: 128 bytes of two, four keys apart), are on different ones.
-template <int D, PromptKind KIND>
+// unit c of row k at c ^ mix(k); in f32 three planes of them, one for each term.  LDS has 64 banks, 256
+// bytes: sixteen lanes that read one unit of consecutive keys, and the rows that one read of the
+// values takes together (64 bytes of four keys), are on different ones.
+template <int D, bool F32>
 struct TileShape {
-    static constexpr uint32_t E = KIND == kF32 ? 4 : 2, CH = D * E / 16;  // bytes of an element, units of a row
-    static constexpr uint32_t RS = CH <= 8 ? 8 : CH <= 16 ? 16 : CH <= 32 ? 32 : 64;
+    static constexpr uint32_t CH = D / 8;  // units of a row
+    static constexpr uint32_t RS = CH <= 8 ? 8 : CH <= 16 ? 16 : 32;
     static constexpr uint32_t RSB = RS * 16;
-    static constexpr uint32_t KT = RS <= 16 && KIND != kSplit ? 64 : 32;
-    static constexpr uint32_t PLANE = KT * RSB, BYTES = PLANE * (KIND == kSplit ? 3 : 1);  // of a term, of K or of V
+    static constexpr uint32_t KT = RS <= 16 && !F32 ? 64 : 32;
+    static constexpr uint32_t PLANE = KT * RSB, BYTES = PLANE * (F32 ? 3 : 1);  // of a term, of K or of V
     // Linear in the bits of k: mix(a ^ b) = mix(a) ^ mix(b).
     static constexpr __device__ uint32_t mix(uint32_t k) {
-        if (KIND == kF32) return (k >> 2 & 1u) << 3 | (k >> 3 & 1u) << 2 | (k & 3u);
         return RS == 8 ? (k >> 1 & 1u) << 2 | (k >> 2 & 3u) : (k & 3u) << 2 | (k >> 2 & 3u);
     }
 };
 
 // What a wave holds of its 32 rows: all dims, or (HALVES 2) half of them.
-template <int D, PromptKind KIND, int WAVES, int HALVES>
+template <int D, bool F32, int HALVES>
 struct PromptWave {
-    using T = TileShape<D, KIND>;
-    static constexpr bool F32 = KIND == kF32;
-    static constexpr int SUB = T::KT / 32, DT = D / 32 / HALVES, QN = (F32 ? D / 8 : D / 16) / HALVES;
-    using Frag = std::conditional_t<F32, f32x4, std::conditional_t<KIND == kSplit, Terms, bf16x8>>;
+    using T = TileShape<D, F32>;
+    static constexpr int SUB = T::KT / 32, DT = D / 32 / HALVES, QN = D / 16 / HALVES;
+    using Frag = std::conditional_t<F32, Terms, bf16x8>;
 
     Frag q[QN];
     f32x16 o[DT];
     float m, l;        // what exponents are from (in powers of two; kNone: nothing seen yet), sum of this lane's
     float c;           // scale in powers of two
     int64_t pos;       // the last key that this lane's row sees, -1: none
-    static constexpr uint32_t KA = T::RS == 8 ? 4 : 8, VA = F32 ? 4 : T::RS == 8 ? 2 : 4;
-    static constexpr uint32_t HALF = D * T::E / HALVES;  // bytes of a half in a row
+    static constexpr uint32_t KA = T::RS == 8 ? 4 : 8, VA = T::RS == 8 ? 2 : 4;
+    static constexpr uint32_t HALF = D * 2 / HALVES;  // bytes of a half in a row
     static_assert(HALVES == 1 || HALF % 256 == 0, "the second half's units do not mix with the first's");
-    uint32_t k_at[KA], v_at[F32 ? 1 : 2][VA];  // this lane's places in a tile
+    uint32_t k_at[KA], v_at[2][VA];  // this lane's places in a tile
 
     __device__ __forceinline__ void places(uint32_t lane, uint32_t half_of_dims) {
         const uint32_t col = lane & 31u, g = lane >> 5, h0 = half_of_dims * HALF;
 #pragma unroll
         for (uint32_t t = 0; t < KA; t++) k_at[t] = h0 + col * T::RSB + (((2 * t + g) ^ T::mix(col)) << 4);
-        if constexpr (F32) {
+        const uint32_t i = lane & 15u, half = (lane >> 4) & 1u;
 #pragma unroll
-            for (uint32_t b = 0; b < 4; b++) v_at[0][b] = h0 + (4 * g + b) * T::RSB + (((col / 4) ^ T::mix(4 * g + b)) << 4) + 4 * (col & 3u);
-        } else {
-            const uint32_t i = lane & 15u, half = (lane >> 4) & 1u;
+        for (uint32_t e = 0; e < 2; e++)
 #pragma unroll
-            for (uint32_t e = 0; e < 2; e++)
-#pragma unroll
-                for (uint32_t p = 0; p < VA; p++) {
-                    const uint32_t row = 8 * e + 4 * g + i / 4;
-                    v_at[e][p] = h0 + row * T::RSB + (((4 * p + 2 * half + (i & 3u) / 2) ^ T::mix(row)) << 4) + 8 * (i & 1u);
-                }
-        }
+            for (uint32_t p = 0; p < VA; p++) {
+                const uint32_t row = 8 * e + 4 * g + i / 4;
+                v_at[e][p] = h0 + row * T::RSB + (((4 * p + 2 * half + (i & 3u) / 2) ^ T::mix(row)) << 4) + 8 * (i & 1u);
+            }
     }
 
     // Of keys k0 + 32 sub + 4 (lane / 32) and on: how many this lane's row sees, up to 32.
@@ -164,25 +154,19 @@ struct PromptWave {
 #pragma unroll
         for (uint32_t t = 0; t < QN; t++) {
             const uint8_t* const at = kt + k_at[t % KA] + (sub * 32 * T::RSB + t / KA * KA * 32);
-            if constexpr (KIND == kSplit) {
+            if constexpr (F32) {
                 Terms k;
 #pragma unroll
                 for (uint32_t i = 0; i < 3; i++) k.t[i] = *reinterpret_cast<const bf16x8*>(at + i * T::PLANE);
                 s = mfma_terms(k, q[t], s);
-                continue;
-            }
-            const auto k = *reinterpret_cast<const std::conditional_t<F32, f32x4, bf16x8>*>(at);
-            if constexpr (F32) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], q[t][j], s, 0, 0, 0);
-            } else if constexpr (KIND == kBf16) {
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[t], s, 0, 0, 0);
+            } else {
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(at), q[t], s, 0, 0, 0);
             }
         }
         return s;
     }
 
-    // The operand of 32 dims of the values of 16 keys (bf16) in the order of P.
+    // The operand of 32 dims of the values of 16 keys in the order of P.
     __device__ __forceinline__ bf16x8 values(const uint8_t* vt, uint32_t s, uint32_t dt) const {
         typedef __attribute__((address_space(3))) i16x4 lds4;
         i16x4 x[2];
@@ -193,54 +177,31 @@ struct PromptWave {
         const u32x2 a = __builtin_bit_cast(u32x2, x[0]), b = __builtin_bit_cast(u32x2, x[1]);
         return __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
     }
-    // (f32): one dim of the value of key number i of 32.
-    __device__ __forceinline__ float value(const uint8_t* vt, uint32_t sub, uint32_t i, uint32_t dt) const {
-        const uint32_t at = v_at[0][i & 3u] ^ ((i >> 2 & 1u) << 6 | (dt & 1u) << 7);  // mix of key 8 (i / 4), and an odd dt
-        return *reinterpret_cast<const float*>(vt + at + ((32 * sub + 8 * (i >> 2)) * T::RSB + (dt >> 1) * 256));
-    }
 
     // P V added to the output.  bf16: the exponentials are rounded to 8 bits of mantissa, an error of the
-    // size of the output's own rounding; few rows, which the keys' bytes bound and not the
-    // products, take a second term, to 16 bits.
+    // size of the output's own rounding.
     __device__ __forceinline__ void add(const f32x16 (&p)[SUB], const uint8_t* vt) {
-        if constexpr (F32) {
 #pragma unroll
-            for (uint32_t sub = 0; sub < SUB; sub++)
+        for (uint32_t s = 0; s < 2 * SUB; s++) {
+            float x[8];
 #pragma unroll
-                for (uint32_t i = 0; i < 16; i++)
+            for (uint32_t j = 0; j < 8; j++) x[j] = p[s / 2][8 * (s & 1u) + j];
+            if constexpr (F32) {
+                const Terms pt = split8(x);
 #pragma unroll
-                    for (uint32_t dt = 0; dt < DT; dt++)
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(value(vt, sub, i, dt), p[sub][i], o[dt], 0, 0, 0);
-        } else {
+                for (uint32_t dt = 0; dt < DT; dt++) {
+                    Terms v;
 #pragma unroll
-            for (uint32_t s = 0; s < 2 * SUB; s++) {
-                float x[8];
-#pragma unroll
-                for (uint32_t j = 0; j < 8; j++) x[j] = p[s / 2][8 * (s & 1u) + j];
-                if constexpr (KIND == kSplit) {
-                    const Terms pt = split8(x);
-#pragma unroll
-                    for (uint32_t dt = 0; dt < DT; dt++) {
-                        Terms v;
-#pragma unroll
-                        for (uint32_t i = 0; i < 3; i++) v.t[i] = values(vt + i * T::PLANE, s, dt);
-                        o[dt] = mfma_terms(v, pt, o[dt]);
-                    }
-                } else {
-                    u32x4 w, u;
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; j++) {
-                        w[j] = f32x2_to_bf16x2_bits(x[2 * j], x[2 * j + 1]);
-                        if (WAVES == 1) u[j] = f32x2_to_bf16x2_bits(x[2 * j] - __uint_as_float(w[j] << 16), x[2 * j + 1] - __uint_as_float(w[j] & 0xFFFF0000u));
-                    }
-#pragma unroll
-                    for (uint32_t dt = 0; dt < DT; dt++) {
-                        const bf16x8 v = values(vt, s, dt);
-                        if constexpr (WAVES == 1)
-                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, u), o[dt], 0, 0, 0);
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, w), o[dt], 0, 0, 0);
-                    }
+                    for (uint32_t i = 0; i < 3; i++) v.t[i] = values(vt + i * T::PLANE, s, dt);
+                    o[dt] = mfma_terms(v, pt, o[dt]);
                 }
+            } else {
+                u32x4 w;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) w[j] = f32x2_to_bf16x2_bits(x[2 * j], x[2 * j + 1]);
+#pragma unroll
+                for (uint32_t dt = 0; dt < DT; dt++)
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(vt, s, dt), __builtin_bit_cast(bf16x8, w), o[dt], 0, 0, 0);
             }
         }
     }
@@ -348,16 +309,18 @@ __device__ __forceinline__ void prompt_row_by_itself(const PromptArgs& a, uint32
 }
 
 // Workgroup (row tile, sequence, kv head, part of the keys), the last row tiles, which see most
-// keys, first.  WAVES groups of 32 rows; of 256 dims, whose registers would leave one wave to a SIMD, two
+// keys, first.  Four groups of 32 rows; of 256 dims, whose registers would leave one wave to a SIMD, two
 // waves share a group: each takes the scores of its half of the dims, the halves are added through LDS,
 // and each keeps its half of the output.  VEC: keys and values lie on 16-byte boundaries, less than 64 MB apart.
-template <int D, PromptKind KIND, int WAVES, bool VEC>
-__global__ __launch_bounds__(64 * WAVES * (WAVES > 1 && D > 128 ? 2 : 1), (WAVES > 1 ? 2 : 1)) void prompt_kernel(PromptArgs a) {
-    constexpr int HALVES = WAVES > 1 && D > 128 ? 2 : 1, ALL = WAVES * HALVES;
-    using T = TileShape<D, KIND>;
-    using W = PromptWave<D, KIND, WAVES, HALVES>;
-    constexpr bool F32 = KIND != kBf16;
-    constexpr uint32_t ROWS = 32 * WAVES, STAGE = 2 * T::BYTES, STAGES = KIND == kSplit ? 1 : 2;
+template <int D>
+constexpr int kPromptHalves = D > 128 ? 2 : 1;
+
+template <int D, bool F32, bool VEC>
+__global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_kernel(PromptArgs a) {
+    constexpr int HALVES = kPromptHalves<D>, ALL = kPromptRows / 32 * HALVES;
+    using T = TileShape<D, F32>;
+    using W = PromptWave<D, F32, HALVES>;
+    constexpr uint32_t ROWS = kPromptRows, STAGE = 2 * T::BYTES, STAGES = F32 ? 1 : 2;
     __shared__ __align__(16) uint8_t lds[STAGES * STAGE];
     __shared__ f32x4 other[HALVES == 2 ? ALL * W::SUB * 4 * 64 : 1];  // scores of the other half
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -402,7 +365,7 @@ __global__ __launch_bounds__(64 * WAVES * (WAVES > 1 && D > 128 ? 2 : 1), (WAVES
         const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
 #pragma unroll
         for (uint32_t t = 0; t < W::QN; t++) {
-            if constexpr (KIND == kBf16) {
+            if constexpr (!F32) {
                 const uint16_t* p = static_cast<const uint16_t*>(a.q.p) + at + 16 * t + 8 * g;
                 u32x4 x;
                 if (a.q.vec) {
@@ -415,11 +378,10 @@ __global__ __launch_bounds__(64 * WAVES * (WAVES > 1 && D > 128 ? 2 : 1), (WAVES
                 for (int j = 0; j < 4; j++) x[j] = a.scale == 0.0f ? 0u : x[j] ^ (a.scale < 0.0f ? 0x80008000u : 0u);
                 w.q[t] = __builtin_bit_cast(bf16x8, x);
             } else {
-                constexpr int N = KIND == kSplit ? 8 : 4;
-                const float* p = static_cast<const float*>(a.q.p) + at + 2 * N * t + N * g;
-                float x[N];
+                const float* p = static_cast<const float*>(a.q.p) + at + 16 * t + 8 * g;
+                float x[8];
 #pragma unroll
-                for (int j = 0; j < N; j += 4) {
+                for (int j = 0; j < 8; j += 4) {
                     if (a.q.vec) {
                         const f32x4 y = *gptr<f32x4>(p + j);
 #pragma unroll
@@ -429,10 +391,7 @@ __global__ __launch_bounds__(64 * WAVES * (WAVES > 1 && D > 128 ? 2 : 1), (WAVES
                         for (int i = 0; i < 4; i++) x[j + i] = gptr<float>(p)[j + i] * sign;
                     }
                 }
-                if constexpr (KIND == kSplit)
-                    w.q[t] = split8(x);
-                else
-                    w.q[t] = f32x4{x[0], x[1], x[2], x[3]};
+                w.q[t] = split8(x);
             }
         }
     };
@@ -470,7 +429,7 @@ __global__ __launch_bounds__(64 * WAVES * (WAVES > 1 && D > 128 ? 2 : 1), (WAVES
         if (live) w.finish(p, lds + at + T::BYTES, k0, lane, (int64_t)(k0 + T::KT) > open);
     };
 
-    if constexpr (KIND == kSplit) {
+    if constexpr (F32) {
         // A tile goes through registers, where it is split into its terms: thread i takes units i + 64 ALL j,
         // eight dims each.  The next tile's loads are in flight while this one is worked on.
         constexpr uint32_t UNITS = T::KT * T::CH, N = (UNITS + 64 * ALL - 1) / (64 * ALL);
@@ -529,10 +488,10 @@ __global__ __launch_bounds__(64 * WAVES * (WAVES > 1 && D > 128 ? 2 : 1), (WAVES
         const uint32_t key0 = wave * PER + lane / T::RS, chunk0 = (lane % T::RS) ^ T::mix(key0);
         const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
         auto first = [&](const KvRows& x) {
-            return scalar64((uint64_t)(uintptr_t)x.p + (uint64_t)((int64_t)r.key0 * x.ts + (int64_t)head * x.hs) * T::E);
+            return scalar64((uint64_t)(uintptr_t)x.p + (uint64_t)((int64_t)r.key0 * x.ts + (int64_t)head * x.hs) * 2);
         };
         const uint64_t from[2] = {first(a.k), first(a.v)};
-        const uint64_t stride[2] = {scalar64((uint64_t)a.k.ts * T::E), scalar64((uint64_t)a.v.ts * T::E)};
+        const uint64_t stride[2] = {scalar64((uint64_t)a.k.ts * 2), scalar64((uint64_t)a.v.ts * 2)};
         auto fetch = [&](uint32_t t) {
             const uint32_t at = ((t - t0) & 1u) * STAGE + wave * 1024;
             const uint32_t left = min(r.nk - t * T::KT, T::KT);  // keys that there are
@@ -549,7 +508,7 @@ __global__ __launch_bounds__(64 * WAVES * (WAVES > 1 && D > 128 ? 2 : 1), (WAVES
                         u32x4 x;
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            x[e] = F32 ? gptr<uint32_t>(p)[e] : gptr<uint16_t>(p)[2 * e] | (uint32_t)gptr<uint16_t>(p)[2 * e + 1] << 16;
+                            x[e] = gptr<uint16_t>(p)[2 * e] | (uint32_t)gptr<uint16_t>(p)[2 * e + 1] << 16;
                         *reinterpret_cast<u32x4*>(lds + to + ALL * j * 1024 + 16 * lane) = x;
                     }
                 } else if (left == T::KT) {
@@ -674,10 +633,7 @@ hipError_t prompt_launch_typed(const PromptArgs& a, const PromptPlan& plan, hipS
         const bool vec = a.k.vec && a.v.vec && std::max(a.k.ts, a.v.ts) * E < (1 << 26);
         auto run = [&](auto v) {
             constexpr bool VEC = decltype(v)::value;
-            if (plan.waves == 1)
-                prompt_kernel<D, F32 ? kF32 : kBf16, 1, VEC><<<(uint32_t)plan.grid, 64, 0, st>>>(a);
-            else
-                prompt_kernel<D, F32 ? kSplit : kBf16, 4, VEC><<<(uint32_t)plan.grid, D > 128 ? 512 : 256, 0, st>>>(a);
+            prompt_kernel<D, F32, VEC><<<(uint32_t)plan.grid, 2 * kPromptRows * kPromptHalves<D>, 0, st>>>(a);
         };
         if (vec)
             run(std::true_type());

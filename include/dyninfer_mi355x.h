@@ -489,8 +489,8 @@ typedef struct dyninfer_prompts {
  * of exponentials, or NULL.  What is masked has no influence, whatever it holds.
  * scale is finite, also times log2(e).
  * Rounding: scores and outputs are sums in f32, of exact products in bf16 and of products to 23 bits in f32.
- * Exponentials are f32; in bf16 they are rounded once to bf16 before the product with v, and to 16 bits
- * of mantissa where max_new * group <= 32.  Scores up to 2^30 in magnitude are resolved.
+ * Exponentials are f32, in bf16 rounded once before the product with v.  Scores up to 2^30 in magnitude
+ * are resolved.
  * workspace: device memory of dyninfer_mi355x_prompt_attention_workspace_bytes, 256-byte aligned (NULL when that is 0),
  * under the rules of dyninfer_mi355x_qlinear's.
  */
