@@ -15,8 +15,9 @@ template <int D>
 constexpr uint32_t kJoinLanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;
 
 // A row (token, query head) by kJoinLanes<D> * groups threads: each group brings every groups-th
-// part to its own maximum, then the groups are joined in LDS.  Bound by latency where rows are
-// few: one token of 32 heads after 16000, 62 parts, by one group took 34 us.
+// part to its own maximum, then the groups are joined in LDS.  What it reads is small (a float a dim and part);
+// bound by latency where rows are few: one token of 32 heads after 16000, 62 parts, by one group took
+// 34 us, by groups of about four parts each 5.
 template <int D>
 __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t groups) {
     constexpr uint32_t L = kJoinLanes<D>;
@@ -102,6 +103,18 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t
 
 }  // namespace
 
+// Tiles of 128 rows, also where there are fewer: waves without rows still copy.  (32 rows by one wave: one token
+// of 32/8 heads of 128 dims after 16000 24 us, with four 21; 8 x 8 tokens after 4000 40 and 31, in f32 107
+// and 74.)
+//
+// A device takes two workgroups to a compute unit at a time (of 256 dims, which fill its LDS, one).  `load` is what
+// one of those places has to do in steps of 64 keys, with half of the new rows' own keys masked.  Where the
+// longest row tile has more, and it pays for the second launch (eight steps), keys are cut into parts of
+// `load` steps, four at least:
+//   2 x 96 rows of 12/4 heads of 64 dims after 24000: parts of load / 1, / 2, / 3 steps 36, 42, 46 us
+//   one token after 16000: parts of four steps at least 23 us, of eight 29
+//   512 rows of 32/8 heads, 8 steps in the longest tile: whole 17 us, in parts 22
+//   3 x 1500 of 8/2 heads of 256 dims in f32: whole 427 us, in parts 263
 PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint32_t heads, uint32_t group, uint32_t dim) {
     PromptPlan p = {};
     const uint64_t rows = (uint64_t)max_new * group;
@@ -109,7 +122,7 @@ PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint3
     const uint64_t units = (uint64_t)seqs * heads * p.row_tiles;
     const double full = dim > 128 ? 256 : 512;  // workgroups at a time
     const uint64_t steps = ((uint64_t)max_keys + 63) / 64;
-    const double load = units * (steps - std::min(max_new, max_keys) / 128.0) / full;  // steps that a place for a workgroup gets
+    const double load = units * (steps - std::min(max_new, max_keys) / 128.0) / full;
     const double each = std::max(std::ceil(load), 4.0);
     p.parts = 1;
     p.each = 0xFFFFFFFFu;

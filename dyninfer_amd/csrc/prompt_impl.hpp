@@ -13,6 +13,16 @@
 //   S: lane l holds keys 8 a + 4 (l / 32) + b of 32, register 4 a + b
 //   P, as operand of 16 keys: lane l holds registers 8 s .. 8 s + 7 of that order
 // The sum over keys may take them in any order if V's operand agrees.
+//
+// What bounds it: 32 rows by 64 keys of 128 dims are 32 MFMAs of 32 cycles, 1024, and some 160 vector
+// instructions, 32 exponentials among them, about as many cycles again; the two waves of a SIMD
+// overlap them in part (1830 cycles for the two kinds, the matrix units busy for 56 %).  16384 tokens of 32/8
+// heads of 128 dims in bf16 take 1.95 ms (1130 TFLOP/s; up to 2.08 by card; a product of two 8192 x
+// 8192 matrices reaches 1370 to 1400), 8192 tokens of 64 dims 284 us (970), of 96 226 (912); 4096 tokens in
+// f32 705 us (195, of six products each).  Prompts of some hundred tokens are bound by the
+// latencies of a tile's beginning and end: 24 x 700 tokens of 16/8 heads 89 us (540).
+// Tried without gain: tiles of 32 keys (2319 us instead of 2068), three waves on a SIMD (registers
+// spill, 2948), two tiles ahead at 64 dims (316 instead of 284), wave priorities.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -61,8 +71,10 @@ __device__ __forceinline__ PromptArgs late_args() {
 }
 
 // f32 in three bf16 terms, x = hi + mid + lo to 2^-24: hi cut off (so that no finite number
-// becomes infinite), the others rounded.  Products of terms below 2^-23 of the whole are left out, so six
-// matrix instructions take the place of sixteen times their cost in f32 ones.
+// becomes infinite), the others rounded.  Products of terms below 2^-23 of the whole are left out: six
+// matrix instructions take the place of eight f32 ones of twice the cycles each (4096 tokens 1230 us with those).
+// Split in the kernel, tile by tile: split beforehand into a workspace they took 654 to 730 us, no
+// faster, and 104 instead of 56 where 16 rows follow 4000.
 struct Terms {
     bf16x8 t[3];
 };
@@ -311,7 +323,7 @@ __device__ __forceinline__ void prompt_row_by_itself(const PromptArgs& a, uint32
 // Workgroup (row tile, sequence, kv head, part of the keys), the last row tiles, which see most
 // keys, first.  Four groups of 32 rows; of 256 dims, whose registers would leave one wave to a SIMD, two
 // waves share a group: each takes the scores of its half of the dims, the halves are added through LDS,
-// and each keeps its half of the output.  VEC: keys and values lie on 16-byte boundaries, less than 64 MB apart.
+// and each keeps its half of the output (8192 tokens of 8/2 heads 400 us, by one wave each 540).  VEC: keys and values lie on 16-byte boundaries, less than 64 MB apart.
 template <int D>
 constexpr int kPromptHalves = D > 128 ? 2 : 1;
 
