@@ -25,20 +25,20 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t
     __shared__ vec sm_o[256];
     __shared__ float sm_m[256 / L], sm_l[256 / L];
     const uint32_t q_heads = a.heads * a.group, lane = threadIdx.x % L, group = threadIdx.x / L % groups;
-    const uint64_t id = (uint64_t)blockIdx.x * (256 / L / groups) + threadIdx.x / L / groups;
-    const uint64_t per = (uint64_t)a.max_new * q_heads;
-    const uint32_t seq = (uint32_t)min(id / per, (uint64_t)a.seqs - 1), i = (uint32_t)(id % per / q_heads), h = (uint32_t)(id % q_heads);
+    const uint32_t id = blockIdx.x * (256 / L / groups) + threadIdx.x / L / groups;  // rows of split calls are below 2^17
+    const uint32_t per = a.max_new * q_heads;
+    const uint32_t seq = min(id / per, a.seqs - 1), i = id % per / q_heads, h = id % q_heads;
     const PromptRange r = prompt_range(a, seq);
     const uint32_t r0 = r.row0, head = h / a.group;
-    const uint64_t row = (uint64_t)i * a.group + (h - head * a.group), tile = row / kPromptRows;
-    const uint64_t last_row = min((tile + 1) * kPromptRows, (uint64_t)r.n * a.group) - 1;
-    const uint32_t parts = i < r.n ? prompt_cut(a, prompt_keys(a, r, last_row)).parts : 1u;
+    const uint32_t row = i * a.group + (h - head * a.group), tile = row / kPromptRows;
+    const uint32_t last_row = min((tile + 1) * kPromptRows, r.n * a.group) - 1;
+    const uint32_t parts = i < r.n ? prompt_cut(a, prompt_keys(r, last_row / a.group)).parts : 1u;
     const bool live = id < per * a.seqs && parts > 1;  // the others are written
     const uint32_t d0 = 4 * lane, from = d0 < D ? d0 : 0;
     float m = -__builtin_inff(), l = 0.0f;
     vec o = {};
     if (live) {
-        const uint64_t unit = (tile * a.seqs + seq) * a.heads + head;
+        const uint64_t unit = (uint64_t)(tile * a.seqs + seq) * a.heads + head;
         const uint64_t at = unit * a.parts * kPromptRows + row % kPromptRows;  // of part 0; parts are kPromptRows apart
         for (uint32_t p0 = group; p0 < parts; p0 += 4 * groups) {  // four loads in flight
             float pm[4], pl[4];

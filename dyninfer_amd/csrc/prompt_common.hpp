@@ -35,9 +35,9 @@ __device__ __forceinline__ PromptRange prompt_range(const PromptArgs& a, uint32_
     return r;
 }
 
-// Keys, from the first on, that some of the rows first..last of one kv head see.
-__device__ __forceinline__ uint32_t prompt_keys(const PromptArgs& a, const PromptRange& r, uint64_t last_row) {
-    const int64_t n = (int64_t)(last_row / a.group) + r.off + 1;
+// Keys, from the first on, that token i of the sequence sees: below 2^31, as rows of one kv head are too.
+__device__ __forceinline__ uint32_t prompt_keys(const PromptRange& r, uint32_t token) {
+    const int64_t n = (int64_t)token + r.off + 1;
     return n <= 0 ? 0u : (uint32_t)n;
 }
 

@@ -135,7 +135,7 @@ struct PromptWave {
     f32x16 o[DT];
     float m, l;        // what exponents are from (in powers of two; kNone: nothing seen yet), sum of this lane's
     float c;           // scale in powers of two
-    int64_t pos;       // the last key that this lane's row sees, -1: none
+    uint32_t sees;     // keys that this lane's row sees
     static constexpr uint32_t KA = T::RS == 8 ? 4 : 8, VA = T::RS == 8 ? 2 : 4;
     static constexpr uint32_t HALF = D * 2 / HALVES;  // bytes of a half in a row
     static_assert(HALVES == 1 || HALF % 256 == 0, "the second half's units do not mix with the first's");
@@ -156,8 +156,9 @@ struct PromptWave {
     }
 
     // Of keys k0 + 32 sub + 4 (lane / 32) and on: how many this lane's row sees, up to 32.
-    __device__ __forceinline__ int32_t seen_of(uint64_t k0, uint32_t sub, uint32_t lane) const {
-        return (int32_t)max(min(pos + 1 - (int64_t)(k0 + 32 * sub + 4 * (lane >> 5)), (int64_t)32), (int64_t)0);
+    __device__ __forceinline__ uint32_t seen_of(uint32_t k0, uint32_t sub, uint32_t lane) const {
+        const uint32_t from = k0 + 32 * sub + 4 * (lane >> 5);
+        return sees > from ? min(sees - from, 32u) : 0u;
     }
 
     // scores of 32 keys
@@ -219,16 +220,16 @@ struct PromptWave {
     }
 
     // A tile of keys from k0 on, from the scores on.  masked: some row does not see all of them.
-    __device__ __forceinline__ void finish(f32x16 (&p)[SUB], const uint8_t* vt, uint64_t k0, uint32_t lane, bool masked) {
+    __device__ __forceinline__ void finish(f32x16 (&p)[SUB], const uint8_t* vt, uint32_t k0, uint32_t lane, bool masked) {
         float top = kNone;
         if (masked) {
             asm volatile("");  // a branch, not a selection in every step
 #pragma unroll
             for (uint32_t sub = 0; sub < SUB; sub++) {
-                const int32_t sees = seen_of(k0, sub, lane);
+                const uint32_t some = seen_of(k0, sub, lane);
 #pragma unroll
-                for (int32_t i = 0; i < 16; i++)
-                    if (8 * (i >> 2) + (i & 3) >= sees) p[sub][i] = kNone;
+                for (uint32_t i = 0; i < 16; i++)
+                    if (8 * (i >> 2) + (i & 3u) >= some) p[sub][i] = kNone;
             }
         }
 #pragma unroll
@@ -347,11 +348,11 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
     const uint32_t seq = id % a.seqs, tile = a.row_tiles - 1 - id / a.seqs;
     PromptRange r = prompt_range(a, seq);
     r = {scalar(r.row0), scalar(r.n), scalar(r.key0), scalar(r.nk), (int64_t)scalar64((uint64_t)r.off)};
-    const uint64_t rows = (uint64_t)r.n * a.group, tile_row = (uint64_t)tile * ROWS;
+    const uint32_t rows = r.n * a.group, tile_row = tile * ROWS;  // below 2^31
     if (tile_row >= rows) return;
-    const uint64_t last_row = min(tile_row + ROWS, rows) - 1;
+    const uint32_t last_row = min(tile_row + ROWS, rows) - 1;
     // keys that some row of the tile sees, and of them this part's
-    const uint32_t keys = prompt_keys(a, r, last_row);
+    const uint32_t keys = prompt_keys(r, last_row / a.group);
     const PromptCut cut = prompt_cut(a, keys);
     if (part >= cut.parts) return;
     constexpr uint32_t PER_STEP = 64 / T::KT;
@@ -360,20 +361,20 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
 
     W w;
     w.places(lane, half);
-    const uint64_t wave_row = tile_row + 32 * group, row = wave_row + col;
-    const uint64_t token = min(row, last_row) / a.group;
-    const uint32_t q_head = head * a.group + (uint32_t)(min(row, last_row) - token * a.group);
-    w.pos = row <= last_row ? (int64_t)token + r.off : -1;
+    const uint32_t wave_row = tile_row + 32 * group, row = wave_row + col;
+    const uint32_t token = min(row, last_row) / a.group;
+    const uint32_t q_head = head * a.group + (min(row, last_row) - token * a.group);
+    w.sees = row <= last_row ? prompt_keys(r, token) : 0u;
     // all keys up to `open` are seen by every row of this wave, none from `shut` on by any
     const bool whole = wave_row + 31 <= last_row;
-    const int64_t open = whole ? (int64_t)(wave_row / a.group) + r.off + 1 : 0;
-    const int64_t shut = wave_row > last_row ? 0 : (int64_t)(min(wave_row + 31, last_row) / a.group) + r.off + 1;
+    const uint32_t open = whole ? prompt_keys(r, wave_row / a.group) : 0u;
+    const uint32_t shut = wave_row > last_row ? 0u : prompt_keys(r, min(wave_row + 31, last_row) / a.group);
 
     // this wave's rows; a negative scale turns their signs, a scale of 0 makes them 0
     const float scale = fabsf(a.scale);
     w.c = scale == 0.0f ? 1.0f : scale * 1.4426950408889634f;
     auto load_rows = [&] {  // behind the first tile's copies: one latency for both
-        const int64_t at = (int64_t)(r.row0 + token) * a.q.ts + (int64_t)q_head * a.q.hs + half * (D / HALVES);
+        const int64_t at = (int64_t)((uint64_t)r.row0 + token) * a.q.ts + (int64_t)q_head * a.q.hs + half * (D / HALVES);
         const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
 #pragma unroll
         for (uint32_t t = 0; t < W::QN; t++) {
@@ -414,8 +415,8 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
 
     // Tile t, whose keys lie at LDS offset `at` and its values behind them: every wave comes here.
     auto step = [&](uint32_t t, uint32_t at) {
-        const uint64_t k0 = (uint64_t)t * T::KT;
-        const bool live = (int64_t)k0 < shut;
+        const uint32_t k0 = t * T::KT;
+        const bool live = k0 < shut;
         f32x16 p[W::SUB];
         if (live) {
 #pragma unroll
@@ -438,7 +439,7 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
                 }
             }
         }
-        if (live) w.finish(p, lds + at + T::BYTES, k0, lane, (int64_t)(k0 + T::KT) > open);
+        if (live) w.finish(p, lds + at + T::BYTES, k0, lane, k0 + T::KT > open);
     };
 
     if constexpr (F32) {
@@ -562,7 +563,7 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
     bool alone = false;  // rows one by one
     if (__any(odd)) {
         bool masked = false;
-        const int64_t first = max((int64_t)(min(wave_row, last_row) / b.group) + r.off + 1, key_begin);
+        const int64_t first = max((int64_t)prompt_keys(r, min(wave_row, last_row) / b.group), key_begin);
         for (int64_t j = max(min(first, key_end - 1), (int64_t)0); j < key_end; j++)  // the last one stands for keys behind the end as well
             for (uint32_t d = lane; d < D; d += 64)
                 masked |= !(fabsf(prompt_element<F32>(b.v, (int64_t)(r.key0 + j) * b.v.ts + (int64_t)head * b.v.hs + d)) < __builtin_inff());
@@ -577,9 +578,9 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
     if (alone) {
 #pragma unroll 1
         for (uint32_t i = 0; i < 32 && wave_row + i <= last_row; i++) {
-            const uint64_t rr = wave_row + i, tok = rr / b.group;
-            const int64_t end = min((int64_t)tok + r.off + 1, key_end);
-            prompt_row_by_itself<D, D / HALVES, F32>(b, half * (D / HALVES), r.row0 + tok, head * b.group + (uint32_t)(rr - tok * b.group),
+            const uint32_t rr = wave_row + i, tok = rr / b.group;
+            const int64_t end = min((int64_t)prompt_keys(r, tok), key_end);
+            prompt_row_by_itself<D, D / HALVES, F32>(b, half * (D / HALVES), (uint64_t)r.row0 + tok, head * b.group + (rr - tok * b.group),
                                                      r.key0, head, key_begin, end, cut.parts > 1, slot0 + i);
         }
         return;
@@ -602,10 +603,11 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
         return;
     }
     const float inv = w.m == kNone ? 0.0f : 1.0f / w.l;
+    const uint32_t i0 = row / b.group, h0 = head * b.group + (row - i0 * b.group);  // computed again, not held
+    const uint64_t to_row = (uint64_t)r.row0 + i0;
     if (b.lse && g == 0 && half == 0)
-        gptr_mut<float>(b.lse)[(r.row0 + token) * (uint64_t)(b.heads * b.group) + q_head] =
-            w.m == kNone ? kNone : (w.m + log2f(w.l)) * 0.69314718055994531f;
-    const int64_t to = (int64_t)(r.row0 + token) * b.out.ts + (int64_t)q_head * b.out.hs + half * (D / HALVES);
+        gptr_mut<float>(b.lse)[to_row * (b.heads * b.group) + h0] = w.m == kNone ? kNone : (w.m + log2f(w.l)) * 0.69314718055994531f;
+    const int64_t to = (int64_t)to_row * b.out.ts + (int64_t)h0 * b.out.hs + half * (D / HALVES);
 #pragma unroll
     for (uint32_t dt = 0; dt < W::DT; dt++)
 #pragma unroll
