@@ -324,7 +324,7 @@ __device__ __forceinline__ void prompt_row_by_itself(const PromptArgs& a, uint32
 // Workgroup (row tile, sequence, kv head, part of the keys), the last row tiles, which see most
 // keys, first.  Four groups of 32 rows; of 256 dims, whose registers would leave one wave to a SIMD, two
 // waves share a group: each takes the scores of its half of the dims, the halves are added through LDS,
-// and each keeps its half of the output (8192 tokens of 8/2 heads 400 us, by one wave each 540).  VEC: keys and values lie on 16-byte boundaries, less than 64 MB apart.
+// and each keeps its half of the output (8192 tokens of 8/2 heads 362 us, by one wave each 540).  VEC: keys and values lie on 16-byte boundaries, less than 64 MB apart.
 template <int D>
 constexpr int kPromptHalves = D > 128 ? 2 : 1;
 
@@ -335,7 +335,8 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
     using W = PromptWave<D, F32, HALVES>;
     constexpr uint32_t ROWS = kPromptRows, STAGE = 2 * T::BYTES, STAGES = F32 ? 1 : 2;
     __shared__ __align__(16) uint8_t lds[STAGES * STAGE];
-    __shared__ f32x4 other[HALVES == 2 ? ALL * W::SUB * 4 * 64 : 1];  // scores of the other half
+    constexpr uint32_t TURNS = HALVES == 2 && !F32 ? 2 : 1;
+    __shared__ f32x4 other[HALVES == 2 ? TURNS * ALL * W::SUB * 4 * 64 : 1];  // scores of the other half
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t group = wave / HALVES, half = wave % HALVES;
     const uint32_t g = lane >> 5, col = lane & 31u;
@@ -413,34 +414,41 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
 #pragma unroll
     for (uint32_t dt = 0; dt < W::DT; dt++) w.o[dt] = f32x16{};
 
-    // Tile t, whose keys lie at LDS offset `at` and its values behind them: every wave comes here.
-    auto step = [&](uint32_t t, uint32_t at) {
-        const uint32_t k0 = t * T::KT;
-        const bool live = k0 < shut;
-        f32x16 p[W::SUB];
-        if (live) {
+    // Tile t: its scores, from its keys at LDS offset `at`, and the rest, from its values.
+    typedef f32x16 Scores[W::SUB];
+    auto live = [&](uint32_t t) { return t * T::KT < shut; };
+    auto scores = [&](uint32_t t, uint32_t at, Scores& p) {
+        if (!live(t)) return;
 #pragma unroll
-            for (uint32_t sub = 0; sub < W::SUB; sub++) p[sub] = w.scores(lds + at, sub);
-        }
-        if constexpr (HALVES == 2) {
-            auto place = [&](uint32_t of, uint32_t i) { return other + (of * W::SUB * 4 + i) * 64 + lane; };
-            if (live) {
-#pragma unroll
-                for (uint32_t i = 0; i < 4 * W::SUB; i++)
-                    *place(wave, i) = f32x4{p[i / 4][4 * (i & 3u)], p[i / 4][4 * (i & 3u) + 1], p[i / 4][4 * (i & 3u) + 2], p[i / 4][4 * (i & 3u) + 3]};
-            }
-            ring_barrier<63>();
-            if (live) {
-#pragma unroll
-                for (uint32_t i = 0; i < 4 * W::SUB; i++) {
-                    const f32x4 x = *place(wave ^ 1u, i);
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; j++) p[i / 4][4 * (i & 3u) + j] += x[j];
-                }
-            }
-        }
-        if (live) w.finish(p, lds + at + T::BYTES, k0, lane, k0 + T::KT > open);
+        for (uint32_t sub = 0; sub < W::SUB; sub++) p[sub] = w.scores(lds + at, sub);
     };
+    auto finish = [&](uint32_t t, uint32_t at, Scores& p) {
+        if (live(t)) w.finish(p, lds + at, t * T::KT, lane, (t + 1) * T::KT > open);
+    };
+    // (HALVES 2) The scores of this half of the dims to the other wave, and its own added.
+    auto place = [&](uint32_t of, uint32_t i) { return other + (of * W::SUB * 4 + i) * 64 + lane; };
+    auto give = [&](uint32_t t, const Scores& p, uint32_t turn) {
+        if (!live(t)) return;
+#pragma unroll
+        for (uint32_t i = 0; i < 4 * W::SUB; i++)
+            *place(turn * ALL + wave, i) = f32x4{p[i / 4][4 * (i & 3u)], p[i / 4][4 * (i & 3u) + 1], p[i / 4][4 * (i & 3u) + 2], p[i / 4][4 * (i & 3u) + 3]};
+    };
+    auto take = [&](uint32_t t, Scores& p, uint32_t turn) {
+        if (!live(t)) return;
+#pragma unroll
+        for (uint32_t i = 0; i < 4 * W::SUB; i++) {
+            const f32x4 x = *place(turn * ALL + (wave ^ 1u), i);
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) p[i / 4][4 * (i & 3u) + j] += x[j];
+        }
+    };
+
+    // Where this head's keys and values begin, and bytes from one to the next.
+    auto first = [&](const KvRows& x) {
+        return scalar64((uint64_t)(uintptr_t)x.p + (uint64_t)((int64_t)r.key0 * x.ts + (int64_t)head * x.hs) * (F32 ? 4 : 2));
+    };
+    const uint64_t from[2] = {first(a.k), first(a.v)};
+    const uint64_t stride[2] = {scalar64((uint64_t)a.k.ts * (F32 ? 4 : 2)), scalar64((uint64_t)a.v.ts * (F32 ? 4 : 2))};
 
     if constexpr (F32) {
         // A tile goes through registers, where it is split into its terms: thread i takes units i + 64 ALL j,
@@ -448,22 +456,21 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
         constexpr uint32_t UNITS = T::KT * T::CH, N = (UNITS + 64 * ALL - 1) / (64 * ALL);
         f32x4 raw[N][2][2];
         auto load = [&](uint32_t t) {
+            const uint32_t left = min(r.nk - t * T::KT, T::KT);  // keys behind the end are the last one
 #pragma unroll
             for (uint32_t j = 0; j < N; j++) {
-                const uint32_t u = min(threadIdx.x + 64 * ALL * j, UNITS - 1);
-                const int64_t at = r.key0 + min((int64_t)t * T::KT + u / T::CH, (int64_t)r.nk - 1);
+                const uint32_t u = min(threadIdx.x + 64 * ALL * j, UNITS - 1), key = min(u / T::CH, left - 1);
 #pragma unroll
                 for (uint32_t i = 0; i < 2; i++) {
-                    const KvRows& x = i ? a.v : a.k;
-                    const float* const from = static_cast<const float*>(x.p) + at * x.ts + (int64_t)head * x.hs + 8 * (u % T::CH);
+                    const char* const base = reinterpret_cast<const char*>(from[i] + t * (stride[i] * T::KT));
+                    if constexpr (VEC) {
+                        const uint32_t at = key * (uint32_t)stride[i] + 32 * (u % T::CH);
 #pragma unroll
-                    for (uint32_t e = 0; e < 2; e++) {
-                        if constexpr (VEC) {
-                            raw[j][i][e] = *gptr<f32x4>(from + 4 * e);
-                        } else {
+                        for (uint32_t e = 0; e < 2; e++) raw[j][i][e] = *gptr<f32x4>(base + at + 16 * e);
+                    } else {
+                        const char* const p = base + key * stride[i] + 32 * (u % T::CH);
 #pragma unroll
-                            for (uint32_t y = 0; y < 4; y++) raw[j][i][e][y] = gptr<float>(from)[4 * e + y];
-                        }
+                        for (uint32_t e = 0; e < 8; e++) raw[j][i][e / 4][e % 4] = gptr<float>(p)[e];
                     }
                 }
             }
@@ -489,7 +496,14 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
             }
             if (t + 1 < t1) load(t + 1);
             ring_barrier<63>();
-            step(t, 0);
+            Scores p;
+            scores(t, 0, p);
+            if constexpr (HALVES == 2) {
+                give(t, p, 0);
+                ring_barrier<63>();
+                take(t, p, 0);
+            }
+            finish(t, T::BYTES, p);
         }
     } else {
         // Copies of a tile: unit blk * 64 + lane of K and of V, blk = wave + ALL j, its key key0 + STEP j,
@@ -500,16 +514,11 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
         static_assert(COPIES * 64 * ALL == T::KT * T::RS, "whole copies");
         const uint32_t key0 = wave * PER + lane / T::RS, chunk0 = (lane % T::RS) ^ T::mix(key0);
         const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-        auto first = [&](const KvRows& x) {
-            return scalar64((uint64_t)(uintptr_t)x.p + (uint64_t)((int64_t)r.key0 * x.ts + (int64_t)head * x.hs) * 2);
-        };
-        const uint64_t from[2] = {first(a.k), first(a.v)};
-        const uint64_t stride[2] = {scalar64((uint64_t)a.k.ts * 2), scalar64((uint64_t)a.v.ts * 2)};
-        auto fetch = [&](uint32_t t) {
+        auto fetch = [&](uint32_t t, uint32_t first, uint32_t count) {  // keys (0), values (1)
             const uint32_t at = ((t - t0) & 1u) * STAGE + wave * 1024;
             const uint32_t left = min(r.nk - t * T::KT, T::KT);  // keys that there are
 #pragma unroll
-            for (uint32_t i = 0; i < 2; i++) {
+            for (uint32_t i = first; i < first + count; i++) {
                 uint64_t base = from[i] + t * (stride[i] * T::KT);
                 const uint32_t to = at + i * T::BYTES;
                 if constexpr (!VEC) {
@@ -542,12 +551,41 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
                 }
             }
         };
-        if (t0 < t1) fetch(t0);
+        if (t0 < t1) fetch(t0, 0, 2);
         load_rows();
-        for (uint32_t t = t0; t < t1; t++) {
-            ring_barrier<0>();  // tile t has landed, and the other stage has been read
-            if (t + 1 < t1) fetch(t + 1);
-            step(t, ((t - t0) & 1u) * STAGE);
+        if constexpr (HALVES == 1) {
+            for (uint32_t t = t0; t < t1; t++) {
+                ring_barrier<0>();  // tile t has landed, and the other stage has been read
+                if (t + 1 < t1) fetch(t + 1, 0, 2);
+                const uint32_t at = ((t - t0) & 1u) * STAGE;
+                if (!live(t)) continue;
+                Scores p;
+#pragma unroll
+                for (uint32_t sub = 0; sub < W::SUB; sub++) p[sub] = w.scores(lds + at, sub);
+                w.finish(p, lds + at + T::BYTES, t * T::KT, lane, (t + 1) * T::KT > open);
+            }
+        } else if (t0 < t1) {
+            // The scores of a tile ahead of the rest of the one before: one barrier a tile, and products beside
+            // exponentials (362 us instead of 397; in f32, whose registers are full, no gain).
+            Scores p, next;
+            if (t0 + 1 < t1) fetch(t0 + 1, 0, 1);
+            ring_barrier<0>();
+            scores(t0, 0, next);
+            give(t0, next, 0);
+            for (uint32_t t = t0; t < t1; t++) {
+                ring_barrier<0>();  // values of t and keys of t + 1 have landed, the stages of those before have been read
+                const uint32_t turn = (t - t0) & 1u;
+                if (t + 1 < t1) fetch(t + 1, 1, 1);
+                if (t + 2 < t1) fetch(t + 2, 0, 1);
+#pragma unroll
+                for (int i = 0; i < W::SUB; i++) p[i] = next[i];
+                take(t, p, turn);
+                if (t + 1 < t1) {
+                    scores(t + 1, (turn ^ 1u) * STAGE, next);
+                    give(t + 1, next, turn ^ 1u);
+                }
+                finish(t, turn * STAGE + T::BYTES, p);
+            }
         }
     }
 
