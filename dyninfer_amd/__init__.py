@@ -866,15 +866,25 @@ class Context:
         kp = 0 if tokens is None else _table(tokens, _T_I64, (n,), "tokens")
         tp = 0 if temperature is None else _table(temperature, _T_F32, (n,), "temperature")
         wp, wn, _keep = self._work(_logprobs_workspace_bytes(n, vocab, top, code), workspace, logits.device, stream)
-        new = lambda shape, dtype: self._new(shape, dtype, logits.device, stream)
-        entropy = new((n,), torch.float32)
-        logprobs = None if tokens is None else new((n,), torch.float32)
-        ranks = None if tokens is None else new((n,), torch.int32)
-        top_tokens = new((n, top), torch.int64) if top else None
-        top_logprobs = new((n, top), torch.float32) if top else None
-        ptr = lambda t: 0 if t is None else t.data_ptr()
-        args = _pack_logprobs(logits.data_ptr(), logits.stride(0), kp, tp, code, n, vocab, top, ptr(logprobs), ptr(ranks),
-                              ptr(entropy), ptr(top_tokens), ptr(top_logprobs))
+        logprobs = ranks = top_tokens = top_logprobs = None
+        if stream is None:  # new_empty, of the type where a tensor has it: 0.3 to 0.6 us less each than torch.empty
+            entropy = logits.new_empty((n,)) if code == DTYPE_F32 else logits.new_empty((n,), dtype=torch.float32)
+            if tokens is not None:
+                logprobs, ranks = entropy.new_empty((n,)), entropy.new_empty((n,), dtype=torch.int32)
+            if top:
+                top_logprobs = entropy.new_empty((n, top))
+                top_tokens = (entropy if tokens is None else tokens).new_empty((n, top), dtype=torch.int64)
+        else:
+            new = lambda shape, dtype: self._new(shape, dtype, logits.device, stream)
+            entropy = new((n,), torch.float32)
+            if tokens is not None:
+                logprobs, ranks = new((n,), torch.float32), new((n,), torch.int32)
+            if top:
+                top_logprobs, top_tokens = new((n, top), torch.float32), new((n, top), torch.int64)
+        given = tokens is not None
+        args = _pack_logprobs(logits.data_ptr(), logits.stride(0), kp, tp, code, n, vocab, top,
+                              logprobs.data_ptr() if given else 0, ranks.data_ptr() if given else 0, entropy.data_ptr(),
+                              top_tokens.data_ptr() if top else 0, top_logprobs.data_ptr() if top else 0)
         _check(self._lib.dyninfer_mi355x_token_logprobs(self._h, args, wp, wn, self._on(stream)))
         return TokenLogprobs(logprobs, ranks, entropy, top_tokens, top_logprobs)
 
