@@ -203,3 +203,33 @@ def test_refused(ctx):
                 dict(rope=d.Rope(rope.table, rope.positions[:5], 64)), dict(rope=d.Rope(rope.table, rope.positions, 128))):
         with pytest.raises(d.DyninferError):
             ctx.qk_norm_rope(**{**good, **bad})
+
+
+@pytest.mark.parametrize("dim,rot,layout", [(128, 128, "half"), (96, 64, "interleaved"), (256, 256, "half")])
+def test_types_apart(ctx, dim, rot, layout):
+    """Queries and keys, and their weights, of different types in one call: as each alone."""
+    rng = np.random.default_rng(dim)
+    rope = d.Rope(dev(kvref.table(90, rot).astype(np.float32)), i32(rng.integers(0, 90, 29)), rot, layout)
+    for a, b, wa, wb in (("f32", "bf16", "f32", "f32"), ("bf16", "f32", "bf16", "f32"), ("bf16", "bf16", "f32", "bf16")):
+        q, k = (dev(rng.normal(0, 2, (29, h, dim)).astype(np.float32), DT[t]) for h, t in ((5, a), (2, b)))
+        nq, nk = (d.HeadNorm(dev(rng.normal(1, 0.2, dim).astype(np.float32), DT[t])) for t in (wa, wb))
+        got = ctx.qk_norm_rope(q, k, rope, nq, nk)
+        assert torch.equal(got[0], ctx.qk_norm_rope(q, None, rope, nq)[0]) and torch.equal(got[1], ctx.qk_norm_rope(k, None, rope, nk)[0])
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+def test_magnitudes_of_aligned_rows(ctx, io):
+    """Overflowing, tiny, zero, infinite and NaN heads beside ordinary ones: each as alone in rows off 16 bytes."""
+    x = torch.randn(9, 4, 128, device="cuda")
+    x[1, 0] *= 1e30
+    x[1, 1] *= 1e-30
+    x[2, 2] = 0
+    x[3, 3, 7], x[4, 0, 9], x[5, 1] = float("inf"), float("nan"), 3e38
+    x = x.to(DT[io])
+    w = torch.rand(128, device="cuda") + 0.5
+    rope = d.Rope(ctx.rope_table(20, 128), i32(np.arange(9)), 128)
+    off = torch.empty(9 * 4 * 128 + 1, device="cuda", dtype=DT[io])[1:].view(9, 4, 128)
+    off.copy_(x)
+    got, want = (ctx.qk_norm_rope(t, None, rope, d.HeadNorm(w))[0].float() for t in (x, off))
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(), want.nan_to_num())
+    assert torch.isfinite(got[1]).all() and torch.isfinite(got[5]).all() and (got[2, 2] == 0).all()
