@@ -144,12 +144,14 @@ struct VerifyArgs {
 // Attention of prompts (prompt.hip): rows and keys of sequences packed one after the other.
 struct PromptPlan {
     uint32_t row_tiles;  // of the sequence with the most rows
+    uint32_t tile_rows;  // of a row tile that parts have room for
     uint32_t parts;      // into which the keys of a row tile are split, at most
     uint32_t each;       // steps of 64 keys of a part
     uint64_t grid;
     uint64_t bytes, stats;  // workspace, and where the parts' statistics begin in it
 };
-PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint32_t heads, uint32_t group, uint32_t dim);
+PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint32_t heads, uint32_t group, uint32_t dim,
+                       bool f32);
 struct PromptArgs {
     KvRows q, k, v, out;
     const int32_t* q_starts;
@@ -157,7 +159,7 @@ struct PromptArgs {
     float* lse;
     float* part_o;  // [row tile][sequence][kv head][part][row][dim], not yet over their sums
     float* stats;   // [..][row][2]: what exponents are from, sum
-    uint32_t seqs, tokens, keys, max_new, heads, group, dim, row_tiles, parts, each;
+    uint32_t seqs, tokens, keys, max_new, heads, group, dim, row_tiles, tile_rows, parts, each;
     float scale;
 };
 hipError_t prompt_launch(PromptArgs a, const PromptPlan& plan, uint8_t* work, hipStream_t st);

@@ -39,14 +39,14 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t
     vec o = {};
     if (live) {
         const uint64_t unit = (uint64_t)(tile * a.seqs + seq) * a.heads + head;
-        const uint64_t at = unit * a.parts * kPromptRows + row % kPromptRows;  // of part 0; parts are kPromptRows apart
+        const uint64_t at = unit * a.parts * a.tile_rows + row % kPromptRows;  // of part 0
         for (uint32_t p0 = group; p0 < parts; p0 += 4 * groups) {  // four loads in flight
             float pm[4], pl[4];
             vec po[4];
 #pragma unroll
             for (uint32_t k = 0; k < 4; k++) {
                 const uint32_t p = p0 + k * groups;
-                const uint64_t slot = at + (uint64_t)min(p, parts - 1) * kPromptRows;
+                const uint64_t slot = at + (uint64_t)min(p, parts - 1) * a.tile_rows;
                 pm[k] = p < parts ? gptr<float>(a.stats)[2 * slot] : -__builtin_inff();
                 pl[k] = gptr<float>(a.stats)[2 * slot + 1];
                 po[k] = *gptr<vec>(a.part_o + slot * D + from);
@@ -107,33 +107,55 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t
 // of 32/8 heads of 128 dims after 16000 24 us, with four 21; 8 x 8 tokens after 4000 40 and 31, in f32 107
 // and 74.)
 //
-// A device takes two workgroups to a compute unit at a time (of 256 dims, which fill its LDS, one).  `load` is what
-// one of those places has to do in steps of 64 keys, with half of the new rows' own keys masked.  Where the
-// longest row tile has more, and it pays for the second launch (eight steps), keys are cut into parts of
-// `load` steps, four at least:
-//   2 x 96 rows of 12/4 heads of 64 dims after 24000: parts of load / 1, / 2, / 3 steps 36, 42, 46 us
-//   one token after 16000: parts of four steps at least 23 us, of eight 29
-//   512 rows of 32/8 heads, 8 steps in the longest tile: whole 17 us, in parts 22
-//   3 x 1500 of 8/2 heads of 256 dims in f32: whole 427 us, in parts 263
-PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint32_t heads, uint32_t group, uint32_t dim) {
+// Whether and into how many parts keys are cut is the least of these times in us, e steps of 64 keys a part:
+//   whole   the longest row tile, or all tiles' steps over the places for workgroups
+//   parts   a part, or all of them over the places, and the second launch with what it reads and was written for it
+// where a workgroup costs some 5 us to begin and end (f32 8), a step what `step` says, as measured on one
+// workgroup a compute unit, and where two share one 1.3 times that (f32 1.75); 256 dims fill a unit's LDS.
+//   one token after 1000, f32 of 32/8 heads of 128 dims: whole 99 us, parts of 4, 2, 1 steps 35, 23, 17
+//   512 tokens of the same: whole 60 us, parts of 2 steps 44, of 1 61; in bf16 whole 17, of 4 22, of 2 24, of 1 37
+//   2 x 700 tokens of 8/2 heads of 256 dims in f32: whole 125 us, parts of 2 steps 89
+//   2 x 96 tokens of 12/4 heads of 64 dims after 24000 in bf16: parts of 18, 9, 6 steps 36, 42, 46 us
+//   3 x 1500 of 8/2 heads of 256 dims in f32: whole 427 us, parts of 13 steps 260
+PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint32_t heads, uint32_t group, uint32_t dim,
+                       bool f32) {
     PromptPlan p = {};
     const uint64_t rows = (uint64_t)max_new * group;
     p.row_tiles = (uint32_t)((rows + kPromptRows - 1) / kPromptRows);
+    p.tile_rows = (uint32_t)std::min(rows, (uint64_t)kPromptRows);
     const uint64_t units = (uint64_t)seqs * heads * p.row_tiles;
-    const double full = dim > 128 ? 256 : 512;  // workgroups at a time
-    const uint64_t steps = ((uint64_t)max_keys + 63) / 64;
-    const double load = units * (steps - std::min(max_new, max_keys) / 128.0) / full;
-    const double each = std::max(std::ceil(load), 4.0);
+    const uint32_t steps = (uint32_t)(((uint64_t)max_keys + 63) / 64);
     p.parts = 1;
     p.each = 0xFFFFFFFFu;
-    if (steps > load && steps > each + 8) {
-        p.each = (uint32_t)each;
-        p.parts = (uint32_t)((steps + p.each - 1) / p.each);
+    if (units && units <= 1024 && steps > 1) {  // 2^17 rows at most
+        const double places = dim > 128 ? 256 : 512;
+        const double step = f32 ? (dim == 64 ? 3.5 : dim == 96 ? 4.9 : dim == 128 ? 6.1 : 10)
+                                : (dim == 64 ? 1 : dim == 96 ? 1.2 : dim == 128 ? 1.35 : 3);
+        const double shared = dim > 128 ? 1 : f32 ? 1.75 : 1.3, ends = f32 ? 8 : 5;
+        const double span = std::min(max_new, max_keys) / 64.0, mean = steps - span / 2;  // steps of a row tile, on average
+        // n workgroups, of `each` steps the longest and `typical` on average
+        auto time = [&](double n, double each, double typical) {
+            const double s = step * (n > 256 ? shared : 1);
+            return std::max(ends + step * each, n > places ? (n / places + 0.5) * (ends + s * typical) : ends + s * typical);
+        };
+        double best = time(units, steps, mean);
+        const double load = units * mean / places;
+        for (uint32_t e = std::max(1u, (uint32_t)(load / 2)); e < steps && e < 8 * load + 64; e += std::max(1u, e / 4)) {
+            const double most = (steps + e - 1) / e, least = std::ceil(std::max(steps - span, 1.0) / e), parts = (most + least) / 2;
+            const double join = 4.5 + 2.0 * seqs * heads * rows * parts * dim * 4 / 3.8e6;  // one write, one read
+            const double t = time(units * parts, e, std::min((double)e, mean / parts)) + join;
+            if (t < best) {
+                best = t;
+                p.each = e;
+                p.parts = (uint32_t)most;
+            }
+        }
     }
     p.grid = units * p.parts;
     if (p.parts > 1) {
-        p.stats = p.grid * kPromptRows * dim * 4;
-        p.bytes = (p.stats + p.grid * kPromptRows * 8 + 255) / 256 * 256;
+        const uint64_t slots = p.grid * p.tile_rows;
+        p.stats = slots * dim * 4;
+        p.bytes = (p.stats + slots * 8 + 255) / 256 * 256;
     }
     return p;
 }
@@ -147,6 +169,7 @@ hipError_t prompt_launch(PromptArgs a, const PromptPlan& plan, uint8_t* work, hi
     if (plan.grid == 0) return hipSuccess;
     if (!launchable(plan.grid, a.dim > 128 ? 512 : 256)) return kTooManyThreads;
     a.row_tiles = plan.row_tiles;
+    a.tile_rows = plan.tile_rows;
     a.parts = plan.parts;
     a.each = plan.each;
     a.part_o = reinterpret_cast<float*>(work);

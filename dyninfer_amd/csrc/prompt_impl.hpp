@@ -590,7 +590,7 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
     }
 
     const PromptArgs b = late_args();
-    const uint64_t slot0 = ((((uint64_t)tile * b.seqs + seq) * b.heads + head) * b.parts + part) * ROWS + 32 * group;
+    const uint64_t slot0 = ((((uint64_t)tile * b.seqs + seq) * b.heads + head) * b.parts + part) * b.tile_rows + 32 * group;
     // An infinity or a NaN in the output: of what the row sees, or of values that are masked for it
     bool odd = false;
 #pragma unroll

@@ -214,8 +214,8 @@ int check_groups(const dyninfer_prompts_t* b, uint32_t q_heads, uint32_t kv_head
     return 0;
 }
 
-dmx::PromptPlan plan_prompts(const dyninfer_prompts_t* b, uint32_t q_heads, uint32_t kv_heads, uint32_t dim) {
-    return dmx::prompt_plan(b->sequences, b->max_new, b->max_keys, kv_heads, q_heads / kv_heads, dim);
+dmx::PromptPlan plan_prompts(const dyninfer_prompts_t* b, uint32_t q_heads, uint32_t kv_heads, uint32_t dim, uint32_t dtype) {
+    return dmx::prompt_plan(b->sequences, b->max_new, b->max_keys, kv_heads, q_heads / kv_heads, dim, dtype == DYNINFER_DTYPE_F32);
 }
 
 int launched(hipError_t e) {
@@ -532,7 +532,7 @@ int dyninfer_mi355x_prompt_attention_workspace_bytes(const dyninfer_prompts_t* b
     if (int rc = check_dim(head_dim)) return rc;
     if (dtype != DYNINFER_DTYPE_F32 && dtype != DYNINFER_DTYPE_BF16) return fail(UNSUPPORTED, "q must be f32 or bf16");
     if (int rc = check_groups(batch, q_heads, kv_heads)) return rc;
-    *out_bytes = plan_prompts(batch, q_heads, kv_heads, head_dim).bytes;
+    *out_bytes = plan_prompts(batch, q_heads, kv_heads, head_dim, dtype).bytes;
     return DYNINFER_MI355X_OK;
 }
 
@@ -562,7 +562,7 @@ int dyninfer_mi355x_prompt_attention(dyninfer_mi355x_ctx_t* ctx, const dyninfer_
             return fail(BAD, "out overlaps k or v");
     }
     if (int rc = check_groups(batch, q->heads, kv_heads)) return rc;
-    const dmx::PromptPlan plan = plan_prompts(batch, q->heads, kv_heads, head_dim);
+    const dmx::PromptPlan plan = plan_prompts(batch, q->heads, kv_heads, head_dim, q->dtype);
     if (int rc = check_workspace(workspace, workspace_bytes, plan.bytes, "prompt_attention")) return rc;
     a.q_starts = batch->starts;
     a.k_starts = batch->key_starts ? batch->key_starts : batch->starts;
