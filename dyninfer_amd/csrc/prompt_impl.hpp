@@ -19,8 +19,8 @@
 // overlap them in part (1830 cycles for the two kinds, the matrix units busy for 56 %).  16384 tokens of 32/8
 // heads of 128 dims in bf16 take 1.95 ms (1130 TFLOP/s; up to 2.08 by card; a product of two 8192 x
 // 8192 matrices reaches 1370 to 1400), 8192 tokens of 64 dims 284 us (970), of 96 226 (912); 4096 tokens in
-// f32 705 us (195, of six products each).  Prompts of some hundred tokens are bound by the
-// latencies of a tile's beginning and end: 24 x 700 tokens of 16/8 heads 89 us (540).
+// f32 705 us (195, of six products each).  Prompts of some hundred tokens are bound by their
+// rows' bytes and the latencies of a tile's beginning and end: 24 x 700 tokens of 16/8 heads 81 to 86 us.
 // Tried without gain: tiles of 32 keys (2319 us instead of 2068), three waves on a SIMD (registers
 // spill, 2948), two tiles ahead at 64 dims (316 instead of 284), wave priorities.
 #pragma once
@@ -374,6 +374,12 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
     // this wave's rows; a negative scale turns their signs, a scale of 0 makes them 0
     const float scale = fabsf(a.scale);
     w.c = scale == 0.0f ? 1.0f : scale * 1.4426950408889634f;
+    // bf16 rows and outputs of up to 128 dims pass through the stage of the tiles that is not in use, whole rows at a
+    // time: read and written in pieces of 16 or 32 bytes, as the products hold them, a row's lines move eight
+    // times (192 x 128 tokens of 16/8 heads of 128 dims 93 us instead of 78, 768 x 64 of 64 dims 74 instead of 59;
+    // 8192 tokens of 64 dims on the other hand 307 instead of 313).
+    constexpr bool kRowsByLds = !F32 && HALVES == 1;
+    static_assert(!kRowsByLds || ROWS * T::RSB <= STAGE, "room for the rows");
     auto load_rows = [&] {  // behind the first tile's copies: one latency for both
         const int64_t at = (int64_t)((uint64_t)r.row0 + token) * a.q.ts + (int64_t)q_head * a.q.hs + half * (D / HALVES);
         const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
@@ -382,7 +388,9 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
             if constexpr (!F32) {
                 const uint16_t* p = static_cast<const uint16_t*>(a.q.p) + at + 16 * t + 8 * g;
                 u32x4 x;
-                if (a.q.vec) {
+                if (kRowsByLds && a.q.vec) {
+                    x = *reinterpret_cast<const u32x4*>(lds + STAGE + 32 * group * T::RSB + w.k_at[t % W::KA] + t / W::KA * W::KA * 32);
+                } else if (a.q.vec) {
                     x = *gptr<u32x4>(p);
                 } else {
 #pragma unroll
@@ -552,18 +560,36 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
             }
         };
         if (t0 < t1) fetch(t0, 0, 2);
+        if (kRowsByLds && a.q.vec) {
+            constexpr uint32_t N = ROWS * T::RS / 64 / ALL;
+#pragma unroll 1
+            for (uint32_t j = 0; j < N; j++) {
+                const uint32_t at = key0 + STEP * j, chunk = (lane % T::RS) ^ T::mix(at), of = min(tile_row + at, last_row);
+                if (T::CH < T::RS && chunk >= T::CH) continue;
+                const uint32_t i = of / a.group, h = head * a.group + (of - i * a.group);
+                copy16(static_cast<const uint8_t*>(a.q.p) + 2 * ((int64_t)((uint64_t)r.row0 + i) * a.q.ts + (int64_t)h * a.q.hs + 8 * chunk),
+                       lds0 + STAGE + wave * 1024 + ALL * j * 1024);
+            }
+            ring_barrier<0>();
+        }
         load_rows();
         if constexpr (HALVES == 1) {
-            for (uint32_t t = t0; t < t1; t++) {
+            auto next_tile = [&](uint32_t t) {
                 ring_barrier<0>();  // tile t has landed, and the other stage has been read
                 if (t + 1 < t1) fetch(t + 1, 0, 2);
+            };
+            // tiles that some row of this wave sees, then those that others see: one loop for both would have the
+            // compiler move an output's registers with every tile
+            const uint32_t mine = max(min((shut + T::KT - 1) / T::KT, t1), t0);
+            for (uint32_t t = t0; t < mine; t++) {
+                next_tile(t);
                 const uint32_t at = ((t - t0) & 1u) * STAGE;
-                if (!live(t)) continue;
                 Scores p;
 #pragma unroll
                 for (uint32_t sub = 0; sub < W::SUB; sub++) p[sub] = w.scores(lds + at, sub);
                 w.finish(p, lds + at + T::BYTES, t * T::KT, lane, (t + 1) * T::KT > open);
             }
+            for (uint32_t t = mine; t < t1; t++) next_tile(t);
         } else if (t0 < t1) {
             // The scores of a tile ahead of the rest of the one before: one barrier a tile, and products beside
             // exponentials (362 us instead of 397; in f32, whose registers are full, no gain).
@@ -592,11 +618,12 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
     const PromptArgs b = late_args();
     const uint64_t slot0 = ((((uint64_t)tile * b.seqs + seq) * b.heads + head) * b.parts + part) * b.tile_rows + 32 * group;
     // An infinity or a NaN in the output: of what the row sees, or of values that are masked for it
-    bool odd = false;
+    float zeros[4] = {};  // NaN as soon as one is not finite
 #pragma unroll
     for (uint32_t dt = 0; dt < W::DT; dt++)
 #pragma unroll
-        for (uint32_t i = 0; i < 16; i++) odd |= !(fabsf(w.o[dt][i]) < __builtin_inff());
+        for (uint32_t i = 0; i < 16; i++) zeros[i & 3u] = __builtin_fmaf(w.o[dt][i], 0.0f, zeros[i & 3u]);
+    const bool odd = !(zeros[0] + zeros[1] + zeros[2] + zeros[3] == 0.0f);
     const int64_t key_end = min((int64_t)t1 * T::KT, (int64_t)r.nk), key_begin = (int64_t)t0 * T::KT;
     bool alone = false;  // rows one by one
     if (__any(odd)) {
@@ -625,8 +652,9 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
     }
 
     w.l += __shfl_xor(w.l, 32);
-    if (row > last_row) return;
+    const bool live_row = row <= last_row;
     if (cut.parts > 1) {
+        if (!live_row) return;
         const uint64_t slot = slot0 + col;
         if (g == 0 && half == 0) {
             gptr_mut<float>(b.stats)[2 * slot] = w.m;
@@ -643,9 +671,38 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
     const float inv = w.m == kNone ? 0.0f : 1.0f / w.l;
     const uint32_t i0 = row / b.group, h0 = head * b.group + (row - i0 * b.group);  // computed again, not held
     const uint64_t to_row = (uint64_t)r.row0 + i0;
-    if (b.lse && g == 0 && half == 0)
+    if (b.lse && g == 0 && half == 0 && live_row)
         gptr_mut<float>(b.lse)[to_row * (b.heads * b.group) + h0] = w.m == kNone ? kNone : (w.m + log2f(w.l)) * 0.69314718055994531f;
     const int64_t to = (int64_t)to_row * b.out.ts + (int64_t)h0 * b.out.hs + half * (D / HALVES);
+    if (kRowsByLds && b.out.vec) {
+        // the stage of the last tile but one, which all waves have left
+        uint8_t* const mine = lds + ((t1 - t0) % 2 ? STAGE : 0) + 32 * group * T::RSB;
+        if (live_row) {
+#pragma unroll
+            for (uint32_t dt = 0; dt < W::DT; dt++)
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) {
+                    float y[4];
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) y[j] = w.m == kNone ? 0.0f : w.o[dt][4 * i + j] * inv;
+                    *reinterpret_cast<u32x2*>(mine + col * T::RSB + (((4 * dt + i) ^ T::mix(col)) << 4) + 8 * g) =
+                        u32x2{f32x2_to_bf16x2_bits(y[0], y[1]), f32x2_to_bf16x2_bits(y[2], y[3])};
+                }
+        }
+        ring_wait<63>();
+        const uint32_t count = wave_row > last_row ? 0u : min(last_row - wave_row + 1, 32u);
+#pragma unroll
+        for (uint32_t j = 0; j < T::CH / 2; j++) {
+            const uint32_t u = 64 * j + lane, of = u / T::CH, chunk = u % T::CH;
+            const int64_t at = (int64_t)((uint64_t)(uint32_t)__shfl((int)(uint32_t)((uint64_t)to >> 32), (int)of) << 32 |
+                                         (uint32_t)__shfl((int)(uint32_t)(uint64_t)to, (int)of));
+            if (of < count)
+                *gptr_mut<u32x4>(static_cast<uint16_t*>(b.out.p) + at + 8 * chunk) =
+                    *reinterpret_cast<const u32x4*>(mine + of * T::RSB + ((chunk ^ T::mix(of)) << 4));
+        }
+        return;
+    }
+    if (!live_row) return;
 #pragma unroll
     for (uint32_t dt = 0; dt < W::DT; dt++)
 #pragma unroll
