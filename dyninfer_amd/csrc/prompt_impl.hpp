@@ -374,12 +374,13 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
     // this wave's rows; a negative scale turns their signs, a scale of 0 makes them 0
     const float scale = fabsf(a.scale);
     w.c = scale == 0.0f ? 1.0f : scale * 1.4426950408889634f;
-    // bf16 rows and outputs of up to 128 dims pass through the stage of the tiles that is not in use, whole rows at a
-    // time: read and written in pieces of 16 or 32 bytes, as the products hold them, a row's lines move eight
-    // times (192 x 128 tokens of 16/8 heads of 128 dims 93 us instead of 78, 768 x 64 of 64 dims 74 instead of 59;
-    // 8192 tokens of 64 dims on the other hand 307 instead of 313).
-    constexpr bool kRowsByLds = !F32 && HALVES == 1;
-    static_assert(!kRowsByLds || ROWS * T::RSB <= STAGE, "room for the rows");
+    // bf16 rows and outputs pass through the stage of the tiles that is not in use (256 dims: rows through the place
+    // of the halves' scores), whole rows at a time: read and written in pieces of 16 or 32 bytes, as the products hold them, a row's lines move eight
+    // times (192 x 128 tokens of 16/8 heads of 128 dims 93 us instead of 78, 768 x 64 of 64 dims 74 instead of 59, 192 x
+    // 256 of 256 dims 498 instead of 404; 8192 tokens of 64 dims on the other hand 307 instead of 313).
+    constexpr bool kRowsByLds = !F32;
+    uint8_t* const held = HALVES == 1 ? lds + STAGE : reinterpret_cast<uint8_t*>(other);  // rows, before the first tile
+    static_assert(!kRowsByLds || ROWS * T::RSB <= (HALVES == 1 ? STAGE : sizeof(other)), "room for the rows");
     auto load_rows = [&] {  // behind the first tile's copies: one latency for both
         const int64_t at = (int64_t)((uint64_t)r.row0 + token) * a.q.ts + (int64_t)q_head * a.q.hs + half * (D / HALVES);
         const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
@@ -389,7 +390,7 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
                 const uint16_t* p = static_cast<const uint16_t*>(a.q.p) + at + 16 * t + 8 * g;
                 u32x4 x;
                 if (kRowsByLds && a.q.vec) {
-                    x = *reinterpret_cast<const u32x4*>(lds + STAGE + 32 * group * T::RSB + w.k_at[t % W::KA] + t / W::KA * W::KA * 32);
+                    x = *reinterpret_cast<const u32x4*>(held + 32 * group * T::RSB + w.k_at[t % W::KA] + t / W::KA * W::KA * 32);
                 } else if (a.q.vec) {
                     x = *gptr<u32x4>(p);
                 } else {
@@ -562,13 +563,14 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
         if (t0 < t1) fetch(t0, 0, 2);
         if (kRowsByLds && a.q.vec) {
             constexpr uint32_t N = ROWS * T::RS / 64 / ALL;
+            const uint32_t held0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)held;
 #pragma unroll 1
             for (uint32_t j = 0; j < N; j++) {
                 const uint32_t at = key0 + STEP * j, chunk = (lane % T::RS) ^ T::mix(at), of = min(tile_row + at, last_row);
                 if (T::CH < T::RS && chunk >= T::CH) continue;
                 const uint32_t i = of / a.group, h = head * a.group + (of - i * a.group);
                 copy16(static_cast<const uint8_t*>(a.q.p) + 2 * ((int64_t)((uint64_t)r.row0 + i) * a.q.ts + (int64_t)h * a.q.hs + 8 * chunk),
-                       lds0 + STAGE + wave * 1024 + ALL * j * 1024);
+                       held0 + wave * 1024 + ALL * j * 1024);
             }
             ring_barrier<0>();
         }
@@ -675,8 +677,9 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
         gptr_mut<float>(b.lse)[to_row * (b.heads * b.group) + h0] = w.m == kNone ? kNone : (w.m + log2f(w.l)) * 0.69314718055994531f;
     const int64_t to = (int64_t)to_row * b.out.ts + (int64_t)h0 * b.out.hs + half * (D / HALVES);
     if (kRowsByLds && b.out.vec) {
-        // the stage of the last tile but one, which all waves have left
-        uint8_t* const mine = lds + ((t1 - t0) % 2 ? STAGE : 0) + 32 * group * T::RSB;
+        // the stage of the last tile but one, which all waves have left; of 256 dims, behind a barrier, both
+        constexpr uint32_t CO = D / HALVES / 8, RO = CO <= 8 ? 128 : 256;  // units of a row (of a half), bytes from one to the next
+        uint8_t* const mine = HALVES == 1 ? lds + ((t1 - t0) % 2 ? STAGE : 0) + 32 * group * RO : lds + 32 * wave * RO;
         if (live_row) {
 #pragma unroll
             for (uint32_t dt = 0; dt < W::DT; dt++)
@@ -685,20 +688,20 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
                     float y[4];
 #pragma unroll
                     for (uint32_t j = 0; j < 4; j++) y[j] = w.m == kNone ? 0.0f : w.o[dt][4 * i + j] * inv;
-                    *reinterpret_cast<u32x2*>(mine + col * T::RSB + (((4 * dt + i) ^ T::mix(col)) << 4) + 8 * g) =
+                    *reinterpret_cast<u32x2*>(mine + col * RO + (((4 * dt + i) ^ T::mix(col)) << 4) + 8 * g) =
                         u32x2{f32x2_to_bf16x2_bits(y[0], y[1]), f32x2_to_bf16x2_bits(y[2], y[3])};
                 }
         }
         ring_wait<63>();
         const uint32_t count = wave_row > last_row ? 0u : min(last_row - wave_row + 1, 32u);
 #pragma unroll
-        for (uint32_t j = 0; j < T::CH / 2; j++) {
-            const uint32_t u = 64 * j + lane, of = u / T::CH, chunk = u % T::CH;
+        for (uint32_t j = 0; j < CO / 2; j++) {
+            const uint32_t u = 64 * j + lane, of = u / CO, chunk = u % CO;
             const int64_t at = (int64_t)((uint64_t)(uint32_t)__shfl((int)(uint32_t)((uint64_t)to >> 32), (int)of) << 32 |
                                          (uint32_t)__shfl((int)(uint32_t)(uint64_t)to, (int)of));
             if (of < count)
                 *gptr_mut<u32x4>(static_cast<uint16_t*>(b.out.p) + at + 8 * chunk) =
-                    *reinterpret_cast<const u32x4*>(mine + of * T::RSB + ((chunk ^ T::mix(of)) << 4));
+                    *reinterpret_cast<const u32x4*>(mine + of * RO + ((chunk ^ T::mix(of)) << 4));
         }
         return;
     }
