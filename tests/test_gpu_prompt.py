@@ -321,3 +321,26 @@ def test_refused(ctx):
     long = torch.ones(5000, 2, 64, device="cuda")
     with pytest.raises(d.DyninferError):  # parts, and no room for them
         ctx.prompt_attention(q, long, long, d.PromptBatch(i32([0, 6]), 6, i32([0, 5000]), 5000), workspace=torch.empty(256, device="cuda"))
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("news,priors", [([1, 64, 65, 200], [0, 0, 0, 0]), ([33, 9], [2500, 700])])
+def test_layouts_have_the_same_bits(ctx, io, dim, news, priors):
+    """Rows and outputs on and off 16-byte boundaries, heads apart, and rows between others that stay."""
+    p = Prompts(29, news, priors, 2, 3, dim, io)
+    want = p.run(ctx)
+    p.check(want)
+    q, t = p.q, sum(news)
+    wide = torch.full((t + 2, 9, dim), 3.0, device="cuda", dtype=DT[io])
+    for how in ("odd", "head_major", "fused"):
+        out, _ = rows(p.rng, t, 6, dim, DT[io], how)
+        p.q, _ = rows(p.rng, t, 6, dim, DT[io], how)
+        p.q.copy_(q)
+        got = p.run(ctx, out=out)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    p.q = q
+    got = p.run(ctx, out=wide[1:-1, 2:8])
+    assert torch.equal(got[0], want[0])
+    wide[1:-1, 2:8] = 3.0
+    assert (wide == 3.0).all()
