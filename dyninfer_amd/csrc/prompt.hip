@@ -15,7 +15,8 @@ template <int D>
 constexpr uint32_t kJoinLanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;
 
 // A row (token, query head) by kJoinLanes<D> * groups threads: each group brings every groups-th
-// part to its own maximum, then the groups are joined in LDS.  What it reads is small (a float a dim and part);
+// part to its own maximum, then the groups are joined in LDS.  A part that has no maximum has a sum of 0 (no
+// keys for the row, or scores of -inf alone) or of NaN (scores of NaN), which times 0 stays that.  What it reads is small (a float a dim and part);
 // bound by latency where rows are few: one token of 32 heads after 16000, 62 parts, by one group took
 // 34 us, by groups of about four parts each 5.
 template <int D>
@@ -48,20 +49,18 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t
                 const uint32_t p = p0 + k * groups;
                 const uint64_t slot = at + (uint64_t)min(p, parts - 1) * a.tile_rows;
                 pm[k] = p < parts ? gptr<float>(a.stats)[2 * slot] : -__builtin_inff();
-                pl[k] = gptr<float>(a.stats)[2 * slot + 1];
+                pl[k] = p < parts ? gptr<float>(a.stats)[2 * slot + 1] : 0.0f;
                 po[k] = *gptr<vec>(a.part_o + slot * D + from);
             }
             const float now = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m);
-            if (now == -__builtin_inff()) continue;  // saw nothing
-            const float f = __builtin_amdgcn_exp2f(m - now);
+            const float ref = now == -__builtin_inff() ? 0.0f : now, f = __builtin_amdgcn_exp2f(m - ref);
             l *= f;
             o *= f;
 #pragma unroll
             for (uint32_t k = 0; k < 4; k++) {
-                if (pm[k] == -__builtin_inff()) continue;
-                const float g = __builtin_amdgcn_exp2f(pm[k] - now);
+                const float g = __builtin_amdgcn_exp2f(pm[k] - ref);
                 l += pl[k] * g;
-                o += po[k] * g;
+                if (pm[k] != -__builtin_inff()) o += po[k] * g;
             }
             m = now;
         }
@@ -75,9 +74,9 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t
         float top = m, sum = 0.0f;
         for (uint32_t g = 1; g < groups; g++) top = fmaxf(top, sm_m[t0 + g]);
         o = vec{};
+        const float ref = top == -__builtin_inff() ? 0.0f : top;
         for (uint32_t g = 0; g < groups; g++) {
-            if (sm_m[t0 + g] == -__builtin_inff()) continue;
-            const float f = __builtin_amdgcn_exp2f(sm_m[t0 + g] - top);
+            const float f = __builtin_amdgcn_exp2f(sm_m[t0 + g] - ref);
             sum += sm_l[t0 + g] * f;
             o += sm_o[threadIdx.x + g * L] * f;
         }
@@ -85,11 +84,11 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t
         l = sum;
     }
     if (!live) return;
-    const bool none = m == -__builtin_inff();
+    const bool none = prompt_keys(r, i) == 0;
     if (a.lse && lane == 0)
-        gptr_mut<float>(a.lse)[(r0 + (uint64_t)i) * q_heads + h] = none ? m : (m + log2f(l)) * 0.69314718055994531f;
+        gptr_mut<float>(a.lse)[(r0 + (uint64_t)i) * q_heads + h] = none ? -__builtin_inff() : (m + log2f(l)) * 0.69314718055994531f;
     if (d0 >= D) return;
-    const float inv = none ? 0.0f : 1.0f / l;
+    const float inv = 1.0f / l;
     const int64_t e = (int64_t)(r0 + (uint64_t)i) * a.out.ts + (int64_t)h * a.out.hs + d0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {

@@ -301,15 +301,14 @@ __device__ __forceinline__ void prompt_row_by_itself(const PromptArgs& a, uint32
         }
     }
     const bool none = from >= to;
-    const float ref = none ? kNone : m == kNone ? 0.0f : m;  // scores without a number: the sum is NaN
     if (parts) {
-        if (lane == 0 && d0 == 0) gptr_mut<float>(a.stats)[2 * slot] = ref, gptr_mut<float>(a.stats)[2 * slot + 1] = l;
+        if (lane == 0 && d0 == 0) gptr_mut<float>(a.stats)[2 * slot] = m, gptr_mut<float>(a.stats)[2 * slot + 1] = l;
         for (int i = 0; i < N; i++)
             if (lane + 64 * i < DO) gptr_mut<float>(a.part_o)[slot * D + d0 + lane + 64 * i] = o[i];
         return;
     }
     if (a.lse && lane == 0 && d0 == 0)
-        gptr_mut<float>(a.lse)[q_row * (a.heads * a.group) + q_head] = none ? kNone : (ref + log2f(l)) * 0.69314718055994531f;
+        gptr_mut<float>(a.lse)[q_row * (a.heads * a.group) + q_head] = none ? kNone : (m + log2f(l)) * 0.69314718055994531f;
     for (int i = 0; i < N; i++) {
         if (lane + 64 * i >= DO) continue;
         const float y = none ? 0.0f : o[i] / l;
@@ -670,11 +669,14 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
                     f32x4{w.o[dt][4 * i], w.o[dt][4 * i + 1], w.o[dt][4 * i + 2], w.o[dt][4 * i + 3]};
         return;
     }
-    const float inv = w.m == kNone ? 0.0f : 1.0f / w.l;
     const uint32_t i0 = row / b.group, h0 = head * b.group + (row - i0 * b.group);  // computed again, not held
     const uint64_t to_row = (uint64_t)r.row0 + i0;
+    // What sees nothing is told by its keys, not by its statistics: scores of NaN, which the maximum passes
+    // over, leave a sum of NaN, scores of -inf alone one of 0, and the quotients are NaN.
+    const bool none = prompt_keys(r, i0) == 0;
+    const float inv = 1.0f / w.l;
     if (b.lse && g == 0 && half == 0 && live_row)
-        gptr_mut<float>(b.lse)[to_row * (b.heads * b.group) + h0] = w.m == kNone ? kNone : (w.m + log2f(w.l)) * 0.69314718055994531f;
+        gptr_mut<float>(b.lse)[to_row * (b.heads * b.group) + h0] = none ? kNone : (w.m + log2f(w.l)) * 0.69314718055994531f;
     const int64_t to = (int64_t)to_row * b.out.ts + (int64_t)h0 * b.out.hs + half * (D / HALVES);
     if (kRowsByLds && b.out.vec) {
         // the stage of the last tile but one, which all waves have left; of 256 dims, behind a barrier, both
@@ -687,7 +689,7 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
                 for (uint32_t i = 0; i < 4; i++) {
                     float y[4];
 #pragma unroll
-                    for (uint32_t j = 0; j < 4; j++) y[j] = w.m == kNone ? 0.0f : w.o[dt][4 * i + j] * inv;
+                    for (uint32_t j = 0; j < 4; j++) y[j] = none ? 0.0f : w.o[dt][4 * i + j] * inv;
                     *reinterpret_cast<u32x2*>(mine + col * RO + (((4 * dt + i) ^ T::mix(col)) << 4) + 8 * g) =
                         u32x2{f32x2_to_bf16x2_bits(y[0], y[1]), f32x2_to_bf16x2_bits(y[2], y[3])};
                 }
@@ -712,7 +714,7 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
         for (uint32_t i = 0; i < 4; i++) {
             float y[4];
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) y[j] = w.m == kNone ? 0.0f : w.o[dt][4 * i + j] * inv;
+            for (uint32_t j = 0; j < 4; j++) y[j] = none ? 0.0f : w.o[dt][4 * i + j] * inv;
             const int64_t d = to + 32 * dt + 8 * i + 4 * g;
             if constexpr (F32) {
                 float* p = static_cast<float*>(b.out.p) + d;

@@ -484,13 +484,14 @@ typedef struct dyninfer_prompts {
  * out[r, h] = sum_j softmax_j(scale * q[r, h] . k[j, h / group]) v[j, h / group] over the keys j <= i +
  * (keys of the sequence - its rows) of row i = r - starts[b]: causal attention on the activations
  * themselves, without a cache.  All of one dtype (f32 or bf16); group = heads of q / heads of k, any whole number;
- * head_dim 64, 96, 128 or 256.  A row that sees nothing (fewer keys than rows) gives 0 and lse -inf.  Rows of
+ * head_dim 64, 96, 128 or 256.  A row that sees nothing (fewer keys than rows) gives 0 and lse -inf; one that
+ * sees a score of NaN is NaN, lse too, and one that sees scores of -inf alone NaN with lse -inf.  Rows of
  * out behind the last sequence are left as they were.  lse: f32 [tokens, heads], the natural logarithm of the sum
  * of exponentials, or NULL.  What is masked has no influence, whatever it holds.
  * scale is finite, also times log2(e).
  * Rounding: scores and outputs are sums in f32, of exact products in bf16 and of products to 23 bits in f32.
  * Exponentials are f32, in bf16 rounded once before the product with v.  Scores up to 2^30 in magnitude
- * are resolved.
+ * are resolved; a row whose largest score is beyond gives what it should or NaN.
  * workspace: device memory of dyninfer_mi355x_prompt_attention_workspace_bytes, 256-byte aligned (NULL when that is 0),
  * under the rules of dyninfer_mi355x_qlinear's.
  */

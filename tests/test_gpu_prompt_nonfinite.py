@@ -1,0 +1,144 @@
+"""Attention of prompts where scores or values are no finite numbers, on the GPU, against the formula
+in 64 bits row by row.  A row that sees a key is never taken for one that sees nothing: scores of NaN
+make it NaN, and so do scores of -inf alone, whose log-sum-exp is -inf."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_prompt import HALF_STEP, P_STEP, Prompts
+
+pytestmark = pytest.mark.gpu
+
+NAN, INF = float("nan"), float("inf")
+DIMS = [64, 96, 128, 256]
+
+
+def expect(p, row, head):
+    """(out, lse, tolerance of each) of row (b, i) and head in 64 bits, of the keys it sees and no other; tolerances
+    as those of finite inputs (test_gpu_prompt.py), of the finite products."""
+    b, i = row
+    r, k0 = p.starts[b] + i, p.key_starts[b]
+    n = max(0, i + p.nks[b] - p.news[b] + 1)
+    if n == 0:
+        return np.zeros(p.dim), -INF, np.zeros(p.dim), 0.0
+    q = p.q[r, head].double().cpu().numpy()
+    k, v = (x[k0:k0 + n, head // p.group].double().cpu().numpy() for x in (p.k, p.v))
+    with np.errstate(all="ignore"):
+        s = (q * k).sum(-1) * p.dim**-0.5
+        ds = 2.0**-24 * (p.dim + 16) * p.dim**-0.5 * np.nan_to_num(np.abs(q * k), nan=0, posinf=0).sum(-1).max()
+        sums = 2.0**-24 * (32 + n / 4)
+        m = s.max()
+        if m == -INF:
+            return np.full(p.dim, NAN), -INF, np.zeros(p.dim), 0.0
+        e = np.exp(s - m)
+        w, z = e / e.sum(), m + np.log(e.sum())
+        o = (w[:, None] * v).sum(0)
+        tol = (2 * ds + P_STEP[p.io] + sums) * (w[:, None] * np.nan_to_num(np.abs(v), nan=0, posinf=0)).sum(0)
+        return o, z, tol + HALF_STEP[p.io] * np.abs(o), ds + sums + 2.0**-23 * (abs(z) + 1)
+
+
+def rows_of(p):
+    return [(b, i, h) for b, n in enumerate(p.news) for i in range(n) for h in range(p.q.shape[1])]
+
+
+def check(p, got):
+    """Where the formula gives no finite number the same, elsewhere within the tolerance."""
+    out, lse = got[0].double().cpu().numpy(), got[1].double().cpu().numpy()
+    for b, i, h in rows_of(p):
+        o, z, tol, ltol = expect(p, (b, i), h)
+        y, x, finite, what = out[p.starts[b] + i, h], lse[p.starts[b] + i, h], np.isfinite(o), (p.io, p.dim, b, i, h)
+        assert np.array_equal(y[~finite], o[~finite], equal_nan=True), what
+        assert (np.abs(y[finite] - o[finite]) <= tol[finite]).all(), what
+        assert abs(x - z) <= ltol if np.isfinite(z) else np.array_equal(x, z, equal_nan=True), what
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("news,priors", [([70, 5], [0, 0]), ([3, 5], [1024, 0])])
+def test_a_query_of_nan(ctx, io, dim, news, priors):
+    """The row is NaN, log-sum-exp too; no other is.  (Not their bits: rows of a wave move the
+    reference of their exponentials together.)"""
+    p = Prompts(31, news, priors, 2, 2, dim, io)
+    p.q = p.q.clone()
+    spoiled = [(0, 1), (news[0] - 1, 3), (int(p.starts[1]), 0)]
+    for r, h in spoiled:
+        p.q[r, h, 7] = NAN
+    got = p.run(ctx)
+    check(p, got)
+    nan = torch.isnan(got[1])
+    assert nan.sum() == len(spoiled) and all(nan[r, h] for r, h in spoiled)
+    assert torch.equal(torch.isnan(got[0]), nan[:, :, None].expand_as(got[0]))
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("key", [0, 63, 64, 500, 1023, 1024])
+def test_a_key_of_nan(ctx, io, dim, key):
+    """One key of NaN, first, last or alone in its part, and all that see it are NaN."""
+    p = Prompts(33, [1, 6], [1024, 0], 2, 2, dim, io)
+    p.k = p.k.clone()
+    p.k[key, 1, 3] = NAN  # of the long sequence
+    p.k[1025, 0, 5] = NAN  # the first of the short one: its first row sees nothing else
+    got = p.run(ctx)
+    check(p, got)
+    assert torch.isnan(got[0][0, 2:]).all() and torch.isnan(got[1][0, 2:]).all() and torch.isfinite(got[0][0, :2]).all()
+    assert torch.isnan(got[0][1:, :2]).all() and torch.isnan(got[1][1:, :2]).all() and torch.isfinite(got[0][1:, 2:]).all()
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("first,last", [(0, 1025), (64, 640), (640, 1025), (0, 700)])
+def test_many_keys_of_nan(ctx, io, dim, first, last):
+    """All of a part's keys, of all parts' but some, or of all."""
+    p = Prompts(35, [1, 2], [1024, 1022], 1, 4, dim, io)
+    p.k = p.k.clone()
+    p.k[first:last, 0, 9] = NAN
+    p.k[1025 + first:1025 + min(last, 1023), 0, 9] = NAN  # its first row does not see the last key
+    got = p.run(ctx)
+    check(p, got)
+    assert torch.isnan(got[0]).all() and torch.isnan(got[1]).all()
+
+
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("news,priors", [([70, 5], [0, 0]), ([2, 5], [1024, 0])])
+def test_scores_of_minus_infinity(ctx, dim, news, priors):
+    """Keys at -inf have no weight; a row that sees no others is NaN, its log-sum-exp -inf."""
+    p = Prompts(37, news, priors, 2, 2, dim, "bf16")
+    p.q, p.k = p.q.abs() + 0.125, p.k.clone()
+    p.k[:9, 0, 3] = -INF                                             # first keys
+    p.k[p.key_starts[1] - 3:p.key_starts[1] - 1, 1, 5] = -INF        # last keys but one
+    p.k[p.key_starts[1]:, 0, 5] = -INF                               # all
+    p.k[p.key_starts[1], 1, 5] = -INF                                # all that the first row sees
+    got = p.run(ctx)
+    check(p, got)
+    s = int(p.starts[1])
+    assert torch.isnan(got[0][s:, :2]).all() and (got[1][s:, :2] == -INF).all() and torch.isnan(got[0][s, 2:]).all()
+    assert torch.isfinite(got[0][s + 1:, 2:]).all() and torch.isfinite(got[1][s + 1:, 2:]).all()
+
+
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("prior", [512, 1024, 2048, 4096])
+def test_a_part_at_minus_infinity_beside_masked_infinities(ctx, dim, prior):
+    """A part whose only key for the row is at -inf, computed by itself for a masked value's sake, while
+    the other parts' scores are far below 0."""
+    p = Prompts(39, [2], [prior], 1, 1, dim, "bf16")
+    p.q, p.k, p.v = torch.full_like(p.q, 2.0), torch.full_like(p.k, -128.0 / dim**0.5), p.v.clone()
+    p.k[prior, 0, 0] = -INF
+    p.v[prior + 1, 0, 1] = INF
+    assert expect(p, (0, 0), 0)[1] < -200
+    check(p, p.run(ctx))
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_what_sees_nothing_stays_0(ctx, io, dim):
+    """Beside keys of NaN rows without keys still give 0 and -inf."""
+    p = Prompts(41, [40, 6], [-30, -6], 2, 2, dim, io, key_spare=1)
+    p.k = p.k.clone()
+    p.k[:, 1, 3] = NAN
+    got = p.run(ctx)
+    nothing = torch.ones(46, dtype=torch.bool, device="cuda")
+    nothing[30:40] = False
+    assert (got[0][nothing] == 0).all() and (got[1][nothing] == -INF).all()
+    assert torch.isnan(got[0][30:40, 2:]).all() and torch.isnan(got[1][30:40, 2:]).all()
+    assert torch.isfinite(got[0][30:40, :2]).all() and torch.isfinite(got[1][30:40, :2]).all()
