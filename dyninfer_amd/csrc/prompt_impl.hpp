@@ -264,7 +264,8 @@ __device__ __forceinline__ float prompt_element(const KvRows& x, int64_t at) {
 }
 
 // Dims d0 .. d0 + DO - 1 of one row by a wave, key after key, each that the row sees and no other: for rows
-// beside which infinite or NaN values are masked, where 0 times the value is not 0.  Takes
+// beside which infinite or NaN values are masked, where 0 times the value is not 0, and in f32 for rows that
+// see an infinity.  Takes
 // some forty times as long as the tiles do.
 template <int D, int DO, bool F32>
 __device__ __forceinline__ void prompt_row_by_itself(const PromptArgs& a, uint32_t d0, uint64_t q_row, uint32_t q_head, uint64_t key0, uint32_t head,
@@ -618,7 +619,9 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
 
     const PromptArgs b = late_args();
     const uint64_t slot0 = ((((uint64_t)tile * b.seqs + seq) * b.heads + head) * b.parts + part) * b.tile_rows + 32 * group;
-    // An infinity or a NaN in the output: of what the row sees, or of values that are masked for it
+    // An infinity or a NaN in the output: of what the row sees, or of values that are masked for it.  In f32 also of
+    // an infinity that it sees: a product of terms is NaN (inf 0, or inf - inf) where that of the numbers is infinite.
+    // A row whose query holds a NaN is what it should be: no search of all keys for its sake.
     float zeros[4] = {};  // NaN as soon as one is not finite
 #pragma unroll
     for (uint32_t dt = 0; dt < W::DT; dt++)
@@ -626,14 +629,36 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
         for (uint32_t i = 0; i < 16; i++) zeros[i & 3u] = __builtin_fmaf(w.o[dt][i], 0.0f, zeros[i & 3u]);
     const bool odd = !(zeros[0] + zeros[1] + zeros[2] + zeros[3] == 0.0f);
     const int64_t key_end = min((int64_t)t1 * T::KT, (int64_t)r.nk), key_begin = (int64_t)t0 * T::KT;
-    bool alone = false;  // rows one by one
-    if (__any(odd)) {
-        bool masked = false;
+    bool bad = false, alone = false;  // alone: rows one by one
+    const uint64_t odd_lanes = __ballot(odd);
+    uint32_t odd_rows = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
+    if constexpr (F32) {
+        for (uint32_t left = odd_rows; left; left &= left - 1) {
+            const uint32_t i = (uint32_t)__builtin_ctz(left), rr = min(wave_row + i, last_row), tok = rr / b.group;
+            const int64_t at = (int64_t)((uint64_t)r.row0 + tok) * b.q.ts + (int64_t)(head * b.group + (rr - tok * b.group)) * b.q.hs;
+            bool nan = false, inf = false;
+            for (uint32_t d = lane; d < D; d += 64) {
+                const float x = prompt_element<F32>(b.q, at + d);
+                nan |= x != x;
+                inf |= fabsf(x) == __builtin_inff();
+            }
+            if (__any(nan))
+                odd_rows &= ~(1u << i);
+            else
+                bad |= inf;
+        }
+    }
+    if (odd_rows) {
         const int64_t first = max((int64_t)prompt_keys(r, min(wave_row, last_row) / b.group), key_begin);
-        for (int64_t j = max(min(first, key_end - 1), (int64_t)0); j < key_end; j++)  // the last one stands for keys behind the end as well
-            for (uint32_t d = lane; d < D; d += 64)
-                masked |= !(fabsf(prompt_element<F32>(b.v, (int64_t)(r.key0 + j) * b.v.ts + (int64_t)head * b.v.hs + d)) < __builtin_inff());
-        alone = __any(masked);
+        const int64_t masked = max(min(first, key_end - 1), (int64_t)0);  // the last one stands for keys behind the end as well
+#pragma unroll 2
+        for (int64_t j = F32 ? key_begin : masked; j < key_end; j++)
+            for (uint32_t d = lane; d < D; d += 64) {
+                const float v = fabsf(prompt_element<F32>(b.v, (int64_t)(r.key0 + j) * b.v.ts + (int64_t)head * b.v.hs + d));
+                bad |= v == __builtin_inff() || (j >= masked && v != v);
+                if (F32) bad |= fabsf(prompt_element<F32>(b.k, (int64_t)(r.key0 + j) * b.k.ts + (int64_t)head * b.k.hs + d)) == __builtin_inff();
+            }
+        alone = __any(bad);
     }
     if constexpr (HALVES == 2) {  // both halves or neither: they share the sum and what exponents are from
         __shared__ bool flag[ALL];

@@ -491,7 +491,9 @@ typedef struct dyninfer_prompts {
  * scale is finite, also times log2(e).
  * Rounding: scores and outputs are sums in f32, of exact products in bf16 and of products to 23 bits in f32.
  * Exponentials are f32, in bf16 rounded once before the product with v.  Scores up to 2^30 in magnitude
- * are resolved; a row whose largest score is beyond gives what it should or NaN.
+ * are resolved; a row whose largest score is beyond gives what it should or NaN.  Infinities that a row sees
+ * count as such, weights below 2^-126 as 0.  Sums of values times exponentials of up to 2^8 are f32, so that
+ * values beyond 2^120 over the number of keys may overflow.
  * workspace: device memory of dyninfer_mi355x_prompt_attention_workspace_bytes, 256-byte aligned (NULL when that is 0),
  * under the rules of dyninfer_mi355x_qlinear's.
  */

@@ -129,6 +129,59 @@ def test_a_part_at_minus_infinity_beside_masked_infinities(ctx, dim, prior):
     check(p, p.run(ctx))
 
 
+SEEN = [([70, 5], [0, 0]), ([1, 5], [1024, 0]), ([40, 1], [3000, 700])]
+
+
+def small(seed, news, priors, dim, io):
+    """Scores so near each other that every weight is a normal f32."""
+    p = Prompts(seed, news, priors, 2, 2, dim, io)
+    p.q, p.k, p.v = p.q * 0.125, p.k.clone(), p.v.clone()
+    return p
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("news,priors", SEEN)
+def test_values_of_infinity(ctx, io, dim, news, priors):
+    """Infinite values that all rows see, or the later ones: infinite where they are, and nowhere else; NaN where both
+    signs meet."""
+    p = small(43, news, priors, dim, io)
+    s = int(p.key_starts[1])
+    p.v[0, 0, 5], p.v[3, 1, 7], p.v[s, 1, 9] = INF, -INF, INF
+    p.v[s - 1, 0, 5], p.v[s - 1, 0, 6] = -INF, INF
+    got = p.run(ctx)
+    check(p, got)
+    assert torch.isnan(got[0][news[0] - 1, :2, 5]).all() and (got[0][news[0] - 1, :2, 6] == INF).all()
+    assert (got[0][news[0] - 1, 2:, 7] == -INF).all() and (got[0][news[0]:, 2:, 9] == INF).all()
+    assert torch.isfinite(got[1]).all()
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("news,priors", SEEN)
+def test_keys_of_infinity(ctx, io, dim, news, priors):
+    """A score of -inf has no weight, one of +inf makes the row NaN."""
+    p = small(45, news, priors, dim, io)
+    p.k[0, 0, 3], p.k[2, 1, 11], p.k[p.key_starts[1], 0, 60] = INF, -INF, -INF
+    got = p.run(ctx)
+    check(p, got)
+    assert torch.isnan(got[0]).any() and torch.isfinite(got[0]).any()
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("news,priors", SEEN)
+def test_queries_of_infinity(ctx, io, dim, news, priors):
+    """No finite score is left: NaN, and the log-sum-exp -inf where all scores are."""
+    p = small(47, news, priors, dim, io)
+    p.k[:, 0] = p.k[:, 0].abs() + 0.125
+    p.q[0, 0, 3], p.q[0, 1, 3], p.q[-1, 2, 5] = INF, -INF, INF
+    got = p.run(ctx)
+    check(p, got)
+    assert torch.isnan(got[0][0, :2]).all() and torch.isnan(got[1][0, 0]) and got[1][0, 1] == -INF
+    assert torch.isfinite(got[0][0, 2:]).all()
+
+
 @pytest.mark.parametrize("io", ["bf16", "f32"])
 @pytest.mark.parametrize("dim", [64, 256])
 def test_what_sees_nothing_stays_0(ctx, io, dim):
