@@ -487,8 +487,8 @@ typedef struct dyninfer_prompts {
  * head_dim 64, 96, 128 or 256.  A row that sees nothing (fewer keys than rows) gives 0 and lse -inf; one that
  * sees a score of NaN is NaN, lse too, and one that sees scores of -inf alone NaN with lse -inf.  Rows of
  * out behind the last sequence are left as they were.  lse: f32 [tokens, heads], the natural logarithm of the sum
- * of exponentials, or NULL.  What is masked has no influence, whatever it holds.
- * scale is finite, also times log2(e).
+ * of exponentials, or NULL.  What is masked has no influence, whatever it holds, but that rows beside masked values
+ * of NaN or infinity are summed in another order, slower.  scale is finite, also times log2(e).
  * Rounding: scores and outputs are sums in f32, of exact products in bf16 and of products to 23 bits in f32.
  * Exponentials are f32, in bf16 rounded once before the product with v.  Scores up to 2^30 in magnitude
  * are resolved; a row whose largest score is beyond gives what it should or NaN.  Infinities that a row sees

@@ -195,3 +195,34 @@ def test_what_sees_nothing_stays_0(ctx, io, dim):
     assert (got[0][nothing] == 0).all() and (got[1][nothing] == -INF).all()
     assert torch.isnan(got[0][30:40, 2:]).all() and torch.isnan(got[1][30:40, 2:]).all()
     assert torch.isfinite(got[0][30:40, :2]).all() and torch.isfinite(got[1][30:40, :2]).all()
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("news,priors", [([70, 200], [0, 0]), ([40, 45], [20, 900])])
+def test_what_masked_contents_leave(ctx, io, dim, news, priors):
+    """The last row's own key and value spoiled, which lie in the tiles of rows before it.  Finite values, however
+    large, change no bit of those.  A key of NaN changes none of waves (32 rows of a kv head) that do not hold the
+    row that sees it; the others of its wave may move their exponentials' reference elsewhere.  Beside values of
+    NaN or infinity rows are summed in another order: within the tolerance, like all of them."""
+    p = Prompts(49, news, priors, 2, 2, dim, io)
+    clean = p.run(ctx)
+    p.check(clean)
+    row, key = sum(news) - 1, int(p.key_starts[2]) - 1
+    keep_k, keep_v = p.k, p.v
+    p.v = keep_v.clone()
+    p.v[key] = -3.0e38
+    got = p.run(ctx)
+    assert torch.equal(got[0][:row], clean[0][:row]) and torch.equal(got[1][:row], clean[1][:row])
+    p.k, p.v = keep_k.clone(), keep_v
+    p.k[key] = NAN
+    got = p.run(ctx)
+    alone = int(p.starts[1]) + (2 * news[1] - 1) // 32 * 32 // 2  # the first token of the last wave
+    assert alone < row and torch.equal(got[0][:alone], clean[0][:alone]) and torch.equal(got[1][:alone], clean[1][:alone])
+    check(p, got)
+    for bad in (NAN, INF):
+        p.k, p.v = keep_k, keep_v.clone()
+        p.v[key, :, 3] = bad
+        got = p.run(ctx)
+        check(p, got)
+        assert torch.equal(got[0][:news[0]], clean[0][:news[0]]) and torch.isfinite(got[0][:row]).all()
