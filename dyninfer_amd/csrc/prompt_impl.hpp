@@ -56,6 +56,11 @@ __device__ __forceinline__ void copy16(const uint8_t* from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(scalar(to)), "v"(from) : "memory");
 }
 
+// 0 times two bf16: NaN where one is not finite.
+__device__ __forceinline__ uint32_t times_0(uint32_t x) {
+    return ((x & 0x7F80u) == 0x7F80u ? 0x7FC0u : 0u) | ((x & 0x7F800000u) == 0x7F800000u ? 0x7FC00000u : 0u);
+}
+
 // The kernel's arguments read again where they are needed: held in scalar registers through the
 // loop over the keys they would push out what the loop itself uses.
 __device__ __forceinline__ PromptArgs late_args() {
@@ -371,7 +376,7 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
     const uint32_t open = whole ? prompt_keys(r, wave_row / a.group) : 0u;
     const uint32_t shut = wave_row > last_row ? 0u : prompt_keys(r, min(wave_row + 31, last_row) / a.group);
 
-    // this wave's rows; a negative scale turns their signs, a scale of 0 makes them 0
+    // this wave's rows; a negative scale turns their signs, a scale of 0 makes them 0 (what is not finite NaN)
     const float scale = fabsf(a.scale);
     w.c = scale == 0.0f ? 1.0f : scale * 1.4426950408889634f;
     // bf16 rows and outputs pass through the stage of the tiles that is not in use (256 dims: rows through the place
@@ -398,7 +403,7 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
                     for (int j = 0; j < 4; j++) x[j] = gptr<uint16_t>(p)[2 * j] | (uint32_t)gptr<uint16_t>(p)[2 * j + 1] << 16;
                 }
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[j] = a.scale == 0.0f ? 0u : x[j] ^ (a.scale < 0.0f ? 0x80008000u : 0u);
+                for (int j = 0; j < 4; j++) x[j] = a.scale == 0.0f ? times_0(x[j]) : x[j] ^ (a.scale < 0.0f ? 0x80008000u : 0u);
                 w.q[t] = __builtin_bit_cast(bf16x8, x);
             } else {
                 const float* p = static_cast<const float*>(a.q.p) + at + 16 * t + 8 * g;

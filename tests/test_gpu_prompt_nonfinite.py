@@ -226,3 +226,20 @@ def test_what_masked_contents_leave(ctx, io, dim, news, priors):
         got = p.run(ctx)
         check(p, got)
         assert torch.equal(got[0][:news[0]], clean[0][:news[0]]) and torch.isfinite(got[0][:row]).all()
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("news,priors", [([70, 5], [0, 0]), ([1, 5], [1024, 0])])
+def test_a_scale_of_0(ctx, io, dim, news, priors):
+    """0 times a query that is not finite is NaN; all other rows weigh their keys alike."""
+    p = Prompts(51, news, priors, 2, 2, dim, io)
+    p.q = p.q.clone()
+    for h, x in enumerate((NAN, INF, -INF)):
+        p.q[0, h, dim - 1 - h] = x
+    got = p.run(ctx, scale=0.0)
+    assert torch.isnan(got[0][0, :3]).all() and torch.isnan(got[1][0, :3]).all()
+    p.q[0, :3] = 1.0
+    out, lse, tol, ltol = p.expect(0.0)
+    assert ((got[0].double() - out).abs() <= tol)[1:].all() and ((got[1].double() - lse).abs() <= ltol)[1:].all()
+    assert ((got[0].double() - out).abs() <= tol)[0, 3].all()
