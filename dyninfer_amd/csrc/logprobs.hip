@@ -274,7 +274,11 @@ __device__ __forceinline__ void select_top(TopLds<THREADS>& l, uint32_t top, con
 template <int THREADS, bool BF16>
 __device__ __forceinline__ void write_row(const LogprobArgs& a, uint32_t row, const Stats& st, float c, const u64* keys) {
     const float m = st.m, log_s = logf(st.s), inv = a.temperature ? c * kLn2 : 1.0f;
-    auto logp = [&](float x) { return x == -kInf ? -kInf : (x - m) * inv - log_s; };
+    auto logp = [&](float x) {
+        if (x == -kInf) return -kInf;
+        const float d = x - m;  // may leave f32 where d / T does not
+        return (d == -kInf ? (0.5f * x - 0.5f * m) * (2.0f * inv) : d * inv) - log_s;
+    };
     for (uint32_t i = threadIdx.x; i < a.top; i += THREADS) {
         const u64 key = keys[i];
         const size_t to = (size_t)row * a.top + i;
