@@ -379,26 +379,23 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
     // this wave's rows; a negative scale turns their signs, a scale of 0 makes them 0 (what is not finite NaN)
     const float scale = fabsf(a.scale);
     w.c = scale == 0.0f ? 1.0f : scale * 1.4426950408889634f;
-    // bf16 rows and outputs pass through the stage of the tiles that is not in use (256 dims: rows through the place
+    // bf16 rows and outputs on 16-byte boundaries pass through the stage of the tiles that is not in use (256 dims: rows through the place
     // of the halves' scores), whole rows at a time: read and written in pieces of 16 or 32 bytes, as the products hold them, a row's lines move eight
     // times (192 x 128 tokens of 16/8 heads of 128 dims 93 us instead of 78, 768 x 64 of 64 dims 74 instead of 59, 192 x
     // 256 of 256 dims 498 instead of 404; 8192 tokens of 64 dims on the other hand 307 instead of 313).
-    constexpr bool kRowsByLds = !F32;
     uint8_t* const held = HALVES == 1 ? lds + STAGE : reinterpret_cast<uint8_t*>(other);  // rows, before the first tile
-    static_assert(!kRowsByLds || ROWS * T::RSB <= (HALVES == 1 ? STAGE : sizeof(other)), "room for the rows");
+    static_assert(F32 || ROWS * T::RSB <= (HALVES == 1 ? STAGE : sizeof(other)), "room for the rows");
     auto load_rows = [&] {  // behind the first tile's copies: one latency for both
         const int64_t at = (int64_t)((uint64_t)r.row0 + token) * a.q.ts + (int64_t)q_head * a.q.hs + half * (D / HALVES);
         const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
 #pragma unroll
         for (uint32_t t = 0; t < W::QN; t++) {
             if constexpr (!F32) {
-                const uint16_t* p = static_cast<const uint16_t*>(a.q.p) + at + 16 * t + 8 * g;
                 u32x4 x;
-                if (kRowsByLds && a.q.vec) {
+                if (a.q.vec) {
                     x = *reinterpret_cast<const u32x4*>(held + 32 * group * T::RSB + w.k_at[t % W::KA] + t / W::KA * W::KA * 32);
-                } else if (a.q.vec) {
-                    x = *gptr<u32x4>(p);
                 } else {
+                    const uint16_t* p = static_cast<const uint16_t*>(a.q.p) + at + 16 * t + 8 * g;
 #pragma unroll
                     for (int j = 0; j < 4; j++) x[j] = gptr<uint16_t>(p)[2 * j] | (uint32_t)gptr<uint16_t>(p)[2 * j + 1] << 16;
                 }
@@ -566,7 +563,7 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
             }
         };
         if (t0 < t1) fetch(t0, 0, 2);
-        if (kRowsByLds && a.q.vec) {
+        if (a.q.vec) {
             constexpr uint32_t N = ROWS * T::RS / 64 / ALL;
             const uint32_t held0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)held;
 #pragma unroll 1
@@ -708,7 +705,7 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
     if (b.lse && g == 0 && half == 0 && live_row)
         gptr_mut<float>(b.lse)[to_row * (b.heads * b.group) + h0] = none ? kNone : (w.m + log2f(w.l)) * 0.69314718055994531f;
     const int64_t to = (int64_t)to_row * b.out.ts + (int64_t)h0 * b.out.hs + half * (D / HALVES);
-    if (kRowsByLds && b.out.vec) {
+    if (!F32 && b.out.vec) {
         // the stage of the last tile but one, which all waves have left; of 256 dims, behind a barrier, both
         constexpr uint32_t CO = D / HALVES / 8, RO = CO <= 8 ? 128 : 256;  // units of a row (of a half), bytes from one to the next
         uint8_t* const mine = HALVES == 1 ? lds + ((t1 - t0) % 2 ? STAGE : 0) + 32 * group * RO : lds + 32 * wave * RO;
@@ -757,12 +754,8 @@ __global__ __launch_bounds__(2 * kPromptRows * kPromptHalves<D>, 2) void prompt_
             } else {
                 uint16_t* p = static_cast<uint16_t*>(b.out.p) + d;
                 const u32x2 x = {f32x2_to_bf16x2_bits(y[0], y[1]), f32x2_to_bf16x2_bits(y[2], y[3])};
-                if (b.out.vec) {
-                    *gptr_mut<u32x2>(p) = x;
-                } else {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) gptr_mut<uint16_t>(p)[j] = (uint16_t)(x[j / 2] >> (16 * (j & 1)));
-                }
+                for (int j = 0; j < 4; j++) gptr_mut<uint16_t>(p)[j] = (uint16_t)(x[j / 2] >> (16 * (j & 1)));
             }
         }
 }
