@@ -258,14 +258,60 @@ __device__ __forceinline__ void store4(const KvRows& r, int64_t at, const float 
     }
 }
 
-// One head of one token: loads, takes its norm (NORM), rotates, stores.  Halves of whole fours: a lane takes four
+// One head of one token: loads, rotates, stores.  Halves of whole fours: a lane takes four
 // pairs (with eight dims of one half it loads their partners as well and twice the cosines:
 // append over 4 x 2048 tokens 36.0 us instead of 30.7, one token 2.2 instead of 1.8).  Otherwise
 // in place is safe as well: a head's lanes are one wave's, which has loaded all of it before its
 // first store.
-template <int D, bool NORM>
+template <int D>
 __device__ __forceinline__ void rope_row(const KvRows& x, const KvRows& y, uint32_t token, uint32_t head, uint32_t lane,
-                                         const RopeView& rp, const NormView& nv) {
+                                         const RopeView& rp) {
+    const uint32_t d0 = 8 * lane;
+    const int64_t row = (int64_t)token * x.ts + (int64_t)head * x.hs;
+    if (rp.half && rp.rot % 8 == 0 && d0 < rp.rot) {
+        const int64_t to = (int64_t)token * y.ts + (int64_t)head * y.hs;
+        const uint32_t i0 = 4 * lane, i1 = i0 + rp.rot / 2;
+        const int32_t pos = gptr<int32_t>(rp.positions)[token];
+        float a[4], b[4], p[4], q[4];
+        load4(x, row + i0, a);
+        load4(x, row + i1, b);
+        const bool in = pos >= 0 && (uint32_t)pos < rp.table_positions;
+        f32x4 cs[2] = {};
+        if (in) {
+            const float* t = rp.table + (size_t)pos * rp.rot + 2 * i0;
+            cs[0] = *gptr<f32x4>(t);
+            cs[1] = *gptr<f32x4>(t + 4);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const f32x4 w = cs[i];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int e = 2 * i + j;
+                const float c = w[2 * j], s = w[2 * j + 1];
+                p[e] = in ? a[e] * c - b[e] * s : __builtin_nanf("");
+                q[e] = in ? a[e] * s + b[e] * c : __builtin_nanf("");
+            }
+        }
+        store4(y, to + i0, p);
+        store4(y, to + i1, q);
+        return;
+    }
+    float v[8];
+    if (d0 < D) {
+        load8(x, row + d0, v);
+        rotate8(x, row, token, d0, rp, NoNorm(), v);
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (d0 < D) store8(y, (int64_t)token * y.ts + (int64_t)head * y.hs + d0, v);
+}
+
+// The same with the head's norm before the rotation.  A function of its own: sharing one, the rotation alone loaded
+// its cosines behind the rows instead of beside them (append over 4 x 2048 tokens and reading back 53.5 us
+// instead of 50.5).
+template <int D>
+__device__ __forceinline__ void norm_rope_row(const KvRows& x, const KvRows& y, uint32_t token, uint32_t head, uint32_t lane,
+                                              const RopeView& rp, const NormView& nv) {
     const uint32_t d0 = 8 * lane;
     const int64_t row = (int64_t)token * x.ts + (int64_t)head * x.hs;
     const int64_t to = (int64_t)token * y.ts + (int64_t)head * y.hs;
@@ -281,48 +327,42 @@ __device__ __forceinline__ void rope_row(const KvRows& x, const KvRows& y, uint3
     } else if (d0 < D) {
         load8(x, row + d0, v);
     }
-    auto finish = [&](const auto& norm) {
-        if (pairs) {
-            const int32_t pos = gptr<int32_t>(rp.positions)[token];
-            float a[4], b[4], p[4], q[4];
+    const HeadNorm norm = head_norm<D>(nv, v);
+    if (pairs) {
+        const int32_t pos = gptr<int32_t>(rp.positions)[token];
+        float a[4], b[4], p[4], q[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) a[i] = v[i], b[i] = v[4 + i];
-            const bool in = pos >= 0 && (uint32_t)pos < rp.table_positions;
-            f32x4 cs[2] = {};
-            if (in) {
-                const float* t = rp.table + (size_t)pos * rp.rot + 2 * i0;
-                cs[0] = *gptr<f32x4>(t);
-                cs[1] = *gptr<f32x4>(t + 4);
-            }
-            norm.apply(i0, a);
-            norm.apply(i1, b);
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const f32x4 w = cs[i];
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int e = 2 * i + j;
-                    const float c = w[2 * j], s = w[2 * j + 1];
-                    p[e] = in ? a[e] * c - b[e] * s : __builtin_nanf("");
-                    q[e] = in ? a[e] * s + b[e] * c : __builtin_nanf("");
-                }
-            }
-            store4(y, to + i0, p);
-            store4(y, to + i1, q);
-            return;
+        for (int i = 0; i < 4; i++) a[i] = v[i], b[i] = v[4 + i];
+        const bool in = pos >= 0 && (uint32_t)pos < rp.table_positions;
+        f32x4 cs[2] = {};
+        if (in) {
+            const float* t = rp.table + (size_t)pos * rp.rot + 2 * i0;
+            cs[0] = *gptr<f32x4>(t);
+            cs[1] = *gptr<f32x4>(t + 4);
         }
-        if (d0 < D) {
-            norm.apply(d0, v);
-            rotate8(x, row, token, d0, rp, norm, v);
+        norm.apply(i0, a);
+        norm.apply(i1, b);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const f32x4 w = cs[i];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int e = 2 * i + j;
+                const float c = w[2 * j], s = w[2 * j + 1];
+                p[e] = in ? a[e] * c - b[e] * s : __builtin_nanf("");
+                q[e] = in ? a[e] * s + b[e] * c : __builtin_nanf("");
+            }
         }
-        __builtin_amdgcn_wave_barrier();
-        if (d0 < D) store8(y, to + d0, v);
-    };
-    if constexpr (NORM) {
-        finish(head_norm<D>(nv, v));
-    } else {
-        finish(NoNorm());
+        store4(y, to + i0, p);
+        store4(y, to + i1, q);
+        return;
     }
+    if (d0 < D) {
+        norm.apply(d0, v);
+        rotate8(x, row, token, d0, rp, norm, v);
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (d0 < D) store8(y, to + d0, v);
 }
 
 // 4099 tokens of 40 heads of 128 dims in f32: 28.9 us, 6.0 TB/s; one token 1.8 us.  (Four
@@ -332,7 +372,7 @@ __global__ __launch_bounds__(256) void rope_kernel(KvRows x, KvRows y, uint32_t 
     constexpr uint32_t L = kLanes<D>;
     const uint64_t i = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
     if (i >= (uint64_t)tokens * heads) return;
-    rope_row<D, false>(x, y, (uint32_t)(i / heads), (uint32_t)(i % heads), threadIdx.x % L, rp, NormView{});
+    rope_row<D>(x, y, (uint32_t)(i / heads), (uint32_t)(i % heads), threadIdx.x % L, rp);
 }
 
 // Queries in the first q_blocks workgroups, then keys.  A head is read once: its squares are
@@ -350,9 +390,9 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(KvRows q, KvRows q_out, 
     const KvRows x = keys ? k : q, y = keys ? k_out : q_out;
     const NormView n = keys ? k_norm : q_norm;
     if (n.on)
-        rope_row<D, true>(x, y, token, head, lane, rp, n);
+        norm_rope_row<D>(x, y, token, head, lane, rp, n);
     else
-        rope_row<D, false>(x, y, token, head, lane, rp, n);
+        rope_row<D>(x, y, token, head, lane, rp);
 }
 
 // The same where every row and weight begins at 16 bytes and rot is whole eights (or none): a lane takes two
@@ -569,9 +609,9 @@ __global__ __launch_bounds__(256) void append_kernel(KvView kv, KvBatch b, KvRow
         if (i >= (uint64_t)b.tokens * q_heads) return;
         const uint32_t token = (uint32_t)(i / q_heads), head = (uint32_t)(i % q_heads);
         if (NORM && q_norm.on)
-            rope_row<D, true>(q, q_out, token, head, lane, rp, q_norm);
+            norm_rope_row<D>(q, q_out, token, head, lane, rp, q_norm);
         else
-            rope_row<D, false>(q, q_out, token, head, lane, rp, q_norm);
+            rope_row<D>(q, q_out, token, head, lane, rp);
         return;
     }
     Chunk c;
@@ -583,15 +623,16 @@ __global__ __launch_bounds__(256) void append_kernel(KvView kv, KvBatch b, KvRow
             const uint32_t token = c.row(t);
             const int64_t row = (int64_t)token * k.ts + (int64_t)c.h * k.hs;
             float x[8] = {};
-            if (d0 < D) load8(k, row + d0, x);
             if (NORM && k_norm.on) {
+                if (d0 < D) load8(k, row + d0, x);
                 const HeadNorm norm = head_norm<D>(k_norm, x);
                 if (d0 < D) {
                     norm.apply(d0, x);
                     if (rp.table) rotate8(k, row, token, d0, rp, norm, x);
                 }
-            } else if (d0 < D && rp.table) {
-                rotate8(k, row, token, d0, rp, NoNorm(), x);
+            } else if (d0 < D) {
+                load8(k, row + d0, x);
+                if (rp.table) rotate8(k, row, token, d0, rp, NoNorm(), x);
             }
             int32_t code[8];
             const uint16_t sc = quantize<KB, 4>(x, code);
