@@ -9,16 +9,20 @@
 // every logit is read once; a second small launch joins a row's pieces.  A row of up to
 // 2048 logits is one wave's, in one launch (8000 rows of 1000 in bf16 18 us with a launch for each row's
 // joining 76).  Bound by the logits' bytes where rows are many (2047 rows of 151936 in bf16, 622 MB:
-// 125 us without tokens, 5.0 TB/s, the rate of a copy; some eleven vector instructions a logit, the
+// 127 us without tokens, 4.9 TB/s, nearly the rate of a copy; some eleven vector instructions a logit, the
 // exponential counted as four, fill four fifths of that), by two launches where they are few (one
 // row 7 us).
 //
 // The order is that of (logit, lower token first), held as one 64-bit key: the
 // float's bits as a whole number of the same order, and the token's complement.
 // A piece's largest `top`: of its threads' largest logits one wave finds a bound
-// that `top` of them reach; what reaches it (few more than `top`, unless many
-// logits tie) is gathered in LDS, in each wave's own order, and one wave puts it in
-// order.  That is latency, not bytes: 5 alternatives cost the 2047 rows 36 us more, 64 some 300.
+// that `top` of them reach; what reaches it is gathered in LDS, in each wave's own order and
+// quarter, and one wave puts it in order.  That is latency, not bytes: the 2047 rows with tokens take 131 to 148 us by
+// card, with 1, 5, 20, 64 alternatives 159, 162, 194, 355.  Few more than `top` reach the bound, unless many logits tie, or
+// fewer than `top` threads hold any that count: then all of them reach it, and where one wave has more than its
+// quarter holds, `top` rounds over the piece find one after another.  So with 64 alternatives where a piece's logits
+// lie in few threads: 1000 rows of 24576 in bf16 take 55 us, of 24976, whose last piece has 400, 290, and under a mask
+// that leaves 300 in a row 970 (300 here and there: 55).
 #include "kvcache.hpp"
 
 #include <type_traits>
@@ -129,7 +133,7 @@ __device__ __forceinline__ void find_bound(TopLds<THREADS>& l, uint32_t top) {
         for (uint32_t i = 0; i < N; i++) n += (uint32_t)__popcll(__ballot(v[i] >= mid));
         if (n >= top) {
             lo = mid;
-            if (n <= top + top / 4 + 6) break;
+            if (n <= top + top / 4 + 6) break;  // exactly `top`: 2047 rows of 151936 with 20 203 us; up to 2 top + 32: 209; so 193
         } else {
             hi = mid - 1;
         }
@@ -247,7 +251,7 @@ __device__ __forceinline__ void select_top(TopLds<THREADS>& l, uint32_t top, con
             finish(std::integral_constant<uint32_t, kGathered / 64>());
         return;
     }
-    // too many (ties): one after another, each the largest below the one before
+    // too many for a wave's quarter: one after another, each the largest below the one before
     u64 last = ~0ull;
     for (uint32_t i = 0; i < top; i++) {
         u64 best = 0;
@@ -477,7 +481,9 @@ __global__ __launch_bounds__(THREADS, BF16 ? 6 : 1) void piece_kernel(LogprobArg
     }
 }
 
-// Workgroup: a row's pieces joined.  Up to 64 kMany keys (20 pieces of 64) are one wave's, in registers.
+// Workgroup: a row's pieces joined.  Up to 64 kMany keys (20 pieces of 64) are one wave's, in registers; up to 64 kFew
+// (19 pieces of 20) in as few as that takes (by kMany 2047 rows of 151936 with 20 alternatives 197 us instead of
+// 193, one row with 5 13.8 instead of 11).
 constexpr uint32_t kJoin = 256, kFew = 6, kMany = 20;
 template <bool BF16, bool TOP>
 __global__ __launch_bounds__(kJoin) void join_kernel(LogprobArgs a, uint32_t pieces) {

@@ -110,12 +110,16 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, uint32_t
 //   whole   the longest row tile, or all tiles' steps over the places for workgroups
 //   parts   a part, or all of them over the places, and the second launch with what it reads and was written for it
 // where a workgroup costs some 5 us to begin and end (f32 8), a step what `step` says, as measured on one
-// workgroup a compute unit, and where two share one 1.3 times that (f32 1.75); 256 dims fill a unit's LDS.
-//   one token after 1000, f32 of 32/8 heads of 128 dims: whole 99 us, parts of 4, 2, 1 steps 35, 23, 17
-//   512 tokens of the same: whole 60 us, parts of 2 steps 44, of 1 61; in bf16 whole 17, of 4 22, of 2 24, of 1 37
-//   2 x 700 tokens of 8/2 heads of 256 dims in f32: whole 125 us, parts of 2 steps 89
-//   2 x 96 tokens of 12/4 heads of 64 dims after 24000 in bf16: parts of 18, 9, 6 steps 36, 42, 46 us
-//   3 x 1500 of 8/2 heads of 256 dims in f32: whole 427 us, parts of 13 steps 260
+// workgroup a compute unit, and where two share one 1.3 times that (f32 1.75); 256 dims fill a unit's LDS.  Of
+// 64 dims more than two fit a unit, which the model leaves out: the places are 512 there too.
+//   one token after 1000, f32 of 32/8 heads of 128 dims: whole 107 us, parts of 4, 2, 1 (taken) steps 35, 22, 16
+//   512 tokens of the same: whole 57 us, parts of 4, 2, 1 steps 44, 42, 57 (taken 46); in bf16 whole (taken) 17, of 4 23,
+//   of 2 24, of 1 37
+//   2 x 700 tokens of 8/2 heads of 256 dims in f32: whole 124 us, parts of 4, 2 steps 66, 83 (taken 89)
+//   2 x 96 tokens of 12/4 heads of 64 dims after 24000 in bf16: whole 349 us, parts of 36, 18, 9, 6 steps 52, 36, 36, 43 (taken 35)
+//   3 x 1500 of 8/2 heads of 256 dims in f32, all of one length: whole 253 us, parts of 13, 6, 4 steps 258, 306, 287 (taken 250)
+// Above 1024 units the model takes no parts (asked for 1025 to 8192 units of many shapes), so it is not asked there, and the
+// join's rows stay below 2^17.
 PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint32_t heads, uint32_t group, uint32_t dim,
                        bool f32) {
     PromptPlan p = {};
@@ -126,7 +130,7 @@ PromptPlan prompt_plan(uint32_t seqs, uint32_t max_new, uint32_t max_keys, uint3
     const uint32_t steps = (uint32_t)(((uint64_t)max_keys + 63) / 64);
     p.parts = 1;
     p.each = 0xFFFFFFFFu;
-    if (units && units <= 1024 && steps > 1) {  // 2^17 rows at most
+    if (units && units <= 1024 && steps > 1) {
         const double places = dim > 128 ? 256 : 512;
         const double step = f32 ? (dim == 64 ? 3.5 : dim == 96 ? 4.9 : dim == 128 ? 6.1 : 10)
                                 : (dim == 64 ? 1 : dim == 96 ? 1.2 : dim == 128 ? 1.35 : 3);

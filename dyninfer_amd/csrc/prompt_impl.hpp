@@ -17,10 +17,11 @@
 // What bounds it: 32 rows by 64 keys of 128 dims are 32 MFMAs of 32 cycles, 1024, and some 160 vector
 // instructions, 32 exponentials among them, about as many cycles again; the two waves of a SIMD
 // overlap them in part (1830 cycles for the two kinds, the matrix units busy for 56 %).  16384 tokens of 32/8
-// heads of 128 dims in bf16 take 1.95 ms (1130 TFLOP/s; up to 2.08 by card; a product of two 8192 x
-// 8192 matrices reaches 1370 to 1400), 8192 tokens of 64 dims 284 us (970), of 96 226 (912); 4096 tokens in
-// f32 705 us (195, of six products each).  Prompts of some hundred tokens are bound by their
-// rows' bytes and the latencies of a tile's beginning and end: 24 x 700 tokens of 16/8 heads 81 to 86 us.
+// heads of 128 dims in bf16 take 2.02 to 2.11 ms by card (1041 to 1091 TFLOP/s; a product of two 8192 x
+// 8192 matrices reaches 1400), 8192 tokens of 64 dims 299 to 309 us (890 to 920), of 16/4 heads of 96 234 to 242 (two
+// waves a SIMD, whose products and exponentials hardly overlap); 4096 tokens of 32/8 heads in f32 724 to 746 us (184 to
+// 190, of six products each).  Prompts of some hundred tokens are bound by their
+// rows' bytes and the latencies of a tile's beginning and end: 24 x 700 tokens of 16/8 heads 84 to 86 us.
 // Tried without gain: tiles of 32 keys (2319 us instead of 2068), three waves on a SIMD (registers
 // spill, 2948), two tiles ahead at 64 dims (316 instead of 284), wave priorities.
 #pragma once
@@ -270,8 +271,8 @@ __device__ __forceinline__ float prompt_element(const KvRows& x, int64_t at) {
 
 // Dims d0 .. d0 + DO - 1 of one row by a wave, key after key, each that the row sees and no other: for rows
 // beside which infinite or NaN values are masked, where 0 times the value is not 0, and in f32 for rows that
-// see an infinity.  Takes
-// some forty times as long as the tiles do.
+// see an infinity.  A wave takes some 0.17 us a row and key (f32 0.05): one infinite value that all rows see makes
+// 4096 tokens of 32/8 heads in f32 35 ms instead of 0.87, one late in them 27, in bf16 24 instead of 0.17.
 template <int D, int DO, bool F32>
 __device__ __forceinline__ void prompt_row_by_itself(const PromptArgs& a, uint32_t d0, uint64_t q_row, uint32_t q_head, uint64_t key0, uint32_t head,
                                                   int64_t from, int64_t to, bool parts, uint64_t slot) {
