@@ -553,7 +553,8 @@ int dyninfer_mi355x_draft_verify_workspace_bytes(uint32_t sequences, uint32_t to
  * resolved, those beyond count as the nearest; a NaN gives NaN.  A NaN logit counts as -inf, +inf as the
  * largest f32.  A token outside the vocabulary (a padded batch's) has logarithm -inf and rank -1.
  * Alternatives are tokens of logits above -inf; where there are fewer, the rest are token -1 with
- * -inf.  A row of -inf only: logarithms -inf, entropy 0.  Sums are f32.
+ * -inf.  A row of -inf only: logarithms -inf, entropy 0.  Sums are f32, without the largest logit's own term:
+ * logarithms near 0 and small entropies are right to their own size.
  */
 typedef struct dyninfer_logprobs {
     const void* logits; /* f32 or bf16, rows logits_stride elements apart */
