@@ -12,7 +12,7 @@
 // every logit is read once; a second small launch joins a row's pieces.  A row of up to
 // 2048 logits is one wave's, in one launch (8000 rows of 1000 in bf16 18 us with a launch for each row's
 // joining 76).  Bound by the logits' bytes where rows are many (2047 rows of 151936 in bf16, 622 MB:
-// 127 us without tokens, 4.9 TB/s, nearly the rate of a copy; some eleven vector instructions a logit, the
+// 130 to 135 us without tokens, 4.6 to 4.8 TB/s, nearly the rate of a copy; some eleven vector instructions a logit, the
 // exponential counted as four, fill four fifths of that), by two launches where they are few (one
 // row 7 us).
 //
@@ -21,11 +21,11 @@
 // A piece's largest `top`: of its threads' largest logits one wave finds a bound
 // that `top` of them reach; what reaches it is gathered in LDS, in each wave's own order and
 // quarter, and one wave puts it in order.  That is latency, not bytes: the 2047 rows with tokens take 131 to 148 us by
-// card, with 1, 5, 20, 64 alternatives 159, 162, 194, 355.  Few more than `top` reach the bound, unless many logits tie, or
+// card, with 1, 5, 20, 64 alternatives 161, 164, 194, 352.  Few more than `top` reach the bound, unless many logits tie, or
 // fewer than `top` threads hold any that count: then all of them reach it, and where one wave has more than its
 // quarter holds, `top` rounds over the piece find one after another.  So with 64 alternatives where a piece's logits
 // lie in few threads: 1000 rows of 24576 in bf16 take 55 us, of 24976, whose last piece has 400, 290, and under a mask
-// that leaves 300 in a row 970 (300 here and there: 55).
+// that leaves 300 in a row 990 (300 here and there: 54).
 #include "kvcache.hpp"
 
 #include <type_traits>
